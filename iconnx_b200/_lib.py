@@ -15,9 +15,26 @@ HEADER = os.path.join(os.path.dirname(HERE), "include", "iconnx_b200.h")
 
 ICX_OK = 0
 ICX_MAX_MINMAX_PARTIALS = 1184
-ICX_U8, ICX_S8, ICX_S32, ICX_F32, ICX_S64, ICX_BOOL = 0, 1, 2, 3, 4, 5
+ICX_U8, ICX_S8, ICX_S32, ICX_F32, ICX_S64, ICX_BOOL, ICX_F16, ICX_BF16 = range(8)
+ICX_DEVICE_BAD_PAGE = 0x201
+ICX_SCALED_MAX_K = 131071
 
 _vp, _sz, _i = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int
+_i64 = ctypes.c_int64
+
+
+class KvCacheArg(ctypes.Structure):
+    """icx_kv_cache"""
+    _fields_ = [("k_codes", _vp), ("v_codes", _vp), ("k_params", _vp), ("v_params", _vp),
+                ("pages", _i64), ("page_size", _i), ("kv_heads", _i), ("head_dim", _i),
+                ("bits", _i), ("group", _i)]
+
+
+class KvTokensArg(ctypes.Structure):
+    """icx_kv_tokens"""
+    _fields_ = [("d_page_table", _vp), ("d_seq_lens", _vp), ("d_cu_tokens", _vp),
+                ("tokens", _i64), ("batch", _i), ("table_width", _i)]
+
 
 # name -> (restype, argtypes)
 PROTOTYPES = {
@@ -40,6 +57,13 @@ PROTOTYPES = {
     "icx_dql_quantize_f32_u8": (_i, [_vp, _vp, _sz, _vp, _i, _vp, _vp, _vp, _vp, _sz]),
     "icx_dequantize_linear": (_i, [_vp, _vp, _i, _sz, _sz, _sz, _vp, _sz, _vp, _vp]),
     "icx_matmul_integer_rowsum": (_i, [_vp, _vp, _i, _sz, _sz, _vp]),
+    "icx_quantize_per_token": (_i, [_vp, _vp, _i, _sz, _sz, _sz, _vp, _vp]),
+    "icx_matmul_integer_scaled": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _sz, _vp, _vp, _vp, _i, _vp]),
+    "icx_kv_cache_append": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i64, _i64, _i64, _i64, _vp, _vp]),
+    "icx_kv_cache_read": (_i, [_vp, _vp, _vp, _i, _vp, _vp]),
+    "icx_kv_cache_attention_workspace_bytes": (_sz, [_vp, _vp, _i]),
+    "icx_kv_cache_attention": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i64, _i64, ctypes.c_float, _vp, _vp,
+                                    _sz]),
     "icx_engine_create": (_vp, [_i]),
     "icx_engine_destroy": (None, [_vp]),
     "icx_engine_add_input": (_i, [_vp, ctypes.c_char_p, _i, _i, _vp]),

@@ -1,0 +1,76 @@
+// Layout of the quantised K/V cache, shared by the kernels that write, read
+// and attend over it.
+//
+// Codes stand in rows of head_dim * bits / 8 bytes, one row per (page, head,
+// token of the page).  Inside a row they are ordered for the attention's
+// matrix instructions (m16n8k16, thread (g, t) of a warp: g = lane / 4,
+// t = lane % 4), so that a thread's operands are consecutive bytes:
+//
+//   K is the left operand of the scores (rows = tokens, contraction over the
+//   dimensions).  Step j of the contraction covers dimensions 16j .. 16j+15,
+//   of which thread t holds 16j + 4t + {0,1,2,3}.  The row is four chunks, one
+//   per t, each with t's dimensions of all steps in order.
+//     4 bits: word w of a chunk holds steps 2w and 2w+1; dimension i of step
+//             2w + o stands in nibble {0, 4, 2, 6}[i] + o.
+//     8 bits: word j of a chunk holds step j; dimension i stands in byte
+//             {0, 2, 1, 3}[i].
+//   V is the left operand of the output (rows = dimensions, contraction over
+//   the tokens).  Row tile m covers dimensions 16m .. 16m+15, of which thread
+//   g holds 16m + 2g + {0,1}.  The row is eight chunks, one per g; dimension
+//   16m + 2g + h is code 2m + h of chunk g, in order of the bits.
+#pragma once
+
+#include "floats.cuh"
+
+namespace icx {
+
+struct KvView {
+  uint8_t* codes[2];    // K, V
+  uint32_t* params[2];  // s (bf16) in the low half, lo (bf16) in the high half
+  int64_t pages;
+  int page_shift, heads, dim, bits, group;
+};
+
+struct KvTokens {
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* cu;  // nullable: one token per sequence
+  int64_t tokens;
+  int batch, width;
+};
+
+// Checks both arguments and fills the device views; `what` names the operator
+// in messages.
+int kv_views(const char* what, const icx_kv_cache* cache, const icx_kv_tokens* where, KvView* view,
+             KvTokens* tokens);
+
+__device__ __forceinline__ float param_scale(uint32_t p) { return __uint_as_float(p << 16); }
+__device__ __forceinline__ float param_low(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
+
+// Sequence of packed row i: the b with cu[b] <= i < cu[b+1], or -1.  Whatever
+// cu holds, b is within the batch.
+__device__ __forceinline__ int kv_sequence(const KvTokens& w, int64_t i) {
+  if (w.cu == nullptr) return i < w.batch ? (int)i : -1;
+  int lo = 0, hi = w.batch;   // first b with cu[b+1] > i
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if ((int64_t)w.cu[mid + 1] > i) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo < w.batch && (int64_t)w.cu[lo] <= i ? lo : -1;
+}
+
+// Page of position p of sequence b, or -1 where the table gives none.
+__device__ __forceinline__ int64_t kv_page(const KvView& c, const KvTokens& w, int b, int p) {
+  const int n = p >> c.page_shift;
+  if (n >= w.width) return -1;
+  const int64_t page = w.table[(int64_t)b * w.width + n];
+  return page >= 0 && page < c.pages ? page : -1;
+}
+
+// Row of (page, head, token of the page) in the codes and params buffers.
+__device__ __forceinline__ int64_t kv_row(const KvView& c, int64_t page, int head, int p) {
+  return (((page * c.heads) + head) << c.page_shift) + (p & ((1 << c.page_shift) - 1));
+}
+
+}  // namespace icx

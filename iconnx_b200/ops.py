@@ -6,7 +6,9 @@ These mirror the reference's op wrappers (src/cuda/ops/quantize.rs):
 * ``gpu_matmul_integer(a, b, a_zp, b_zp)`` -> s32                           (:398)
 * ``gpu_dequantize_linear(x, scale, zp, axis)`` -> f32                      (:24)
 
-plus the fused chain this build adds (``quant_linear``).  Errors are raised
+plus the fused chain this build adds (``quant_linear``) and the int8 linear
+layer with a scale per token and per output channel
+(``gpu_quantize_per_token``, ``gpu_matmul_integer_scaled``).  Errors are raised
 as :class:`IcxError` (the reference returns ``CudaError::Kernel``), before any
 launch.  torch only supplies device memory and the current stream; every
 computation runs in libiconnx_b200.so.
@@ -20,11 +22,13 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._lib import ICX_S8, ICX_S32, ICX_U8, IcxError, check
+from ._lib import ICX_BF16, ICX_F16, ICX_F32, ICX_S8, ICX_S32, ICX_U8, IcxError, check
 
 _TYPE = {torch.uint8: ICX_U8, torch.int8: ICX_S8, torch.int32: ICX_S32}
+_FLOAT_TYPE = {torch.float32: ICX_F32, torch.float16: ICX_F16, torch.bfloat16: ICX_BF16}
 _DT_NAME = {torch.float32: "Float32", torch.uint8: "UInt8", torch.int8: "Int8",
-            torch.int32: "Int32", torch.int64: "Int64", torch.float16: "Float16"}
+            torch.int32: "Int32", torch.int64: "Int64", torch.float16: "Float16",
+            torch.bfloat16: "BFloat16"}
 
 
 def _name(dt) -> str:
@@ -42,6 +46,32 @@ def _ptr(t: torch.Tensor | None):
 def _cuda(t: torch.Tensor, what: str) -> torch.Tensor:
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise IcxError(-1, f"{what}: expected a CUDA tensor")
+    return t.contiguous()
+
+
+def _on(device: torch.device, fn, *args) -> None:
+    """Calls a C entry with ``device`` current (its launches go there)."""
+    if torch.cuda.current_device() == device.index:
+        check(fn(*args))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args))
+
+
+def _float_type(dtype, what: str) -> int:
+    t = _FLOAT_TYPE.get(dtype)
+    if t is None:
+        raise IcxError(-1, f"{what} must be Float32, Float16 or BFloat16, got {_name(dtype)}")
+    return t
+
+
+def _operand(t: torch.Tensor, dtype, shape, device, what: str) -> torch.Tensor:
+    """t as a contiguous CUDA tensor of that type, shape and device."""
+    if not isinstance(t, torch.Tensor) or t.device != device:
+        raise IcxError(-1, f"{what}: expected a tensor on {device}")
+    if t.dtype != dtype or t.shape != shape:
+        raise IcxError(-1, f"{what}: expected {_name(dtype)} {list(shape)}, "
+                           f"got {_name(t.dtype)} {list(t.shape)}")
     return t.contiguous()
 
 
@@ -279,3 +309,71 @@ def dynamic_quant_linear(x: torch.Tensor, w: PreparedWeight, w_scale: torch.Tens
     rows = outs[3] if b_zp is not None else None
     out = quant_linear(y, s, z, w, w_scale, bias, b_zp, rows, gelu, minmax=out_minmax)
     return out, y, s, z
+
+
+def gpu_quantize_per_token(x: torch.Tensor):
+    """Symmetric int8 quantisation with one scale per row of the last axis.
+
+    x: Float32 / Float16 / BFloat16 [..., K].  Returns ``(q, scale)``: Int8 of
+    x's shape and Float32 [...], ``scale = max|x| / 127`` and
+    ``q = clamp(round_half_even(x / scale), -127, 127)``.  A row of zeros has
+    scale 0; a row that holds a NaN or an infinity has scale NaN and q = 0, so
+    that a product with it is NaN.  No gradient flows through it.
+    """
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise IcxError(-1, "QuantizePerToken: expected a CUDA tensor")
+    t = _float_type(x.dtype, "QuantizePerToken: input")
+    if x.dim() == 0:
+        raise IcxError(-1, "QuantizePerToken: a scalar has no token axis")
+    K = x.shape[-1]
+    # rows at one stride are read in place (a slice of wider rows), others copied
+    if x.dim() != 2 or (x.stride(1) != 1 and K > 1) or (x.stride(0) < K and x.shape[0] > 1):
+        x = x.contiguous()
+    rows = x.numel() // K if K else x.shape[:-1].numel()
+    stride = x.stride(0) if x.dim() == 2 and x.shape[0] > 1 else K
+    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    _on(x.device, _lib.load().icx_quantize_per_token, _stream(x), x.data_ptr(), t, rows, K, stride,
+        q.data_ptr(), scale.data_ptr())
+    return q, scale
+
+
+def gpu_matmul_integer_scaled(q: torch.Tensor, q_scale: torch.Tensor, w: PreparedWeight,
+                              w_scale: torch.Tensor, bias: torch.Tensor | None = None,
+                              residual: torch.Tensor | None = None,
+                              out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """Int8 product with a scale per token and per output channel.
+
+    ``out[m, n] = (sum_k q[m, k] w[k, n]) * q_scale[m] * w_scale[n] [+ bias[n]]
+    [+ residual[m, n]]``: the sum exact in s32 (K at most 131071), the rest in
+    f32, rounded once to ``out_dtype``.
+
+    q: Int8 [..., K], q_scale: Float32 [...] (:func:`gpu_quantize_per_token`);
+    w: an Int8 :func:`prepare_weight`; w_scale, bias: Float32 [N]; residual:
+    ``out_dtype`` [..., N].  No gradient flows through it.
+    """
+    what = "MatMulIntegerScaled"
+    if not isinstance(q, torch.Tensor) or not q.is_cuda:
+        raise IcxError(-1, f"{what}: expected a CUDA tensor")
+    if q.dtype != torch.int8 or q.dim() == 0:
+        raise IcxError(-1, f"{what}: q must be Int8 [..., K], got {_name(q.dtype)} {list(q.shape)}")
+    if w.dtype != torch.int8 or q.shape[-1] != w.K:
+        raise IcxError(-1, f"{what}: weight must be Int8 with matching K (q {list(q.shape)}, "
+                           f"weight {_name(w.dtype)} [{w.K}, {w.N}])")
+    t = _float_type(out_dtype, f"{what}: out_dtype")
+    dev, lead = q.device, q.shape[:-1]
+    if w.bt.device != dev:
+        raise IcxError(-1, f"{what}: weight is on {w.bt.device}, q on {dev}")
+    q = q.contiguous()
+    q_scale = _operand(q_scale, torch.float32, lead, dev, f"{what}: q_scale")
+    w_scale = _operand(w_scale, torch.float32, (w.N,), dev, f"{what}: w_scale")
+    shape = (*lead, w.N)
+    if bias is not None:
+        bias = _operand(bias, torch.float32, (w.N,), dev, f"{what}: bias")
+    if residual is not None:
+        residual = _operand(residual, out_dtype, shape, dev, f"{what}: residual")
+    out = torch.empty(shape, dtype=out_dtype, device=dev)
+    _on(dev, _lib.load().icx_matmul_integer_scaled, _stream(q), q.data_ptr(), q_scale.data_ptr(),
+        w.bt.data_ptr(), lead.numel(), w.K, w.N, w_scale.data_ptr(), _ptr(bias), _ptr(residual), t,
+        out.data_ptr())
+    return out

@@ -19,7 +19,8 @@
  *     kernel entry points never allocate; scratch space is passed in as a
  *     caller-owned workspace whose size a *_workspace_bytes query returns.
  *   - Matrices are row-major and contiguous.
- *   - Element type codes: ICX_U8, ICX_S8, ICX_S32, ICX_F32.
+ *   - Element type codes: ICX_U8, ICX_S8, ICX_S32, ICX_F32; the decoder-layer
+ *     operators also take ICX_F16 and ICX_BF16.
  */
 #ifndef ICONNX_B200_H
 #define ICONNX_B200_H
@@ -51,6 +52,10 @@ extern "C" {
 #define ICX_DEVICE_TIMEOUT_MMA 0x102
 #define ICX_DEVICE_TIMEOUT_EPILOGUE 0x103
 #define ICX_DEVICE_TIMEOUT_SELFTEST 0x1ff
+/* a cache operator met a position without a usable page (and touched nothing
+ * there): the page table's entry is outside the pool, or the sequence is
+ * longer than its row of the table */
+#define ICX_DEVICE_BAD_PAGE 0x201
 
 /* Upper bound on the (min, max) partial pairs a producer writes for a
  * following DynamicQuantizeLinear (icx_quant_linear d_minmax, and the
@@ -64,6 +69,8 @@ extern "C" {
 #define ICX_F32 3
 #define ICX_S64 4
 #define ICX_BOOL 5
+#define ICX_F16 6
+#define ICX_BF16 7
 
 /* Message for the last failing call on this thread ("" if none). */
 ICX_API const char* icx_last_error(void);
@@ -246,6 +253,109 @@ ICX_API int icx_dequantize_linear(void* stream, const void* d_x, int x_type,
  * MatMulInteger path replacing src/cuda/ops/quantize.rs:398-615. */
 ICX_API int icx_matmul_integer_rowsum(void* stream, const void* d_a, int a_type, size_t M,
                                       size_t K, int32_t* d_rowsum);
+
+/* ======================================================================== *
+ * Integer side of a decoder layer (no reference counterpart: the reference
+ * has one scale per tensor and no cache).  Float operands are ICX_F32,
+ * ICX_F16 or ICX_BF16.
+ *
+ * Per-token quantisation of x [rows, cols] (row_stride elements apart,
+ * row_stride >= cols):
+ *   s = f32(max|x| / 127), q = clamp(rte(x / s), -127, 127)   (exact quotient)
+ * A row of zeros (or one whose scale rounds to 0): s = 0, q = 0.  A row that
+ * holds a NaN or an infinity: s = NaN, q = 0.
+ * Outputs: d_q s8 [rows, cols] contiguous, d_scale f32 [rows].
+ * ======================================================================== */
+ICX_API int icx_quantize_per_token(void* stream, const void* d_x, int x_type, size_t rows,
+                                   size_t cols, size_t row_stride, int8_t* d_q, float* d_scale);
+
+/* Product of per-token quantised activations with a prepared weight
+ * (icx_prepare_b of an s8 weight with a scale per output channel):
+ *   out[m,n] = (sum_k q[m,k] * w[k,n]) * q_scale[m] * w_scale[n]
+ *              [+ bias[n]] [+ residual[m,n]]
+ * The sum is exact in s32 (K <= ICX_SCALED_MAX_K, so it cannot wrap); the
+ * rest is f32, rounded once to out_type.  bias: f32 [N] or NULL; residual:
+ * out_type [M, N] or NULL. */
+#define ICX_SCALED_MAX_K 131071
+ICX_API int icx_matmul_integer_scaled(void* stream, const int8_t* d_q, const float* d_q_scale,
+                                      const int8_t* d_wt, size_t M, size_t K, size_t N,
+                                      const float* d_w_scale, const float* d_bias,
+                                      const void* d_residual, int out_type, void* d_out);
+
+/* A paged K/V cache held in 4 or 8 bits.  Per (token, kv head) the head_dim
+ * values are quantised in groups of `group` (32 or 64), L = 2^bits - 1:
+ *   lo = bf16 rounded down (min x), not below -bf16max
+ *   s  = bf16 rounded up ((max x - lo) / L)
+ *   c  = clamp(rte((x - lo) / s), 0, L)   (exact quotient; s = 0: c = 0)
+ * and stand for c * s + lo.  Rounding lo down and s up keeps the whole group
+ * inside [lo, lo + L s].  A group that holds a NaN or an infinity is stored
+ * as NaN.  Position p of a sequence stands in page page_table[p / page_size].
+ * Buffers (device): codes [pages, kv_heads, page_size, head_dim * bits / 8]
+ * bytes, params [pages, kv_heads, page_size, head_dim / group] words (s in
+ * the low half, lo in the high half); the order of the codes inside a row is
+ * private to these entry points.  page_size: a power of two, 16..1024;
+ * head_dim: 64, 128 or 256.  All four buffers are 16-byte aligned. */
+typedef struct icx_kv_cache {
+  void* k_codes;
+  void* v_codes;
+  void* k_params;
+  void* v_params;
+  int64_t pages;
+  int page_size;
+  int kv_heads;
+  int head_dim;
+  int bits;
+  int group;
+} icx_kv_cache;
+
+/* The tokens of one call: sequence b of `batch` has seq_lens[b] tokens in the
+ * cache (this call's included); its new tokens are rows cu_tokens[b] ..
+ * cu_tokens[b+1]-1 of the packed operands and stand at its last positions.
+ * d_cu_tokens (s32 [batch + 1]) may be NULL: one token per sequence.  Rows
+ * outside [cu_tokens[0], cu_tokens[batch]) are left as they were.  All
+ * index arrays are s32 on the device; page_table is [batch, table_width]. */
+typedef struct icx_kv_tokens {
+  const int32_t* d_page_table;
+  const int32_t* d_seq_lens;
+  const int32_t* d_cu_tokens;
+  int64_t tokens; /* rows of the packed operands */
+  int batch;
+  int table_width;
+} icx_kv_tokens;
+
+/* Quantises k and v ([tokens, kv_heads, head_dim], strides in elements, the
+ * last dimension contiguous) into the cache.  d_k_values / d_v_values
+ * (nullable, contiguous, of k's type) receive the values the cache stands
+ * for.  A page that receives tokens belongs to one sequence: if two tokens of
+ * a call fall on one slot, the slot holds an undefined mixture of both. */
+ICX_API int icx_kv_cache_append(void* stream, const icx_kv_cache* cache, const icx_kv_tokens* where,
+                                const void* d_k, const void* d_v, int type, int64_t k_token_stride,
+                                int64_t k_head_stride, int64_t v_token_stride,
+                                int64_t v_head_stride, void* d_k_values, void* d_v_values);
+
+/* Dequantises the tokens that `where` names into contiguous
+ * [tokens, kv_heads, head_dim] buffers; either may be NULL.  Positions that
+ * do not exist (before a sequence's start, without a usable page) are left
+ * as they were. */
+ICX_API int icx_kv_cache_read(void* stream, const icx_kv_cache* cache, const icx_kv_tokens* where,
+                              int type, void* d_k, void* d_v);
+
+/* Causal attention of the tokens that `where` names over the cache (whose
+ * last tokens are these themselves):
+ *   o = sum_p softmax_p(scale * q . k[p]) v[p],  p = 0 .. own position
+ * q: [tokens, q_heads, head_dim] (strides in elements, last dimension
+ * contiguous), q_heads a multiple of kv_heads (consecutive query heads share
+ * a kv head); out: contiguous, of q's type.  A row without any position gives
+ * zeros.  Positions without a usable page take no part.
+ * Scores, softmax statistics and sums are f32. */
+ICX_API size_t icx_kv_cache_attention_workspace_bytes(const icx_kv_cache* cache,
+                                                      const icx_kv_tokens* where, int q_heads);
+
+ICX_API int icx_kv_cache_attention(void* stream, const icx_kv_cache* cache,
+                                   const icx_kv_tokens* where, const void* d_q, int type,
+                                   int q_heads, int64_t q_token_stride, int64_t q_head_stride,
+                                   float scale, void* d_out, void* d_workspace,
+                                   size_t workspace_bytes);
 
 /* ======================================================================== *
  * Graph executor.  Replaces GpuGraphExecutor (src/cuda/inference/mod.rs:

@@ -1,0 +1,486 @@
+"""The quantised K/V cache (append, read) and the attention over it against a
+plain 64-bit implementation.  Stored values are exact; the attention's
+tolerance is derived in decoder_reference.attention_tolerance."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from iconnx_b200 import IcxError, _lib, kv_cache
+from iconnx_b200.kv_cache import (KvCache, gpu_kv_cache_append, gpu_kv_cache_attention,
+                                  gpu_kv_cache_read)
+from tests import decoder_reference as ref
+
+DEV = "cuda:0"
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def f64(t):
+    return t.detach().cpu().double().numpy()
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def ends(counts):
+    return [0, *np.cumsum(counts).tolist()]
+
+
+def status():
+    v = ctypes.c_int(0)
+    assert _lib.load().icx_device_status(0, ctypes.byref(v)) == 0
+    return v.value
+
+
+class Case:
+    """A pool filled with whole sequences of given lengths, pages in random order."""
+
+    def __init__(self, lens, kv_heads=2, dim=64, bits=4, group=64, page=16, dtype=torch.float32, seed=0,
+                 spread=1.0, width_extra=1):
+        g = torch.Generator().manual_seed(seed)
+        self.lens, self.page = lens, page
+        need = [-(-n // page) for n in lens]
+        pool = sum(need) + 2
+        perm = torch.randperm(pool, generator=g).tolist()
+        table = torch.full((len(lens), max(need, default=0) + width_extra), -1, dtype=torch.int32)
+        for b, n in enumerate(need):
+            for i in range(n):
+                table[b, i] = perm.pop()
+        self.table = table.to(DEV)
+        self.cache = KvCache(pool, page, kv_heads, dim, bits, group, DEV)
+        shape = (sum(lens), kv_heads, dim)
+        self.k = (torch.randn(shape, generator=g) * spread + torch.randn(kv_heads, dim, generator=g)).to(dtype)
+        self.v = torch.randn(shape, generator=g).to(dtype)
+        gpu_kv_cache_append(self.cache, self.k.to(DEV), self.v.to(DEV), self.table, i32(lens), i32(ends(lens)))
+        self.kv = [ref.cached_values(f64(x), bits, group) for x in (self.k, self.v)]
+
+    def sequence(self, b):
+        e = ends(self.lens)
+        return [x[e[b]:e[b + 1]] for x in self.kv]
+
+
+# ---------------------------------------------------------------- refusals
+def c_args(**over):
+    cache = dict(k_codes=16, v_codes=16, k_params=16, v_params=16, pages=4, page_size=16, kv_heads=2,
+                 head_dim=64, bits=4, group=32)
+    where = dict(d_page_table=16, d_seq_lens=16, d_cu_tokens=None, tokens=3, batch=3, table_width=4)
+    for k, v in over.items():
+        (cache if k in cache else where)[k] = v
+    return _lib.KvCacheArg(*cache.values()), _lib.KvTokensArg(*where.values())
+
+
+@pytest.mark.parametrize("over,text", [
+    (dict(bits=5), b"bits"), (dict(head_dim=80), b"head_dim"), (dict(group=16), b"group"),
+    (dict(page_size=24), b"page_size"), (dict(page_size=8), b"page_size"), (dict(page_size=2048), b"page_size"),
+    (dict(kv_heads=0), b"kv_heads"), (dict(pages=-1), b"pages"), (dict(batch=-1), b"batch"),
+    (dict(tokens=4), b"one token per sequence"), (dict(d_seq_lens=None), b"null index"),
+    (dict(k_codes=None), b"null cache"), (dict(v_params=24), b"aligned"),
+    (dict(table_width=1 << 28), b"2\\^31")])
+def test_refusals_before_any_launch(over, text):
+    import re
+    L = _lib.load()
+    p = ctypes.c_void_p(64)
+    c, w = c_args(**over)
+    for rc in (L.icx_kv_cache_append(None, ctypes.byref(c), ctypes.byref(w), p, p, 3, 64, 64, 64, 64, None, None),
+               L.icx_kv_cache_read(None, ctypes.byref(c), ctypes.byref(w), 3, p, p),
+               L.icx_kv_cache_attention(None, ctypes.byref(c), ctypes.byref(w), p, 3, 2, 128, 64, 1.0, p, None, 0)):
+        assert rc == -1
+        assert re.search(text, L.icx_last_error()), L.icx_last_error()
+
+
+def test_operand_refusals_before_any_launch():
+    L = _lib.load()
+    p = ctypes.c_void_p(64)
+    c, w = (ctypes.byref(a) for a in c_args())
+    assert L.icx_kv_cache_append(None, None, w, p, p, 3, 1, 1, 1, 1, None, None) == -1
+    assert L.icx_kv_cache_append(None, c, w, p, p, 0, 1, 1, 1, 1, None, None) == -1
+    assert L.icx_kv_cache_append(None, c, w, None, p, 3, 1, 1, 1, 1, None, None) == -1
+    assert L.icx_kv_cache_append(None, c, w, p, p, 3, -1, 1, 1, 1, None, None) == -1
+    assert L.icx_kv_cache_append(None, c, w, p, p, 3, 1, 1, 1, 1, ctypes.c_void_p(8), None) == -1
+    assert L.icx_kv_cache_read(None, c, w, 2, p, p) == -1
+    assert L.icx_kv_cache_read(None, c, w, 3, ctypes.c_void_p(4), p) == -1
+    for kw in (dict(t=1), dict(h=3), dict(h=0), dict(stride=-1), dict(scale=float("nan")), dict(q=None),
+               dict(out=None)):
+        a = dict(t=3, h=4, stride=64, scale=1.0, q=p, out=p) | kw
+        assert L.icx_kv_cache_attention(None, c, w, a["q"], a["t"], a["h"], a["stride"], 64, a["scale"], a["out"],
+                                        p, 1 << 30) == -1, kw
+    with pytest.raises(IcxError, match="CUDA device"):
+        KvCache(4, 16, 2, 64, device="cpu")
+    for kw in (dict(bits=2), dict(head_dim=96), dict(group=128), dict(page_size=20), dict(kv_heads=0), dict(pages=-1)):
+        with pytest.raises(IcxError):
+            KvCache(**(dict(pages=4, page_size=16, kv_heads=2, head_dim=64) | kw))
+
+
+@pytest.mark.gpu
+def test_python_refusals():
+    c = KvCache(4, 16, 2, 64, device=DEV)
+    k = torch.zeros(2, 2, 64, device=DEV)
+    table, lens = i32([[0], [1]]), i32([1, 1])
+    gpu_kv_cache_append(c, k, k, table, lens)
+    for a in ((k[:, :1], k, table, lens), (k, k.half(), table, lens), (k, k[:1], table, lens),
+              (k.cpu(), k, table, lens), (k, k, table.long(), lens), (k, k, table, lens[:1]),
+              (k, k, table[:1], lens[:1]), (k, k, table, lens, i32([0, 2])), (k.int(), k.int(), table, lens)):
+        with pytest.raises(IcxError):
+            gpu_kv_cache_append(c, *a)
+    with pytest.raises(IcxError, match="tokens is needed"):
+        gpu_kv_cache_read(c, table, lens, i32([0, 1, 2]))
+    for kw in (dict(tokens=3), dict(dtype=torch.int8), dict(out=(k, k[:1])), dict(out=(k, k.half()))):
+        with pytest.raises(IcxError):
+            gpu_kv_cache_read(c, table, lens, **kw)
+    q = torch.zeros(2, 4, 64, device=DEV)
+    for a, kw in (((q[:, :3], table, lens), {}), ((q[..., :32], table, lens), {}), ((q[:1], table, lens), {}),
+                  ((q, table, lens), dict(scale=float("inf"))), ((q, table, lens), dict(out=q.half())),
+                  ((q.double(), table, lens), {})):
+        with pytest.raises(IcxError):
+            gpu_kv_cache_attention(c, *a, **kw)
+
+
+# --------------------------------------------------------- append and read
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,bits,group,page", [(64, 4, 32, 16), (64, 8, 64, 32), (128, 4, 64, 16), (128, 8, 32, 64),
+                                                 (256, 4, 32, 16), (256, 8, 64, 1024), (128, 4, 32, 128)])
+def test_append_then_read_is_exact(dim, bits, group, page, dtype):
+    lens = [1, 37, 16, 0, 65]
+    c = Case(lens, 3, dim, bits, group, page, dtype, seed=dim + bits)
+    got = gpu_kv_cache_read(c.cache, c.table, i32(lens), i32(ends(lens)), tokens=sum(lens))
+    for g, want in zip(got, c.kv):
+        # c * s + lo rounds once in f32
+        np.testing.assert_array_equal(f64(g), want.astype(np.float32).astype(np.float64))
+    # the newest tokens alone, in their own type
+    news = [1, 5, 0, 0, 17]
+    got = gpu_kv_cache_read(c.cache, c.table, i32(lens), i32(ends(news)), tokens=sum(news), dtype=dtype)
+    for x, g in zip(c.kv, got):
+        e = ends(lens)
+        want = np.concatenate([x[e[b + 1] - n:e[b + 1]] for b, n in enumerate(news)])
+        assert torch.equal(g.cpu(), torch.from_numpy(want).float().to(dtype))
+    assert status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 8])
+def test_append_values_strides_and_positions(bits):
+    """Packed QKV rows appended step by step equal one append of the whole."""
+    H, D, page = 2, 128, 16
+    lens = [21, 40]
+    whole = Case(lens, H, D, bits, 64, page, torch.bfloat16, seed=4)
+    c = KvCache(whole.cache.pages, page, H, D, bits, 64, DEV)
+    done = [0, 0]
+    while done != lens:
+        news = [min(n - d, s) for n, d, s in zip(lens, done, (1, 7))]
+        e = ends(lens)
+        at = torch.cat([torch.arange(e[b] + done[b], e[b] + done[b] + n) for b, n in enumerate(news)])
+        packed = torch.zeros(len(at), 3 * H * D + 3, dtype=torch.bfloat16, device=DEV)
+        qkv = packed[:, 1:1 + 3 * H * D].view(len(at), 3 * H, D)   # rows off any alignment
+        qkv[:, H:2 * H], qkv[:, 2 * H:] = whole.k[at].to(DEV), whole.v[at].to(DEV)
+        done = [d + n for d, n in zip(done, news)]
+        vals = gpu_kv_cache_append(c, qkv[:, H:2 * H], qkv[:, 2 * H:], whole.table, i32(done), i32(ends(news)),
+                                   return_values=True)
+        for got, x in zip(vals, whole.kv):
+            assert torch.equal(got.cpu(), torch.from_numpy(x[at.numpy()]).float().bfloat16())
+    for a, b in ((c.k_codes, whole.cache.k_codes), (c.v_codes, whole.cache.v_codes),
+                 (c.k_params, whole.cache.k_params), (c.v_params, whole.cache.v_params)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 8])
+def test_append_special_groups(bits):
+    """Constant groups, ties, subnormal and huge ranges, NaN and infinities."""
+    D, H, rows = 128, 1, 16
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(rows, H, D, generator=g)
+    top = torch.finfo(torch.float32).max
+    x[0] = 0
+    x[1] = 0.1
+    x[2] = -3.25
+    x[3, 0, :64], x[3, 0, 64:] = torch.arange(64) * 0.5, torch.arange(64) * -0.25
+    x[4] *= 1e-39
+    x[5] *= 1e38
+    x[6, 0, 3], x[6, 0, 4] = top, -top
+    x[7, 0, 70] = float("nan")
+    x[8, 0, 1] = float("inf")
+    x[9, 0, 127] = float("-inf")
+    x[10] = 1 + torch.arange(D) * 2.0 ** -23
+    x[11] = -top
+    x[12, 0] = torch.arange(D) * 2.0 ** -149
+    x[13, 0, :64] = torch.arange(64) * 7.5 - 3   # exact halves of the step
+    x[14] = 2.0 ** -133
+    cache = KvCache(1, 16, H, D, bits, 64, DEV)
+    vals = gpu_kv_cache_append(cache, x.to(DEV), x.to(DEV), i32([[0]]), i32([rows]), i32([0, rows]), return_values=True)
+    want = ref.cached_values(f64(x), bits, 64).astype(np.float32)
+    read = gpu_kv_cache_read(cache, i32([[0]]), i32([rows]), i32([0, rows]), tokens=rows)
+    for got in (*vals, *read):
+        np.testing.assert_array_equal(got.cpu().numpy(), want)
+
+
+@pytest.mark.gpu
+def test_rows_and_pages_that_are_not_named_stay():
+    c = Case([20, 33], seed=1)
+    before = [t.clone() for t in (c.cache.k_codes, c.cache.v_codes, c.cache.k_params, c.cache.v_params)]
+    k = torch.randn(9, 2, 64, device=DEV)
+    # rows 0, 1 and 7, 8 lie outside cu_tokens; sequence 0 has none; positions before 0 are skipped
+    for lens, cu in (([20, 2], [2, 2, 7]), ([0, 0], [0, 4, 9])):
+        gpu_kv_cache_append(c.cache, k, k, c.table, i32(lens), i32(cu))
+        out = [torch.full((9, 2, 64), 5.0, device=DEV) for _ in range(2)]
+        gpu_kv_cache_read(c.cache, c.table, i32(lens), i32(cu), tokens=9, out=out)
+        stored = range(5, 7) if lens[1] else range(0)
+        for o in out:
+            for r in range(9):
+                assert (o[r] == 5.0).all() != (r in stored)
+    after = (c.cache.k_codes, c.cache.v_codes, c.cache.k_params, c.cache.v_params)
+    page = int(c.table[1, 0])
+    for a, b in zip(before, after):
+        changed = (a != b).flatten(3).any(-1)          # [pages, heads, token]
+        changed[page, :, :2] = False
+        assert not changed.any()
+    assert status() == 0
+
+
+@pytest.mark.gpu
+def test_unusable_pages_are_skipped_and_noted():
+    c = Case([40, 40], seed=3)
+    table = c.table.clone()
+    table[0, 1] = -1
+    table[1, 2] = c.cache.pages
+    lens = i32([40, 40])
+    k = torch.randn(80, 2, 64, device=DEV)
+    before = c.cache.k_codes.clone()
+    out = [torch.full((80, 2, 64), 5.0, device=DEV) for _ in range(2)]
+    gpu_kv_cache_read(c.cache, table, lens, i32([0, 40, 80]), tokens=80, out=out)
+    assert status() == _lib.ICX_DEVICE_BAD_PAGE
+    for o in out:
+        left = (o == 5.0).flatten(1).all(1).cpu()
+        want = torch.zeros(80, dtype=torch.bool)
+        want[16:32] = True
+        want[72:80] = True
+        assert torch.equal(left, want)
+    gpu_kv_cache_append(c.cache, k, k, table, lens, i32([0, 40, 80]))
+    assert status() == _lib.ICX_DEVICE_BAD_PAGE
+    assert torch.equal(before[c.table[0, 1].long()], c.cache.k_codes[c.table[0, 1].long()])
+    # a sequence longer than its row of the table
+    gpu_kv_cache_read(c.cache, c.table[:, :1], lens, i32([0, 40, 80]), tokens=80, out=out)
+    assert status() == _lib.ICX_DEVICE_BAD_PAGE
+    # attention: the positions without a page take no part
+    q = torch.randn(2, 2, 64, device=DEV)
+    got = f64(gpu_kv_cache_attention(c.cache, q, table, lens))
+    assert status() == _lib.ICX_DEVICE_BAD_PAGE
+    kv = gpu_kv_cache_read(c.cache, c.table, lens, i32([0, 40, 80]), tokens=80)
+    for b, gone in ((0, range(16, 32)), (1, range(32, 40))):
+        keep = [40 * b + p for p in range(40) if p not in gone]
+        kb, vb = (f64(x)[keep] for x in kv)
+        want = ref.attention(f64(q[b:b + 1]), kb, vb, 0.125)
+        tol = ref.attention_tolerance(f64(q[b:b + 1]), kb, vb, 0.125, torch.float32, want)
+        assert (np.abs(got[b] - want[0]) <= tol[0]).all()
+
+
+# --------------------------------------------------------------- attention
+def check_attention(c, news, q_heads, dtype, scale=None, seed=0, q_scale=1.0, pad=0):
+    lens, D = c.lens, c.cache.head_dim
+    g = torch.Generator().manual_seed(seed)
+    q = (torch.randn(sum(news) + pad, q_heads, D, generator=g) * q_scale).to(dtype)
+    cu = None if all(n == 1 for n in news) and not pad else i32(ends(news))
+    out = torch.full((sum(news) + pad, q_heads, D), 7.0, dtype=dtype, device=DEV)
+    got = gpu_kv_cache_attention(c.cache, q.to(DEV), c.table, i32(lens), cu, scale, out=out)
+    assert got is out
+    e = ends(news)
+    s = D ** -0.5 if scale is None else scale
+    for b, n in enumerate(news):
+        if n == 0:
+            continue
+        k, v = c.sequence(b)
+        qb = f64(q[e[b]:e[b + 1]])
+        o = f64(out[e[b]:e[b + 1]])
+        want = ref.attention(qb, k, v, s)
+        if lens[b] == 0:
+            assert (o == 0).all()
+            continue
+        tol = ref.attention_tolerance(qb, k, v, s, dtype, want)
+        assert (np.abs(o - want) <= tol).all(), (b, np.abs(o - want).max(), tol.min())
+    assert (out[sum(news):] == 7.0).all()
+    assert status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dim,group,heads,share", [(64, 32, 3, 1), (64, 64, 1, 8), (128, 64, 2, 4), (128, 32, 1, 7),
+                                                   (256, 64, 1, 3), (256, 32, 2, 2)])
+def test_attention_one_token(dim, group, heads, share, bits, dtype):
+    lens = [1, 2, 15, 16, 17, 130, 0, 300]
+    c = Case(lens, heads, dim, bits, group, 16, dtype, seed=dim + share)
+    check_attention(c, [1] * len(lens), heads * share, dtype, seed=share)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,bits,share,news", [(128, 4, 4, [3, 1, 0, 16]), (64, 8, 1, [40, 7, 1, 100]),
+                                                 (128, 4, 2, [200, 64, 33, 129]), (256, 4, 5, [9, 30, 2, 70]),
+                                                 (128, 8, 16, [5, 1, 1, 21]), (64, 4, 3, [200, 180, 5, 129])])
+def test_attention_several_tokens(dim, bits, share, news, dtype):
+    lens = [200, 180, 33, 129]
+    c = Case(lens, 2, dim, bits, 32 if dim == 64 else 64, 32, dtype, seed=dim + share)
+    check_attention(c, news, 2 * share, dtype, seed=share, pad=3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [16, 64, 1024])
+def test_attention_long_and_ragged(page):
+    """Long sequences beside short ones: work split over the positions and joined."""
+    lens = [5000, 3, 1029, 0, 2048]
+    c = Case(lens, 1, 128, 4, 64, page, torch.float32, seed=page)
+    check_attention(c, [1] * 5, 4, torch.float32, seed=1)
+    check_attention(c, [3, 1, 2, 0, 1], 4, torch.float32, seed=2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_attention_many_rows(dim):
+    """Long runs of new tokens, with and without a cached prefix."""
+    lens = [700, 257, 300]
+    c = Case(lens, 2, dim, 4, 64, 64, torch.bfloat16, seed=dim)
+    check_attention(c, [300, 257, 1], 8, torch.bfloat16, seed=3, pad=5)
+    c = Case(lens, 1, dim, 8, 32, 16, torch.float32, seed=dim + 1)
+    check_attention(c, [130, 200, 300], 3, torch.float32, seed=4)
+
+
+@pytest.mark.gpu
+def test_attention_scales_and_strong_scores():
+    """Scores of order 100 (one position takes all), scale 0, negative scale, tiny and huge q."""
+    for spread, q_scale, scale in ((4.0, 4.0, 0.5), (1.0, 1.0, 0.0), (1.0, 1.0, -0.3), (1.0, 1e-6, None),
+                                   (1e-3, 3e4, 1e-3), (1.0, 300.0, 1.0)):
+        c = Case([77, 400], 2, 128, 8, 64, 16, torch.float32, seed=11, spread=spread)
+        check_attention(c, [1, 1], 4, torch.float32, scale, seed=5, q_scale=q_scale)
+
+
+@pytest.mark.gpu
+def test_attention_values_of_unequal_size():
+    """Values whose groups differ by many orders of magnitude, token by token."""
+    c = Case([90], 1, 128, 4, 64, 16, torch.float32, seed=12)
+    k = c.k.to(DEV)
+    v = (c.v * torch.pow(10.0, torch.arange(90) % 13 - 6.0)[:, None, None]).to(DEV)
+    gpu_kv_cache_append(c.cache, k, v, c.table, i32([90]), i32([0, 90]))
+    c.kv[1] = ref.cached_values(f64(v), 4, 64)
+    check_attention(c, [1], 4, torch.float32, seed=6)
+    check_attention(c, [80], 2, torch.float32, seed=7)
+
+
+@pytest.mark.gpu
+def test_attention_ignores_what_lies_behind():
+    """NaN in unused rows of pages, and in other sequences, reaches nobody."""
+    c = Case([21, 30, 260], 2, 128, 4, 64, 16, torch.bfloat16, seed=13)
+    nan = torch.full((64, 2, 128), float("nan"), device=DEV, dtype=torch.bfloat16)
+    lens = i32(c.lens)
+    for b, n in enumerate(c.lens):   # fill the tail of each last page
+        tail = -n % 16
+        table = c.table[b:b + 1]
+        if tail:
+            gpu_kv_cache_append(c.cache, nan[:tail], nan[:tail], table, i32([n + tail]), i32([0, tail]))
+    check_attention(c, [1, 1, 1], 8, torch.bfloat16, seed=1)
+    check_attention(c, [5, 30, 250], 8, torch.bfloat16, seed=2)
+    # a NaN inside a sequence does reach that sequence's later rows, and them alone
+    gpu_kv_cache_append(c.cache, nan[:1], nan[:1], c.table[1:2], i32([30]), i32([0, 1]))
+    out = gpu_kv_cache_attention(c.cache, torch.randn(32, 8, 128, device=DEV, dtype=torch.bfloat16), c.table, lens,
+                                 i32([0, 1, 31, 32]))
+    bad = out.isnan().flatten(1)
+    assert bad[30].all() and not bad[:30].any() and not bad[31].any()
+
+
+@pytest.mark.gpu
+def test_attention_strided_queries_and_more_new_tokens_than_positions():
+    c = Case([10, 50], 2, 64, 8, 32, 16, torch.float16, seed=14)
+    packed = torch.randn(60, 12, 64, device=DEV).half()
+    q = packed[:, 4:8]
+    got = gpu_kv_cache_attention(c.cache, q, c.table, i32([10, 50]), i32([0, 30, 60]))
+    want = gpu_kv_cache_attention(c.cache, q.contiguous(), c.table, i32([10, 50]), i32([0, 30, 60]))
+    assert torch.equal(got, want)
+    assert (got[:20] == 0).all() and (got[20:] != 0).flatten(1).any(1).all()
+    part = gpu_kv_cache_attention(c.cache, q[20:30], c.table[:1], i32([10]), i32([0, 10]))
+    np.testing.assert_allclose(f64(part), f64(got[20:30]), atol=2e-3)
+    every_other = gpu_kv_cache_attention(c.cache, packed[::2, ::3], c.table[1:], i32([50]), i32([0, 30]))
+    want = gpu_kv_cache_attention(c.cache, packed[::2, ::3].contiguous(), c.table[1:], i32([50]), i32([0, 30]))
+    assert torch.equal(every_other, want)
+
+
+@pytest.mark.gpu
+def test_empty_calls():
+    c = KvCache(0, 16, 2, 64, device=DEV)
+    none = torch.zeros(0, 2, 64, device=DEV)
+    table, lens = torch.zeros(0, 4, dtype=torch.int32, device=DEV), i32([])
+    assert gpu_kv_cache_append(c, none, none, table, lens) is None
+    assert gpu_kv_cache_read(c, table, lens)[0].shape == (0, 2, 64)
+    assert gpu_kv_cache_attention(c, none, table, lens).shape == (0, 2, 64)
+    # a batch without positions in an empty pool
+    table, lens = torch.zeros(3, 0, dtype=torch.int32, device=DEV), i32([0, 0, 0])
+    out = gpu_kv_cache_attention(c, torch.ones(3, 2, 64, device=DEV), table, lens)
+    assert (out == 0).all()
+    assert status() == 0
+
+
+@pytest.mark.gpu
+def test_same_call_twice_is_equal_and_streams_agree():
+    c = Case([3000, 70, 900], 2, 128, 4, 64, 32, torch.float32, seed=15)
+    q = torch.randn(3, 8, 128, device=DEV)
+    lens = i32(c.lens)
+    want = gpu_kv_cache_attention(c.cache, q, c.table, lens)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(DEV) for _ in range(3)]
+    outs = []
+    for i in range(9):
+        with torch.cuda.stream(streams[i % 3]):
+            outs.append(gpu_kv_cache_attention(c.cache, q, c.table, lens))
+    torch.cuda.synchronize()
+    for o in outs:
+        assert torch.equal(o, want)
+
+
+@pytest.mark.gpu
+def test_decode_steps_captured_in_graphs():
+    """Two captured decode steps (append and attention) of different batches, replayed
+    in turn and with other lengths, against eager calls."""
+    H, D, page = 2, 64, 16
+    cache = KvCache(40, page, H, D, 4, 32, DEV)
+    eager = KvCache(40, page, H, D, 4, 32, DEV)
+    tables = [i32(np.arange(20).reshape(2, 10)), i32(np.arange(20, 40).reshape(4, 5))]
+    g = torch.Generator(DEV).manual_seed(3)
+    graphs = []
+    for table in tables:
+        b = table.shape[0]
+        lens = torch.ones(b, dtype=torch.int32, device=DEV)
+        x = [torch.randn(b, H, D, generator=g, device=DEV) for _ in range(3)]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            gpu_kv_cache_append(cache, x[0], x[1], table, lens)
+            out = gpu_kv_cache_attention(cache, x[2], table, lens)
+        graphs.append((graph, lens, x, out, table))
+    for step in range(60):
+        for graph, lens, x, out, table in graphs:
+            lens.fill_(step + 1)
+            for t in x:
+                t.normal_(generator=g)
+            graph.replay()
+            gpu_kv_cache_append(eager, x[0], x[1], table, lens)
+            want = gpu_kv_cache_attention(eager, x[2], table, lens)
+            torch.cuda.synchronize()
+            assert torch.equal(out, want), step
+    assert torch.equal(cache.k_codes, eager.k_codes) and torch.equal(cache.v_params, eager.v_params)
+
+
+@pytest.mark.gpu
+def test_far_pages():
+    """A pool whose later pages start beyond 2^31 bytes, and rows beyond 2^31 codes."""
+    D, H, page = 256, 4, 256
+    pages = (1 << 31) // (page * H * D) + 40
+    cache = KvCache(pages, page, H, D, 8, 64, DEV)
+    k = torch.randn(300, H, D, device=DEV)
+    v = torch.randn(300, H, D, device=DEV)
+    near, far = i32([[0, 1]]), i32([[pages - 1, pages - 2]])
+    lens, cu = i32([300]), i32([0, 300])
+    for table in (near, far):
+        gpu_kv_cache_append(cache, k, v, table, lens, cu)
+    a, b = (gpu_kv_cache_read(cache, t, lens, cu, tokens=300) for t in (near, far))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    q = torch.randn(1, 2 * H, D, device=DEV)
+    assert torch.equal(gpu_kv_cache_attention(cache, q, near, lens), gpu_kv_cache_attention(cache, q, far, lens))
