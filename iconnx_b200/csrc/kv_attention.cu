@@ -1,87 +1,38 @@
-// Causal attention over the quantised K/V cache.
+// Causal attention over the quantised K/V cache: checks, plan and dispatch.
 #include <cmath>
 
-#include "capi.cuh"
-#include "common.cuh"
-#include "kv_cache.cuh"
+#include "kv_attention.cuh"
 
 namespace icx {
 
-template <typename T>
-struct QueryArgs {
-  const T* q;
-  int64_t token_stride, head_stride;
-  int q_heads;
-  float scale;   // of the scores, times log2(e)
-  T* out;
-};
-
-__device__ __forceinline__ uint32_t k_code(const uint8_t* row, int dim, int bits, int d) {
-  const int j = d >> 4, t = (d >> 2) & 3, i = d & 3;
-  const uint8_t* chunk = row + t * (dim * bits / 32);
-  if (bits == 8) return chunk[4 * j + (((i & 1) << 1) | (i >> 1))];
-  const int nib = (((i & 1) << 2) | (i & 2)) + (j & 1);
-  return (chunk[4 * (j >> 1) + (nib >> 1)] >> (4 * (nib & 1))) & 15u;
-}
-
-__device__ __forceinline__ uint32_t v_code(const uint8_t* row, int dim, int bits, int d) {
-  const int m = d >> 4, g = (d >> 1) & 7, k = 2 * m + (d & 1);
-  const uint8_t* chunk = row + g * (dim * bits / 64);
-  return bits == 8 ? chunk[k] : (chunk[k >> 1] >> (4 * (k & 1))) & 15u;
-}
-
-// One warp per (token, query head), one position at a time.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) kv_attend_kernel(const KvView c, const KvTokens w, const QueryArgs<T> a) {
-  pdl_wait();
-  pdl_trigger();
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (item >= w.tokens * a.q_heads) return;
-  const int64_t token = item / a.q_heads;
-  const int hq = (int)(item % a.q_heads), head = hq / (a.q_heads / c.heads);
-  const int b = kv_sequence(w, token);
-  if (b < 0) return;
-  const int64_t end = w.cu ? (int64_t)w.cu[b + 1] : token + 1;
-  const int64_t last = (int64_t)w.lens[b] - end + token;
-  float q[E], o[E] = {};
-#pragma unroll
-  for (int e = 0; e < E; ++e)
-    q[e] = to_f32(a.q[token * a.token_stride + hq * a.head_stride + lane + 32 * e]) * a.scale;
-  float m = -INFINITY, l = 0.0f;
-  for (int p = 0; p <= last; ++p) {
-    const int64_t page = kv_page(c, w, b, p);
-    if (page < 0) {
-      record_status(ICX_DEVICE_BAD_PAGE);
-      continue;
-    }
-    const int64_t row = kv_row(c, page, head, p);
-    const uint8_t* kr = c.codes[0] + row * (D * c.bits / 8);
-    const uint8_t* vr = c.codes[1] + row * (D * c.bits / 8);
-    float s = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int d = lane + 32 * e;
-      const uint32_t pr = c.params[0][row * (D / c.group) + d / c.group];
-      s = fmaf(q[e], fmaf((float)k_code(kr, D, c.bits, d), param_scale(pr), param_low(pr)), s);
-    }
-#pragma unroll
-    for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    const float mn = fmaxf(m, s);
-    const float f = m == -INFINITY ? 0.0f : exp2f(m - mn), pw = exp2f(s - mn);
-    m = mn;
-    l = fmaf(l, f, pw);
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int d = lane + 32 * e;
-      const uint32_t pr = c.params[1][row * (D / c.group) + d / c.group];
-      o[e] = fmaf(o[e], f, pw * fmaf((float)v_code(vr, D, c.bits, d), param_scale(pr), param_low(pr)));
-    }
+static int sm_count() {
+  int dev = 0, n = 148;
+  cudaGetDevice(&dev);
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+    cudaGetLastError();
+    n = 148;
   }
-#pragma unroll
-  for (int e = 0; e < E; ++e)
-    a.out[(token * a.q_heads + hq) * D + lane + 32 * e] = from_f32<T>(l != 0.0f ? o[e] / l : 0.0f);
+  return n;
+}
+
+AttendPlan plan_attend(const KvView& c, const KvTokens& w, int q_heads) {
+  AttendPlan p{};
+  const int share = q_heads / c.heads;
+  // rows that share one read of the cache: as many as the average sequence
+  // has, up to what the registers hold
+  const int64_t rows = (w.tokens + w.batch - 1) / w.batch * share;
+  p.nt = rows <= 8 ? 1 : rows <= 16 || c.dim == 256 ? 2 : 4;
+  const int R = 8 * p.nt;
+  const int64_t blocks = (((int64_t)w.width << c.page_shift) + kAttBlock - 1) / kAttBlock;
+  const int64_t units = (w.tokens * share / R + w.batch) * c.heads * (blocks > 1 ? blocks : 1);
+  const int64_t resident = (int64_t)sm_count() * (c.dim * p.nt <= 128 ? 2 : 1);
+  p.ctas = (int)(units < resident ? units : resident);
+  p.split = blocks > 1;
+  if (p.split) {
+    p.prefix_bytes = ((size_t)(w.batch + 1) * 8 + 255) & ~size_t(255);
+    p.bytes = p.prefix_bytes + (size_t)p.ctas * 2 * R * (c.dim + 2) * 4;
+  }
+  return p;
 }
 
 }  // namespace icx
@@ -90,7 +41,12 @@ using namespace icx;
 
 extern "C" size_t icx_kv_cache_attention_workspace_bytes(const icx_kv_cache* cache, const icx_kv_tokens* where,
                                                          int q_heads) {
-  return 0;
+  KvView c;
+  KvTokens w;
+  if (kv_views("KvCacheAttention", cache, where, &c, &w) || w.tokens == 0 || w.batch == 0 || q_heads < 1 ||
+      q_heads % c.heads)
+    return 0;
+  return plan_attend(c, w, q_heads).bytes;
 }
 
 extern "C" int icx_kv_cache_attention(void* stream, const icx_kv_cache* cache, const icx_kv_tokens* where,
@@ -105,16 +61,32 @@ extern "C" int icx_kv_cache_attention(void* stream, const icx_kv_cache* cache, c
   ICX_REQUIRE(q_heads >= 1 && q_heads % c.heads == 0, "KvCacheAttention: q_heads %d is no multiple of kv_heads %d",
               q_heads, c.heads);
   ICX_REQUIRE(q_token_stride >= 0 && q_head_stride >= 0, "KvCacheAttention: negative stride");
+  scale *= 1.4426950408889634f;
   ICX_REQUIRE(std::isfinite(scale), "KvCacheAttention: scale must be finite");
+  ICX_REQUIRE(w.tokens * q_heads < (1ll << 31), "KvCacheAttention: tokens x q_heads beyond 2^31");
   if (w.tokens == 0 || w.batch == 0) return ICX_OK;
   ICX_REQUIRE(d_q && d_out, "KvCacheAttention: null operand");
+  ICX_REQUIRE((reinterpret_cast<uintptr_t>(d_out) & 15) == 0, "KvCacheAttention: out must be 16-byte aligned");
+  const AttendPlan p = plan_attend(c, w, q_heads);
+  if (p.bytes > 0 && (!d_workspace || workspace_bytes < p.bytes)) {
+    set_error("KvCacheAttention: workspace %zu bytes < %zu required", d_workspace ? workspace_bytes : 0, p.bytes);
+    return ICX_ERR_WORKSPACE;
+  }
+  ICX_REQUIRE((reinterpret_cast<uintptr_t>(d_workspace) & 15) == 0, "KvCacheAttention: workspace must be 16-byte aligned");
+  const size_t e = float_bytes(type);
+  AttendArgs a{};
+  a.q = d_q;
+  a.q_token_stride = q_token_stride;
+  a.q_head_stride = q_head_stride;
+  a.q_heads = q_heads;
+  a.q_vec = (reinterpret_cast<uintptr_t>(d_q) | (size_t)q_token_stride * e | (size_t)q_head_stride * e) % (4 * e) == 0;
+  a.scale = scale;
+  a.out = d_out;
+  a.split = p.split;
+  a.prefix = static_cast<int64_t*>(d_workspace);
+  a.partial = reinterpret_cast<float*>(static_cast<char*>(d_workspace) + p.prefix_bytes);
   cudaStream_t s = as_stream(stream);
-  const dim3 grid((unsigned)((w.tokens * q_heads + 7) / 8));
-  ICX_FLOAT_DISPATCH(type, {
-    QueryArgs<T> a{static_cast<const T*>(d_q), q_token_stride, q_head_stride, q_heads, scale * 1.4426950408889634f,
-                   static_cast<T*>(d_out)};
-    auto kern = c.dim == 64 ? kv_attend_kernel<T, 64> : c.dim == 128 ? kv_attend_kernel<T, 128> : kv_attend_kernel<T, 256>;
-    ICX_CUDA(launch_pdl(kern, grid, dim3(256), 0, s, c, w, a));
-  });
-  return ICX_OK;
+  int r = ICX_OK;
+  ICX_FLOAT_DISPATCH(type, r = launch_attend<T>(s, c, w, a, p));
+  return r;
 }

@@ -1,0 +1,806 @@
+// Attention of few query rows over the quantised K/V cache (decoding).
+//
+// Bound: the cache is read once, 4 D / 32 .. bytes per position with some tens
+// of operations per byte, so HBM sets the floor and the instruction issue rate
+// comes next.  Codes are therefore never dequantised: with K[p] = c s + lo per
+// group of dimensions,
+//     q . K[p] = sum_groups  s (q . c) + lo sum(q)
+//     sum_p w_p V[p] = sum_p (w_p s_p) c_p + sum_p w_p lo_p
+// and the two contractions run on m16n8k16 matrix instructions whose left
+// operand is the codes themselves.  A code c in the low bits of a half word
+// *is* the f16 number c * 2^-24 (a subnormal, which the matrix units take at
+// full precision), so one mask per two codes makes an operand; a code left in
+// bits 4..7 is 16 times that, which the other operand (q) or the final scaling
+// (output rows) undoes.  The positions (scores) and the dimensions (output)
+// are the 16-row side, the query rows that share a K/V head the 8-column side.
+//
+// Right operands: q is scaled per row by a power of two into f16's range and
+// split into f16 + f16 where it has more than 11 bits (f32 input); w s is scaled
+// per group by a power of two that follows the largest s met so far, and split
+// into f16 + f16 unless the output is bf16, whose 8 bits one f16 (11 bits)
+// does not disturb.  Everything summed is f32.
+//
+// Softmax: one pass.  Weights are taken relative to a reference m that only
+// moves (rescaling the sums) when a score passes m + 8, so that most tiles
+// need one vote and no exchange between lanes: 2^8 more range costs f16
+// nothing.  Each lane adds its own positions' weights; lanes are joined once
+// per run of positions.
+//
+// Work: a unit is 128 positions of one (sequence, K/V head, tile of query
+// rows); each CTA takes an equal, contiguous share of all units, found on the
+// device from seq_lens and cu_tokens, so ragged batches balance and a captured
+// call can be replayed with other lengths.  Eight warps of a CTA take 16
+// positions each and are joined through shared memory; rows whose units went
+// to several CTAs leave (m, l, o) in the workspace for the join kernel.  All
+// joins run in a fixed order, so equal calls give equal results.
+#pragma once
+
+#include <type_traits>
+
+#include "capi.cuh"
+#include "common.cuh"
+#include "kv_cache.cuh"
+
+namespace icx {
+
+constexpr int kAttWarps = 8;
+constexpr int kAttBlock = 16 * kAttWarps;   // positions per unit
+constexpr float kNoScore = -1.7e38f;        // m before the first score
+
+struct AttendArgs {
+  const void* q;
+  int64_t q_token_stride, q_head_stride;
+  int q_heads;
+  int q_vec;        // four elements of q can be read in one access
+  float scale;      // of the scores, times log2(e)
+  void* out;
+  int64_t* prefix;  // workspace: units before each sequence [batch + 1]
+  float* partial;   // workspace: two slots per CTA of R x (D + 2) floats
+  int split;        // rows may go to several CTAs
+};
+
+// Units of a sequence: its row tiles x K/V heads x blocks of positions.
+struct SeqUnits {
+  int from, n, len, rows, tiles, blocks;
+  int64_t units;
+};
+
+__device__ __forceinline__ SeqUnits seq_units(const KvView& c, const KvTokens& w, int share, int R, int b) {
+  SeqUnits u;
+  u.from = b;
+  u.n = 1;
+  if (w.cu) {
+    // rows outside the packed operands do not exist, whatever cu holds
+    const int64_t from = max((int64_t)w.cu[b], (int64_t)0);
+    const int64_t to = min((int64_t)w.cu[b + 1], w.tokens);
+    u.from = (int)from;
+    u.n = to > from ? (int)(to - from) : 0;
+  }
+  u.len = max(w.lens[b], 0);
+  u.rows = u.n * share;
+  u.tiles = (u.rows + R - 1) / R;
+  const int reach = (int)min((int64_t)u.len, (int64_t)w.width << c.page_shift);
+  u.blocks = max(1, (reach + kAttBlock - 1) / kAttBlock);
+  u.units = (int64_t)u.tiles * c.heads * u.blocks;
+  return u;
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t u) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&u));
+}
+
+// W consecutive words, W a power of two, naturally aligned up to 16 bytes.
+template <int W>
+__device__ __forceinline__ void load_words(const uint32_t* p, uint32_t (&r)[W]) {
+  if constexpr (W >= 4) {
+#pragma unroll
+    for (int i = 0; i < W / 4; ++i) {
+      const uint4 u = reinterpret_cast<const uint4*>(p)[i];
+      r[4 * i] = u.x;
+      r[4 * i + 1] = u.y;
+      r[4 * i + 2] = u.z;
+      r[4 * i + 3] = u.w;
+    }
+  } else if constexpr (W == 2) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    r[0] = u.x;
+    r[1] = u.y;
+  } else {
+    r[0] = *p;
+  }
+}
+
+// Contiguous global -> shared copy (16-byte aligned, a multiple of 16 bytes),
+// counted on `bar`.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_addr(dst)),
+               "l"(src), "r"(bytes), "r"(smem_addr(bar))
+               : "memory");
+}
+
+// Position (of 16) that stands in row g of the scores' left operand, and
+// g + 8 for the upper eight: an order in which neither the K rows of lanes
+// that read together nor the V rows do share banks.
+__device__ __forceinline__ int row_position(int g) { return g ^ (((g >> 1) ^ (g >> 2)) & 1); }
+
+template <typename T, int D, int BITS, int GROUP, int NT>
+struct AttConfig {
+  static constexpr bool QLO = sizeof(T) == 4;
+  static constexpr bool PLO = !std::is_same<T, __nv_bfloat16>::value;
+  static constexpr int R = 8 * NT;
+  static constexpr int G = D / GROUP;
+  // two CTAs per SM where 128 registers hold the sums
+  static constexpr int kMinBlocks = D * NT <= 128 ? 2 : 1;
+  // q stays in registers where it takes at most 16
+  static constexpr bool kQReg = NT == 1 && (D / 16) * 2 * (QLO ? 2 : 1) <= 16;
+  static constexpr int kRowFloats = D + 2;
+  // a warp's ring: 16 positions of K and V codes and parameters per stage
+  static constexpr int ROW = D * BITS / 8;
+  static constexpr int kCodes = 16 * ROW, kParams = 16 * G * 4;
+  static constexpr int kStage = 2 * (kCodes + kParams);
+  static constexpr int kFit = (kMinBlocks == 2 ? 80 : 160) * 1024 / (kAttWarps * kStage);
+  static constexpr int kStages = kFit > 4 ? 4 : kFit < 2 ? 2 : kFit;
+  static constexpr int kRing = kAttWarps * kStages * kStage;
+  // joining the warps: half of them put down R rows at a time, over the ring
+  static constexpr int kJoin = (kAttWarps / 2) * R * kRowFloats * 4;
+  static constexpr int kQOffset = kRing > kJoin ? kRing : kJoin;
+  static constexpr int kQBytes = kQReg ? 0 : NT * (D / 16) * (QLO ? 2 : 1) * 32 * 8;
+  static constexpr int kSmem = kQOffset + kQBytes;
+};
+
+template <typename T, int D, int BITS, int GROUP, int NT>
+__global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, NT>::kMinBlocks))
+    kv_attend_rows_kernel(const __grid_constant__ KvView c, const __grid_constant__ KvTokens w,
+                          const __grid_constant__ AttendArgs a) {
+  using C = AttConfig<T, D, BITS, GROUP, NT>;
+  constexpr int G = C::G, R = C::R, KS = D / 16, SG = GROUP / 16, MT = D / 16;
+  constexpr int KW = D * BITS / 128, VW = D * BITS / 256;   // words of a K and a V chunk
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ __align__(8) uint64_t full[kAttWarps][C::kStages];
+  __shared__ int64_t s_prefix, s_total;
+  __shared__ int s_seq;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int share = a.q_heads / c.heads;
+  if (lane < C::kStages) mbar_init(&full[warp][lane], 1);
+  fence_barrier_init();
+  pdl_wait();
+  pdl_trigger();
+
+  // this CTA's units [u0, u1) of all
+  if (warp == 0) {
+    int64_t total = 0;
+    for (int b = lane; b < w.batch; b += 32) total += seq_units(c, w, share, R, b).units;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const int64_t first = total * blockIdx.x / gridDim.x;
+    const bool write = a.split && blockIdx.x == 0;
+    int64_t before = 0;
+    int seq = w.batch;
+    int64_t at = 0;
+    for (int b0 = 0; b0 < w.batch; b0 += 32) {
+      const int b = b0 + lane;
+      const int64_t n = b < w.batch ? seq_units(c, w, share, R, b).units : 0;
+      int64_t inc = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += x;
+      }
+      if (write && b < w.batch) a.prefix[b + 1] = before + inc;
+      const uint32_t hit = __ballot_sync(0xffffffffu, before + inc > first);
+      if (hit && seq == w.batch) {
+        const int l = __ffs(hit) - 1;
+        seq = b0 + l;
+        at = before + __shfl_sync(0xffffffffu, inc - n, l);
+        if (!write) break;
+      }
+      before += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    if (lane == 0) {
+      if (write) a.prefix[0] = 0;
+      s_total = total;
+      s_seq = seq;
+      s_prefix = at;
+    }
+  }
+  __syncthreads();
+  const int64_t u0 = s_total * blockIdx.x / gridDim.x, u1 = s_total * (blockIdx.x + 1) / gridDim.x;
+  int seq = s_seq;
+  int64_t base = s_prefix;
+  if (u0 >= u1) return;
+  SeqUnits su = seq_units(c, w, share, R, seq);
+  uint32_t phase = 0;   // parity of each stage's barrier
+  bool ok = true;       // false once a bounded wait gave up
+
+  for (int64_t u = u0; u < u1;) {
+    while (u >= base + su.units) {
+      base += su.units;
+      su = seq_units(c, w, share, R, ++seq);
+    }
+    const int64_t in = u - base;
+    const int block0 = (int)(in % su.blocks);
+    const int block1 = (int)min((int64_t)su.blocks, block0 + (u1 - u));
+    const int rest = (int)(in / su.blocks);
+    const int head = rest / su.tiles, r0 = (rest % su.tiles) * R;
+    u += block1 - block0;
+    const int row_base = su.from;   // packed row of the sequence's first new token
+    const int64_t first_pos = (int64_t)su.len - su.n;
+    const int nrows = min(R, su.rows - r0);
+    // positions that some row of the tile sees, and that every row sees
+    const int reach = (int)min((int64_t)su.len, (int64_t)w.width << c.page_shift);
+    const int see_any = (int)max((int64_t)0, min(first_pos + (r0 + nrows - 1) / share + 1, (int64_t)reach));
+    const int see_all = (int)max((int64_t)0, min(first_pos + r0 / share + 1, (int64_t)reach));
+    if (threadIdx.x == 0 && su.len > reach) record_status(ICX_DEVICE_BAD_PAGE);
+
+    // ------------------------------------------------------ query operand
+    // column g of tile x is row r0 + 8 x + g; step j's contraction index of
+    // this thread is dimensions 16 j + 4 t + {0,1} and {2,3}
+    constexpr int QP = C::QLO ? 2 : 1;   // f16 parts of q
+    uint32_t qr[C::kQReg ? KS : 1][QP][2];
+    uint2* q_smem = reinterpret_cast<uint2*>(smem + C::kQOffset) + lane;   // [NT][KS][QP][32]
+    float qsum[NT][G][2], qf[NT][2];   // per column 2t and 2t+1: sums by group, score factor
+    int see[NT][2];                    // positions that row sees
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+      const int r = r0 + 8 * x + g;
+      const bool ok = r < su.rows;
+      const T* q = static_cast<const T*>(a.q) + (int64_t)(row_base + (ok ? r / share : 0)) * a.q_token_stride +
+                   (int64_t)(head * share + (ok ? r % share : 0)) * a.q_head_stride;
+      float peak = 0.0f, v[4];
+#pragma unroll
+      for (int j = 0; j < KS; ++j) {
+        load_f32<T, 4>(q + 16 * j + 4 * t, v, a.q_vec);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) peak = fmaxf(peak, ok ? fabsf(v[i]) : 0.0f);
+      }
+      peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
+      peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
+      // 2^e with peak * 2^e in [2^14, 2^15)
+      const int e = peak > 0.0f ? max(-60, min(120, 14 - (int)((__float_as_uint(peak) >> 23) & 255) + 127)) : 0;
+      const float up = __uint_as_float((uint32_t)(e + 127) << 23);
+      float sums[G] = {};
+#pragma unroll
+      for (int j = 0; j < KS; ++j) {
+        load_f32<T, 4>(q + 16 * j + 4 * t, v, a.q_vec);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[i] = ok ? v[i] : 0.0f;
+          sums[j / SG] += v[i];
+          v[i] *= up * ((BITS == 4 && (j & 1)) ? 0.0625f : 1.0f);
+        }
+        uint32_t part[2][2];
+        part[0][0] = pack_f16(v[0], v[1]);
+        part[0][1] = pack_f16(v[2], v[3]);
+        const float2 h0 = unpack_f16(part[0][0]), h1 = unpack_f16(part[0][1]);
+        part[1][0] = pack_f16(v[0] - h0.x, v[1] - h0.y);
+        part[1][1] = pack_f16(v[2] - h1.x, v[3] - h1.y);
+#pragma unroll
+        for (int i = 0; i < QP; ++i) {
+          if constexpr (C::kQReg) {
+            qr[j][i][0] = part[i][0];
+            qr[j][i][1] = part[i][1];
+          } else if (warp == 0) {
+            q_smem[((x * KS + j) * QP + i) * 32] = make_uint2(part[i][0], part[i][1]);
+          }
+        }
+      }
+      const float f = a.scale * 16777216.0f * __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int from = (2 * t + h) * 4;   // a lane that holds column 2t + h
+        qf[x][h] = __shfl_sync(0xffffffffu, f, from);
+        const int rr = r0 + 8 * x + 2 * t + h;
+        see[x][h] = rr < su.rows ? (int)max((int64_t)0, min(first_pos + rr / share + 1, (int64_t)reach)) : 0;
+      }
+#pragma unroll
+      for (int k = 0; k < G; ++k) {
+        float s = sums[k];
+        s += __shfl_xor_sync(0xffffffffu, s, 1);
+        s += __shfl_xor_sync(0xffffffffu, s, 2);
+        s *= a.scale;
+        qsum[x][k][0] = __shfl_sync(0xffffffffu, s, 8 * t);
+        qsum[x][k][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
+      }
+    }
+
+    if (!C::kQReg) __syncthreads();
+    // -------------------------------------------------------- running sums
+    float o[NT][MT][4] = {};
+    float m[NT][2], l[NT][2], vlo[NT][G][2];
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        m[x][h] = kNoScore;
+        l[x][h] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < G; ++k) vlo[x][k][h] = 0.0f;
+      }
+    // w s is held times 2^-ve, with the largest s at most 2^7 (w at most 2^8)
+    float vmax[G], vdown[G];
+#pragma unroll
+    for (int k = 0; k < G; ++k) {
+      vmax[k] = 0.0f;
+      vdown[k] = 0.0f;
+    }
+
+    uint8_t* ring = smem + warp * C::kStages * C::kStage;
+    auto load = [&](int stage, int64_t page, int pos) {   // pos: first of 16
+      if (lane == 0) {
+        const int64_t row = kv_row(c, page, head, pos);
+        uint8_t* dst = ring + stage * C::kStage;
+        uint64_t* bar = &full[warp][stage];
+        mbar_arrive_expect_tx(bar, C::kStage);
+        bulk_load(dst, c.codes[0] + row * C::ROW, C::kCodes, bar);
+        bulk_load(dst + C::kCodes, c.params[0] + row * G, C::kParams, bar);
+        bulk_load(dst + C::kCodes + C::kParams, c.codes[1] + row * C::ROW, C::kCodes, bar);
+        bulk_load(dst + 2 * C::kCodes + C::kParams, c.params[1] + row * G, C::kParams, bar);
+      }
+    };
+
+    auto process = [&](int stage, int pos) {
+      const bool edge = pos + 16 > see_all;
+      const uint8_t* kc = ring + stage * C::kStage;
+      const uint32_t* kprm = reinterpret_cast<const uint32_t*>(kc + C::kCodes);
+      const uint8_t* vc = kc + C::kCodes + C::kParams;
+      const uint32_t* vprm = reinterpret_cast<const uint32_t*>(vc + C::kCodes);
+      uint32_t kw[2][KW];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int at = row_position(g) + 8 * h;
+#pragma unroll
+        for (int i = 0; i < KW; i += 4) {
+          if constexpr (KW >= 4) {
+            const uint4 u = *reinterpret_cast<const uint4*>(kc + at * C::ROW + k_word_at<C::ROW>(at, t, i));
+            kw[h][i] = u.x;
+            kw[h][i + 1] = u.y;
+            kw[h][i + 2] = u.z;
+            kw[h][i + 3] = u.w;
+          } else {
+            load_words(reinterpret_cast<const uint32_t*>(kc + at * C::ROW + k_word_at<C::ROW>(at, t, i)), kw[h]);
+          }
+        }
+      }
+      uint32_t kp[2][G];
+      load_words(kprm + row_position(g) * G, kp[0]);
+      load_words(kprm + (row_position(g) + 8) * G, kp[1]);
+      // -- scores: positions pos + g, pos + g + 8 (rows) x columns 2t, 2t+1
+      float s[NT][4] = {};
+#pragma unroll
+      for (int k = 0; k < G; ++k) {
+        float acc[NT][4] = {};
+#pragma unroll
+        for (int js = 0; js < SG; ++js) {
+          const int j = k * SG + js;
+          uint32_t A[4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (BITS == 4) {
+              const uint32_t mask = (j & 1) ? 0x00f000f0u : 0x000f000fu;
+              const uint32_t word = kw[h][j >> 1];
+              A[h] = word & mask;
+              A[2 + h] = (word >> 8) & mask;
+            } else {
+              const uint32_t word = kw[h][j];
+              A[h] = word & 0x00ff00ffu;
+              A[2 + h] = (word >> 8) & 0x00ff00ffu;
+            }
+          }
+#pragma unroll
+          for (int x = 0; x < NT; ++x) {
+#pragma unroll
+            for (int i = 0; i < QP; ++i) {
+              if constexpr (C::kQReg) {
+                mma_f16(acc[x], A, qr[j][i][0], qr[j][i][1]);
+              } else {
+                const uint2 b = q_smem[((x * KS + j) * QP + i) * 32];
+                mma_f16(acc[x], A, b.x, b.y);
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t p = kp[i >> 1][k];
+            s[x][i] = fmaf(param_scale(p), acc[x][i] * qf[x][i & 1], s[x][i]);
+            s[x][i] = fmaf(param_low(p), qsum[x][k][i & 1], s[x][i]);
+          }
+      }
+      if (edge) {
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (pos + row_position(g) + 8 * (i >> 1) >= see[x][i & 1]) s[x][i] = -INFINITY;
+      }
+      // -- the reference follows the scores in steps of at least 8
+      bool move = false;
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) move |= fmaxf(s[x][h], s[x][2 + h]) > m[x][h] + 8.0f;
+      if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float top = fmaxf(s[x][h], s[x][2 + h]);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            top = fmaxf(top, m[x][h]);
+            const float f = ex2(m[x][h] - top);
+            m[x][h] = top;
+            l[x][h] *= f;
+#pragma unroll
+            for (int k = 0; k < G; ++k) vlo[x][k][h] *= f;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              o[x][i][h] *= f;
+              o[x][i][2 + h] *= f;
+            }
+          }
+      }
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[x][i] = ex2(s[x][i] - m[x][i & 1]);
+          l[x][i & 1] += s[x][i];
+        }
+      // -- the scale of w s follows the largest s
+      bool grow = false;
+      uint32_t vp[2][G];
+      load_words(vprm + row_position(g) * G, vp[0]);
+      load_words(vprm + (row_position(g) + 8) * G, vp[1]);
+#pragma unroll
+      for (int k = 0; k < G; ++k)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          // positions behind the last hold whatever the page held before
+          if (edge && pos + row_position(g) + 8 * h >= see_any) vp[h][k] = 0u;
+          grow |= param_scale(vp[h][k]) > vmax[k];
+        }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int k = 0; k < G; ++k) {
+          float top = fmaxf(vmax[k], fmaxf(param_scale(vp[0][k]), param_scale(vp[1][k])));
+          top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+          if (!(top > vmax[k])) continue;
+          // top in [2^(E-1), 2^E): 2^(5-E) leaves it below 2^5, with room for 4 times as much
+          const int E = min(max((int)(__float_as_uint(top) >> 23) - 126, -90), 128);
+          const float down = __uint_as_float((uint32_t)(5 - E + 127) << 23);
+          const float f = vmax[k] > 0.0f ? down / vdown[k] : 0.0f;
+          vmax[k] = __uint_as_float((uint32_t)(min(E + 2, 127) + 127) << 23);
+          vdown[k] = down;
+#pragma unroll
+          for (int x = 0; x < NT; ++x)
+#pragma unroll
+            for (int i = 0; i < GROUP / 16; ++i)
+#pragma unroll
+              for (int q = 0; q < 4; ++q) o[x][k * (GROUP / 16) + i][q] *= f;
+        }
+      }
+      // -- output: rows are dimensions, the contraction runs over the positions;
+      // contraction indices 2t, 2t+1, 2t+8, 2t+9 are the score rows of that name
+      uint32_t vw[4][VW];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = row_position(2 * t + (i & 1)) + 8 * (i >> 1);
+#pragma unroll
+        for (int j = 0; j < VW; j += 4) {
+          const uint32_t* p = reinterpret_cast<const uint32_t*>(vc + at * C::ROW + v_word_at<C::ROW>(at, g, j));
+          if constexpr (VW >= 4) {
+            const uint4 u = *reinterpret_cast<const uint4*>(p);
+            vw[i][j] = u.x;
+            vw[i][j + 1] = u.y;
+            vw[i][j + 2] = u.z;
+            vw[i][j + 3] = u.w;
+          } else {
+            load_words(p, vw[i]);
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < G; ++k) {
+        uint32_t ph[NT][2], pl[C::PLO ? NT : 1][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float sv = param_scale(vp[h][k]) * vdown[k], lo = param_low(vp[h][k]);
+#pragma unroll
+          for (int x = 0; x < NT; ++x) {
+            float p0 = s[x][2 * h], p1 = s[x][2 * h + 1];
+            float w0 = p0 * sv, w1 = p1 * sv, z0 = p0 * lo, z1 = p1 * lo;
+            if (edge) {   // a position that a row does not see gives it nothing, NaN or not
+              const int at = pos + row_position(g) + 8 * h;
+              if (at >= see[x][0]) w0 = z0 = 0.0f;
+              if (at >= see[x][1]) w1 = z1 = 0.0f;
+            }
+            vlo[x][k][0] += z0;
+            vlo[x][k][1] += z1;
+            const uint32_t hi = pack_f16(w0, w1);
+            ph[x][h] = transpose_8x8(hi);
+            if constexpr (C::PLO) {
+              const float2 f = unpack_f16(hi);
+              pl[x][h] = transpose_8x8(pack_f16(w0 - f.x, w1 - f.y));
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < GROUP / 16; ++i) {
+          const int mt = k * (GROUP / 16) + i;
+          uint32_t A[4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {   // positions 2t, 2t+1 and 2t+8, 2t+9
+            if (BITS == 4) {
+              const uint32_t pair = __byte_perm(vw[2 * h][mt >> 2], vw[2 * h + 1][mt >> 2],
+                                                (mt & 2) ? 0x7632 : 0x5410) >> (8 * (mt & 1));
+              A[2 * h] = pair & 0x000f000fu;
+              A[2 * h + 1] = pair & 0x00f000f0u;
+            } else {
+              const uint32_t pair = __byte_perm(vw[2 * h][mt >> 1], vw[2 * h + 1][mt >> 1],
+                                                (mt & 1) ? 0x7632 : 0x5410);
+              A[2 * h] = pair & 0x00ff00ffu;
+              A[2 * h + 1] = (pair >> 8) & 0x00ff00ffu;
+            }
+          }
+#pragma unroll
+          for (int x = 0; x < NT; ++x) {
+            mma_f16(o[x][mt], A, ph[x][0], ph[x][1]);
+            if constexpr (C::PLO) mma_f16(o[x][mt], A, pl[x][0], pl[x][1]);
+          }
+        }
+      }
+    };
+
+    // ------------------------------------------------------ the positions
+    const int end = min(block1 * kAttBlock, see_any);
+    const int p0 = block0 * kAttBlock + warp * 16;
+    const int tiles = p0 < end ? (end - p0 + kAttBlock - 1) / kAttBlock : 0;
+    uint32_t bad = 0;   // stages whose tile has no page
+    // lane i holds the page of this warp's tile (32 n + i)
+    int my_page = -1;
+    auto fetch_pages = [&](int from) {
+      const int p = p0 + (from + lane) * kAttBlock;
+      my_page = from + lane < tiles ? (int)kv_page(c, w, seq, p) : -1;
+      if (from + lane < tiles && my_page < 0) record_status(ICX_DEVICE_BAD_PAGE);
+    };
+    // pages are taken in order, and the ring holds the next kStages - 1 tiles
+    auto advance = [&](int i) {
+      if (i >= tiles || !ok) return;
+      if ((i & 31) == 0) fetch_pages(i);
+      const int page = __shfl_sync(0xffffffffu, my_page, i & 31);
+      if (page >= 0) load(i % C::kStages, page, p0 + i * kAttBlock);
+      else bad |= 1u << (i % C::kStages);
+    };
+    for (int i = 0; i < C::kStages - 1; ++i) advance(i);
+    for (int i = 0; i < tiles; ++i) {
+      const int stage = i % C::kStages;
+      __syncwarp();   // every lane is done with the stage that is filled next
+      advance(i + C::kStages - 1);
+      if (bad >> stage & 1) {
+        bad &= ~(1u << stage);
+        continue;
+      }
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][stage], phase >> stage & 1, ICX_DEVICE_TIMEOUT_CACHE));
+      phase ^= 1u << stage;
+      if (ok) process(stage, p0 + i * kAttBlock);
+    }
+
+    // --------------------------------------------- join lanes, then warps
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int k = 0; k < G; ++k) {
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) vlo[x][k][h] += __shfl_xor_sync(0xffffffffu, vlo[x][k][h], d);
+          // o in units of the cached values
+          const float up = vdown[k] > 0.0f ? 1.0f / vdown[k] : 0.0f;
+#pragma unroll
+          for (int i = 0; i < GROUP / 16; ++i) {
+            float* ot = o[x][k * (GROUP / 16) + i];
+            ot[h] = fmaf(ot[h] * 16777216.0f, up, vlo[x][k][h]);
+            ot[2 + h] = fmaf(ot[2 + h] * (BITS == 4 ? 1048576.0f : 16777216.0f), up, vlo[x][k][h]);
+          }
+        }
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[x][h] += __shfl_xor_sync(0xffffffffu, l[x][h], d);
+      }
+    __syncthreads();   // the ring is free
+#pragma unroll
+    for (int half = kAttWarps / 2; half >= 1; half >>= 1) {
+      float* mine = reinterpret_cast<float*>(smem) + (size_t)(warp % half) * R * C::kRowFloats;
+      if (warp >= half && warp < 2 * half) {
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float* row = mine + (8 * x + 2 * t + h) * C::kRowFloats;
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+              *reinterpret_cast<float2*>(row + 16 * i + 2 * g) = make_float2(o[x][i][h], o[x][i][2 + h]);
+            if (g == 0) *reinterpret_cast<float2*>(row + D) = make_float2(m[x][h], l[x][h]);
+          }
+      }
+      __syncthreads();
+      if (warp < half) {
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float* row = mine + (8 * x + 2 * t + h) * C::kRowFloats;
+            const float2 ml = *reinterpret_cast<const float2*>(row + D);
+            const float top = fmaxf(m[x][h], ml.x);
+            const float fa = ex2(m[x][h] - top), fb = ex2(ml.x - top);
+            m[x][h] = top;
+            l[x][h] = l[x][h] * fa + ml.y * fb;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              const float2 v = *reinterpret_cast<const float2*>(row + 16 * i + 2 * g);
+              o[x][i][h] = o[x][i][h] * fa + v.x * fb;
+              o[x][i][2 + h] = o[x][i][2 + h] * fa + v.y * fb;
+            }
+          }
+      }
+      __syncthreads();
+    }
+    fence_proxy_async_smem();   // before the next bulk copies over what was written here
+    if (warp == 0) {
+      const bool whole = block0 == 0 && block1 == su.blocks;
+      float* slot = a.partial + ((int64_t)blockIdx.x * 2 + (block0 == 0 ? 1 : 0)) * R * C::kRowFloats;
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = r0 + 8 * x + 2 * t + h;
+          if (r >= su.rows) continue;
+          if (whole) {
+            const float inv = l[x][h] != 0.0f ? 1.0f / l[x][h] : 0.0f;
+            T* out = static_cast<T*>(a.out) +
+                     ((int64_t)(row_base + r / share) * a.q_heads + head * share + r % share) * D;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              const float v[2] = {o[x][i][h] * inv, o[x][i][2 + h] * inv};
+              store_f32<T, 2>(out + 16 * i + 2 * g, v);
+            }
+          } else {
+            float* row = slot + (r - r0) * C::kRowFloats;
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+              *reinterpret_cast<float2*>(row + 16 * i + 2 * g) = make_float2(o[x][i][h], o[x][i][2 + h]);
+            if (g == 0) *reinterpret_cast<float2*>(row + D) = make_float2(m[x][h], l[x][h]);
+          }
+        }
+    }
+  }
+}
+
+// Joins the rows whose units went to several CTAs: one warp per (token, query
+// head), the CTAs in order.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv_attend_join_kernel(const KvView c, const KvTokens w, const AttendArgs a,
+                                                             int R, int ctas) {
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (item >= w.tokens * a.q_heads) return;
+  const int share = a.q_heads / c.heads;
+  const int64_t token = item / a.q_heads;
+  const int hq = (int)(item % a.q_heads);
+  const int b = kv_sequence(w, token);
+  if (b < 0) return;
+  const SeqUnits su = seq_units(c, w, share, R, b);
+  const int64_t row = token - su.from;
+  const int r = (int)row * share + hq % share;
+  const int64_t total = a.prefix[w.batch];
+  const int64_t s0 = a.prefix[b] + ((int64_t)(hq / share) * su.tiles + r / R) * su.blocks, s1 = s0 + su.blocks;
+  if (total <= 0) return;
+  // the CTA that holds unit s is the last with total * cta / ctas <= s
+  const int first = (int)(((s0 + 1) * ctas - 1) / total), last = (int)((s1 * ctas - 1) / total);
+  if (first == last) return;   // written whole
+  constexpr int E = D / 32;
+  float m = kNoScore, l = 0.0f, o[E] = {};
+  for (int i = first; i <= last; ++i) {
+    if (total * i / ctas == total * (i + 1) / ctas) continue;   // more CTAs than units: this one had none
+    const float* p = a.partial + (((int64_t)i * 2 + (i == first ? 1 : 0)) * R + r % R) * (D + 2);
+    const float mi = p[D], li = p[D + 1];
+    const float top = fmaxf(m, mi), fa = ex2(m - top), fb = ex2(mi - top);
+    m = top;
+    l = l * fa + li * fb;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = o[e] * fa + p[lane + 32 * e] * fb;
+  }
+  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    static_cast<T*>(a.out)[(token * a.q_heads + hq) * D + lane + 32 * e] = from_f32<T>(o[e] * inv);
+}
+
+// Which kernel, on how many CTAs.
+struct AttendPlan {
+  int nt;      // query rows per tile / 8
+  int ctas;
+  bool split;
+  size_t prefix_bytes, bytes;   // workspace
+};
+
+AttendPlan plan_attend(const KvView& c, const KvTokens& w, int q_heads);
+
+template <typename T>
+int launch_attend(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a, const AttendPlan& p);
+
+template <>
+int launch_attend<float>(cudaStream_t, const KvView&, const KvTokens&, const AttendArgs&, const AttendPlan&);
+template <>
+int launch_attend<__half>(cudaStream_t, const KvView&, const KvTokens&, const AttendArgs&, const AttendPlan&);
+template <>
+int launch_attend<__nv_bfloat16>(cudaStream_t, const KvView&, const KvTokens&, const AttendArgs&, const AttendPlan&);
+
+template <typename T, int D, int BITS, int GROUP, int NT>
+int launch_attend_rows(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a,
+                       const AttendPlan& p) {
+  using C = AttConfig<T, D, BITS, GROUP, NT>;
+  auto kern = kv_attend_rows_kernel<T, D, BITS, GROUP, NT>;
+  if (C::kSmem > 40 * 1024)   // beside the static part
+    ICX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+  ICX_CUDA(launch_pdl(kern, dim3(p.ctas), dim3(32 * kAttWarps), C::kSmem, s, c, w, a));
+  if (p.split)
+    ICX_CUDA(launch_pdl(kv_attend_join_kernel<T, D>, dim3((unsigned)((w.tokens * a.q_heads + 7) / 8)), dim3(256), 0,
+                        s, c, w, a, C::R, p.ctas));
+  return ICX_OK;
+}
+
+template <typename T, int D, int BITS, int GROUP>
+int launch_attend_nt(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a, const AttendPlan& p) {
+  if (p.nt == 1) return launch_attend_rows<T, D, BITS, GROUP, 1>(s, c, w, a, p);
+  if (p.nt == 2 || D == 256) return launch_attend_rows<T, D, BITS, GROUP, 2>(s, c, w, a, p);
+  return launch_attend_rows<T, D, BITS, GROUP, D == 256 ? 2 : 4>(s, c, w, a, p);
+}
+
+template <typename T, int D>
+int launch_attend_dim(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a, const AttendPlan& p) {
+  if (c.bits == 4)
+    return c.group == 32 ? launch_attend_nt<T, D, 4, 32>(s, c, w, a, p) : launch_attend_nt<T, D, 4, 64>(s, c, w, a, p);
+  return c.group == 32 ? launch_attend_nt<T, D, 8, 32>(s, c, w, a, p) : launch_attend_nt<T, D, 8, 64>(s, c, w, a, p);
+}
+
+#define ICX_ATTEND_INSTANCE(T)                                                                             \
+  template <>                                                                                              \
+  int launch_attend<T>(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a,            \
+                       const AttendPlan& p) {                                                              \
+    return c.dim == 64    ? launch_attend_dim<T, 64>(s, c, w, a, p)                                        \
+           : c.dim == 128 ? launch_attend_dim<T, 128>(s, c, w, a, p)                                       \
+                          : launch_attend_dim<T, 256>(s, c, w, a, p);                                      \
+  }
+
+}  // namespace icx

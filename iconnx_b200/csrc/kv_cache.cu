@@ -108,57 +108,58 @@ __device__ __forceinline__ uint32_t group_code(float x, float lo, float s, float
 
 // One 64-dimension block: four dimensions per lane of the half warp.  The
 // shuffles stay inside the half warp; all 32 lanes take part.
-template <int BITS>
-__device__ __forceinline__ void store_block(uint8_t* row, int which, int dim, int block, int l,
+template <int BITS, int D>
+__device__ __forceinline__ void store_block(uint8_t* row, int token, int which, int block, int l,
                                             const uint32_t (&c)[4], bool valid) {
+  constexpr int ROW = D * BITS / 8;
   const int j = l >> 2, t = l & 3;   // 16-dimension step within the block, quarter of it
+  auto put = [&](int at, uint32_t w) { *reinterpret_cast<uint32_t*>(row + at) = w; };
   if (which == 0) {
-    uint8_t* chunk = row + t * (dim * BITS / 32);
     if (BITS == 4) {
       uint32_t w = (c[0] | (c[1] << 16) | (c[2] << 8) | (c[3] << 24)) << (4 * (j & 1));
       w |= __shfl_xor_sync(0xffffffffu, w, 4);
-      if (valid && !(j & 1)) reinterpret_cast<uint32_t*>(chunk)[block * 2 + (j >> 1)] = w;
+      if (valid && !(j & 1)) put(k_word_at<ROW>(token, t, block * 2 + (j >> 1)), w);
     } else {
       const uint32_t w = c[0] | (c[1] << 16) | (c[2] << 8) | (c[3] << 24);
-      if (valid) reinterpret_cast<uint32_t*>(chunk)[block * 4 + j] = w;
+      if (valid) put(k_word_at<ROW>(token, t, block * 4 + j), w);
     }
   } else {
     // this lane: chunks 2t and 2t+1, codes 2j and 2j+1 of the block
-    const int cb = dim * BITS / 64;   // bytes per chunk
     if (BITS == 4) {
       uint32_t a = (c[0] | (c[1] << 4)) << (8 * j), b = (c[2] | (c[3] << 4)) << (8 * j);
       a |= __shfl_xor_sync(0xffffffffu, a, 4);
       b |= __shfl_xor_sync(0xffffffffu, b, 4);
       a |= __shfl_xor_sync(0xffffffffu, a, 8);
       b |= __shfl_xor_sync(0xffffffffu, b, 8);
-      if (valid && j < 2) reinterpret_cast<uint32_t*>(row + (2 * t + j) * cb)[block] = j ? b : a;
+      if (valid && j < 2) put(v_word_at<ROW>(token, 2 * t + j, block), j ? b : a);
     } else {
       uint32_t a = (c[0] | (c[1] << 8)) << (16 * (j & 1)), b = (c[2] | (c[3] << 8)) << (16 * (j & 1));
       a |= __shfl_xor_sync(0xffffffffu, a, 4);
       b |= __shfl_xor_sync(0xffffffffu, b, 4);
-      if (valid) reinterpret_cast<uint32_t*>(row + (2 * t + (j & 1)) * cb)[block * 2 + (j >> 1)] = (j & 1) ? b : a;
+      if (valid) put(v_word_at<ROW>(token, 2 * t + (j & 1), block * 2 + (j >> 1)), (j & 1) ? b : a);
     }
   }
 }
 
-template <int BITS>
-__device__ __forceinline__ void load_block(const uint8_t* row, int which, int dim, int block, int l,
+template <int BITS, int D>
+__device__ __forceinline__ void load_block(const uint8_t* row, int token, int which, int block, int l,
                                            uint32_t (&c)[4]) {
+  constexpr int ROW = D * BITS / 8;
   const int j = l >> 2, t = l & 3;
   constexpr uint32_t mask = (1u << BITS) - 1;
+  auto get = [&](int at) { return *reinterpret_cast<const uint32_t*>(row + at); };
   if (which == 0) {
-    const uint32_t* chunk = reinterpret_cast<const uint32_t*>(row + t * (dim * BITS / 32));
-    const uint32_t w = BITS == 4 ? chunk[block * 2 + (j >> 1)] >> (4 * (j & 1)) : chunk[block * 4 + j];
+    const uint32_t w = BITS == 4 ? get(k_word_at<ROW>(token, t, block * 2 + (j >> 1))) >> (4 * (j & 1))
+                                 : get(k_word_at<ROW>(token, t, block * 4 + j));
     c[0] = w & mask;
     c[1] = (w >> 16) & mask;
     c[2] = (w >> 8) & mask;
     c[3] = (w >> 24) & mask;
   } else {
-    const int cb = dim * BITS / 64;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint32_t* chunk = reinterpret_cast<const uint32_t*>(row + (2 * t + h) * cb);
-      const uint32_t w = BITS == 4 ? chunk[block] >> (8 * j) : chunk[block * 2 + (j >> 1)] >> (16 * (j & 1));
+      const uint32_t w = BITS == 4 ? get(v_word_at<ROW>(token, 2 * t + h, block)) >> (8 * j)
+                                   : get(v_word_at<ROW>(token, 2 * t + h, block * 2 + (j >> 1))) >> (16 * (j & 1));
       c[2 * h] = w & mask;
       c[2 * h + 1] = (w >> BITS) & mask;
     }
@@ -172,11 +173,11 @@ struct KvSource {
   int vec[2];        // four elements can be read in one access
 };
 
-template <typename T, int BITS>
+template <typename T, int BITS, int D>
 __global__ void __launch_bounds__(256) kv_append_kernel(const KvView c, const KvTokens w, const KvSource src) {
   pdl_wait();
   pdl_trigger();
-  const int blocks = c.dim / 64;
+  constexpr int blocks = D / 64;
   const int64_t items = w.tokens * c.heads * blocks * 2;
   const int l = threadIdx.x & 15;
   const int64_t step = (int64_t)gridDim.x * 16;
@@ -226,23 +227,23 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvView c, const Kv
       for (int k = 0; k < 4; ++k) code[k] = group_code<BITS>(x[k], lo, s, inv);
     }
     const int64_t row = valid ? kv_row(c, page, head, pos) : 0;
-    store_block<BITS>(c.codes[which] + row * (c.dim * BITS / 8), which, c.dim, block, l, code, valid);
+    store_block<BITS, D>(c.codes[which] + row * (D * BITS / 8), pos, which, block, l, code, valid);
     if (valid && 4 * l % c.group == 0)
-      c.params[which][row * (c.dim / c.group) + d / c.group] = p;
+      c.params[which][row * (D / c.group) + d / c.group] = p;
     if (valid && src.values[which]) {
       float v[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) v[k] = fmaf((float)code[k], s, lo);
-      store_f32<T, 4>(static_cast<T*>(src.values[which]) + (token * c.heads + head) * c.dim + d, v);
+      store_f32<T, 4>(static_cast<T*>(src.values[which]) + (token * c.heads + head) * D + d, v);
     }
   }
 }
 
-template <typename T, int BITS>
+template <typename T, int BITS, int D>
 __global__ void __launch_bounds__(256) kv_read_kernel(const KvView c, const KvTokens w, T* k_out, T* v_out) {
   pdl_wait();
   pdl_trigger();
-  const int blocks = c.dim / 64;
+  constexpr int blocks = D / 64;
   const int64_t items = w.tokens * c.heads * blocks * 2;
   const int l = threadIdx.x & 15;
   for (int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); i < items; i += (int64_t)gridDim.x * 16) {
@@ -262,15 +263,19 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvView c, const KvTo
     }
     const int64_t row = kv_row(c, page, head, pos);
     const int d = block * 64 + 4 * l;
-    const uint32_t p = c.params[which][row * (c.dim / c.group) + d / c.group];
+    const uint32_t p = c.params[which][row * (D / c.group) + d / c.group];
     uint32_t code[4];
-    load_block<BITS>(c.codes[which] + row * (c.dim * BITS / 8), which, c.dim, block, l, code);
+    load_block<BITS, D>(c.codes[which] + row * (D * BITS / 8), pos, which, block, l, code);
     float v[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] = fmaf((float)code[k], param_scale(p), param_low(p));
-    store_f32<T, 4>(out + (token * c.heads + head) * c.dim + d, v);
+    store_f32<T, 4>(out + (token * c.heads + head) * D + d, v);
   }
 }
+
+#define ICX_KV_DISPATCH(kernel)                                                                        \
+  (c.bits == 4 ? (c.dim == 64 ? kernel<T, 4, 64> : c.dim == 128 ? kernel<T, 4, 128> : kernel<T, 4, 256>) \
+               : (c.dim == 64 ? kernel<T, 8, 64> : c.dim == 128 ? kernel<T, 8, 128> : kernel<T, 8, 256>))
 
 static unsigned item_grid(int64_t items) {
   const int64_t blocks = (items + 15) / 16;
@@ -305,8 +310,8 @@ extern "C" int icx_kv_cache_append(void* stream, const icx_kv_cache* cache, cons
                {vec(d_k, k_token_stride, k_head_stride), vec(d_v, v_token_stride, v_head_stride)}};
   const dim3 grid(item_grid(w.tokens * c.heads * (c.dim / 64) * 2));
   cudaStream_t s = as_stream(stream);
-  ICX_FLOAT_DISPATCH(type, ICX_CUDA(launch_pdl(c.bits == 4 ? kv_append_kernel<T, 4> : kv_append_kernel<T, 8>, grid,
-                                               dim3(256), 0, s, c, w, src)));
+  ICX_FLOAT_DISPATCH(type,
+                     ICX_CUDA(launch_pdl(ICX_KV_DISPATCH(kv_append_kernel), grid, dim3(256), 0, s, c, w, src)));
   return ICX_OK;
 }
 
@@ -322,7 +327,7 @@ extern "C" int icx_kv_cache_read(void* stream, const icx_kv_cache* cache, const 
   if (w.tokens == 0 || w.batch == 0) return ICX_OK;
   const dim3 grid(item_grid(w.tokens * c.heads * (c.dim / 64) * 2));
   cudaStream_t s = as_stream(stream);
-  ICX_FLOAT_DISPATCH(type, ICX_CUDA(launch_pdl(c.bits == 4 ? kv_read_kernel<T, 4> : kv_read_kernel<T, 8>, grid,
-                                               dim3(256), 0, s, c, w, static_cast<T*>(d_k), static_cast<T*>(d_v))));
+  ICX_FLOAT_DISPATCH(type, ICX_CUDA(launch_pdl(ICX_KV_DISPATCH(kv_read_kernel), grid, dim3(256), 0, s, c, w,
+                                               static_cast<T*>(d_k), static_cast<T*>(d_v))));
   return ICX_OK;
 }

@@ -2,14 +2,19 @@
 // and attend over it.
 //
 // Codes stand in rows of head_dim * bits / 8 bytes, one row per (page, head,
-// token of the page).  Inside a row they are ordered for the attention's
-// matrix instructions (m16n8k16, thread (g, t) of a warp: g = lane / 4,
-// t = lane % 4), so that a thread's operands are consecutive bytes:
+// token of the page), so 16 consecutive tokens are one contiguous piece that a
+// bulk copy brings to shared memory as it stands.  Inside a row the codes are
+// ordered for the attention's matrix instructions (m16n8k16, thread (g, t) of
+// a warp: g = lane / 4, t = lane % 4): what a thread needs is consecutive, and
+// the places are exchanged by token so that a warp's reads meet no shared
+// memory bank twice.
 //
 //   K is the left operand of the scores (rows = tokens, contraction over the
 //   dimensions).  Step j of the contraction covers dimensions 16j .. 16j+15,
 //   of which thread t holds 16j + 4t + {0,1,2,3}.  The row is four chunks, one
-//   per t, each with t's dimensions of all steps in order.
+//   per t, each with t's dimensions of all steps in order; chunks longer than
+//   16 bytes are cut into pieces of 16, pieces n of all chunks stand together
+//   (64 bytes), and odd tokens exchange pieces 2n and 2n + 1.
 //     4 bits: word w of a chunk holds steps 2w and 2w+1; dimension i of step
 //             2w + o stands in nibble {0, 4, 2, 6}[i] + o.
 //     8 bits: word j of a chunk holds step j; dimension i stands in byte
@@ -17,7 +22,10 @@
 //   V is the left operand of the output (rows = dimensions, contraction over
 //   the tokens).  Row tile m covers dimensions 16m .. 16m+15, of which thread
 //   g holds 16m + 2g + {0,1}.  The row is eight chunks, one per g; dimension
-//   16m + 2g + h is code 2m + h of chunk g, in order of the bits.
+//   16m + 2g + h is code 2m + h of chunk g, in order of the bits.  Chunks of
+//   32 bytes are cut into two pieces, first all first ones.  Chunk g stands at
+//   place g ^ 2h (16-byte pieces) or g ^ 4 (h & 1) (8 bytes), h = bits 1 and 2
+//   of the token.
 #pragma once
 
 #include "floats.cuh"
@@ -71,6 +79,22 @@ __device__ __forceinline__ int64_t kv_page(const KvView& c, const KvTokens& w, i
 // Row of (page, head, token of the page) in the codes and params buffers.
 __device__ __forceinline__ int64_t kv_row(const KvView& c, int64_t page, int head, int p) {
   return (((page * c.heads) + head) << c.page_shift) + (p & ((1 << c.page_shift) - 1));
+}
+
+// Byte where word w of K chunk t stands in the row of a token, and word w of
+// V chunk g.  ROW = bytes per row.
+template <int ROW>
+__device__ __forceinline__ int k_word_at(int token, int t, int w) {
+  if (ROW == 32) return t * 8 + w * 4;
+  const int piece = ROW == 64 ? 0 : (w >> 2) ^ (token & 1);
+  return piece * 64 + t * 16 + (w & 3) * 4;
+}
+template <int ROW>
+__device__ __forceinline__ int v_word_at(int token, int g, int w) {
+  const int h = (token >> 1) & 3;
+  if (ROW == 32) return g * 4;
+  if (ROW == 64) return (g ^ (4 * (h & 1))) * 8 + w * 4;
+  return (w >> 2) * 128 + (g ^ (2 * h)) * 16 + (w & 3) * 4;
 }
 
 }  // namespace icx

@@ -51,6 +51,7 @@ extern "C" {
 #define ICX_DEVICE_TIMEOUT_PRODUCER 0x101
 #define ICX_DEVICE_TIMEOUT_MMA 0x102
 #define ICX_DEVICE_TIMEOUT_EPILOGUE 0x103
+#define ICX_DEVICE_TIMEOUT_CACHE 0x104
 #define ICX_DEVICE_TIMEOUT_SELFTEST 0x1ff
 /* a cache operator met a position without a usable page (and touched nothing
  * there): the page table's entry is outside the pool, or the sequence is
