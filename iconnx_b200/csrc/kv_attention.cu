@@ -2,18 +2,9 @@
 #include <cmath>
 
 #include "kv_attention.cuh"
+#include "tmap.cuh"
 
 namespace icx {
-
-static int sm_count() {
-  int dev = 0, n = 148;
-  cudaGetDevice(&dev);
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
-    cudaGetLastError();
-    n = 148;
-  }
-  return n;
-}
 
 AttendPlan plan_attend(const KvView& c, const KvTokens& w, int q_heads) {
   AttendPlan p{};

@@ -32,6 +32,7 @@
 
 #include "capi.cuh"
 #include "common.cuh"
+#include "tmap.cuh"
 
 namespace icx {
 
@@ -160,30 +161,6 @@ struct Cfg {
 template <int EW>
 __device__ __forceinline__ void epi_sync() {
   asm volatile("bar.sync 1, %0;" ::"n"(32 * EW) : "memory");
-}
-
-// 2-D TMA store shared -> global of one 32x32 box (tracked by bulk groups).
-__device__ __forceinline__ void tma_store_2d(const void* tmap, const void* src,
-                                             int c0, int c1) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
-          tmap),
-      "r"(smem_addr(src)), "r"(c0), "r"(c1)
-      : "memory");
-}
-__device__ __forceinline__ void bulk_commit() {
-  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-}
-__device__ __forceinline__ void bulk_wait_read0() {
-  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-}
-// Waits until at most N bulk groups of this thread still read shared memory.
-template <int N>
-__device__ __forceinline__ void bulk_wait_read() {
-  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void bulk_wait0() {
-  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
 // Packed fp32 pairs (sm_100 f32x2 instructions).  Used only inside the GELU,
@@ -1135,14 +1112,7 @@ __global__ void qgemm_simt_kernel(const void* __restrict__ a, int a_signed,
 }
 
 // ---------------------------------------------------------------- host side
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
-                                  void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*,
-                                  CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion,
-                                  CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_fn() {
+EncodeTiledFn encode_fn() {
   static EncodeTiledFn fn = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {
@@ -1158,8 +1128,7 @@ static EncodeTiledFn encode_fn() {
 
 // K-major byte matrix [rows, K] -> tensor map with a box of box_rows x 128
 // bytes and the 128-byte swizzle.  Out-of-range rows/columns read as zero.
-static int make_tmap(CUtensorMap* map, const void* base, size_t rows, size_t K,
-                     int box_rows) {
+int make_tmap(CUtensorMap* map, const void* base, size_t rows, size_t K, int box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) {
     set_error("cuTensorMapEncodeTiled unavailable from the driver");
@@ -1180,7 +1149,7 @@ static int make_tmap(CUtensorMap* map, const void* base, size_t rows, size_t K,
   return ICX_OK;
 }
 
-static int sm_count() {
+int sm_count() {
   int dev = 0, n = 148;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);

@@ -1,0 +1,667 @@
+// Scaled int8 product on the 5th-generation tensor cores:
+//   out[m,n] = (sum_k q[m,k] w[n,k]) * q_scale[m] * w_scale[n] [+ bias[n]]
+//              [+ residual[m,n]],  rounded once to f32 / f16 / bf16.
+// The s32 sum is exact (tcgen05.mma kind::i8, K <= 131071) and stays in tensor
+// memory; the rest happens in registers on its way out.  Three kernels:
+//
+//   scaled_rows_kernel    many tokens: 128 (one CTA) or 256 (a CTA pair,
+//                         cta_group::2) tokens x 128 / 256 channels per tile,
+//                         persistent, bound by the tensor cores.
+//   scaled_stream_kernel  up to 128 tokens: the weight is the 128-row operand
+//                         and the tokens the narrow one, so that nothing is
+//                         padded to 128 tokens; bound by reading the weight
+//                         once, which all SMs share by splitting K over the
+//                         CTAs of a cluster, summed in s32 through distributed
+//                         shared memory (exact, so in any order).
+//   scaled_tile_kernel    any K and alignment (TMA needs K % 16 == 0 and
+//                         16-byte bases): dp4a on 64 x 64 tiles.
+#include <type_traits>
+
+#include "capi.cuh"
+#include "common.cuh"
+#include "floats.cuh"
+#include "tmap.cuh"
+
+namespace icx {
+
+struct ScaledArgs {
+  const int8_t* q;
+  const float* q_scale;
+  const int8_t* wt;  // [N, K]
+  int M, K, N;
+  const float* w_scale;
+  const float* bias;      // nullable
+  const void* residual;   // nullable, out type
+  void* out;
+};
+
+// One rounding per operation: the product with the token's scale, then with
+// the channel's (fused with the bias), then the residual's sum.
+__device__ __forceinline__ float scaled_value(int acc, float sa, float sw, float bias) {
+  return fmaf(__int2float_rn(acc) * sa, sw, bias);
+}
+
+// ------------------------------------------------- any K and any alignment
+template <typename T>
+__global__ void __launch_bounds__(256) scaled_tile_kernel(const ScaledArgs p) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ int sa[64][17], sb[64][17];   // 64 rows of 64 bytes, padded
+  const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  int acc[4][4] = {};
+  for (int k0 = 0; k0 < p.K; k0 += 64) {
+    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
+      const int r = i >> 6, c = i & 63;
+      const bool kv = k0 + c < p.K;
+      reinterpret_cast<int8_t*>(&sa[r][0])[c] =
+          kv && m0 + r < p.M ? p.q[(size_t)(m0 + r) * p.K + k0 + c] : (int8_t)0;
+      reinterpret_cast<int8_t*>(&sb[r][0])[c] =
+          kv && n0 + r < p.N ? p.wt[(size_t)(n0 + r) * p.K + k0 + c] : (int8_t)0;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(sa[ty + 16 * i][k], sb[tx + 16 * j][k], acc[i][j]);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
+      if (m >= p.M || n >= p.N) continue;
+      const size_t o = (size_t)m * p.N + n;
+      float v = scaled_value(acc[i][j], p.q_scale[m], p.w_scale[n], p.bias ? p.bias[n] : 0.0f);
+      if (p.residual) v += to_f32(static_cast<const T*>(p.residual)[o]);
+      static_cast<T*>(p.out)[o] = from_f32<T>(v);
+    }
+}
+
+constexpr int kRows = 128;    // rows of the wide operand per CTA
+constexpr int kStep = 128;    // K bytes per stage (one 128-byte swizzle atom)
+
+// ------------------------------------------------------------- many tokens
+// Warp 0 loads (TMA, 128-byte swizzle), warp 1 issues the matrix
+// instructions into two accumulators of BN columns, warps 2..9 finish: each
+// takes the 32 tokens of its TMEM quadrant and every other box of 128 output
+// bytes per token, which leaves through a swizzled staging box (two per warp)
+// by TMA, or row by row where N or the output is not 16-byte aligned.
+constexpr int kRowsEpi = 8;
+constexpr int kRowsThreads = 64 + 32 * kRowsEpi;
+
+template <int BN, int CG>
+struct RowsConfig {
+  static constexpr int kABytes = kRows * kStep;
+  static constexpr int kBBytes = (BN / CG) * kStep;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kStages = (224 * 1024 - kRowsEpi * (2 * 4096 + 512) - 2048) / kStageBytes;
+  static constexpr int kBoxOffset = kStages * kStageBytes;
+  static constexpr int kOpOffset = kBoxOffset + kRowsEpi * 2 * 4096;
+  static constexpr int kBarOffset = kOpOffset + kRowsEpi * 512;
+  static constexpr int kSmem = kBarOffset + 512 + 1024;   // + alignment slack
+  static constexpr int kTmemCols = 2 * BN;
+  static_assert(kStages >= 3 && (2 * kStages + 4) * 8 + 8 <= 512 && kSmem <= 227 * 1024, "shared memory");
+};
+
+template <typename T, int BN, int CG>
+__global__ void __launch_bounds__(kRowsThreads, 1)
+    scaled_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                       const __grid_constant__ CUtensorMap tmOut, const __grid_constant__ ScaledArgs p,
+                       int tma_store, int vec_residual) {
+  using C = RowsConfig<BN, CG>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + C::kStages * C::kABytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOffset);
+  uint64_t* empty = full + C::kStages;
+  uint64_t* tfull = empty + C::kStages;
+  uint64_t* tempty = tfull + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int num_n = (p.N + BN - 1) / BN, num_m = (p.M + kRows * CG - 1) / (kRows * CG);
+  const int ntiles = num_m * num_n, nk = (p.K + kStep - 1) / kStep;
+  const uint32_t rank = CG == 2 ? cluster_ctarank() : 0u;
+  const int tile0 = CG == 2 ? (int)cluster_id_x() : (int)blockIdx.x;
+  const int tstep = CG == 2 ? (int)nclusters_x() : (int)gridDim.x;
+  // tiles in bands of 16 token tiles, channel by channel inside a band: the
+  // CTAs that run together share few rows of both operands, which stay in L2
+  auto tile_at = [&](int t, int& m0, int& n0) {
+    const int band = t / (16 * num_n), in = t - band * 16 * num_n;
+    const int height = min(16, num_m - band * 16);
+    m0 = (band * 16 + in % height) * kRows * CG + (int)rank * kRows;
+    n0 = in / height * BN;
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull[a], 1);
+      mbar_init(&tempty[a], CG * kRowsEpi);   // the leader's counts both CTAs' warps
+    }
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+    if (tma_store) tma_prefetch_desc(&tmOut);
+  }
+  if (warp == 1) {
+    if (CG == 2) {
+      tmem_alloc_pair(tmem_slot, C::kTmemCols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_slot, C::kTmemCols);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  if (CG == 2) cluster_sync();
+  else __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_trigger();
+
+  if (warp == 0) {
+    if (elect_one()) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = tile0; t < ntiles && ok; t += tstep) {
+        int m0, n0;
+        tile_at(t, m0, n0);
+        n0 += (int)rank * (BN / CG);
+        for (int kb = 0; kb < nk; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, ICX_DEVICE_TIMEOUT_PRODUCER)) {
+            ok = false;
+            break;
+          }
+          if (CG == 2) {
+            const uint32_t fb = cluster_addr(&full[stage], 0);
+            if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * C::kStageBytes);
+            tma_load_2d_pair(sA + stage * C::kABytes, &tmA, fb, kb * kStep, m0);
+            tma_load_2d_pair(sB + stage * C::kBBytes, &tmB, fb, kb * kStep, n0);
+          } else {
+            mbar_arrive_expect_tx(&full[stage], C::kStageBytes);
+            tma_load_2d(sA + stage * C::kABytes, &tmA, &full[stage], kb * kStep, m0);
+            tma_load_2d(sB + stage * C::kBBytes, &tmB, &full[stage], kb * kStep, n0);
+          }
+          if (++stage == C::kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && elect_one()) {
+      const uint32_t idesc = idesc_i8(kRows * CG, BN, true, true);
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int t = tile0; t < ntiles && ok; t += tstep) {
+        if (!mbar_wait(&tempty[acc], acc_phase ^ 1, ICX_DEVICE_TIMEOUT_MMA)) break;
+        tc_fence_after();
+        const uint32_t d = tmem + (uint32_t)(acc * BN);
+        for (int kb = 0; kb < nk; ++kb) {
+          if (!mbar_wait(&full[stage], phase, ICX_DEVICE_TIMEOUT_MMA)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t da = smem_desc_k128(smem_addr(sA + stage * C::kABytes));
+          const uint64_t db = smem_desc_k128(smem_addr(sB + stage * C::kBBytes));
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (CG == 2) mma_i8_pair(d, da + (uint64_t)(k * 2), db + (uint64_t)(k * 2), idesc, (kb | k) != 0);
+            else mma_i8(d, da + (uint64_t)(k * 2), db + (uint64_t)(k * 2), idesc, (kb | k) != 0);
+          }
+          if (CG == 2) {
+            mma_commit_pair(cluster_addr(&empty[stage], 0));
+            mma_commit_pair(cluster_addr(&empty[stage], 1));
+          } else {
+            mma_commit(&empty[stage]);
+          }
+          if (++stage == C::kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        if (CG == 2) {
+          mma_commit_pair(cluster_addr(&tfull[acc], 0));
+          mma_commit_pair(cluster_addr(&tfull[acc], 1));
+        } else {
+          mma_commit(&tfull[acc]);
+        }
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1;
+      }
+    }
+  } else {
+    constexpr int CB = 128 / (int)sizeof(T);   // columns of a box
+    constexpr int kPiece = 16 / (int)sizeof(T);   // columns of 16 bytes
+    const int e = warp - 2, quad = warp & 3, part = e >> 2;
+    uint8_t* box0 = smem + C::kBoxOffset + e * 2 * 4096;
+    float* ops = reinterpret_cast<float*>(smem + C::kOpOffset + e * 512);   // [CB] scales, [CB] biases
+    const T* residual = static_cast<const T*>(p.residual);
+    int acc = 0, buf = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int t = tile0; t < ntiles; t += tstep) {
+      int m0, n0;
+      tile_at(t, m0, n0);
+      const int mrow0 = m0 + quad * 32, m = mrow0 + lane;
+      const float sa = m < p.M ? __ldg(p.q_scale + m) : 0.0f;
+      const int nboxes = (min(BN, p.N - n0) + CB - 1) / CB;
+      if (ok) ok = mbar_wait_warp(&tfull[acc], acc_phase, ICX_DEVICE_TIMEOUT_EPILOGUE);
+      tc_fence_after();
+      const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN);
+      const bool rows_here = mrow0 < p.M;
+      for (int bx = part; ok && bx < nboxes; bx += kRowsEpi / 4) {
+        const int nb = n0 + bx * CB;
+        uint8_t* box = box0 + buf * 4096;
+        uint8_t* row = box + lane * 128;
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(trow + (uint32_t)(bx * CB), r);
+        // the box's store of two boxes ago has been read out
+        if (tma_store && lane == 0) bulk_wait_read<1>();
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < CB / 32; ++i) {
+          const int c = i * 32 + lane, n = nb + c;
+          ops[c] = n < p.N ? __ldg(p.w_scale + n) : 0.0f;
+          ops[CB + c] = p.bias && n < p.N ? __ldg(p.bias + n) : 0.0f;
+        }
+        if (residual && rows_here) {
+          // the residual's box, into the places its outputs will take
+          if (vec_residual && nb + CB <= p.N) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int rr = (lane >> 3) + 4 * i, c = lane & 7;
+              uint4 v = make_uint4(0, 0, 0, 0);
+              if (mrow0 + rr < p.M)
+                v = __ldg(reinterpret_cast<const uint4*>(residual + (size_t)(mrow0 + rr) * p.N + nb) + c);
+              *reinterpret_cast<uint4*>(box + rr * 128 + ((c ^ (rr & 7)) << 4)) = v;
+            }
+          } else {
+            for (int rr = 0; rr < 32 && mrow0 + rr < p.M; ++rr)
+#pragma unroll
+              for (int i = 0; i < CB / 32; ++i) {
+                const int c = i * 32 + lane;
+                if (nb + c < p.N)
+                  *reinterpret_cast<T*>(box + rr * 128 + (((c / kPiece) ^ (rr & 7)) << 4) + c % kPiece * sizeof(T)) =
+                      residual[(size_t)(mrow0 + rr) * p.N + nb + c];
+              }
+          }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int half = 0; half < CB / 32; ++half) {
+          if (half) tmem_ld_32x32b_x32(trow + (uint32_t)(bx * CB + 32), r);
+          tmem_ld_wait_regs(r);
+#pragma unroll
+          for (int q = 0; q < 32 / kPiece; ++q) {
+            const int pc = half * (32 / kPiece) + q;   // piece of the row
+            Vec<T, kPiece>* at = reinterpret_cast<Vec<T, kPiece>*>(row + ((pc ^ (lane & 7)) << 4));
+            float v[kPiece];
+#pragma unroll
+            for (int i = 0; i < kPiece; i += 4) {
+              const float4 sw = *reinterpret_cast<const float4*>(ops + pc * kPiece + i);
+              const float4 bi = *reinterpret_cast<const float4*>(ops + CB + pc * kPiece + i);
+              v[i] = scaled_value((int)r[q * kPiece + i], sa, sw.x, bi.x);
+              v[i + 1] = scaled_value((int)r[q * kPiece + i + 1], sa, sw.y, bi.y);
+              v[i + 2] = scaled_value((int)r[q * kPiece + i + 2], sa, sw.z, bi.z);
+              v[i + 3] = scaled_value((int)r[q * kPiece + i + 3], sa, sw.w, bi.w);
+            }
+            Vec<T, kPiece> u;
+            if (residual) {
+              u = *at;
+#pragma unroll
+              for (int i = 0; i < kPiece; ++i) v[i] += to_f32(u.v[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < kPiece; ++i) u.v[i] = from_f32<T>(v[i]);
+            *at = u;
+          }
+        }
+        if (tma_store) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (rows_here) tma_store_2d(&tmOut, box, nb, mrow0);
+            bulk_commit();
+          }
+          buf ^= 1;
+        } else {
+          __syncwarp();
+          T* out = static_cast<T*>(p.out);
+          for (int rr = 0; rr < 32 && mrow0 + rr < p.M; ++rr)
+#pragma unroll
+            for (int i = 0; i < CB / 32; ++i) {
+              const int c = i * 32 + lane;
+              if (nb + c < p.N)
+                out[(size_t)(mrow0 + rr) * p.N + nb + c] = *reinterpret_cast<const T*>(
+                    box + rr * 128 + (((c / kPiece) ^ (rr & 7)) << 4) + c % kPiece * sizeof(T));
+            }
+          __syncwarp();
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (CG == 2) mbar_arrive_cluster(cluster_addr(&tempty[acc], 0));
+        else mbar_arrive(&tempty[acc]);
+      }
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1;
+    }
+    if (tma_store && lane == 0) bulk_wait0();
+  }
+  tc_fence_before();
+  __syncwarp();
+  if (CG == 2) cluster_sync();   // neither CTA leaves while the other may still signal or read it
+  else __syncthreads();
+  tc_fence_after();
+  if (warp == 1) {
+    if (CG == 2) tmem_dealloc_pair(tmem, C::kTmemCols);
+    else tmem_dealloc(tmem, C::kTmemCols);
+  }
+}
+
+// -------------------------------------------------------------- few tokens
+// One tile of 128 channels per cluster; CTA r of the cluster takes its share
+// of K.  Warp 0 loads, warp 1 multiplies, and all six finish: the s32 sums go
+// through shared memory ([token][channel]), and CTA r sums and writes its
+// share of the tokens.
+constexpr int kStreamThreads = 192;
+
+template <int TOK>
+struct StreamConfig {
+  static constexpr int kABytes = kRows * kStep, kBBytes = TOK * kStep;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kFit = (200 * 1024) / kStageBytes;
+  static constexpr int kStages = kFit > 8 ? 8 : kFit;
+  static constexpr int kBarOffset = kStages * kStageBytes;
+  static constexpr int kSmem = kBarOffset + 512 + 1024;
+  static constexpr int kTmemCols = TOK < 32 ? 32 : TOK;
+  static_assert(TOK * kRows * 4 <= kStages * kStageBytes, "sums over the ring");
+};
+
+__device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <typename T, int TOK>
+__global__ void __launch_bounds__(kStreamThreads, 1)
+    scaled_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmQ,
+                         const __grid_constant__ ScaledArgs p, int split) {
+  using C = StreamConfig<TOK>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sW = smem;
+  uint8_t* sQ = smem + C::kStages * C::kABytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOffset);
+  uint64_t* empty = full + C::kStages;
+  uint64_t* done = empty + C::kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = split > 1 ? (int)cluster_ctarank() : 0;
+  const int n0 = (int)blockIdx.x / split * kRows;
+  const int nk = (p.K + kStep - 1) / kStep;
+  const int kb0 = nk * rank / split, kb1 = nk * (rank + 1) / split;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(done, 1);
+    fence_barrier_init();
+    fence_proxy_async_smem();
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmQ);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_trigger();
+
+  bool ok = true;
+  if (warp == 0) {
+    if (elect_one()) {
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const int i = kb - kb0, stage = i % C::kStages;
+        if (!mbar_wait(&empty[stage], (uint32_t)(i / C::kStages & 1) ^ 1, ICX_DEVICE_TIMEOUT_PRODUCER)) break;
+        mbar_arrive_expect_tx(&full[stage], C::kStageBytes);
+        tma_load_2d(sW + stage * C::kABytes, &tmW, &full[stage], kb * kStep, n0);
+        tma_load_2d(sQ + stage * C::kBBytes, &tmQ, &full[stage], kb * kStep, 0);
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const uint32_t idesc = idesc_i8(kRows, TOK, true, true);
+      bool good = true;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const int i = kb - kb0, stage = i % C::kStages;
+        good = mbar_wait(&full[stage], (uint32_t)(i / C::kStages & 1), ICX_DEVICE_TIMEOUT_MMA);
+        if (!good) break;
+        tc_fence_after();
+        const uint64_t da = smem_desc_k128(smem_addr(sW + stage * C::kABytes));
+        const uint64_t db = smem_desc_k128(smem_addr(sQ + stage * C::kBBytes));
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          mma_i8(tmem, da + (uint64_t)(k * 2), db + (uint64_t)(k * 2), idesc, (i | k) != 0);
+        mma_commit(&empty[stage]);
+      }
+      if (good) mma_commit(done);
+    }
+  }
+  __syncwarp();
+  // every warp: its share of the finishing below starts when the sums are whole
+  ok = mbar_wait_warp(done, 0, ICX_DEVICE_TIMEOUT_EPILOGUE);
+  tc_fence_after();
+  int* sums = reinterpret_cast<int*>(smem);   // [TOK][128] over the ring, all of it read by now
+  if (warp >= 2 && ok && kb1 > kb0) {
+    const int quad = warp & 3;
+#pragma unroll
+    for (int c0 = 0; c0 < TOK; c0 += 16) {
+      if (c0 >= p.M) break;
+      uint32_t r[16];
+      tmem_ld_32x32b_x16(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)c0, r);
+      tmem_ld_wait_regs16(r);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sums[(c0 + i) * kRows + quad * 32 + lane] = (int)r[i];
+    }
+  }
+  tc_fence_before();
+  if (split > 1) cluster_sync();
+  else __syncthreads();
+  if (ok) {
+    const int m_from = p.M * rank / split, m_to = p.M * (rank + 1) / split;
+    for (int i = threadIdx.x; i < (m_to - m_from) * kRows; i += kStreamThreads) {
+      const int m = m_from + i / kRows, c = i % kRows, n = n0 + c;
+      int acc = 0;
+      if (split > 1) {
+        for (int r = 0; r < split; ++r)
+          if (nk * (r + 1) / split > nk * r / split) acc += ld_cluster_s32(cluster_addr(sums + m * kRows + c, (uint32_t)r));
+      } else {
+        acc = sums[m * kRows + c];
+      }
+      if (n < p.N) {
+        float v = scaled_value(acc, __ldg(p.q_scale + m), __ldg(p.w_scale + n), p.bias ? __ldg(p.bias + n) : 0.0f);
+        const size_t o = (size_t)m * p.N + n;
+        if (p.residual) v += to_f32(static_cast<const T*>(p.residual)[o]);
+        static_cast<T*>(p.out)[o] = from_f32<T>(v);
+      }
+    }
+  }
+  if (split > 1) cluster_sync();   // no CTA leaves while another reads its sums
+  else __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, C::kTmemCols);
+}
+
+// ---------------------------------------------------------------- host side
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <typename T>
+static int make_out_map(CUtensorMap* map, void* out, int M, int N) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) {
+    set_error("cuTensorMapEncodeTiled unavailable from the driver");
+    return ICX_ERR_CUDA;
+  }
+  const CUtensorMapDataType type = sizeof(T) == 4                      ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)M}, strides[1] = {(cuuint64_t)N * sizeof(T)};
+  cuuint32_t box[2] = {128 / sizeof(T), 32}, estr[2] = {1, 1};
+  const CUresult r = fn(map, type, 2, out, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled (output) failed (%d) M=%d N=%d", (int)r, M, N);
+    return ICX_ERR_CUDA;
+  }
+  return ICX_OK;
+}
+
+// CTA pairs of a kernel that can be resident at once (per device).
+template <typename T, int BN>
+static int max_pairs() {
+  static int cached[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return 0;
+  if (cached[dev]) return cached[dev];
+  using C = RowsConfig<BN, 2>;
+  auto kern = scaled_rows_kernel<T, BN, 2>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess) return 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * 74);
+  cfg.blockDim = dim3(kRowsThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    return 0;
+  }
+  cached[dev] = n;
+  return n;
+}
+
+template <typename T, int BN, int CG>
+static int launch_rows(cudaStream_t s, const ScaledArgs& p, int units) {
+  using C = RowsConfig<BN, CG>;
+  auto kern = scaled_rows_kernel<T, BN, CG>;
+  CUtensorMap ta, tb, to = {};
+  int rc = make_tmap(&ta, p.q, p.M, p.K, kRows);
+  if (rc) return rc;
+  rc = make_tmap(&tb, p.wt, p.N, p.K, BN / CG);
+  if (rc) return rc;
+  const bool pitch16 = (size_t)p.N * sizeof(T) % 16 == 0;
+  const int tma_store = pitch16 && aligned16(p.out);
+  if (tma_store) {
+    rc = make_out_map<T>(&to, p.out, p.M, p.N);
+    if (rc) return rc;
+  }
+  const int vec_residual = pitch16 && p.residual && aligned16(p.residual);
+  ICX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+  const long tiles = (long)((p.M + kRows * CG - 1) / (kRows * CG)) * ((p.N + BN - 1) / BN);
+  const unsigned grid = (unsigned)(tiles < units ? tiles : units) * CG;
+  if (CG == 2)
+    ICX_CUDA(launch_pdl_cluster(kern, dim3(grid), dim3(kRowsThreads), C::kSmem, s, 2u, ta, tb, to, p, tma_store,
+                                vec_residual));
+  else
+    ICX_CUDA(launch_pdl(kern, dim3(grid), dim3(kRowsThreads), C::kSmem, s, ta, tb, to, p, tma_store, vec_residual));
+  return ICX_OK;
+}
+
+template <typename T, int TOK>
+static int launch_stream(cudaStream_t s, const ScaledArgs& p) {
+  using C = StreamConfig<TOK>;
+  auto kern = scaled_stream_kernel<T, TOK>;
+  CUtensorMap tw, tq;
+  int rc = make_tmap(&tw, p.wt, p.N, p.K, kRows);
+  if (rc) return rc;
+  rc = make_tmap(&tq, p.q, p.M, p.K, TOK);
+  if (rc) return rc;
+  ICX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+  // split K while the SMs are not all busy and a CTA keeps at least four steps
+  const int tiles = (p.N + kRows - 1) / kRows, nk = (p.K + kStep - 1) / kStep, sms = sm_count();
+  int split = 1;
+  while (split < 8 && tiles * split * 2 <= sms && nk / (split * 2) >= 4) split *= 2;
+  ICX_CUDA(launch_pdl_cluster(kern, dim3((unsigned)(tiles * split)), dim3(kStreamThreads), C::kSmem, s,
+                              (unsigned)split, tw, tq, p, split));
+  return ICX_OK;
+}
+
+template <typename T>
+static int launch_scaled(cudaStream_t s, const ScaledArgs& p) {
+  if (p.K == 0 || p.K % 16 != 0 || !aligned16(p.q) || !aligned16(p.wt)) {
+    const dim3 grid((unsigned)((p.N + 63) / 64), (unsigned)((p.M + 63) / 64));
+    ICX_CUDA(launch_pdl(scaled_tile_kernel<T>, grid, dim3(256), 0, s, p));
+    return ICX_OK;
+  }
+  if (p.M <= 16) return launch_stream<T, 16>(s, p);
+  if (p.M <= 32) return launch_stream<T, 32>(s, p);
+  if (p.M <= 64) return launch_stream<T, 64>(s, p);
+  if (p.M <= 128) return launch_stream<T, 128>(s, p);
+  const int sms = sm_count();
+  const long nm = (p.M + kRows - 1) / kRows;
+  const int pairs = p.M >= 1024 && p.N > 128 ? max_pairs<T, 256>() : 0;
+  // the kernel whose busiest CTA does the least: tiles per CTA x columns of a
+  // tile (plus what a tile costs beside its columns); pairs move half the
+  // weight bytes per product and win where they keep all SMs busy
+  const long c1 = (nm * ((p.N + 127) / 128) + sms - 1) / sms * (128 + 64);
+  const long c2 = (nm * ((p.N + 255) / 256) + sms - 1) / sms * (256 + 64);
+  const long cp = pairs ? (((nm + 1) / 2) * ((p.N + 255) / 256) + pairs - 1) / pairs * (256 + 32) : c1 + c2;
+  if (cp <= c1 && cp <= c2) return launch_rows<T, 256, 2>(s, p, pairs);
+  return c2 <= c1 ? launch_rows<T, 256, 1>(s, p, sms) : launch_rows<T, 128, 1>(s, p, sms);
+}
+
+}  // namespace icx
+
+using namespace icx;
+
+extern "C" int icx_matmul_integer_scaled(void* stream, const int8_t* d_q, const float* d_q_scale,
+                                         const int8_t* d_wt, size_t M, size_t K, size_t N,
+                                         const float* d_w_scale, const float* d_bias,
+                                         const void* d_residual, int out_type, void* d_out) {
+  ICX_REQUIRE(is_float_type(out_type), "MatMulIntegerScaled: output must be Float32, Float16 or BFloat16");
+  ICX_REQUIRE(K <= ICX_SCALED_MAX_K, "MatMulIntegerScaled: K %zu above %d, where the s32 sum could wrap", K,
+              ICX_SCALED_MAX_K);
+  ICX_REQUIRE(M < (1ull << 22) && N < (1ull << 22), "MatMulIntegerScaled: shape too large");
+  if (M == 0 || N == 0) return ICX_OK;
+  ICX_REQUIRE(d_out && d_q_scale && d_w_scale && (K == 0 || (d_q && d_wt)),
+              "MatMulIntegerScaled: null operand");
+  const ScaledArgs a{d_q, d_q_scale, d_wt, (int)M, (int)K, (int)N, d_w_scale, d_bias, d_residual, d_out};
+  int rc = ICX_OK;
+  ICX_FLOAT_DISPATCH(out_type, rc = launch_scaled<T>(as_stream(stream), a));
+  return rc;
+}
