@@ -1,8 +1,9 @@
 // Quantised K/V cache: append (quantise) and read (dequantise).
 //
-// Half a warp takes 64 dimensions of one (token, head) of K or V, four
-// consecutive ones per lane, so a quantisation group is 8 or 16 lanes and
-// every code word of the layout is put together from lanes of one half warp.
+// Bound by HBM.  Eight lanes take 64 dimensions of one (token, head) of K or V,
+// eight consecutive ones (one or two 16-byte accesses) per lane, so a
+// quantisation group is 4 or 8 lanes and every code word of the layout is put
+// together from lanes of one such eighth.
 #include "kv_cache.cuh"
 
 #include "capi.cuh"
@@ -86,82 +87,144 @@ __device__ __forceinline__ uint32_t group_params(float mn, float mx) {
   return s | (lo << 16);
 }
 
-// rte((x - lo) / s) clamped to [0, L]: rounded from an f32 quotient (off by
-// less than 1e-4 of a step), and where that is within 2e-4 of a half, decided
-// by comparing x with the midpoint in 64 bits ((k + 1/2) * s is exact).
-// Scales whose reciprocal or range may not be finite take the 64-bit quotient.
+// rte((x - lo) / s) clamped to [0, L], as integers and as floats.  An f32
+// quotient is off by less than 5e-5 (three roundings at most 255); where it is
+// within 2e-4 of a half, x is compared with the midpoint in 64 bits ((k + 1/2) s
+// is exact).  Scales whose reciprocal or range may not be finite take the 64-bit
+// quotient.
 template <int BITS>
-__device__ __forceinline__ uint32_t group_code(float x, float lo, float s, float inv) {
+__device__ __noinline__ float code_near_half(float x, float lo, float s, float u) {
+  const float k = floorf(u);
+  const double d = ((double)x - (double)lo) - (double)k * (double)s - 0.5 * (double)s;
+  const float c = d > 0.0 ? k + 1.0f : d < 0.0 ? k : 2.0f * rintf(0.5f * k + 0.25f);
+  return fminf(c, (float)((1 << BITS) - 1));
+}
+
+template <int BITS>
+__device__ __forceinline__ void group_codes(const float (&x)[8], float lo, float s, bool finite, uint32_t (&code)[8],
+                                            float (&c)[8]) {
   constexpr float L = (float)((1 << BITS) - 1);
-  if (s < 1e-36f || s > 1e36f)
-    return (uint32_t)fmin(fmax(rint(((double)x - (double)lo) / (double)s), 0.0), (double)L);
-  const float u = fminf(fmaxf((x - lo) * inv, 0.0f), L);
-  float c = rintf(u);
-  if (fabsf(u - c) > 0.4998f) {
-    const float k = floorf(u);
-    const double d = ((double)x - (double)lo) - (double)k * (double)s - 0.5 * (double)s;
-    c = d > 0.0 ? k + 1.0f : d < 0.0 ? k : 2.0f * rintf(0.5f * k + 0.25f);
-    c = fminf(c, L);
-  }
-  return (uint32_t)c;
-}
-
-// One 64-dimension block: four dimensions per lane of the half warp.  The
-// shuffles stay inside the half warp; all 32 lanes take part.
-template <int BITS, int D>
-__device__ __forceinline__ void store_block(uint8_t* row, int token, int which, int block, int l,
-                                            const uint32_t (&c)[4], bool valid) {
-  constexpr int ROW = D * BITS / 8;
-  const int j = l >> 2, t = l & 3;   // 16-dimension step within the block, quarter of it
-  auto put = [&](int at, uint32_t w) { *reinterpret_cast<uint32_t*>(row + at) = w; };
-  if (which == 0) {
-    if (BITS == 4) {
-      uint32_t w = (c[0] | (c[1] << 16) | (c[2] << 8) | (c[3] << 24)) << (4 * (j & 1));
-      w |= __shfl_xor_sync(0xffffffffu, w, 4);
-      if (valid && !(j & 1)) put(k_word_at<ROW>(token, t, block * 2 + (j >> 1)), w);
-    } else {
-      const uint32_t w = c[0] | (c[1] << 16) | (c[2] << 8) | (c[3] << 24);
-      if (valid) put(k_word_at<ROW>(token, t, block * 4 + j), w);
+  constexpr float kRound = 12582912.0f;   // adding it rounds to an integer (half to even)
+  if (finite && s >= 1e-36f && s <= 1e36f) {
+    const float inv = __frcp_rn(s);
+    float worst = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float u = fminf(fmaxf((x[k] - lo) * inv, 0.0f), L);
+      c[k] = __fsub_rn(__fadd_rn(u, kRound), kRound);
+      worst = fmaxf(worst, fabsf(u - c[k]));
     }
-  } else {
-    // this lane: chunks 2t and 2t+1, codes 2j and 2j+1 of the block
-    if (BITS == 4) {
-      uint32_t a = (c[0] | (c[1] << 4)) << (8 * j), b = (c[2] | (c[3] << 4)) << (8 * j);
-      a |= __shfl_xor_sync(0xffffffffu, a, 4);
-      b |= __shfl_xor_sync(0xffffffffu, b, 4);
-      a |= __shfl_xor_sync(0xffffffffu, a, 8);
-      b |= __shfl_xor_sync(0xffffffffu, b, 8);
-      if (valid && j < 2) put(v_word_at<ROW>(token, 2 * t + j, block), j ? b : a);
-    } else {
-      uint32_t a = (c[0] | (c[1] << 8)) << (16 * (j & 1)), b = (c[2] | (c[3] << 8)) << (16 * (j & 1));
-      a |= __shfl_xor_sync(0xffffffffu, a, 4);
-      b |= __shfl_xor_sync(0xffffffffu, b, 4);
-      if (valid) put(v_word_at<ROW>(token, 2 * t + (j & 1), block * 2 + (j >> 1)), (j & 1) ? b : a);
+    if (worst > 0.4998f) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float u = fminf(fmaxf((x[k] - lo) * inv, 0.0f), L);
+        if (fabsf(u - c[k]) > 0.4998f) c[k] = code_near_half<BITS>(x[k], lo, s, u);
+      }
     }
-  }
-}
-
-template <int BITS, int D>
-__device__ __forceinline__ void load_block(const uint8_t* row, int token, int which, int block, int l,
-                                           uint32_t (&c)[4]) {
-  constexpr int ROW = D * BITS / 8;
-  const int j = l >> 2, t = l & 3;
-  constexpr uint32_t mask = (1u << BITS) - 1;
-  auto get = [&](int at) { return *reinterpret_cast<const uint32_t*>(row + at); };
-  if (which == 0) {
-    const uint32_t w = BITS == 4 ? get(k_word_at<ROW>(token, t, block * 2 + (j >> 1))) >> (4 * (j & 1))
-                                 : get(k_word_at<ROW>(token, t, block * 4 + j));
-    c[0] = w & mask;
-    c[1] = (w >> 16) & mask;
-    c[2] = (w >> 8) & mask;
-    c[3] = (w >> 24) & mask;
   } else {
 #pragma unroll
+    for (int k = 0; k < 8; ++k)
+      c[k] = finite && s > 0.0f ? (float)fmin(fmax(rint(((double)x[k] - (double)lo) / (double)s), 0.0), (double)L) : 0.0f;
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) code[k] = __float_as_uint(c[k] + 8388608.0f) & (uint32_t)((1 << BITS) - 1);
+}
+
+// One block of 64 dimensions: eight lanes (l = 0..7) of eight consecutive
+// dimensions.  Lane l holds step / row tile j = l / 2 of the block, quarters
+// 2 (l & 1) and 2 (l & 1) + 1 of it (K), or thread chunks g = 4 (l & 1) .. + 3
+// (V).  The shuffles stay inside the eight lanes; all 32 lanes take part.
+template <int BITS, int D>
+__device__ __forceinline__ void store_block(uint8_t* row, int token, int which, int block, int l,
+                                            const uint32_t (&c)[8], bool valid) {
+  constexpr int ROW = D * BITS / 8;
+  const int j = l >> 1, odd = l & 1;
+  auto put = [&](int at, uint32_t w) {
+    if (valid) *reinterpret_cast<uint32_t*>(row + at) = w;
+  };
+  if (which == 0) {
+    uint32_t a = c[0] | (c[1] << 16) | (c[2] << 8) | (c[3] << 24), b = c[4] | (c[5] << 16) | (c[6] << 8) | (c[7] << 24);
+    if (BITS == 4) {
+      // words of both quarters need steps 2n and 2n+1, which are lanes l and l ^ 2
+      a <<= 4 * (j & 1);
+      b <<= 4 * (j & 1);
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, (j & 1) ? a : b, 2);
+      put(k_word_at<ROW>(token, 2 * odd + (j & 1), block * 2 + (j >> 1)), ((j & 1) ? b : a) | other);
+    } else {
+      put(k_word_at<ROW>(token, 2 * odd, block * 4 + j), a);
+      put(k_word_at<ROW>(token, 2 * odd + 1, block * 4 + j), b);
+    }
+  } else if (BITS == 4) {
+    // byte i: chunk 4 odd + i, codes 2j and 2j+1; a 4 x 4 byte transposition
+    // over the lanes j leaves lane j with the word of chunk 4 odd + j
+    uint32_t u = (c[0] | (c[1] << 4)) | (c[2] << 8) | (c[3] << 12) | (c[4] << 16) | (c[5] << 20) | (c[6] << 24) |
+                 (c[7] << 28);
+    uint32_t v = __shfl_xor_sync(0xffffffffu, u, 2);
+    u = (j & 1) ? __byte_perm(v, u, 0x7351) : __byte_perm(u, v, 0x6240);
+    v = __shfl_xor_sync(0xffffffffu, u, 4);
+    u = (j & 2) ? __byte_perm(v, u, 0x7632) : __byte_perm(u, v, 0x5410);
+    put(v_word_at<ROW>(token, 4 * odd + j, block), u);
+  } else {
+    // half words of chunks 4 odd + {0,1} and {2,3}; lanes j and j ^ 1 exchange
+    // so that each holds whole words of two chunks
+    const uint32_t a = c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24), b = c[4] | (c[5] << 8) | (c[6] << 16) | (c[7] << 24);
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, (j & 1) ? a : b, 2);
+    const uint32_t lo = (j & 1) ? other : a, hi = (j & 1) ? b : other;
+    const int g = 4 * odd + 2 * (j & 1), w = block * 2 + (j >> 1);
+    put(v_word_at<ROW>(token, g, w), __byte_perm(lo, hi, 0x5410));
+    put(v_word_at<ROW>(token, g + 1, w), __byte_perm(lo, hi, 0x7632));
+  }
+}
+
+// The inverse: the codes of this lane's eight dimensions.  Split in two, so
+// that several blocks' loads can be in flight.
+template <int BITS, int D>
+__device__ __forceinline__ void load_block_words(const uint8_t* row, int token, int which, int block, int l,
+                                                 uint32_t (&w)[2]) {
+  constexpr int ROW = D * BITS / 8;
+  const int j = l >> 1, odd = l & 1;
+  auto get = [&](int at) { return *reinterpret_cast<const uint32_t*>(row + at); };
+  if (which == 0) {
+    const int n = BITS == 4 ? block * 2 + (j >> 1) : block * 4 + j;
+    w[0] = get(k_word_at<ROW>(token, 2 * odd, n));
+    w[1] = get(k_word_at<ROW>(token, 2 * odd + 1, n));
+  } else if (BITS == 4) {
+    w[0] = get(v_word_at<ROW>(token, 4 * odd + j, block));
+  } else {
+    const int g = 4 * odd + 2 * (j & 1), n = block * 2 + (j >> 1);
+    w[0] = get(v_word_at<ROW>(token, g, n));
+    w[1] = get(v_word_at<ROW>(token, g + 1, n));
+  }
+}
+template <int BITS>
+__device__ __forceinline__ void block_codes(int which, int l, const uint32_t (&w)[2], uint32_t (&c)[8]) {
+  const int j = l >> 1;
+  constexpr uint32_t mask = (1u << BITS) - 1;
+  if (which == 0) {
+#pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint32_t w = BITS == 4 ? get(v_word_at<ROW>(token, 2 * t + h, block)) >> (8 * j)
-                                   : get(v_word_at<ROW>(token, 2 * t + h, block * 2 + (j >> 1))) >> (16 * (j & 1));
-      c[2 * h] = w & mask;
-      c[2 * h + 1] = (w >> BITS) & mask;
+      const uint32_t u = BITS == 4 ? w[h] >> (4 * (j & 1)) : w[h];
+      c[4 * h] = u & mask;
+      c[4 * h + 1] = (u >> 16) & mask;
+      c[4 * h + 2] = (u >> 8) & mask;
+      c[4 * h + 3] = (u >> 24) & mask;
+    }
+  } else if (BITS == 4) {
+    uint32_t u = w[0];
+    uint32_t v = __shfl_xor_sync(0xffffffffu, u, 2);
+    u = (j & 1) ? __byte_perm(v, u, 0x7351) : __byte_perm(u, v, 0x6240);
+    v = __shfl_xor_sync(0xffffffffu, u, 4);
+    u = (j & 2) ? __byte_perm(v, u, 0x7632) : __byte_perm(u, v, 0x5410);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = (u >> (4 * i)) & 15u;
+  } else {
+    const uint32_t lo = __byte_perm(w[0], w[1], 0x5410), hi = __byte_perm(w[0], w[1], 0x7632);
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, (j & 1) ? lo : hi, 2);
+    const uint32_t a = (j & 1) ? other : lo, b = (j & 1) ? hi : other;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      c[i] = (a >> (8 * i)) & 255u;
+      c[4 + i] = (b >> (8 * i)) & 255u;
     }
   }
 }
@@ -170,117 +233,176 @@ struct KvSource {
   const void* x[2];
   int64_t token_stride[2], head_stride[2];
   void* values[2];   // nullable
-  int vec[2];        // four elements can be read in one access
+  int vec[2];        // eight elements can be read in 16-byte accesses
 };
 
+// A warp takes one token's K or V: `per` blocks of 64 dimensions of its
+// heads, four at a time, `U` fours in flight.  The token's sequence and page
+// are looked up once.
+struct TokenPart {
+  int64_t token, row0;   // row0: cache row of head 0
+  int which, from, to;   // blocks
+  int pos;
+  bool valid;
+};
+
+__device__ __forceinline__ TokenPart token_part(const KvView& c, const KvTokens& w, int64_t item, int parts, int per,
+                                                int blocks) {
+  TokenPart p;
+  const int part = (int)(item % parts);
+  p.which = (int)((item / parts) & 1);
+  p.token = item / (2 * parts);
+  p.from = part * per;
+  p.to = min(p.from + per, blocks);
+  int b;
+  p.pos = token_position(w, p.token, &b);
+  p.valid = p.pos >= 0;
+  p.row0 = 0;
+  if (p.valid) {
+    const int64_t page = kv_page(c, w, b, p.pos);
+    if (page < 0) {
+      p.valid = false;
+      record_status(ICX_DEVICE_BAD_PAGE);
+    } else {
+      p.row0 = kv_row(c, page, 0, p.pos);
+    }
+  }
+  return p;
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8], bool vec) {
+  if (sizeof(T) == 2) {
+    load_f32<T, 8>(p, x, vec);
+  } else {
+    load_f32<T, 4>(p, *reinterpret_cast<float(*)[4]>(&x[0]), vec);
+    load_f32<T, 4>(p + 4, *reinterpret_cast<float(*)[4]>(&x[4]), vec);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+  if (sizeof(T) == 2) {
+    store_f32<T, 8>(p, x);
+  } else {
+    store_f32<T, 4>(p, *reinterpret_cast<const float(*)[4]>(&x[0]));
+    store_f32<T, 4>(p + 4, *reinterpret_cast<const float(*)[4]>(&x[4]));
+  }
+}
+
 template <typename T, int BITS, int D>
-__global__ void __launch_bounds__(256) kv_append_kernel(const KvView c, const KvTokens w, const KvSource src) {
+__global__ void __launch_bounds__(128)
+    kv_append_kernel(const __grid_constant__ KvView c, const __grid_constant__ KvTokens w,
+                     const __grid_constant__ KvSource src, int parts, int per) {
   pdl_wait();
   pdl_trigger();
-  constexpr int blocks = D / 64;
-  const int64_t items = w.tokens * c.heads * blocks * 2;
-  const int l = threadIdx.x & 15;
-  const int64_t step = (int64_t)gridDim.x * 16;
-  // both halves of a warp run the same number of rounds: shuffles use all lanes
-  for (int64_t base = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 5) * 2; base < items; base += step) {
-    const int64_t it = base + ((threadIdx.x >> 4) & 1);
-    bool valid = it < items;
-    const int64_t i = valid ? it : 0;
-    const int block = (int)(i % blocks);
-    const int which = (int)((i / blocks) & 1);
-    const int head = (int)((i / (2 * blocks)) % c.heads);
-    const int64_t token = i / ((int64_t)2 * blocks * c.heads);
-    int b;
-    const int pos = token_position(w, token, &b);
-    valid = valid && pos >= 0;
-    int64_t page = -1;
-    if (valid) {
-      page = kv_page(c, w, b, pos);
-      if (page < 0) {
-        valid = false;
-        record_status(ICX_DEVICE_BAD_PAGE);
+  constexpr int kPerHead = D / 64, U = 2;
+  const int blocks = c.heads * kPerHead;
+  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (item >= w.tokens * 2 * parts) return;
+  const TokenPart p = token_part(c, w, item, parts, per, blocks);
+  if (!p.valid) return;
+  const int l = threadIdx.x & 7, sub = (threadIdx.x >> 3) & 3;
+  const T* x0 = static_cast<const T*>(src.x[p.which]) + p.token * src.token_stride[p.which];
+  for (int b0 = p.from; b0 < p.to; b0 += 4 * U) {
+    float x[U][8];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int b = b0 + 4 * i + sub;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[i][k] = 0.0f;
+      if (b < p.to)
+        load8<T>(x0 + (b / kPerHead) * src.head_stride[p.which] + b % kPerHead * 64 + 8 * l, x[i], src.vec[p.which]);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (b0 + 4 * i >= p.to) break;
+      const int b = b0 + 4 * i + sub, head = b / kPerHead, block = b % kPerHead;
+      const bool valid = b < p.to;
+      float mn = x[i][0], mx = x[i][0];
+      uint32_t peak = 0;   // |x| by its bits: NaN and infinity are at the top
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        mn = fminf(mn, x[i][k]);
+        mx = fmaxf(mx, x[i][k]);
+        peak = max(peak, __float_as_uint(fabsf(x[i][k])));
       }
-    }
-    const int d = block * 64 + 4 * l;
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
-    if (valid)
-      load_f32<T, 4>(static_cast<const T*>(src.x[which]) + token * src.token_stride[which] +
-                         head * src.head_stride[which] + d,
-                     x, src.vec[which]);
-    float mn = fminf(fminf(x[0], x[1]), fminf(x[2], x[3]));
-    float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-    uint32_t peak = 0;   // |x| by its bits: NaN and infinity are at the top
+      for (int o = 1; o < c.group / 8; o <<= 1) {
+        mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, o));
+      }
+      const bool finite = peak < 0x7f800000u;
+      const uint32_t prm = finite ? group_params<BITS>(mn, mx) : 0x7fc07fc0u;
+      const float s = param_scale(prm), lo = param_low(prm);
+      uint32_t code[8] = {};
+      float v[8];
+      group_codes<BITS>(x[i], lo, s, finite, code, v);
+      const int64_t row = p.row0 + ((int64_t)(valid ? head : 0) << c.page_shift);
+      store_block<BITS, D>(c.codes[p.which] + row * (D * BITS / 8), p.pos, p.which, block, l, code, valid);
+      if (valid) {
+        const int d = block * 64 + 8 * l;
+        if (8 * l % c.group == 0) c.params[p.which][row * (D / c.group) + d / c.group] = prm;
+        if (src.values[p.which]) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) peak = max(peak, __float_as_uint(fabsf(x[k])));
-    for (int o = 1; o < c.group / 4; o <<= 1) {
-      mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, o));
-    }
-    const bool finite = peak < 0x7f800000u;
-    const uint32_t p = finite ? group_params<BITS>(mn, mx) : 0x7fc07fc0u;
-    const float s = param_scale(p), lo = param_low(p);
-    uint32_t code[4] = {0, 0, 0, 0};
-    if (finite && s > 0.0f) {
-      const float inv = __frcp_rn(s);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) code[k] = group_code<BITS>(x[k], lo, s, inv);
-    }
-    const int64_t row = valid ? kv_row(c, page, head, pos) : 0;
-    store_block<BITS, D>(c.codes[which] + row * (D * BITS / 8), pos, which, block, l, code, valid);
-    if (valid && 4 * l % c.group == 0)
-      c.params[which][row * (D / c.group) + d / c.group] = p;
-    if (valid && src.values[which]) {
-      float v[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = fmaf((float)code[k], s, lo);
-      store_f32<T, 4>(static_cast<T*>(src.values[which]) + (token * c.heads + head) * D + d, v);
+          for (int k = 0; k < 8; ++k) v[k] = fmaf(v[k], s, lo);
+          store8<T>(static_cast<T*>(src.values[p.which]) + (p.token * c.heads + head) * D + d, v);
+        }
+      }
     }
   }
 }
 
 template <typename T, int BITS, int D>
-__global__ void __launch_bounds__(256) kv_read_kernel(const KvView c, const KvTokens w, T* k_out, T* v_out) {
+__global__ void __launch_bounds__(128)
+    kv_read_kernel(const __grid_constant__ KvView c, const __grid_constant__ KvTokens w, T* k_out, T* v_out, int parts,
+                   int per) {
   pdl_wait();
   pdl_trigger();
-  constexpr int blocks = D / 64;
-  const int64_t items = w.tokens * c.heads * blocks * 2;
-  const int l = threadIdx.x & 15;
-  for (int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); i < items; i += (int64_t)gridDim.x * 16) {
-    const int block = (int)(i % blocks);
-    const int which = (int)((i / blocks) & 1);
-    T* out = which ? v_out : k_out;
-    if (!out) continue;
-    const int head = (int)((i / (2 * blocks)) % c.heads);
-    const int64_t token = i / ((int64_t)2 * blocks * c.heads);
-    int b;
-    const int pos = token_position(w, token, &b);
-    if (pos < 0) continue;
-    const int64_t page = kv_page(c, w, b, pos);
-    if (page < 0) {
-      record_status(ICX_DEVICE_BAD_PAGE);
-      continue;
-    }
-    const int64_t row = kv_row(c, page, head, pos);
-    const int d = block * 64 + 4 * l;
-    const uint32_t p = c.params[which][row * (D / c.group) + d / c.group];
-    uint32_t code[4];
-    load_block<BITS, D>(c.codes[which] + row * (D * BITS / 8), pos, which, block, l, code);
-    float v[4];
+  constexpr int kPerHead = D / 64, U = 4;
+  const int blocks = c.heads * kPerHead;
+  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (item >= w.tokens * 2 * parts) return;
+  const TokenPart p = token_part(c, w, item, parts, per, blocks);
+  T* out = p.which ? v_out : k_out;
+  if (!p.valid || !out) return;
+  const int l = threadIdx.x & 7, sub = (threadIdx.x >> 3) & 3;
+  for (int b0 = p.from; b0 < p.to; b0 += 4 * U) {
+    uint32_t words[U][2], prm[U];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = fmaf((float)code[k], param_scale(p), param_low(p));
-    store_f32<T, 4>(out + (token * c.heads + head) * D + d, v);
+    for (int i = 0; i < U; ++i) {
+      const int b = min(b0 + 4 * i + sub, p.to - 1), block = b % kPerHead;
+      const int64_t row = p.row0 + ((int64_t)(b / kPerHead) << c.page_shift);
+      load_block_words<BITS, D>(c.codes[p.which] + row * (D * BITS / 8), p.pos, p.which, block, l, words[i]);
+      prm[i] = c.params[p.which][row * (D / c.group) + (block * 64 + 8 * l) / c.group];
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (b0 + 4 * i >= p.to) break;
+      const int b = b0 + 4 * i + sub;
+      uint32_t code[8];
+      block_codes<BITS>(p.which, l, words[i], code);
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)   // a code below 2^23 on 2^23's bits is 2^23 + code
+        v[k] = fmaf(__uint_as_float(0x4b000000u | code[k]) - 8388608.0f, param_scale(prm[i]), param_low(prm[i]));
+      if (b < p.to) store8<T>(out + (p.token * c.heads + b / kPerHead) * D + b % kPerHead * 64 + 8 * l, v);
+    }
   }
+}
+
+// Warps per token and side: one, unless there are too few tokens to fill the
+// GPU (then up to one per four blocks).
+static void token_parts(const KvView& c, const KvTokens& w, int* parts, int* per) {
+  const int blocks = c.heads * (c.dim / 64), fours = (blocks + 3) / 4;
+  int n = 1;
+  while (n < fours && w.tokens * 2 * n < 148 * 16) ++n;
+  *per = (fours + n - 1) / n * 4;
+  *parts = (blocks + *per - 1) / *per;
 }
 
 #define ICX_KV_DISPATCH(kernel)                                                                        \
   (c.bits == 4 ? (c.dim == 64 ? kernel<T, 4, 64> : c.dim == 128 ? kernel<T, 4, 128> : kernel<T, 4, 256>) \
                : (c.dim == 64 ? kernel<T, 8, 64> : c.dim == 128 ? kernel<T, 8, 128> : kernel<T, 8, 256>))
-
-static unsigned item_grid(int64_t items) {
-  const int64_t blocks = (items + 15) / 16;
-  return (unsigned)(blocks < 148 * 32 ? blocks : 148 * 32);
-}
 
 }  // namespace icx
 
@@ -301,17 +423,19 @@ extern "C" int icx_kv_cache_append(void* stream, const icx_kv_cache* cache, cons
   ICX_REQUIRE(d_k && d_v, "KvCacheAppend: null operand");
   const size_t e = float_bytes(type);
   auto vec = [&](const void* p, int64_t ts, int64_t hs) {
-    return (int)((reinterpret_cast<uintptr_t>(p) | (size_t)ts * e | (size_t)hs * e) % (4 * e) == 0);
+    return (int)((reinterpret_cast<uintptr_t>(p) | (size_t)ts * e | (size_t)hs * e) % 16 == 0);
   };
   ICX_REQUIRE(((reinterpret_cast<uintptr_t>(d_k_values) | reinterpret_cast<uintptr_t>(d_v_values)) & 15) == 0,
               "KvCacheAppend: value buffers must be 16-byte aligned");
   KvSource src{{d_k, d_v}, {k_token_stride, v_token_stride}, {k_head_stride, v_head_stride},
                {d_k_values, d_v_values},
                {vec(d_k, k_token_stride, k_head_stride), vec(d_v, v_token_stride, v_head_stride)}};
-  const dim3 grid(item_grid(w.tokens * c.heads * (c.dim / 64) * 2));
+  int parts, per;
+  token_parts(c, w, &parts, &per);
+  const dim3 grid((unsigned)((w.tokens * 2 * parts + 3) / 4));
   cudaStream_t s = as_stream(stream);
   ICX_FLOAT_DISPATCH(type,
-                     ICX_CUDA(launch_pdl(ICX_KV_DISPATCH(kv_append_kernel), grid, dim3(256), 0, s, c, w, src)));
+                     ICX_CUDA(launch_pdl(ICX_KV_DISPATCH(kv_append_kernel), grid, dim3(128), 0, s, c, w, src, parts, per)));
   return ICX_OK;
 }
 
@@ -325,9 +449,11 @@ extern "C" int icx_kv_cache_read(void* stream, const icx_kv_cache* cache, const 
   ICX_REQUIRE(((reinterpret_cast<uintptr_t>(d_k) | reinterpret_cast<uintptr_t>(d_v)) & 15) == 0,
               "KvCacheRead: output buffers must be 16-byte aligned");
   if (w.tokens == 0 || w.batch == 0) return ICX_OK;
-  const dim3 grid(item_grid(w.tokens * c.heads * (c.dim / 64) * 2));
+  int parts, per;
+  token_parts(c, w, &parts, &per);
+  const dim3 grid((unsigned)((w.tokens * 2 * parts + 3) / 4));
   cudaStream_t s = as_stream(stream);
-  ICX_FLOAT_DISPATCH(type, ICX_CUDA(launch_pdl(ICX_KV_DISPATCH(kv_read_kernel), grid, dim3(256), 0, s, c, w,
-                                               static_cast<T*>(d_k), static_cast<T*>(d_v))));
+  ICX_FLOAT_DISPATCH(type, ICX_CUDA(launch_pdl(ICX_KV_DISPATCH(kv_read_kernel), grid, dim3(128), 0, s, c, w,
+                                               static_cast<T*>(d_k), static_cast<T*>(d_v), parts, per)));
   return ICX_OK;
 }
