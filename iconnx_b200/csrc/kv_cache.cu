@@ -69,12 +69,14 @@ __device__ __forceinline__ uint32_t bf16_up(float x) {     // finite x >= 0
   return (u >> 16) + ((u & 0xffffu) ? 1u : 0u);
 }
 
-// Low end and scale of a group's range [mn, mx] (finite).  The quotient
-// (mx - lo) / L is bounded from above in 64 bits, rounded up to bf16, and the
-// bf16 below is taken instead if it is already enough: no division, and the
-// result is the exact quotient rounded up.
+// Low end and scale of a group's range [mn, mx] (finite).  t bounds the
+// quotient (mx - lo) / L from above and is rounded up to bf16; the bf16 below
+// is taken instead if it is already enough: below * L is exact, and with the
+// difference rounded up, "difference <= below * L" decides exactly (an f32 is
+// not below the exact difference if and only if it is not below that
+// difference rounded up).  Ranges that pass f32 are done in 64 bits.
 template <int BITS>
-__device__ __forceinline__ uint32_t group_params(float mn, float mx) {
+__device__ __noinline__ uint32_t group_params_wide(float mn, float mx) {
   constexpr int L = (1 << BITS) - 1;
   const uint32_t lo = bf16_down(mn);
   // (not negative: a maximum below the lowest finite bf16 gives s = 0)
@@ -84,6 +86,17 @@ __device__ __forceinline__ uint32_t group_params(float mn, float mx) {
     const double below = (double)__uint_as_float((s - 1) << 16);
     if (range <= below * L) --s;
   }
+  return s | (lo << 16);
+}
+
+template <int BITS>
+__device__ __forceinline__ uint32_t group_params(float mn, float mx) {
+  constexpr int L = (1 << BITS) - 1;
+  if (fmaxf(fabsf(mn), fabsf(mx)) > 1e38f) return group_params_wide<BITS>(mn, mx);
+  const uint32_t lo = bf16_down(mn);
+  const float range = __fsub_ru(mx, __uint_as_float(lo << 16));
+  uint32_t s = bf16_up(__fmul_ru(range, (float)((1.0 + 1e-6) / L)));
+  if (s > 0 && range <= __uint_as_float((s - 1) << 16) * (float)L) --s;
   return s | (lo << 16);
 }
 
@@ -100,34 +113,45 @@ __device__ __noinline__ float code_near_half(float x, float lo, float s, float u
   return fminf(c, (float)((1 << BITS) - 1));
 }
 
+// The codes, each on the bits of kRound (the code in the low byte), and as
+// floats.
+constexpr float kRound = 12582912.0f;   // 1.5 * 2^23: adding it rounds to an integer (half to even)
+
 template <int BITS>
 __device__ __forceinline__ void group_codes(const float (&x)[8], float lo, float s, bool finite, uint32_t (&code)[8],
                                             float (&c)[8]) {
-  constexpr float L = (float)((1 << BITS) - 1);
-  constexpr float kRound = 12582912.0f;   // adding it rounds to an integer (half to even)
-  if (finite && s >= 1e-36f && s <= 1e36f) {
+  if (finite && s >= 1e-36f && s <= 1e36f && lo > -3e38f) {
+    // here lo <= x <= lo + L s, so that the quotient needs no clamp
     const float inv = __frcp_rn(s);
     float worst = 0.0f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const float u = fminf(fmaxf((x[k] - lo) * inv, 0.0f), L);
-      c[k] = __fsub_rn(__fadd_rn(u, kRound), kRound);
+      const float u = (x[k] - lo) * inv, r = __fadd_rn(u, kRound);
+      c[k] = __fsub_rn(r, kRound);
       worst = fmaxf(worst, fabsf(u - c[k]));
+      code[k] = __float_as_uint(r);
     }
     if (worst > 0.4998f) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float u = fminf(fmaxf((x[k] - lo) * inv, 0.0f), L);
+        const float u = (x[k] - lo) * inv;
         if (fabsf(u - c[k]) > 0.4998f) c[k] = code_near_half<BITS>(x[k], lo, s, u);
+        code[k] = __float_as_uint(c[k] + kRound);
       }
     }
   } else {
+    constexpr float L = (float)((1 << BITS) - 1);
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
+    for (int k = 0; k < 8; ++k) {
       c[k] = finite && s > 0.0f ? (float)fmin(fmax(rint(((double)x[k] - (double)lo) / (double)s), 0.0), (double)L) : 0.0f;
+      code[k] = __float_as_uint(c[k] + kRound);
+    }
   }
-#pragma unroll
-  for (int k = 0; k < 8; ++k) code[k] = __float_as_uint(c[k] + 8388608.0f) & (uint32_t)((1 << BITS) - 1);
+}
+
+// The low bytes of four words.
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
 // One block of 64 dimensions: eight lanes (l = 0..7) of eight consecutive
@@ -143,7 +167,7 @@ __device__ __forceinline__ void store_block(uint8_t* row, int token, int which, 
     if (valid) *reinterpret_cast<uint32_t*>(row + at) = w;
   };
   if (which == 0) {
-    uint32_t a = c[0] | (c[1] << 16) | (c[2] << 8) | (c[3] << 24), b = c[4] | (c[5] << 16) | (c[6] << 8) | (c[7] << 24);
+    uint32_t a = low_bytes(c[0], c[2], c[1], c[3]), b = low_bytes(c[4], c[6], c[5], c[7]);
     if (BITS == 4) {
       // words of both quarters need steps 2n and 2n+1, which are lanes l and l ^ 2
       a <<= 4 * (j & 1);
@@ -157,8 +181,7 @@ __device__ __forceinline__ void store_block(uint8_t* row, int token, int which, 
   } else if (BITS == 4) {
     // byte i: chunk 4 odd + i, codes 2j and 2j+1; a 4 x 4 byte transposition
     // over the lanes j leaves lane j with the word of chunk 4 odd + j
-    uint32_t u = (c[0] | (c[1] << 4)) | (c[2] << 8) | (c[3] << 12) | (c[4] << 16) | (c[5] << 20) | (c[6] << 24) |
-                 (c[7] << 28);
+    uint32_t u = low_bytes(c[0], c[2], c[4], c[6]) | (low_bytes(c[1], c[3], c[5], c[7]) << 4);
     uint32_t v = __shfl_xor_sync(0xffffffffu, u, 2);
     u = (j & 1) ? __byte_perm(v, u, 0x7351) : __byte_perm(u, v, 0x6240);
     v = __shfl_xor_sync(0xffffffffu, u, 4);
@@ -167,7 +190,7 @@ __device__ __forceinline__ void store_block(uint8_t* row, int token, int which, 
   } else {
     // half words of chunks 4 odd + {0,1} and {2,3}; lanes j and j ^ 1 exchange
     // so that each holds whole words of two chunks
-    const uint32_t a = c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24), b = c[4] | (c[5] << 8) | (c[6] << 16) | (c[7] << 24);
+    const uint32_t a = low_bytes(c[0], c[1], c[2], c[3]), b = low_bytes(c[4], c[5], c[6], c[7]);
     const uint32_t other = __shfl_xor_sync(0xffffffffu, (j & 1) ? a : b, 2);
     const uint32_t lo = (j & 1) ? other : a, hi = (j & 1) ? b : other;
     const int g = 4 * odd + 2 * (j & 1), w = block * 2 + (j >> 1);
@@ -229,6 +252,18 @@ __device__ __forceinline__ void block_codes(int which, int l, const uint32_t (&w
   }
 }
 
+// Minimum and maximum that a NaN passes through.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 struct KvSource {
   const void* x[2];
   int64_t token_stride[2], head_stride[2];
@@ -236,35 +271,44 @@ struct KvSource {
   int vec[2];        // eight elements can be read in 16-byte accesses
 };
 
-// A warp takes one token's K or V: `per` blocks of 64 dimensions of its
-// heads, four at a time, `U` fours in flight.  The token's sequence and page
-// are looked up once.
-struct TokenPart {
-  int64_t token, row0;   // row0: cache row of head 0
-  int which, from, to;   // blocks
-  int pos;
-  bool valid;
+// A warp takes K or V of `run` consecutive tokens (at most 32): `per` blocks of
+// 64 dimensions of their heads, four at a time, several fours in flight.  Lane
+// i looks up the sequence and page of token i, all at once, since each lookup
+// is a chain of dependent loads.
+struct WarpPart {
+  int64_t token0, row0;   // row0: this lane's token's cache row of head 0
+  int tokens, which, from, to;
+  int pos;                // this lane's token's position, or -1: nothing to do
 };
 
-__device__ __forceinline__ TokenPart token_part(const KvView& c, const KvTokens& w, int64_t item, int parts, int per,
-                                                int blocks) {
-  TokenPart p;
-  const int part = (int)(item % parts);
-  p.which = (int)((item / parts) & 1);
-  p.token = item / (2 * parts);
-  p.from = part * per;
-  p.to = min(p.from + per, blocks);
-  int b;
-  p.pos = token_position(w, p.token, &b);
-  p.valid = p.pos >= 0;
+struct Parts {
+  int run, parts, per;
+  int64_t items;
+};
+
+__device__ __forceinline__ WarpPart warp_part(const KvView& c, const KvTokens& w, const Parts& n, int64_t item,
+                                              int blocks) {
+  WarpPart p;
+  const int lane = threadIdx.x & 31;
+  const int part = (int)(item % n.parts);
+  p.which = (int)((item / n.parts) & 1);
+  p.token0 = item / (2 * n.parts) * n.run;
+  p.tokens = (int)min((int64_t)n.run, w.tokens - p.token0);
+  p.from = part * n.per;
+  p.to = min(p.from + n.per, blocks);
+  p.pos = -1;
   p.row0 = 0;
-  if (p.valid) {
-    const int64_t page = kv_page(c, w, b, p.pos);
-    if (page < 0) {
-      p.valid = false;
-      record_status(ICX_DEVICE_BAD_PAGE);
-    } else {
-      p.row0 = kv_row(c, page, 0, p.pos);
+  if (lane < p.tokens) {
+    int b;
+    p.pos = token_position(w, p.token0 + lane, &b);
+    if (p.pos >= 0) {
+      const int64_t page = kv_page(c, w, b, p.pos);
+      if (page < 0) {
+        p.pos = -1;
+        record_status(ICX_DEVICE_BAD_PAGE);
+      } else {
+        p.row0 = kv_row(c, page, 0, p.pos);
+      }
     }
   }
   return p;
@@ -292,17 +336,20 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
 template <typename T, int BITS, int D>
 __global__ void __launch_bounds__(128)
     kv_append_kernel(const __grid_constant__ KvView c, const __grid_constant__ KvTokens w,
-                     const __grid_constant__ KvSource src, int parts, int per) {
+                     const __grid_constant__ KvSource src, const Parts n) {
   pdl_wait();
   pdl_trigger();
   constexpr int kPerHead = D / 64, U = 2;
   const int blocks = c.heads * kPerHead;
   const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (item >= w.tokens * 2 * parts) return;
-  const TokenPart p = token_part(c, w, item, parts, per, blocks);
-  if (!p.valid) return;
+  if (item >= n.items) return;
+  const WarpPart p = warp_part(c, w, n, item, blocks);
   const int l = threadIdx.x & 7, sub = (threadIdx.x >> 3) & 3;
-  const T* x0 = static_cast<const T*>(src.x[p.which]) + p.token * src.token_stride[p.which];
+  for (int i0 = 0; i0 < p.tokens; ++i0) {
+  const int pos = __shfl_sync(0xffffffffu, p.pos, i0);
+  const int64_t row0 = __shfl_sync(0xffffffffu, p.row0, i0), token = p.token0 + i0;
+  if (pos < 0) continue;
+  const T* x0 = static_cast<const T*>(src.x[p.which]) + token * src.token_stride[p.which];
   for (int b0 = p.from; b0 < p.to; b0 += 4 * U) {
     float x[U][8];
 #pragma unroll
@@ -319,60 +366,62 @@ __global__ void __launch_bounds__(128)
       const int b = b0 + 4 * i + sub, head = b / kPerHead, block = b % kPerHead;
       const bool valid = b < p.to;
       float mn = x[i][0], mx = x[i][0];
-      uint32_t peak = 0;   // |x| by its bits: NaN and infinity are at the top
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        mn = fminf(mn, x[i][k]);
-        mx = fmaxf(mx, x[i][k]);
-        peak = max(peak, __float_as_uint(fabsf(x[i][k])));
+      for (int k = 1; k < 8; ++k) {
+        mn = min_nan(mn, x[i][k]);
+        mx = max_nan(mx, x[i][k]);
       }
       for (int o = 1; o < c.group / 8; o <<= 1) {
-        mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, o));
+        mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+        mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
       }
-      const bool finite = peak < 0x7f800000u;
+      const bool finite = fabsf(mn) < INFINITY && fabsf(mx) < INFINITY;
       const uint32_t prm = finite ? group_params<BITS>(mn, mx) : 0x7fc07fc0u;
       const float s = param_scale(prm), lo = param_low(prm);
       uint32_t code[8] = {};
       float v[8];
       group_codes<BITS>(x[i], lo, s, finite, code, v);
-      const int64_t row = p.row0 + ((int64_t)(valid ? head : 0) << c.page_shift);
-      store_block<BITS, D>(c.codes[p.which] + row * (D * BITS / 8), p.pos, p.which, block, l, code, valid);
+      const int64_t row = row0 + ((int64_t)(valid ? head : 0) << c.page_shift);
+      store_block<BITS, D>(c.codes[p.which] + row * (D * BITS / 8), pos, p.which, block, l, code, valid);
       if (valid) {
         const int d = block * 64 + 8 * l;
         if (8 * l % c.group == 0) c.params[p.which][row * (D / c.group) + d / c.group] = prm;
         if (src.values[p.which]) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) v[k] = fmaf(v[k], s, lo);
-          store8<T>(static_cast<T*>(src.values[p.which]) + (p.token * c.heads + head) * D + d, v);
+          store8<T>(static_cast<T*>(src.values[p.which]) + (token * c.heads + head) * D + d, v);
         }
       }
     }
+  }
   }
 }
 
 template <typename T, int BITS, int D>
 __global__ void __launch_bounds__(128)
-    kv_read_kernel(const __grid_constant__ KvView c, const __grid_constant__ KvTokens w, T* k_out, T* v_out, int parts,
-                   int per) {
+    kv_read_kernel(const __grid_constant__ KvView c, const __grid_constant__ KvTokens w, T* k_out, T* v_out,
+                   const Parts n) {
   pdl_wait();
   pdl_trigger();
   constexpr int kPerHead = D / 64, U = 4;
   const int blocks = c.heads * kPerHead;
   const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (item >= w.tokens * 2 * parts) return;
-  const TokenPart p = token_part(c, w, item, parts, per, blocks);
+  if (item >= n.items) return;
+  const WarpPart p = warp_part(c, w, n, item, blocks);
   T* out = p.which ? v_out : k_out;
-  if (!p.valid || !out) return;
+  if (!out) return;
   const int l = threadIdx.x & 7, sub = (threadIdx.x >> 3) & 3;
+  for (int i0 = 0; i0 < p.tokens; ++i0) {
+  const int pos = __shfl_sync(0xffffffffu, p.pos, i0);
+  const int64_t row0 = __shfl_sync(0xffffffffu, p.row0, i0), token = p.token0 + i0;
+  if (pos < 0) continue;
   for (int b0 = p.from; b0 < p.to; b0 += 4 * U) {
     uint32_t words[U][2], prm[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const int b = min(b0 + 4 * i + sub, p.to - 1), block = b % kPerHead;
-      const int64_t row = p.row0 + ((int64_t)(b / kPerHead) << c.page_shift);
-      load_block_words<BITS, D>(c.codes[p.which] + row * (D * BITS / 8), p.pos, p.which, block, l, words[i]);
+      const int64_t row = row0 + ((int64_t)(b / kPerHead) << c.page_shift);
+      load_block_words<BITS, D>(c.codes[p.which] + row * (D * BITS / 8), pos, p.which, block, l, words[i]);
       prm[i] = c.params[p.which][row * (D / c.group) + (block * 64 + 8 * l) / c.group];
     }
 #pragma unroll
@@ -385,19 +434,25 @@ __global__ void __launch_bounds__(128)
 #pragma unroll
       for (int k = 0; k < 8; ++k)   // a code below 2^23 on 2^23's bits is 2^23 + code
         v[k] = fmaf(__uint_as_float(0x4b000000u | code[k]) - 8388608.0f, param_scale(prm[i]), param_low(prm[i]));
-      if (b < p.to) store8<T>(out + (p.token * c.heads + b / kPerHead) * D + b % kPerHead * 64 + 8 * l, v);
+      if (b < p.to) store8<T>(out + (token * c.heads + b / kPerHead) * D + b % kPerHead * 64 + 8 * l, v);
     }
+  }
   }
 }
 
-// Warps per token and side: one, unless there are too few tokens to fill the
-// GPU (then up to one per four blocks).
-static void token_parts(const KvView& c, const KvTokens& w, int* parts, int* per) {
+// Enough warps to fill the GPU: with few tokens their heads are divided (down
+// to four blocks per warp), with many a warp takes up to eight tokens.
+static Parts make_parts(const KvView& c, const KvTokens& w) {
   const int blocks = c.heads * (c.dim / 64), fours = (blocks + 3) / 4;
-  int n = 1;
-  while (n < fours && w.tokens * 2 * n < 148 * 16) ++n;
-  *per = (fours + n - 1) / n * 4;
-  *parts = (blocks + *per - 1) / *per;
+  constexpr int64_t kWarps = 148 * 32;
+  Parts n{1, 1, 0, 0};
+  while (n.parts < fours && w.tokens * 2 * n.parts < kWarps) ++n.parts;
+  n.per = (fours + n.parts - 1) / n.parts * 4;
+  n.parts = (blocks + n.per - 1) / n.per;
+  if (n.parts == 1)
+    while (n.run < 8 && w.tokens * 2 / (n.run * 2) >= kWarps) n.run *= 2;
+  n.items = (w.tokens + n.run - 1) / n.run * 2 * n.parts;
+  return n;
 }
 
 #define ICX_KV_DISPATCH(kernel)                                                                        \
@@ -430,12 +485,11 @@ extern "C" int icx_kv_cache_append(void* stream, const icx_kv_cache* cache, cons
   KvSource src{{d_k, d_v}, {k_token_stride, v_token_stride}, {k_head_stride, v_head_stride},
                {d_k_values, d_v_values},
                {vec(d_k, k_token_stride, k_head_stride), vec(d_v, v_token_stride, v_head_stride)}};
-  int parts, per;
-  token_parts(c, w, &parts, &per);
-  const dim3 grid((unsigned)((w.tokens * 2 * parts + 3) / 4));
+  const Parts n = make_parts(c, w);
+  const dim3 grid((unsigned)((n.items + 3) / 4));
   cudaStream_t s = as_stream(stream);
   ICX_FLOAT_DISPATCH(type,
-                     ICX_CUDA(launch_pdl(ICX_KV_DISPATCH(kv_append_kernel), grid, dim3(128), 0, s, c, w, src, parts, per)));
+                     ICX_CUDA(launch_pdl(ICX_KV_DISPATCH(kv_append_kernel), grid, dim3(128), 0, s, c, w, src, n)));
   return ICX_OK;
 }
 
@@ -449,11 +503,10 @@ extern "C" int icx_kv_cache_read(void* stream, const icx_kv_cache* cache, const 
   ICX_REQUIRE(((reinterpret_cast<uintptr_t>(d_k) | reinterpret_cast<uintptr_t>(d_v)) & 15) == 0,
               "KvCacheRead: output buffers must be 16-byte aligned");
   if (w.tokens == 0 || w.batch == 0) return ICX_OK;
-  int parts, per;
-  token_parts(c, w, &parts, &per);
-  const dim3 grid((unsigned)((w.tokens * 2 * parts + 3) / 4));
+  const Parts n = make_parts(c, w);
+  const dim3 grid((unsigned)((n.items + 3) / 4));
   cudaStream_t s = as_stream(stream);
   ICX_FLOAT_DISPATCH(type, ICX_CUDA(launch_pdl(ICX_KV_DISPATCH(kv_read_kernel), grid, dim3(128), 0, s, c, w,
-                                               static_cast<T*>(d_k), static_cast<T*>(d_v), parts, per)));
+                                               static_cast<T*>(d_k), static_cast<T*>(d_v), n)));
   return ICX_OK;
 }

@@ -69,6 +69,32 @@ __device__ __forceinline__ void token_codes(const float (&x)[N], float s, float 
   }
 }
 
+// Largest |x| by its bits: f32 bits, or for 16-bit types the larger of both
+// half words, which peak_f32_bits turns into the f32 value's.
+template <typename T, int E>
+__device__ __forceinline__ uint32_t vec_peak(const Vec<T, E>& v) {
+  uint32_t p = 0;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) p = max(p, __float_as_uint(fabsf(v.v[i])));
+  } else if constexpr (E == 1) {
+    p = *reinterpret_cast<const uint16_t*>(&v.v[0]) & 0x7fffu;
+  } else {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&v);
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+    p = max(m >> 16, m & 0xffffu);
+  }
+  return p;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t peak_f32_bits(uint32_t p) {
+  if constexpr (sizeof(T) == 4) return p;
+  const uint16_t h = (uint16_t)p;
+  return __float_as_uint(to_f32(*reinterpret_cast<const T*>(&h)));
+}
+
 // W warps per row; a thread holds V accesses of E values (E = 16 bytes' worth,
 // or 1 where the row cannot be read in 16-byte pieces).
 template <typename T, int W, int V, int E>
@@ -83,22 +109,17 @@ __global__ void __launch_bounds__(256)
   const int row = blockIdx.x * (256 / kThreads) + threadIdx.x / kThreads;
   const bool here = row < rows;
   const T* src = x + (size_t)(here ? row : 0) * stride;
-  float v[V][E];
+  Vec<T, E> v[V];   // as they are: half the registers of their f32 values
   uint32_t peak = 0;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int at = (i * kThreads + t) * E;
-    if (here && at < cols) {
-      load_f32<T, E>(src + at, v[i], true);
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) v[i][e] = 0.0f;
-    }
+    v[i] = Vec<T, E>{};
+    if (here && at < cols) v[i] = *reinterpret_cast<const Vec<T, E>*>(src + at);
   }
 #pragma unroll
-  for (int i = 0; i < V; ++i)
-#pragma unroll
-    for (int e = 0; e < E; ++e) peak = max(peak, __float_as_uint(fabsf(v[i][e])));
+  for (int i = 0; i < V; ++i) peak = max(peak, vec_peak(v[i]));
+  peak = peak_f32_bits<T>(peak);
   peak = __reduce_max_sync(0xffffffffu, peak);
   if (W > 1) {
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = peak;
@@ -116,7 +137,10 @@ __global__ void __launch_bounds__(256)
     const int at = (i * kThreads + t) * E;
     if (at >= cols) break;
     uint32_t c[(E + 3) / 4];
-    token_codes<E>(v[i], s, inv, c);
+    float f[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] = to_f32(v[i].v[e]);
+    token_codes<E>(f, s, inv, c);
     if (E == 8) *reinterpret_cast<uint2*>(out + at) = make_uint2(c[0], c[(E + 3) / 4 - 1]);
     else if (E == 4) *reinterpret_cast<uint32_t*>(out + at) = c[0];
     else out[at] = (int8_t)c[0];
