@@ -42,7 +42,7 @@ int kv_views(const char* what, const icx_kv_cache* c, const icx_kv_tokens* w, Kv
   }
   *view = KvView{{static_cast<uint8_t*>(c->k_codes), static_cast<uint8_t*>(c->v_codes)},
                  {static_cast<uint32_t*>(c->k_params), static_cast<uint32_t*>(c->v_params)},
-                 c->pages, shift, c->kv_heads, c->head_dim, c->bits, c->group};
+                 c->pages, shift, c->kv_heads, c->head_dim, c->bits, c->group, c->group == 32 ? 5 : 6};
   *tokens = KvTokens{w->d_page_table, w->d_seq_lens, w->d_cu_tokens, w->tokens, w->batch, w->table_width};
   return ICX_OK;
 }
@@ -100,43 +100,53 @@ __device__ __forceinline__ uint32_t group_params(float mn, float mx) {
   return s | (lo << 16);
 }
 
-// rte((x - lo) / s) clamped to [0, L], as integers and as floats.  An f32
-// quotient is off by less than 5e-5 (three roundings at most 255); where it is
-// within 2e-4 of a half, x is compared with the midpoint in 64 bits ((k + 1/2) s
-// is exact).  Scales whose reciprocal or range may not be finite take the 64-bit
-// quotient.
-template <int BITS>
-__device__ __noinline__ float code_near_half(float x, float lo, float s, float u) {
-  const float k = floorf(u);
-  const double d = ((double)x - (double)lo) - (double)k * (double)s - 0.5 * (double)s;
-  const float c = d > 0.0 ? k + 1.0f : d < 0.0 ? k : 2.0f * rintf(0.5f * k + 0.25f);
-  return fminf(c, (float)((1 << BITS) - 1));
+// rte((x - lo) / s) clamped to [0, L].  An f32 quotient is off by less than 7e-5
+// (roundings of 2^-24, 2^-23 and 2^-24 at most at 255); where it is within 2e-4
+// of a half, x is compared with the midpoint lo + m, m = (k + 1/2) s, in f32
+// alone: m is exact (9 + 8 bits), t + e = lo + m exactly, and x - t is exact
+// where x and t are within a factor of two, while otherwise t is all but
+// cancelled, so that e = 0 and the sign of x - t is what counts.
+__device__ __forceinline__ float code_near_half(float x, float lo, float s, float u) {
+  const float k = floorf(u), m = (k + 0.5f) * s;
+  const float t = __fadd_rn(lo, m), b = __fsub_rn(t, lo);
+  const float e = __fadd_rn(__fsub_rn(lo, __fsub_rn(t, b)), __fsub_rn(m, b));
+  const float d = __fsub_rn(x, t);
+  return d > e ? k + 1.0f : d < e ? k : 2.0f * rintf(0.5f * k + 0.25f);
 }
 
 // The codes, each on the bits of kRound (the code in the low byte), and as
 // floats.
 constexpr float kRound = 12582912.0f;   // 1.5 * 2^23: adding it rounds to an integer (half to even)
 
+// Scales whose reciprocal or range may not be finite take the 64-bit quotient.
 template <int BITS>
 __device__ __forceinline__ void group_codes(const float (&x)[8], float lo, float s, bool finite, uint32_t (&code)[8],
                                             float (&c)[8]) {
   if (finite && s >= 1e-36f && s <= 1e36f && lo > -3e38f) {
     // here lo <= x <= lo + L s, so that the quotient needs no clamp
-    const float inv = __frcp_rn(s);
-    float worst = 0.0f;
+    float inv, worst = 0.0f;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    const F2 lo2 = f2(-lo, -lo), inv2 = f2(inv, inv), up = f2(kRound, kRound), down = f2(-kRound, -kRound);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float u = (x[k] - lo) * inv, r = __fadd_rn(u, kRound);
-      c[k] = __fsub_rn(r, kRound);
-      worst = fmaxf(worst, fabsf(u - c[k]));
-      code[k] = __float_as_uint(r);
+    for (int k = 0; k < 8; k += 2) {
+      const F2 u = f2_mul(f2_add(f2(x[k], x[k + 1]), lo2), inv2), r = f2_add(u, up), n = f2_add(r, down);
+      float r0, r1, u0, u1;
+      f2_split(r, r0, r1);
+      f2_split(u, u0, u1);
+      f2_split(n, c[k], c[k + 1]);
+      code[k] = __float_as_uint(r0);
+      code[k + 1] = __float_as_uint(r1);
+      worst = fmaxf(worst, fmaxf(fabsf(u0 - c[k]), fabsf(u1 - c[k + 1])));
     }
     if (worst > 0.4998f) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < 8; ++k) {   // few lanes have one, and seldom the same: a branch for each
         const float u = (x[k] - lo) * inv;
-        if (fabsf(u - c[k]) > 0.4998f) c[k] = code_near_half<BITS>(x[k], lo, s, u);
-        code[k] = __float_as_uint(c[k] + kRound);
+        const bool near = fabsf(u - c[k]) > 0.4998f;
+        if (__any_sync(__activemask(), near)) {
+          if (near) c[k] = fminf(code_near_half(x[k], lo, s, u), (float)((1 << BITS) - 1));
+          code[k] = __float_as_uint(c[k] + kRound);
+        }
       }
     }
   } else {
@@ -219,18 +229,24 @@ __device__ __forceinline__ void load_block_words(const uint8_t* row, int token, 
     w[1] = get(v_word_at<ROW>(token, g + 1, n));
   }
 }
+// Eight codes, each on the bits of 2^23 (2^23 + code as an f32).
+constexpr uint32_t kCodeOne = 0x4b000000u;
+
+__device__ __forceinline__ uint32_t code_at(uint32_t bytes, int i) {   // byte i of a word
+  return __byte_perm(bytes, kCodeOne, 0x7440 + i);
+}
+
 template <int BITS>
 __device__ __forceinline__ void block_codes(int which, int l, const uint32_t (&w)[2], uint32_t (&c)[8]) {
   const int j = l >> 1;
-  constexpr uint32_t mask = (1u << BITS) - 1;
   if (which == 0) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint32_t u = BITS == 4 ? w[h] >> (4 * (j & 1)) : w[h];
-      c[4 * h] = u & mask;
-      c[4 * h + 1] = (u >> 16) & mask;
-      c[4 * h + 2] = (u >> 8) & mask;
-      c[4 * h + 3] = (u >> 24) & mask;
+      const uint32_t u = BITS == 4 ? (w[h] >> (4 * (j & 1))) & 0x0f0f0f0fu : w[h];
+      c[4 * h] = code_at(u, 0);
+      c[4 * h + 1] = code_at(u, 2);
+      c[4 * h + 2] = code_at(u, 1);
+      c[4 * h + 3] = code_at(u, 3);
     }
   } else if (BITS == 4) {
     uint32_t u = w[0];
@@ -238,16 +254,20 @@ __device__ __forceinline__ void block_codes(int which, int l, const uint32_t (&w
     u = (j & 1) ? __byte_perm(v, u, 0x7351) : __byte_perm(u, v, 0x6240);
     v = __shfl_xor_sync(0xffffffffu, u, 4);
     u = (j & 2) ? __byte_perm(v, u, 0x7632) : __byte_perm(u, v, 0x5410);
+    const uint32_t even = u & 0x0f0f0f0fu, odd = (u >> 4) & 0x0f0f0f0fu;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = (u >> (4 * i)) & 15u;
+    for (int i = 0; i < 4; ++i) {
+      c[2 * i] = code_at(even, i);
+      c[2 * i + 1] = code_at(odd, i);
+    }
   } else {
     const uint32_t lo = __byte_perm(w[0], w[1], 0x5410), hi = __byte_perm(w[0], w[1], 0x7632);
     const uint32_t other = __shfl_xor_sync(0xffffffffu, (j & 1) ? lo : hi, 2);
     const uint32_t a = (j & 1) ? other : lo, b = (j & 1) ? hi : other;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      c[i] = (a >> (8 * i)) & 255u;
-      c[4 + i] = (b >> (8 * i)) & 255u;
+      c[i] = code_at(a, i);
+      c[4 + i] = code_at(b, i);
     }
   }
 }
@@ -334,123 +354,128 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
 }
 
 template <typename T, int BITS, int D>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(128, 8)
     kv_append_kernel(const __grid_constant__ KvView c, const __grid_constant__ KvTokens w,
                      const __grid_constant__ KvSource src, const Parts n) {
   pdl_wait();
   pdl_trigger();
-  constexpr int kPerHead = D / 64, U = 2;
-  const int blocks = c.heads * kPerHead;
+  constexpr int kPerHead = D / 64, ROW = D * BITS / 8;
   const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (item >= n.items) return;
-  const WarpPart p = warp_part(c, w, n, item, blocks);
+  const WarpPart p = warp_part(c, w, n, item, c.heads * kPerHead);
   const int l = threadIdx.x & 7, sub = (threadIdx.x >> 3) & 3;
-  for (int i0 = 0; i0 < p.tokens; ++i0) {
-  const int pos = __shfl_sync(0xffffffffu, p.pos, i0);
-  const int64_t row0 = __shfl_sync(0xffffffffu, p.row0, i0), token = p.token0 + i0;
-  if (pos < 0) continue;
-  const T* x0 = static_cast<const T*>(src.x[p.which]) + token * src.token_stride[p.which];
-  for (int b0 = p.from; b0 < p.to; b0 += 4 * U) {
-    float x[U][8];
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int b = b0 + 4 * i + sub;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) x[i][k] = 0.0f;
-      if (b < p.to)
-        load8<T>(x0 + (b / kPerHead) * src.head_stride[p.which] + b % kPerHead * 64 + 8 * l, x[i], src.vec[p.which]);
-    }
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      if (b0 + 4 * i >= p.to) break;
-      const int b = b0 + 4 * i + sub, head = b / kPerHead, block = b % kPerHead;
-      const bool valid = b < p.to;
-      float mn = x[i][0], mx = x[i][0];
+  const bool vec = src.vec[p.which] != 0, store_group = (8 * l & (c.group - 1)) == 0;
+  const int64_t x_step = src.token_stride[p.which], v_step = (int64_t)c.heads * D;
+  for (int b0 = p.from; b0 < p.to; b0 += 4) {
+    // this lane's place in every token
+    const int b = min(b0 + sub, p.to - 1), head = b / kPerHead, block = b % kPerHead, d = block * 64 + 8 * l;
+    const bool valid = b0 + sub < p.to;
+    const T* x_at = static_cast<const T*>(src.x[p.which]) + p.token0 * x_step + head * src.head_stride[p.which] + d;
+    T* v_at = static_cast<T*>(src.values[p.which]);
+    const bool values = valid && v_at != nullptr;
+    v_at += (p.token0 * c.heads + head) * D + d;
+    const int64_t head_row = (int64_t)head << c.page_shift;
+    uint8_t* codes = c.codes[p.which] + head_row * ROW;
+    uint32_t* params = c.params[p.which] + (head_row * D + d >> c.group_shift);
+    for (int i = 0; i < p.tokens; ++i, x_at += x_step, v_at += v_step) {
+      const int pos = __shfl_sync(0xffffffffu, p.pos, i);
+      const int64_t row0 = __shfl_sync(0xffffffffu, p.row0, i);
+      if (pos < 0) continue;
+      float x[8];
+      load8<T>(x_at, x, vec);
+      float mn = x[0], mx = x[0];
 #pragma unroll
       for (int k = 1; k < 8; ++k) {
-        mn = min_nan(mn, x[i][k]);
-        mx = max_nan(mx, x[i][k]);
+        mn = min_nan(mn, x[k]);
+        mx = max_nan(mx, x[k]);
       }
-      for (int o = 1; o < c.group / 8; o <<= 1) {
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) {
+        if (o == 4 && c.group == 32) break;
         mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, o));
         mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
       }
       const bool finite = fabsf(mn) < INFINITY && fabsf(mx) < INFINITY;
       const uint32_t prm = finite ? group_params<BITS>(mn, mx) : 0x7fc07fc0u;
       const float s = param_scale(prm), lo = param_low(prm);
-      uint32_t code[8] = {};
+      uint32_t code[8];
       float v[8];
-      group_codes<BITS>(x[i], lo, s, finite, code, v);
-      const int64_t row = row0 + ((int64_t)(valid ? head : 0) << c.page_shift);
-      store_block<BITS, D>(c.codes[p.which] + row * (D * BITS / 8), pos, p.which, block, l, code, valid);
-      if (valid) {
-        const int d = block * 64 + 8 * l;
-        if (8 * l % c.group == 0) c.params[p.which][row * (D / c.group) + d / c.group] = prm;
-        if (src.values[p.which]) {
+      group_codes<BITS>(x, lo, s, finite, code, v);
+      store_block<BITS, D>(codes + row0 * ROW, pos, p.which, block, l, code, valid);
+      if (valid && store_group) params[row0 * D >> c.group_shift] = prm;
+      if (values) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] = fmaf(v[k], s, lo);
-          store8<T>(static_cast<T*>(src.values[p.which]) + (token * c.heads + head) * D + d, v);
+        for (int k = 0; k < 8; k += 2) {
+          const F2 y = f2_fma(f2(v[k], v[k + 1]), f2(s, s), f2(lo, lo));
+          f2_split(y, v[k], v[k + 1]);
         }
+        store8<T>(v_at, v);
       }
     }
-  }
   }
 }
 
 template <typename T, int BITS, int D>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(128, 8)
     kv_read_kernel(const __grid_constant__ KvView c, const __grid_constant__ KvTokens w, T* k_out, T* v_out,
                    const Parts n) {
   pdl_wait();
   pdl_trigger();
-  constexpr int kPerHead = D / 64, U = 4;
-  const int blocks = c.heads * kPerHead;
+  constexpr int kPerHead = D / 64, ROW = D * BITS / 8, U = 4;   // tokens in flight
   const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (item >= n.items) return;
-  const WarpPart p = warp_part(c, w, n, item, blocks);
+  const WarpPart p = warp_part(c, w, n, item, c.heads * kPerHead);
   T* out = p.which ? v_out : k_out;
   if (!out) return;
   const int l = threadIdx.x & 7, sub = (threadIdx.x >> 3) & 3;
-  for (int i0 = 0; i0 < p.tokens; ++i0) {
-  const int pos = __shfl_sync(0xffffffffu, p.pos, i0);
-  const int64_t row0 = __shfl_sync(0xffffffffu, p.row0, i0), token = p.token0 + i0;
-  if (pos < 0) continue;
-  for (int b0 = p.from; b0 < p.to; b0 += 4 * U) {
-    uint32_t words[U][2], prm[U];
+  const int64_t step = (int64_t)c.heads * D;
+  for (int b0 = p.from; b0 < p.to; b0 += 4) {
+    const int b = min(b0 + sub, p.to - 1), head = b / kPerHead, block = b % kPerHead, d = block * 64 + 8 * l;
+    const bool valid = b0 + sub < p.to;
+    const int64_t head_row = (int64_t)head << c.page_shift;
+    const uint8_t* codes = c.codes[p.which] + head_row * ROW;
+    const uint32_t* params = c.params[p.which] + (head_row * D + d >> c.group_shift);
+    T* out_at = out + (p.token0 * c.heads + head) * D + d;
+    for (int i0 = 0; i0 < p.tokens; i0 += U, out_at += U * step) {
+      uint32_t words[U][2], prm[U];
+      int pos[U];
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int b = min(b0 + 4 * i + sub, p.to - 1), block = b % kPerHead;
-      const int64_t row = row0 + ((int64_t)(b / kPerHead) << c.page_shift);
-      load_block_words<BITS, D>(c.codes[p.which] + row * (D * BITS / 8), pos, p.which, block, l, words[i]);
-      prm[i] = c.params[p.which][row * (D / c.group) + (block * 64 + 8 * l) / c.group];
+      for (int i = 0; i < U; ++i) {
+        pos[i] = i0 + i < p.tokens ? __shfl_sync(0xffffffffu, p.pos, i0 + i) : -1;
+        const int64_t row0 = __shfl_sync(0xffffffffu, p.row0, (i0 + i) & 31);
+        if (pos[i] < 0) continue;
+        load_block_words<BITS, D>(codes + row0 * ROW, pos[i], p.which, block, l, words[i]);
+        prm[i] = params[row0 * D >> c.group_shift];
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        if (pos[i] < 0) continue;
+        uint32_t code[8];
+        block_codes<BITS>(p.which, l, words[i], code);
+        const float s = param_scale(prm[i]), lo = param_low(prm[i]);
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k += 2) {
+          const F2 q = f2_add(f2(__uint_as_float(code[k]), __uint_as_float(code[k + 1])), f2(-8388608.0f, -8388608.0f));
+          f2_split(f2_fma(q, f2(s, s), f2(lo, lo)), v[k], v[k + 1]);
+        }
+        if (valid) store8<T>(out_at + i * step, v);
+      }
     }
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      if (b0 + 4 * i >= p.to) break;
-      const int b = b0 + 4 * i + sub;
-      uint32_t code[8];
-      block_codes<BITS>(p.which, l, words[i], code);
-      float v[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k)   // a code below 2^23 on 2^23's bits is 2^23 + code
-        v[k] = fmaf(__uint_as_float(0x4b000000u | code[k]) - 8388608.0f, param_scale(prm[i]), param_low(prm[i]));
-      if (b < p.to) store8<T>(out + (token * c.heads + b / kPerHead) * D + b % kPerHead * 64 + 8 * l, v);
-    }
-  }
   }
 }
 
 // Enough warps to fill the GPU: with few tokens their heads are divided (down
-// to four blocks per warp), with many a warp takes up to eight tokens.
+// to four blocks per warp), with many a warp takes up to four tokens.
 static Parts make_parts(const KvView& c, const KvTokens& w) {
   const int blocks = c.heads * (c.dim / 64), fours = (blocks + 3) / 4;
-  constexpr int64_t kWarps = 148 * 32;
+  constexpr int64_t kWarps = 148 * 48;
   Parts n{1, 1, 0, 0};
   while (n.parts < fours && w.tokens * 2 * n.parts < kWarps) ++n.parts;
   n.per = (fours + n.parts - 1) / n.parts * 4;
   n.parts = (blocks + n.per - 1) / n.per;
   if (n.parts == 1)
-    while (n.run < 8 && w.tokens * 2 / (n.run * 2) >= kWarps) n.run *= 2;
+    while (n.run < 4 && w.tokens * 2 / (n.run * 2) >= kWarps) n.run *= 2;
   n.items = (w.tokens + n.run - 1) / n.run * 2 * n.parts;
   return n;
 }

@@ -36,7 +36,7 @@ struct KvView {
   uint8_t* codes[2];    // K, V
   uint32_t* params[2];  // s (bf16) in the low half, lo (bf16) in the high half
   int64_t pages;
-  int page_shift, heads, dim, bits, group;
+  int page_shift, heads, dim, bits, group, group_shift;
 };
 
 struct KvTokens {
