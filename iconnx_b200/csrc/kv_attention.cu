@@ -58,7 +58,8 @@ extern "C" int icx_kv_cache_attention(void* stream, const icx_kv_cache* cache, c
   if (w.tokens == 0 || w.batch == 0) return ICX_OK;
   ICX_REQUIRE(d_q && d_out, "KvCacheAttention: null operand");
   ICX_REQUIRE((reinterpret_cast<uintptr_t>(d_out) & 15) == 0, "KvCacheAttention: out must be 16-byte aligned");
-  const AttendPlan p = plan_attend(c, w, q_heads);
+  const bool prompt = prompt_preferred(c, w, q_heads, type);
+  const AttendPlan p = prompt ? AttendPlan{} : plan_attend(c, w, q_heads);
   if (p.bytes > 0 && (!d_workspace || workspace_bytes < p.bytes)) {
     set_error("KvCacheAttention: workspace %zu bytes < %zu required", d_workspace ? workspace_bytes : 0, p.bytes);
     return ICX_ERR_WORKSPACE;
@@ -77,6 +78,7 @@ extern "C" int icx_kv_cache_attention(void* stream, const icx_kv_cache* cache, c
   a.prefix = static_cast<int64_t*>(d_workspace);
   a.partial = reinterpret_cast<float*>(static_cast<char*>(d_workspace) + p.prefix_bytes);
   cudaStream_t s = as_stream(stream);
+  if (prompt) return launch_prompt(s, c, w, a, type);
   int r = ICX_OK;
   ICX_FLOAT_DISPATCH(type, r = launch_attend<T>(s, c, w, a, p));
   return r;

@@ -756,6 +756,10 @@ struct AttendPlan {
 
 AttendPlan plan_attend(const KvView& c, const KvTokens& w, int q_heads);
 
+// Many rows per sequence: the tensor-memory kernel (kv_prompt.cu).
+bool prompt_preferred(const KvView& c, const KvTokens& w, int q_heads, int type);
+int launch_prompt(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a, int type);
+
 template <typename T>
 int launch_attend(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a, const AttendPlan& p);
 
