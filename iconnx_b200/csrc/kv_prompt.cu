@@ -95,6 +95,12 @@ __device__ __forceinline__ uint4 spread(uint32_t w0, uint32_t w1) {
   return make_uint4(w0 & 0x00ff00ffu, (w0 >> 8) & 0x00ff00ffu, w1 & 0x00ff00ffu, (w1 >> 8) & 0x00ff00ffu);
 }
 
+// All lanes poll: the roles hand over several times per tile, and a lane that
+// sleeps between polls wakes too late for that.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
+}
+
 template <typename T, int D, int BITS>
 __global__ void __launch_bounds__(kPrThreads, 2)
     kv_prompt_kernel(const __grid_constant__ KvView c, const __grid_constant__ KvTokens w,
@@ -250,7 +256,7 @@ __global__ void __launch_bounds__(kPrThreads, 2)
       if (tiles > 0) fetch(0);
       for (int i = 0; i < tiles; ++i) {
         const int st = i & 1;
-        if (ok) ok = mbar_wait_warp(&empty[st], ((i >> 1) & 1) ^ 1, ICX_DEVICE_TIMEOUT_PRODUCER);
+        if (ok) ok = wait_warp(&empty[st], ((i >> 1) & 1) ^ 1, ICX_DEVICE_TIMEOUT_PRODUCER);
         // spread to f16: row = position, piece n at place n ^ (row & 7)
 #pragma unroll
         for (int k = 0; k < G; ++k) {
@@ -407,8 +413,8 @@ __global__ void __launch_bounds__(kPrThreads, 2)
       bool ok = true;
       for (int i = 0; i < tiles; ++i) {
         const int st = i & 1;
-        if (ok) ok = mbar_wait_warp(&full[st], (i >> 1) & 1, ICX_DEVICE_TIMEOUT_EPILOGUE);
-        if (ok) ok = mbar_wait_warp(s_full, i & 1, ICX_DEVICE_TIMEOUT_EPILOGUE);
+        if (ok) ok = wait_warp(&full[st], (i >> 1) & 1, ICX_DEVICE_TIMEOUT_EPILOGUE);
+        if (ok) ok = wait_warp(s_full, i & 1, ICX_DEVICE_TIMEOUT_EPILOGUE);
         if (!ok) break;
         tc_fence_after();
         const float* prm = s_p(st);
@@ -540,7 +546,7 @@ __global__ void __launch_bounds__(kPrThreads, 2)
         if (lane == 0) mbar_arrive(p_full);
       }
       // ----------------------------------------------------------- output
-      if (tiles > 0 && ok) ok = mbar_wait_warp(o_full, 0, ICX_DEVICE_TIMEOUT_EPILOGUE);
+      if (tiles > 0 && ok) ok = wait_warp(o_full, 0, ICX_DEVICE_TIMEOUT_EPILOGUE);
       tc_fence_after();
       const float inv = l != 0.0f ? 1.0f / l : 0.0f;
       T* out = static_cast<T*>(a.out) +
