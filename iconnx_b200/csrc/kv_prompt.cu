@@ -24,15 +24,9 @@
 //               stands, position by position: MN-major).
 // Bound by the softmax warps (about ten instructions per score, pairs of f32 in
 // one) beside the tensor cores.
-#include <type_traits>
-
-#include "capi.cuh"
-#include "common.cuh"
-#include "kv_attention.cuh"
+#include "kv_prompt.cuh"
 
 namespace icx {
-
-constexpr int kPrRows = 128, kPrKeys = 64, kPrGroup = 64, kPrThreads = 256;
 
 template <int D>
 struct PromptConfig {
@@ -46,68 +40,13 @@ struct PromptConfig {
   static constexpr int kTmemCols = D == 64 ? 128 : 256;
 };
 
-// kind::f16, f32 accumulator, M = 128: [4,6) D format 1, A and B f16 (0), [16]
-// B MN-major, [17,23) N >> 3, [24,29) M >> 4.
-constexpr uint32_t prompt_idesc(int n, bool b_mn) {
-  return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kPrRows >> 4) << 24);
-}
-__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
-      : "memory");
-}
-
-// The eight f16 of a 16-byte piece come from one 4-bit word or two 8-bit ones.
-// K: piece 2 t + n of a group's 64 dimensions, r-th value: dimension
-// 16 step + 4 t + i of the group.
-template <int BITS>
-__host__ __device__ constexpr int k_step(int n, int r) {
-  return BITS == 4 ? 2 * n + ((r >> 1) & 1) : 2 * n + (r >> 2);
-}
-template <int BITS>
-__host__ __device__ constexpr int k_dim(int r) {
-  return BITS == 4 ? (r & 1) + 2 * (r >> 2) : ((r >> 1) & 1) * 2 + (r & 1);
-}
-// V: piece g, r-th value: dimension 16 m + 2 g + h of the group.
-template <int BITS>
-__host__ __device__ constexpr int v_tile(int r) {
-  return BITS == 4 ? 2 * (r & 1) + (r >> 2) : (r & 1) + 2 * (r >> 2);
-}
-__host__ __device__ constexpr int v_half(int r) { return (r >> 1) & 1; }
-// 4 bits: these values are sixteen times their code
-template <int BITS>
-__host__ __device__ constexpr bool times16(int r) {
-  return BITS == 4 && ((r >> 1) & 1);
-}
-
-template <int BITS>
-__device__ __forceinline__ uint4 spread(uint32_t w0, uint32_t w1) {
-  if (BITS == 4) return make_uint4(w0 & 0x000f000fu, w0 & 0x00f000f0u, (w0 >> 8) & 0x000f000fu, (w0 >> 8) & 0x00f000f0u);
-  return make_uint4(w0 & 0x00ff00ffu, (w0 >> 8) & 0x00ff00ffu, w1 & 0x00ff00ffu, (w1 >> 8) & 0x00ff00ffu);
-}
-
-// All lanes poll: the roles hand over several times per tile, and a lane that
-// sleeps between polls wakes too late for that.
-__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int code) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
-}
-
 template <typename T, int D, int BITS>
 __global__ void __launch_bounds__(kPrThreads, 2)
     kv_prompt_kernel(const __grid_constant__ KvView c, const __grid_constant__ KvTokens w,
                      const __grid_constant__ AttendArgs a) {
   using C = PromptConfig<D>;
-  constexpr int G = C::G, ROW = D * BITS / 8;
-  constexpr bool PLO = !std::is_same<T, __nv_bfloat16>::value;
+  constexpr int G = C::G;
+  constexpr bool PLO = true;   // w s as two f16: an f16 output has as many bits as one
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* s_q = smem;
@@ -140,33 +79,7 @@ __global__ void __launch_bounds__(kPrThreads, 2)
   }
   pdl_wait();
   pdl_trigger();
-  // the blockIdx.x-th row tile of the batch, the last tiles of a sequence (the
-  // longest) first
-  if (warp == 0) {
-    const int want = blockIdx.x;
-    int before = 0, seq = -1, tile = 0;
-    for (int b0 = 0; b0 < w.batch && seq < 0; b0 += 32) {
-      const int b = b0 + lane;
-      const int n = b < w.batch ? seq_units(c, w, share, kPrRows, b).tiles : 0;
-      int inc = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += x;
-      }
-      const uint32_t hit = __ballot_sync(0xffffffffu, before + inc > want);
-      if (hit) {
-        const int l = __ffs(hit) - 1;
-        seq = b0 + l;
-        tile = __shfl_sync(0xffffffffu, n, l) - 1 - (want - before - __shfl_sync(0xffffffffu, inc - n, l));
-      }
-      before += __shfl_sync(0xffffffffu, inc, 31);
-    }
-    if (lane == 0) {
-      s_seq = seq;
-      s_tile = tile;
-    }
-  }
+  if (warp == 0) find_row_tile(c, w, share, blockIdx.x, &s_seq, &s_tile);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -185,9 +98,7 @@ __global__ void __launch_bounds__(kPrThreads, 2)
     if (warp >= 4) {
       // ------------------------------------------------------------ codes
       const int p = threadIdx.x - 128, key = p >> 1, half = p & 1;
-      // words of K chunks 2 half, 2 half + 1 and of V chunks 4 half .. + 3
-      constexpr int KW = D * BITS / 128, VW = KW / 2;
-      uint32_t kw[2][KW], vw[4][VW];
+      RawCodes<D, BITS> raw;
       int hole = 0;            // this position has no page (or does not exist)
       uint32_t kp[2][G], vp[2][G];   // warp 4: parameters of positions lane, lane + 32
       bool pvalid[2] = {false, false};
@@ -196,29 +107,7 @@ __global__ void __launch_bounds__(kPrThreads, 2)
         const int64_t page = pos < see_any ? kv_page(c, w, seq, pos) : -1;
         hole = pos < see_any && page < 0;
         if (hole && half == 0) record_status(ICX_DEVICE_BAD_PAGE);
-        if (page >= 0) {
-          const int64_t row = kv_row(c, page, head, pos);
-          const uint8_t* kr = c.codes[0] + row * ROW;
-          const uint8_t* vr = c.codes[1] + row * ROW;
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if constexpr (KW < 4) {
-              load_words(reinterpret_cast<const uint32_t*>(kr + k_word_at<ROW>(pos, 2 * half + x, 0)), kw[x]);
-            } else {
-#pragma unroll
-              for (int n = 0; n < KW; n += 4) {
-                const uint4 u = *reinterpret_cast<const uint4*>(kr + k_word_at<ROW>(pos, 2 * half + x, n));
-                kw[x][n] = u.x;
-                kw[x][n + 1] = u.y;
-                kw[x][n + 2] = u.z;
-                kw[x][n + 3] = u.w;
-              }
-            }
-          }
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            load_words(reinterpret_cast<const uint32_t*>(vr + v_word_at<ROW>(pos, 4 * half + x, 0)), vw[x]);
-        }
+        if (page >= 0) raw.load(c, kv_row(c, page, head, pos), pos, half);
         if (warp == 4) {
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
@@ -267,12 +156,12 @@ __global__ void __launch_bounds__(kPrThreads, 2)
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
               const int piece = 2 * (2 * half + x) + n, at = BITS == 4 ? 2 * k + n : 4 * k + 2 * n;
-              *reinterpret_cast<uint4*>(kr + ((piece ^ (key & 7)) << 4)) = spread<BITS>(kw[x][at], kw[x][BITS == 4 ? at : at + 1]);
+              *reinterpret_cast<uint4*>(kr + ((piece ^ (key & 7)) << 4)) = spread<BITS>(raw.k[x][at], raw.k[x][BITS == 4 ? at : at + 1]);
             }
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const int piece = 4 * half + x, at = BITS == 4 ? k : 2 * k;
-            *reinterpret_cast<uint4*>(vr + ((piece ^ (key & 7)) << 4)) = spread<BITS>(vw[x][at], vw[x][BITS == 4 ? at : at + 1]);
+            *reinterpret_cast<uint4*>(vr + ((piece ^ (key & 7)) << 4)) = spread<BITS>(raw.v[x][at], raw.v[x][BITS == 4 ? at : at + 1]);
           }
         }
         const uint32_t holes = __ballot_sync(0xffffffffu, hole);   // bit: two lanes per position
@@ -357,51 +246,9 @@ __global__ void __launch_bounds__(kPrThreads, 2)
       {
         const T* q = static_cast<const T*>(a.q) + (int64_t)(su.from + (mine ? r / share : 0)) * a.q_token_stride +
                      (int64_t)(head * share + (mine ? r % share : 0)) * a.q_head_stride;
-        float peak = 0.0f;
+        put_query<T, G, BITS, true>(a, q, mine, row, s_q, &f, qsum);
 #pragma unroll
-        for (int d = 0; d < D; d += 4) {
-          float v[4];
-          load_f32<T, 4>(q + d, v, a.q_vec);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) peak = fmaxf(peak, fabsf(v[i]));
-        }
-        const int e = mine && peak > 0.0f ? max(-60, min(120, 14 - (int)((__float_as_uint(peak) >> 23) & 255) + 127)) : 0;
-        // the score's factor is positive: a negative scale turns q round
-        const float up = mine && a.scale != 0.0f ? copysignf(__uint_as_float((uint32_t)(e + 127) << 23), a.scale) : 0.0f;
-        f = a.scale != 0.0f ? fabsf(a.scale) * 16777216.0f * __uint_as_float((uint32_t)(127 - e) << 23) : 1.0f;
-#pragma unroll 1
-        for (int k = 0; k < G; ++k) {
-          float sum = 0.0f;
-#pragma unroll 1
-          for (int t = 0; t < 4; ++t) {
-            // step j's dimensions 16 j + 4 t .. + 3 of the group
-            float v[4][4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              load_f32<T, 4>(q + k * kPrGroup + 16 * j + 4 * t, v[j], a.q_vec);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                v[j][i] = up != 0.0f ? v[j][i] * up : 0.0f;
-                sum += v[j][i];
-              }
-            }
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-              float x[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                x[i] = v[k_step<BITS>(n, i)][k_dim<BITS>(i)] * (times16<BITS>(i) ? 0.0625f : 1.0f);
-              const int piece = 2 * t + n;
-              *reinterpret_cast<uint4*>(s_q + k * kPrRows * 128 + row * 128 + ((piece ^ (row & 7)) << 4)) =
-                  make_uint4(pack_f16(x[0], x[1]), pack_f16(x[2], x[3]), pack_f16(x[4], x[5]), pack_f16(x[6], x[7]));
-            }
-          }
-          // in the accumulators' units, where a code counts 2^-24
-          const float qs = sum * 5.9604644775390625e-8f;
-#pragma unroll
-          for (int kk = 0; kk < G; ++kk)
-            if (kk == k) qsum[kk] = qs;
-        }
+        for (int k = 0; k < G; ++k) qsum[k] *= 5.9604644775390625e-8f;   // in units where a code counts 2^-24
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);
@@ -601,8 +448,8 @@ static int launch_prompt_kernel(cudaStream_t s, const KvView& c, const KvTokens&
   return ICX_OK;
 }
 
-template <typename T>
-static int launch_prompt_typed(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a) {
+static int launch_prompt_f16(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a) {
+  using T = __half;
   if (c.dim == 64) return c.bits == 4 ? launch_prompt_kernel<T, 64, 4>(s, c, w, a) : launch_prompt_kernel<T, 64, 8>(s, c, w, a);
   return c.bits == 4 ? launch_prompt_kernel<T, 128, 4>(s, c, w, a) : launch_prompt_kernel<T, 128, 8>(s, c, w, a);
 }
@@ -614,7 +461,7 @@ bool prompt_preferred(const KvView& c, const KvTokens& w, int q_heads, int type)
 }
 
 int launch_prompt(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a, int type) {
-  return type == ICX_F16 ? launch_prompt_typed<__half>(s, c, w, a) : launch_prompt_typed<__nv_bfloat16>(s, c, w, a);
+  return type == ICX_F16 ? launch_prompt_f16(s, c, w, a) : launch_prompt_bf16(s, c, w, a);
 }
 
 }  // namespace icx

@@ -1,0 +1,182 @@
+// Pieces shared by the two kernels for prompt chunks over the quantised K/V
+// cache: the spread of codes over 16-byte pieces, matrix instructions of
+// kind::f16, and the row tiles.
+#pragma once
+
+#include "capi.cuh"
+#include "common.cuh"
+#include "kv_attention.cuh"
+
+namespace icx {
+
+constexpr int kPrRows = 128, kPrKeys = 64, kPrGroup = 64, kPrThreads = 256;
+
+// kind::f16, f32 accumulator, M = 128: [4,6) D format 1, A and B f16 (0), [16]
+// B MN-major, [17,23) N >> 3, [24,29) M >> 4.
+constexpr uint32_t prompt_idesc(int n, bool b_mn) {
+  return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kPrRows >> 4) << 24);
+}
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+
+// The eight f16 of a 16-byte piece come from one 4-bit word or two 8-bit ones.
+// K: piece 2 t + n of a group's 64 dimensions, r-th value: dimension
+// 16 step + 4 t + i of the group.
+template <int BITS>
+__host__ __device__ constexpr int k_step(int n, int r) {
+  return BITS == 4 ? 2 * n + ((r >> 1) & 1) : 2 * n + (r >> 2);
+}
+template <int BITS>
+__host__ __device__ constexpr int k_dim(int r) {
+  return BITS == 4 ? (r & 1) + 2 * (r >> 2) : ((r >> 1) & 1) * 2 + (r & 1);
+}
+// V: piece g, r-th value: dimension 16 m + 2 g + h of the group.
+template <int BITS>
+__host__ __device__ constexpr int v_tile(int r) {
+  return BITS == 4 ? 2 * (r & 1) + (r >> 2) : (r & 1) + 2 * (r >> 2);
+}
+__host__ __device__ constexpr int v_half(int r) { return (r >> 1) & 1; }
+// 4 bits: these values are sixteen times their code
+template <int BITS>
+__host__ __device__ constexpr bool times16(int r) {
+  return BITS == 4 && ((r >> 1) & 1);
+}
+
+template <int BITS>
+__device__ __forceinline__ uint4 spread(uint32_t w0, uint32_t w1) {
+  if (BITS == 4) return make_uint4(w0 & 0x000f000fu, w0 & 0x00f000f0u, (w0 >> 8) & 0x000f000fu, (w0 >> 8) & 0x00f000f0u);
+  return make_uint4(w0 & 0x00ff00ffu, (w0 >> 8) & 0x00ff00ffu, w1 & 0x00ff00ffu, (w1 >> 8) & 0x00ff00ffu);
+}
+
+// All lanes poll: the roles hand over several times per tile, and a lane that
+// sleeps between polls wakes too late for that.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
+}
+
+// The want-th row tile of the batch, the last tiles of a sequence (the longest)
+// first; *seq = -1 if there is none.  One warp.
+__device__ __forceinline__ void find_row_tile(const KvView& c, const KvTokens& w, int share, int want, int* seq_out,
+                                              int* tile_out) {
+  const int lane = threadIdx.x & 31;
+  int before = 0, seq = -1, tile = 0;
+  for (int b0 = 0; b0 < w.batch && seq < 0; b0 += 32) {
+    const int b = b0 + lane;
+    const int n = b < w.batch ? seq_units(c, w, share, kPrRows, b).tiles : 0;
+    int inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += x;
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, before + inc > want);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      seq = b0 + l;
+      tile = __shfl_sync(0xffffffffu, n, l) - 1 - (want - before - __shfl_sync(0xffffffffu, inc - n, l));
+    }
+    before += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  if (lane == 0) {
+    *seq_out = seq;
+    *tile_out = tile;
+  }
+}
+
+// The codes of one position: words of K chunks 2 half, 2 half + 1 and of V
+// chunks 4 half .. 4 half + 3.
+template <int D, int BITS>
+struct RawCodes {
+  static constexpr int ROW = D * BITS / 8, KW = D * BITS / 128, VW = KW / 2;
+  uint32_t k[2][KW], v[4][VW];
+  __device__ __forceinline__ void load(const KvView& c, int64_t row, int pos, int half) {
+    const uint8_t* kr = c.codes[0] + row * ROW;
+    const uint8_t* vr = c.codes[1] + row * ROW;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      if constexpr (KW < 4) {
+        load_words(reinterpret_cast<const uint32_t*>(kr + k_word_at<ROW>(pos, 2 * half + x, 0)), k[x]);
+      } else {
+#pragma unroll
+        for (int n = 0; n < KW; n += 4) {
+          const uint4 u = *reinterpret_cast<const uint4*>(kr + k_word_at<ROW>(pos, 2 * half + x, n));
+          k[x][n] = u.x;
+          k[x][n + 1] = u.y;
+          k[x][n + 2] = u.z;
+          k[x][n + 3] = u.w;
+        }
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      load_words(reinterpret_cast<const uint32_t*>(vr + v_word_at<ROW>(pos, 4 * half + x, 0)), v[x]);
+  }
+};
+
+// A query row as the left operand: scaled by 2^e into f16's range (and by the
+// sign of the scale, so that the score's factor is positive), in the order of
+// the K pieces.  *f is the factor from products with codes that count 2^-24
+// (exact) or with values (24 bits less) to scores in powers of two; sum[k] the
+// sum of the scaled row over group k.
+template <typename T, int G, int BITS, bool CODES>
+__device__ __forceinline__ void put_query(const AttendArgs& a, const T* q, bool mine, int row, uint8_t* s_q, float* f,
+                                          float (&sum)[G]) {
+  float peak = 0.0f;
+#pragma unroll
+  for (int d = 0; d < G * kPrGroup; d += 4) {
+    float v[4];
+    load_f32<T, 4>(q + d, v, a.q_vec);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) peak = fmaxf(peak, fabsf(v[i]));
+  }
+  const int e = mine && peak > 0.0f ? max(-60, min(120, 14 - (int)((__float_as_uint(peak) >> 23) & 255) + 127)) : 0;
+  const float up = mine && a.scale != 0.0f ? copysignf(__uint_as_float((uint32_t)(e + 127) << 23), a.scale) : 0.0f;
+  *f = a.scale != 0.0f ? fabsf(a.scale) * (CODES ? 16777216.0f : 1.0f) * __uint_as_float((uint32_t)(127 - e) << 23) : 1.0f;
+#pragma unroll 1
+  for (int k = 0; k < G; ++k) {
+    float total = 0.0f;
+#pragma unroll 1
+    for (int t = 0; t < 4; ++t) {
+      // step j's dimensions 16 j + 4 t .. + 3 of the group
+      float v[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        load_f32<T, 4>(q + k * kPrGroup + 16 * j + 4 * t, v[j], a.q_vec);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[j][i] = up != 0.0f ? v[j][i] * up : 0.0f;
+          total += v[j][i];
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          x[i] = v[k_step<BITS>(n, i)][k_dim<BITS>(i)] * (CODES && times16<BITS>(i) ? 0.0625f : 1.0f);
+        const int piece = 2 * t + n;
+        *reinterpret_cast<uint4*>(s_q + k * kPrRows * 128 + row * 128 + ((piece ^ (row & 7)) << 4)) =
+            make_uint4(pack_f16(x[0], x[1]), pack_f16(x[2], x[3]), pack_f16(x[4], x[5]), pack_f16(x[6], x[7]));
+      }
+    }
+#pragma unroll
+    for (int kk = 0; kk < G; ++kk)
+      if (kk == k) sum[kk] = total;
+  }
+}
+
+int launch_prompt_bf16(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a);
+
+}  // namespace icx
