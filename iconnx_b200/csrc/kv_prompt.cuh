@@ -102,8 +102,17 @@ struct RawCodes {
   static constexpr int ROW = D * BITS / 8, KW = D * BITS / 128, VW = KW / 2;
   uint32_t k[2][KW], v[4][VW];
   __device__ __forceinline__ void load(const KvView& c, int64_t row, int pos, int half) {
-    const uint8_t* kr = c.codes[0] + row * ROW;
+    load_k(c, row, pos, half);
+    load_v(c, row, pos, half);
+  }
+  __device__ __forceinline__ void load_v(const KvView& c, int64_t row, int pos, int half) {
     const uint8_t* vr = c.codes[1] + row * ROW;
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      load_words(reinterpret_cast<const uint32_t*>(vr + v_word_at<ROW>(pos, 4 * half + x, 0)), v[x]);
+  }
+  __device__ __forceinline__ void load_k(const KvView& c, int64_t row, int pos, int half) {
+    const uint8_t* kr = c.codes[0] + row * ROW;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       if constexpr (KW < 4) {
@@ -119,9 +128,6 @@ struct RawCodes {
         }
       }
     }
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-      load_words(reinterpret_cast<const uint32_t*>(vr + v_word_at<ROW>(pos, 4 * half + x, 0)), v[x]);
   }
 };
 
