@@ -3,11 +3,15 @@
 //
 // A bf16 output has 8 significant bits, so here K and V are dequantised to f16
 // (11 bits: half a step is 2^-12, an eighth of the output's) on their way into
-// shared memory, scaled by powers of two into f16's range (K by tile, V by the
-// largest value met so far), and the weights are rounded to one f16.  Scores,
-// their maximum and all sums stay f32.  That leaves the softmax warps with
-// about five instructions per score, against ten in kv_prompt.cu, whose
-// operands are exact and which f16 outputs take.
+// shared memory, scaled by powers of two into f16's range, and the weights are
+// rounded to one f16.  Scores, their maximum and all sums stay f32.  That leaves
+// the softmax warps with about five instructions per score, against ten in
+// kv_prompt.cu, whose operands are exact and which f16 outputs take.
+//
+// Dequantising is one fused multiply-add per pair: a code in the low bits of a
+// half word is the f16 number code * 2^-24, so code * (s 2^24 2^-E) + lo 2^-E is
+// the value times 2^-E.  The CTA looks over the scales of all its positions
+// first (a sixteenth of the cache) to choose E for K and for V.
 //
 // A CTA takes 128 query rows of one (sequence, K/V head), 48 positions at a
 // time, two CTAs per SM:
@@ -22,7 +26,9 @@
 // (48 positions rather than 64: three warps fill them, the fourth of that
 // group is free to issue, and a row's scores stay in 128 registers.)
 // Rows that do not see a position must not meet its NaN: a V group that holds
-// one is stored as zeros and noted, and the rows that see it end as NaN.
+// one is stored as zeros, and the rows that see it end as NaN.  That and pages
+// that are missing are found in the first look; only then do the softmax warps
+// ask for them, tile by tile.
 #include "kv_prompt.cuh"
 
 namespace icx {
@@ -41,49 +47,40 @@ struct PromptB16Config {
 };
 
 
-// What a tile's scores and output need beside the operands; a ring of four:
-// a K stage is free when the scores of two tiles ago are there, which were
-// issued after the weights of four tiles ago were.
-struct TileNote {
-  float k_unit;           // scores: accumulator x f x k_unit
-  float v_fix;            // factor of the output so far
-  float v_unit;           // output: accumulator x v_unit
-  uint32_t special;       // any of the following: bit (tile / 4) % 32, left set once it is
-  uint32_t holes[4];      // positions without a page: two equal bits each, 16 positions per word
-  uint32_t v_nan[4][2];   // positions whose V group holds a NaN, likewise, per group
-};
-
 __device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t taddr, const uint32_t (&r)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
                "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
 
-// 2^-E that brings top into [2^(n-1), 2^n), and 2^E.
-__device__ __forceinline__ void unit_for(float top, int n, float& down, float& up) {
-  const int E = min(max((int)(__float_as_uint(top) >> 23) - 126 - n, -100), 120);
-  down = __uint_as_float((uint32_t)(127 - E) << 23);
-  up = __uint_as_float((uint32_t)(127 + E) << 23);
+// E for groups with scales up to s_top and low ends up to lo_top: s 2^24 2^-E and
+// lo 2^-E stay below 2^15 (and codes x scale mostly in f16's normal range).
+__device__ __forceinline__ int unit_for(uint32_t s_top, uint32_t lo_top) {
+  const int s = (int)(s_top >> 23) - 126, lo = (int)(lo_top >> 23) - 126;   // below 2^s, 2^lo
+  return min(max(max(s + 9, lo - 15), -100), 120);
 }
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
-// Eight dequantised values of a 16-byte piece: code x s + lo, one rounding.
-// s16 is s / 16 for the values that come out sixteen times too large.
+// Scale (for codes that count 2^-24, and for those that count 2^-20) and low
+// end of a group in f16.
+struct GroupF16 {
+  __half2 s, s16, lo;
+  __device__ __forceinline__ GroupF16(uint32_t p, float up24, float down, bool zero) {
+    const float a = zero ? 0.0f : param_scale(p) * up24, b = zero ? 0.0f : param_low(p) * down;
+    s = __float2half2_rn(a);
+    s16 = __float2half2_rn(a * 0.0625f);
+    lo = __float2half2_rn(b);
+  }
+};
+
+// Eight dequantised values of a 16-byte piece, one rounding each.
 template <int BITS>
-__device__ __forceinline__ uint4 dequantize(uint32_t w0, uint32_t w1, __half2 s, __half2 s16, __half2 lo) {
-  const uint32_t one = 0x64006400u;   // 1024 in both halves: a code in its low bits is 1024 + code
-  const __half2 base = __float2half2_rn(1024.0f);
-  uint4 u;
-  if (BITS == 4)
-    u = make_uint4((w0 & 0x000f000fu) | one, (w0 & 0x00f000f0u) | one, ((w0 >> 8) & 0x000f000fu) | one,
-                   ((w0 >> 8) & 0x00f000f0u) | one);
-  else
-    u = make_uint4((w0 & 0x00ff00ffu) | one, ((w0 >> 8) & 0x00ff00ffu) | one, (w1 & 0x00ff00ffu) | one,
-                   ((w1 >> 8) & 0x00ff00ffu) | one);
+__device__ __forceinline__ uint4 dequantize(uint32_t w0, uint32_t w1, const GroupF16& g) {
+  uint4 u = spread<BITS>(w0, w1);
   uint32_t* v = reinterpret_cast<uint32_t*>(&u);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const __half2 c = __hsub2(*reinterpret_cast<const __half2*>(&v[i]), base);
-    const __half2 y = __hfma2(c, times16<BITS>(2 * i) ? s16 : s, lo);
+    const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&v[i]), times16<BITS>(2 * i) ? g.s16 : g.s, g.lo);
     v[i] = *reinterpret_cast<const uint32_t*>(&y);
   }
   return u;
@@ -96,27 +93,22 @@ __global__ void __launch_bounds__(kB16Threads, 2)
   using T = __nv_bfloat16;
   using C = PromptB16Config<D>;
   constexpr int G = C::G;
-  constexpr float L = (float)((1 << BITS) - 1);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* s_q = smem;
   auto s_k = [&](int n) { return smem + C::kQ + n * C::kTile; };
   auto s_v = [&](int n) { return smem + C::kQ + (2 + n) * C::kTile; };
-  __shared__ __align__(8) uint64_t bars[18];
+  __shared__ __align__(8) uint64_t bars[14];
   uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6, *s_full = bars + 8,
-           *p_full = bars + 10, *q_full = bars + 12, *o_full = bars + 13, *note_full = bars + 14;
-  __shared__ __align__(16) TileNote note[4];
-  __shared__ uint32_t s_top[2][3][2];
+           *p_full = bars + 10, *q_full = bars + 12, *o_full = bars + 13;
+  __shared__ uint32_t s_look[5];   // largest s and |lo| of K, of V; whether anything is special
   __shared__ uint32_t tmem_slot;
   __shared__ int s_seq, s_tile;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int share = a.q_heads / c.heads;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 4; ++i) {
-      note[i].special = 0u;
-      mbar_init(&note_full[i], 3);
-    }
+    for (int i = 0; i < 5; ++i) s_look[i] = 0u;
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 3);    // one arrival per warp
       mbar_init(&v_full[i], 3);
@@ -150,6 +142,45 @@ __global__ void __launch_bounds__(kB16Threads, 2)
     const int see_all = (int)max((int64_t)0, min(first_pos + r0 / share + 1, (int64_t)reach));
     const int tiles = (see_any + kB16Keys - 1) / kB16Keys;
     if (threadIdx.x == 0 && su.len > reach) record_status(ICX_DEVICE_BAD_PAGE);
+
+    // the first look
+    {
+      uint32_t top[4] = {0, 0, 0, 0}, special = 0;
+#pragma unroll 4
+      for (int pos = threadIdx.x; pos < see_any; pos += kB16Threads) {
+        const int64_t page = kv_page(c, w, seq, pos);
+        if (page < 0) {
+          special = 1;
+          record_status(ICX_DEVICE_BAD_PAGE);
+          continue;
+        }
+        uint32_t prm[2][G];
+        const int64_t row = kv_row(c, page, head, pos) * G;
+        load_words(c.params[0] + row, prm[0]);
+        load_words(c.params[1] + row, prm[1]);
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int k = 0; k < G; ++k) {
+            const float sc = param_scale(prm[x][k]), lo = fabsf(param_low(prm[x][k]));
+            if (isnan(sc)) {
+              special |= x;
+            } else {
+              top[2 * x] = max(top[2 * x], __float_as_uint(sc));
+              top[2 * x + 1] = max(top[2 * x + 1], __float_as_uint(lo));
+            }
+          }
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        top[x] = __reduce_max_sync(0xffffffffu, top[x]);
+        if (lane == 0) atomicMax(&s_look[x], top[x]);
+      }
+      if (special) s_look[4] = 1u;
+      __syncthreads();
+    }
+    const int k_exp = unit_for(s_look[0], s_look[1]), v_exp = unit_for(s_look[2], s_look[3]);
+    const bool special = s_look[4] != 0u;
 
     if (warp == 7) {
       // ---------------------------------------------------------- products
@@ -206,12 +237,9 @@ __global__ void __launch_bounds__(kB16Threads, 2)
       RawCodes<D, BITS> raw;
       uint32_t kp[G], vp[G];
       int64_t row = -1, row_next = -1;   // cache row of this thread's position, or -1
-      bool hole = false, hole_next = false;
       auto find = [&](int i) {
         const int pos = i * kB16Keys + key;
         const int64_t page = pos < see_any ? kv_page(c, w, seq, pos) : -1;
-        hole_next = pos < see_any && page < 0;
-        if (hole_next && half == 0) record_status(ICX_DEVICE_BAD_PAGE);
         row_next = page >= 0 ? kv_row(c, page, head, pos) : -1;
       };
       auto fetch_k = [&](int i) {
@@ -223,66 +251,25 @@ __global__ void __launch_bounds__(kB16Threads, 2)
       auto fetch_v = [&](int i) {
         if (row >= 0) raw.load_v(c, row, i * kB16Keys + key, half);
       };
-      float v_max = 0.0f, v_down = 0.0f, v_up = 0.0f;
+      const float k_down = power_of_two(-k_exp), v_down = power_of_two(-v_exp);
+      const float k_up24 = k_down * 16777216.0f, v_up24 = v_down * 16777216.0f;
       bool ok = true;
       if (tiles > 0) {
         find(0);
         fetch_k(0);
         row = row_next;
-        hole = hole_next;
         fetch_v(0);
         if (tiles > 1) find(1);
       }
       for (int i = 0; i < tiles; ++i) {
         const int st = i & 1;
-        TileNote& nt = note[i & 3];
-        // the largest |value| a group can stand for, over the tile
-        float k_top = 0.0f, v_top = 0.0f;
-        bool nan[G];
+        uint32_t vq[G];
 #pragma unroll
-        for (int k = 0; k < G; ++k) {
-          if (row < 0) kp[k] = vp[k] = 0u;
-          nan[k] = isnan(param_scale(vp[k]));
-          k_top = fmaxf(k_top, fmaxf(fabsf(param_low(kp[k])), fabsf(fmaf(L, param_scale(kp[k]), param_low(kp[k])))));
-          v_top = fmaxf(v_top, fmaxf(fabsf(param_low(vp[k])), fabsf(fmaf(L, param_scale(vp[k]), param_low(vp[k])))));
-        }
-        const uint32_t kt = __reduce_max_sync(0xffffffffu, __float_as_uint(k_top));
-        const uint32_t vt = __reduce_max_sync(0xffffffffu, __float_as_uint(v_top));
-        if (lane == 0) {
-          s_top[st][warp - 4][0] = kt;
-          s_top[st][warp - 4][1] = vt;
-        }
-        asm volatile("bar.sync 1, 96;" ::: "memory");   // warps 4..6
-        k_top = v_top = 0.0f;
-#pragma unroll
-        for (int x = 0; x < 3; ++x) {
-          k_top = fmaxf(k_top, __uint_as_float(s_top[st][x][0]));
-          v_top = fmaxf(v_top, __uint_as_float(s_top[st][x][1]));
-        }
-        float k_down, k_up, v_fix = 1.0f;
-        unit_for(k_top, 8, k_down, k_up);
-        if (v_top > v_max) {   // room for four times as much before the next change
-          float down, up;
-          unit_for(v_top, 6, down, up);
-          v_fix = v_max > 0.0f ? down * v_up : 1.0f;
-          v_down = down;
-          v_up = up;
-          v_max = up * 256.0f;
-        }
-        __half2 vs2[G], vs16[G], vlo2[G];
-#pragma unroll
-        for (int k = 0; k < G; ++k) {
-          const float s = nan[k] ? 0.0f : param_scale(vp[k]) * v_down, lo = nan[k] ? 0.0f : param_low(vp[k]) * v_down;
-          vs2[k] = __float2half2_rn(s);
-          vs16[k] = __float2half2_rn(s * 0.0625f);
-          vlo2[k] = __float2half2_rn(lo);
-        }
-        // -- K, and the tile's note
+        for (int k = 0; k < G; ++k) vq[k] = vp[k];
         if (ok) ok = wait_warp(&k_empty[st], ((i >> 1) & 1) ^ 1, ICX_DEVICE_TIMEOUT_PRODUCER);
 #pragma unroll
         for (int k = 0; k < G; ++k) {
-          const float s = param_scale(kp[k]) * k_down, lo = param_low(kp[k]) * k_down;
-          const __half2 s2 = __float2half2_rn(s), s16 = __float2half2_rn(s * 0.0625f), lo2 = __float2half2_rn(lo);
+          const GroupF16 g(kp[k], k_up24, k_down, row < 0);
           uint8_t* kr = s_k(st) + k * kB16Keys * 128 + key * 128;
 #pragma unroll
           for (int x = 0; x < 2; ++x)
@@ -290,50 +277,29 @@ __global__ void __launch_bounds__(kB16Threads, 2)
             for (int n = 0; n < 2; ++n) {
               const int piece = 2 * (2 * half + x) + n, at = BITS == 4 ? 2 * k + n : 4 * k + 2 * n;
               *reinterpret_cast<uint4*>(kr + ((piece ^ (key & 7)) << 4)) =
-                  dequantize<BITS>(raw.k[x][at], raw.k[x][BITS == 4 ? at : at + 1], s2, s16, lo2);
+                  dequantize<BITS>(raw.k[x][at], raw.k[x][BITS == 4 ? at : at + 1], g);
             }
-        }
-        {
-          const uint32_t holes = __ballot_sync(0xffffffffu, hole);
-          uint32_t special = holes;
-          if (lane == 0) nt.holes[warp - 4] = holes;
-#pragma unroll
-          for (int k = 0; k < G; ++k) {
-            const uint32_t n = __ballot_sync(0xffffffffu, nan[k]);
-            special |= n;
-            if (lane == 0) nt.v_nan[warp - 4][k] = n;
-          }
-          if (lane == 0 && special) atomicOr(&nt.special, 1u << (i >> 2 & 31));
-          if (p == 0) {
-            nt.k_unit = k_up;
-            nt.v_fix = v_fix;
-            nt.v_unit = v_up;
-          }
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&note_full[i & 3]);
-          mbar_arrive(&k_full[st]);
-        }
+        if (lane == 0) mbar_arrive(&k_full[st]);
         if (i + 1 < tiles) fetch_k(i + 1);
-        // -- V
         if (ok) ok = wait_warp(&v_empty[st], ((i >> 1) & 1) ^ 1, ICX_DEVICE_TIMEOUT_PRODUCER);
 #pragma unroll
         for (int k = 0; k < G; ++k) {
+          const GroupF16 g(vq[k], v_up24, v_down, row < 0 || isnan(param_scale(vq[k])));
           uint8_t* vr = s_v(st) + k * kB16Keys * 128 + key * 128;
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const int piece = 4 * half + x, at = BITS == 4 ? k : 2 * k;
             *reinterpret_cast<uint4*>(vr + ((piece ^ (key & 7)) << 4)) =
-                dequantize<BITS>(raw.v[x][at], raw.v[x][BITS == 4 ? at : at + 1], vs2[k], vs16[k], vlo2[k]);
+                dequantize<BITS>(raw.v[x][at], raw.v[x][BITS == 4 ? at : at + 1], g);
           }
         }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&v_full[st]);
         row = row_next;
-        hole = hole_next;
         if (i + 1 < tiles) fetch_v(i + 1);
         if (i + 2 < tiles) find(i + 2);
       }
@@ -351,40 +317,45 @@ __global__ void __launch_bounds__(kB16Threads, 2)
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
+      const float ft = fminf(fmaxf(f * power_of_two(k_exp), 1e-37f), 1e37f);   // neither 0 nor infinity beside a masked -infinity
       float m = kNoScore, l = 0.0f;   // m: in powers of two
       bool vnan[G];
 #pragma unroll
       for (int k = 0; k < G; ++k) vnan[k] = false;
       for (int i = 0; i < tiles && ok; ++i) {
         const int st = i & 1;
-        ok = wait_warp(&note_full[i & 3], (i >> 2) & 1, ICX_DEVICE_TIMEOUT_EPILOGUE);
-        if (ok) ok = wait_warp(&s_full[st], (i >> 1) & 1, ICX_DEVICE_TIMEOUT_EPILOGUE);
+        ok = wait_warp(&s_full[st], (i >> 1) & 1, ICX_DEVICE_TIMEOUT_EPILOGUE);
         if (!ok) break;
         tc_fence_after();
         const uint32_t t_s = tmem + t_lane + (uint32_t)(st * kB16Cols);
         uint32_t x0[32], x1[16];
         tmem_ld_32x32b_x32(t_s, x0);
         tmem_ld_32x32b_x16(t_s + 32, x1);
-        const float4 nt = *reinterpret_cast<const float4*>(&note[i & 3]);
-        const bool special = (__float_as_uint(nt.w) >> (i >> 2 & 31) & 1u) != 0;
         tmem_ld_wait_regs(x0);
         tmem_ld_wait_regs16(x1);
         float s[kB16Keys];
 #pragma unroll
         for (int j = 0; j < kB16Keys; ++j) s[j] = __uint_as_float(j < 32 ? x0[j & 31] : x1[j & 15]);
-        if ((i + 1) * kB16Keys > see_all || special) {
-          const uint32_t hw[3] = {note[i & 3].holes[0], note[i & 3].holes[1], note[i & 3].holes[2]};
+        if ((i + 1) * kB16Keys > see_all) {
+#pragma unroll
+          for (int j = 0; j < kB16Keys; ++j)
+            if (i * kB16Keys + j >= see) s[j] = -INFINITY;
+        }
+        if (special) {
 #pragma unroll
           for (int j = 0; j < kB16Keys; ++j) {
-            if (i * kB16Keys + j >= see || (hw[j >> 4] >> (2 * (j & 15)) & 1u)) {
+            const int pos = i * kB16Keys + j;
+            if (pos >= see) continue;
+            const int64_t page = kv_page(c, w, seq, pos);
+            if (page < 0) {
               s[j] = -INFINITY;
-            } else if (special) {
-#pragma unroll
-              for (int k = 0; k < G; ++k) vnan[k] |= (note[i & 3].v_nan[j >> 4][k] >> (2 * (j & 15)) & 1u) != 0;
+              continue;
             }
+#pragma unroll
+            for (int k = 0; k < G; ++k)
+              vnan[k] |= isnan(param_scale(c.params[1][kv_row(c, page, head, pos) * G + k]));
           }
         }
-        const float ft = fminf(fmaxf(f * nt.x, 1e-37f), 1e37f);   // neither 0 nor infinity beside a masked -infinity
         float tops[4] = {s[0], s[1], s[2], s[3]};   // four chains
 #pragma unroll
         for (int j = 4; j < kB16Keys; j += 4)
@@ -392,7 +363,7 @@ __global__ void __launch_bounds__(kB16Threads, 2)
           for (int x = 0; x < 4; ++x) tops[x] = fmaxf(tops[x], s[j + x]);
         const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * ft;
         const bool move = top > m + 8.0f;
-        if (__any_sync(0xffffffffu, move) || nt.y != 1.0f) {
+        if (__any_sync(0xffffffffu, move)) {
           const float nm = move ? top : m;
           const float alpha = ex2(m - nm);
           m = nm;
@@ -402,14 +373,13 @@ __global__ void __launch_bounds__(kB16Threads, 2)
             ok = wait_warp(&v_empty[(i - 1) & 1], ((i - 1) >> 1) & 1, ICX_DEVICE_TIMEOUT_EPILOGUE);
             if (!ok) break;
             tc_fence_after();
-            const float g = alpha * nt.y;
 #pragma unroll 1
             for (int n = 0; n < D; n += 16) {
               uint32_t x[16];
               tmem_ld_32x32b_x16(t_o + t_lane + (uint32_t)n, x);
               tmem_ld_wait_regs16(x);
 #pragma unroll
-              for (int j = 0; j < 16; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * g);
+              for (int j = 0; j < 16; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * alpha);
               tmem_st_32x32b_x16(t_o + t_lane + (uint32_t)n, x);
             }
           }
@@ -448,7 +418,7 @@ __global__ void __launch_bounds__(kB16Threads, 2)
       if (tiles > 0 && ok) ok = wait_warp(o_full, 0, ICX_DEVICE_TIMEOUT_EPILOGUE);
       tc_fence_after();
       const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-      const float up = tiles > 0 ? note[(tiles - 1) & 3].v_unit : 0.0f;
+      const float up = power_of_two(v_exp);
       T* out = static_cast<T*>(a.out) +
                ((int64_t)(su.from + (mine ? r / share : 0)) * a.q_heads + head * share + (mine ? r % share : 0)) * D;
       if (ok) {
