@@ -30,7 +30,7 @@ import torch
 
 from . import _lib
 from ._lib import IcxError, KvCacheArg, KvTokensArg
-from .ops import _float_type, _name, _on, _ptr, _stream
+from .ops import _float_type, _name, _on, _ptr
 
 
 class KvCache:
@@ -73,13 +73,13 @@ class KvCache:
         self.device = self.k_codes.device
         self._arg = KvCacheArg(self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.k_params.data_ptr(),
                                self.v_params.data_ptr(), pages, page_size, kv_heads, head_dim, bits, group)
+        self._ref = ctypes.byref(self._arg)
 
 
 def _index(t, shape, device, what: str) -> torch.Tensor:
     if not isinstance(t, torch.Tensor) or t.device != device:
         raise IcxError(-1, f"{what}: expected a tensor on {device}")
-    if t.dtype != torch.int32 or t.dim() != len(shape) or any(
-            want is not None and n != want for n, want in zip(t.shape, shape)):
+    if t.dtype != torch.int32 or t.dim() != len(shape) or (shape[0] is not None and t.shape[0] != shape[0]):
         raise IcxError(-1, f"{what}: expected Int32 [{', '.join('*' if n is None else str(n) for n in shape)}], "
                            f"got {_name(t.dtype)} {list(t.shape)}")
     return t.contiguous()
@@ -111,8 +111,6 @@ def _rows(t, heads, dim, device, what: str) -> torch.Tensor:
 
 
 def _new_rows(out, shape, dtype, device, what: str) -> torch.Tensor:
-    if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
     if (not isinstance(out, torch.Tensor) or out.device != device or out.dtype != dtype
             or out.shape != shape or not out.is_contiguous() or out.data_ptr() % 16):
         raise IcxError(-1, f"{what}: expected a contiguous, 16-byte aligned {_name(dtype)} "
@@ -142,8 +140,8 @@ def gpu_kv_cache_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, page_t
         raise IcxError(-1, f"{what}: v is {_name(v.dtype)} {list(v.shape)}, "
                            f"k {_name(k.dtype)} {list(k.shape)}")
     arg, keep = _where(cache, page_table, seq_lens, cu_tokens, k.shape[0], what)
-    values = [torch.empty(k.shape, dtype=k.dtype, device=k.device) for _ in range(2)] if return_values else [None] * 2
-    _on(cache.device, _lib.load().icx_kv_cache_append, _stream(k), ctypes.byref(cache._arg), ctypes.byref(arg),
+    values = [torch.empty_like(k, memory_format=torch.contiguous_format) for _ in range(2)] if return_values else (None, None)
+    _on(cache.device, _lib.load().icx_kv_cache_append, cache._ref, ctypes.byref(arg),
         k.data_ptr(), v.data_ptr(), t, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
         _ptr(values[0]), _ptr(values[1]))
     return tuple(values) if return_values else None
@@ -170,8 +168,12 @@ def gpu_kv_cache_read(cache: KvCache, page_table: torch.Tensor, seq_lens: torch.
         raise IcxError(-1, f"{what}: tokens must not be negative")
     arg, keep = _where(cache, page_table, seq_lens, cu_tokens, tokens, what)
     shape = (tokens, cache.kv_heads, cache.head_dim)
-    k, v = (_new_rows(o, shape, dtype, cache.device, f"{what}: out") for o in (out or (None, None)))
-    _on(cache.device, _lib.load().icx_kv_cache_read, _stream(k), ctypes.byref(cache._arg), ctypes.byref(arg), t,
+    if out is None:
+        k = seq_lens.new_empty(shape, dtype=dtype)
+        v = torch.empty_like(k)
+    else:
+        k, v = (_new_rows(o, shape, dtype, cache.device, f"{what}: out") for o in out)
+    _on(cache.device, _lib.load().icx_kv_cache_read, cache._ref, ctypes.byref(arg), t,
         k.data_ptr(), v.data_ptr())
     return k, v
 
@@ -199,10 +201,13 @@ def gpu_kv_cache_attention(cache: KvCache, q: torch.Tensor, page_table: torch.Te
     if not math.isfinite(scale):
         raise IcxError(-1, f"{what}: scale must be finite")
     arg, keep = _where(cache, page_table, seq_lens, cu_tokens, q.shape[0], what)
-    out = _new_rows(out, q.shape, q.dtype, cache.device, f"{what}: out")
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    else:
+        out = _new_rows(out, q.shape, q.dtype, cache.device, f"{what}: out")
     L = _lib.load()
-    size = L.icx_kv_cache_attention_workspace_bytes(ctypes.byref(cache._arg), ctypes.byref(arg), heads)
-    ws = torch.empty(size, dtype=torch.uint8, device=cache.device) if size else None
-    _on(cache.device, L.icx_kv_cache_attention, _stream(q), ctypes.byref(cache._arg), ctypes.byref(arg),
+    size = L.icx_kv_cache_attention_workspace_bytes(cache._ref, ctypes.byref(arg), heads)
+    ws = q.new_empty(size, dtype=torch.uint8) if size else None
+    _on(cache.device, L.icx_kv_cache_attention, cache._ref, ctypes.byref(arg),
         q.data_ptr(), t, heads, q.stride(0), q.stride(1), scale, out.data_ptr(), _ptr(ws), size)
     return out

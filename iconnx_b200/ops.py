@@ -49,13 +49,23 @@ def _cuda(t: torch.Tensor, what: str) -> torch.Tensor:
     return t.contiguous()
 
 
+# The current stream's handle without the Stream object around it: the small
+# calls' time is the host's.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _on(device: torch.device, fn, *args) -> None:
-    """Calls a C entry with ``device`` current (its launches go there)."""
-    if torch.cuda.current_device() == device.index:
-        check(fn(*args))
+    """Calls a C entry with ``device`` current (its launches go there) and that
+    device's current stream as the first argument."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        status = fn(_raw_stream(index), *args)
     else:
         with torch.cuda.device(device):
-            check(fn(*args))
+            status = fn(_raw_stream(index), *args)
+    if status:
+        check(status)
 
 
 def _float_type(dtype, what: str) -> int:
@@ -331,10 +341,10 @@ def gpu_quantize_per_token(x: torch.Tensor):
         x = x.contiguous()
     rows = x.numel() // K if K else x.shape[:-1].numel()
     stride = x.stride(0) if x.dim() == 2 and x.shape[0] > 1 else K
-    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    _on(x.device, _lib.load().icx_quantize_per_token, _stream(x), x.data_ptr(), t, rows, K, stride,
-        q.data_ptr(), scale.data_ptr())
+    q = torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    _on(x.device, _lib.load().icx_quantize_per_token, x.data_ptr(), t, rows, K, stride, q.data_ptr(),
+        scale.data_ptr())
     return q, scale
 
 
@@ -372,8 +382,8 @@ def gpu_matmul_integer_scaled(q: torch.Tensor, q_scale: torch.Tensor, w: Prepare
         bias = _operand(bias, torch.float32, (w.N,), dev, f"{what}: bias")
     if residual is not None:
         residual = _operand(residual, out_dtype, shape, dev, f"{what}: residual")
-    out = torch.empty(shape, dtype=out_dtype, device=dev)
-    _on(dev, _lib.load().icx_matmul_integer_scaled, _stream(q), q.data_ptr(), q_scale.data_ptr(),
+    out = q.new_empty(shape, dtype=out_dtype)
+    _on(dev, _lib.load().icx_matmul_integer_scaled, q.data_ptr(), q_scale.data_ptr(),
         w.bt.data_ptr(), lead.numel(), w.K, w.N, w_scale.data_ptr(), _ptr(bias), _ptr(residual), t,
         out.data_ptr())
     return out
