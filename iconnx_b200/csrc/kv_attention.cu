@@ -14,7 +14,8 @@ AttendPlan plan_attend(const KvView& c, const KvTokens& w, int q_heads) {
   const int64_t rows = (w.tokens + w.batch - 1) / w.batch * share;
   p.nt = rows <= 8 ? 1 : rows <= 16 || c.dim == 256 ? 2 : 4;
   const int R = 8 * p.nt;
-  const int64_t blocks = (((int64_t)w.width << c.page_shift) + kAttBlock - 1) / kAttBlock;
+  const int block = att_block(c.dim, c.bits, R);
+  const int64_t blocks = (((int64_t)w.width << c.page_shift) + block - 1) / block;
   const int64_t units = (w.tokens * share / R + w.batch) * c.heads * (blocks > 1 ? blocks : 1);
   const int64_t resident = (int64_t)sm_count() * (c.dim * p.nt <= 128 ? 2 : 1);
   p.ctas = (int)(units < resident ? units : resident);

@@ -26,11 +26,11 @@
 // nothing.  Each lane adds its own positions' weights; lanes are joined once
 // per run of positions.
 //
-// Work: a unit is 128 positions of one (sequence, K/V head, tile of query
-// rows); each CTA takes an equal, contiguous share of all units, found on the
+// Work: a unit is a block of positions (16 or 32 per warp) of one (sequence, K/V
+// head, tile of query rows); each CTA takes an equal, contiguous share of all units, found on the
 // device from seq_lens and cu_tokens, so ragged batches balance and a captured
-// call can be replayed with other lengths.  Eight warps of a CTA take 16
-// positions each and are joined through shared memory; rows whose units went
+// call can be replayed with other lengths.  Eight warps of a CTA take
+// the block's positions in turn and are joined through shared memory; rows whose units went
 // to several CTAs leave (m, l, o) in the workspace for the join kernel.  All
 // joins run in a fixed order, so equal calls give equal results.
 #pragma once
@@ -44,7 +44,13 @@
 namespace icx {
 
 constexpr int kAttWarps = 8;
-constexpr int kAttBlock = 16 * kAttWarps;   // positions per unit
+
+// Tiles of 16 positions that a warp takes at once: two where codes and sums are
+// small enough, which halves what a step costs beside its arithmetic.
+__host__ __device__ constexpr int att_subtiles(int dim, int bits, int R) { return dim * bits <= 512 && R <= 8 ? 2 : 1; }
+__host__ __device__ constexpr int att_block(int dim, int bits, int R) {
+  return 16 * kAttWarps * att_subtiles(dim, bits, R);
+}
 constexpr float kNoScore = -1.7e38f;        // m before the first score
 
 struct AttendArgs {
@@ -66,6 +72,7 @@ struct SeqUnits {
 };
 
 __device__ __forceinline__ SeqUnits seq_units(const KvView& c, const KvTokens& w, int share, int R, int b) {
+  const int block = att_block(c.dim, c.bits, R);
   SeqUnits u;
   u.from = b;
   u.n = 1;
@@ -80,13 +87,13 @@ __device__ __forceinline__ SeqUnits seq_units(const KvView& c, const KvTokens& w
   u.rows = u.n * share;
   u.tiles = (u.rows + R - 1) / R;
   const int reach = (int)min((int64_t)u.len, (int64_t)w.width << c.page_shift);
-  u.blocks = max(1, (reach + kAttBlock - 1) / kAttBlock);
+  u.blocks = max(1, (reach + block - 1) / block);
   u.units = (int64_t)u.tiles * c.heads * u.blocks;
   return u;
 }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -94,7 +101,7 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
 
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
 
@@ -142,10 +149,15 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
-// Position (of 16) that stands in row g of the scores' left operand, and
-// g + 8 for the upper eight: an order in which neither the K rows of lanes
-// that read together nor the V rows do share banks.
-__device__ __forceinline__ int row_position(int g) { return g ^ (((g >> 1) ^ (g >> 2)) & 1); }
+// Four 8 x 8 matrices of half words, transposed: lane (g, t) gets column g,
+// rows 2t and 2t+1 of each.  Lane i gives the address of row i % 8 of matrix
+// i / 8.
+__device__ __forceinline__ void load_transposed(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
 
 template <typename T, int D, int BITS, int GROUP, int NT>
 struct AttConfig {
@@ -158,10 +170,11 @@ struct AttConfig {
   // q stays in registers where it takes at most 16
   static constexpr bool kQReg = NT == 1 && (D / 16) * 2 * (QLO ? 2 : 1) <= 16;
   static constexpr int kRowFloats = D + 2;
-  // a warp's ring: 16 positions of K and V codes and parameters per stage
-  static constexpr int ROW = D * BITS / 8;
+  // a warp's ring: per stage SUB tiles of 16 positions, each K codes, K
+  // parameters, V codes, V parameters
+  static constexpr int ROW = D * BITS / 8, SUB = att_subtiles(D, BITS, R);
   static constexpr int kCodes = 16 * ROW, kParams = 16 * G * 4;
-  static constexpr int kStage = 2 * (kCodes + kParams);
+  static constexpr int kTile = 2 * (kCodes + kParams), kStage = SUB * kTile;
   static constexpr int kFit = (kMinBlocks == 2 ? 80 : 160) * 1024 / (kAttWarps * kStage);
   static constexpr int kStages = kFit > 4 ? 4 : kFit < 2 ? 2 : kFit;
   static constexpr int kRing = kAttWarps * kStages * kStage;
@@ -178,7 +191,8 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
                           const __grid_constant__ AttendArgs a) {
   using C = AttConfig<T, D, BITS, GROUP, NT>;
   constexpr int G = C::G, R = C::R, KS = D / 16, SG = GROUP / 16, MT = D / 16;
-  constexpr int KW = D * BITS / 128, VW = D * BITS / 256;   // words of a K and a V chunk
+  constexpr int KW = D * BITS / 128;   // words of a K chunk
+  constexpr int ROW = C::ROW, SUB = C::SUB, kBlock = att_block(D, BITS, R);
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t full[kAttWarps][C::kStages];
   __shared__ int64_t s_prefix, s_total;
@@ -263,7 +277,7 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
     constexpr int QP = C::QLO ? 2 : 1;   // f16 parts of q
     uint32_t qr[C::kQReg ? KS : 1][QP][2];
     uint2* q_smem = reinterpret_cast<uint2*>(smem + C::kQOffset) + lane;   // [NT][KS][QP][32]
-    float qsum[NT][G][2], qf[NT][2];   // per column 2t and 2t+1: sums by group, score factor
+    float qsum[NT][G][2], qf[NT][2], step[NT][2];   // per column 2t and 2t+1: sums by group, score factor, 8 / factor
     int see[NT][2];                    // positions that row sees
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
@@ -282,16 +296,17 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
       peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
       // 2^e with peak * 2^e in [2^14, 2^15)
       const int e = peak > 0.0f ? max(-60, min(120, 14 - (int)((__float_as_uint(peak) >> 23) & 255) + 127)) : 0;
-      const float up = __uint_as_float((uint32_t)(e + 127) << 23);
+      // scores are held in units of 1 / f, f > 0: a negative scale turns q round
+      const float up = a.scale != 0.0f ? copysignf(__uint_as_float((uint32_t)(e + 127) << 23), a.scale) : 0.0f;
       float sums[G] = {};
 #pragma unroll
       for (int j = 0; j < KS; ++j) {
         load_f32<T, 4>(q + 16 * j + 4 * t, v, a.q_vec);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          v[i] = ok ? v[i] : 0.0f;
+          v[i] = ok && up != 0.0f ? v[i] * up : 0.0f;
           sums[j / SG] += v[i];
-          v[i] *= up * ((BITS == 4 && (j & 1)) ? 0.0625f : 1.0f);
+          if (BITS == 4 && (j & 1)) v[i] *= 0.0625f;
         }
         uint32_t part[2][2];
         part[0][0] = pack_f16(v[0], v[1]);
@@ -309,11 +324,12 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
           }
         }
       }
-      const float f = a.scale * 16777216.0f * __uint_as_float((uint32_t)(127 - e) << 23);
+      const float f = a.scale != 0.0f ? fabsf(a.scale) * 16777216.0f * __uint_as_float((uint32_t)(127 - e) << 23) : 1.0f;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int from = (2 * t + h) * 4;   // a lane that holds column 2t + h
         qf[x][h] = __shfl_sync(0xffffffffu, f, from);
+        step[x][h] = 8.0f / qf[x][h];
         const int rr = r0 + 8 * x + 2 * t + h;
         see[x][h] = rr < su.rows ? (int)max((int64_t)0, min(first_pos + rr / share + 1, (int64_t)reach)) : 0;
       }
@@ -322,7 +338,7 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
         float s = sums[k];
         s += __shfl_xor_sync(0xffffffffu, s, 1);
         s += __shfl_xor_sync(0xffffffffu, s, 2);
-        s *= a.scale;
+        s *= 5.9604644775390625e-8f;   // a code counts 2^-24
         qsum[x][k][0] = __shfl_sync(0xffffffffu, s, 8 * t);
         qsum[x][k][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
       }
@@ -336,7 +352,7 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
     for (int x = 0; x < NT; ++x)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        m[x][h] = kNoScore;
+        m[x][h] = kNoScore;   // in units of 1 / f
         l[x][h] = 0.0f;
 #pragma unroll
         for (int k = 0; k < G; ++k) vlo[x][k][h] = 0.0f;
@@ -350,114 +366,155 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
     }
 
     uint8_t* ring = smem + warp * C::kStages * C::kStage;
-    auto load = [&](int stage, int64_t page, int pos) {   // pos: first of 16
-      if (lane == 0) {
-        const int64_t row = kv_row(c, page, head, pos);
-        uint8_t* dst = ring + stage * C::kStage;
-        uint64_t* bar = &full[warp][stage];
-        mbar_arrive_expect_tx(bar, C::kStage);
-        bulk_load(dst, c.codes[0] + row * C::ROW, C::kCodes, bar);
-        bulk_load(dst + C::kCodes, c.params[0] + row * G, C::kParams, bar);
-        bulk_load(dst + C::kCodes + C::kParams, c.codes[1] + row * C::ROW, C::kCodes, bar);
-        bulk_load(dst + 2 * C::kCodes + C::kParams, c.params[1] + row * G, C::kParams, bar);
+    const int end = min(block1 * kBlock, see_any);
+    const int p0 = block0 * kBlock + warp * 16 * SUB;
+    const int tiles = p0 < end ? (end - p0 + kBlock - 1) / kBlock : 0;   // steps of SUB tiles
+    // lane i < 4 SUB brings piece i % 4 (K codes, K parameters, V codes, V
+    // parameters) of tile i / 4
+    const int my_piece = lane & 3, my_sub = (lane >> 2) & (SUB - 1);
+    const uint32_t my_bytes = (my_piece & 1) ? C::kParams : C::kCodes;
+    const int64_t my_row = (my_piece & 1) ? G * 4 : ROW;
+    const uint8_t* my_src = ((my_piece & 1) ? reinterpret_cast<const uint8_t*>(c.params[my_piece >> 1]) : c.codes[my_piece >> 1]) +
+                            ((int64_t)head << c.page_shift) * my_row;
+    const int64_t my_page_bytes = ((int64_t)c.heads << c.page_shift) * my_row;
+    const int my_dst = my_sub * C::kTile + (my_piece >> 1) * (C::kCodes + C::kParams) + (my_piece & 1) * C::kCodes;
+    // lane i holds the page of this warp's i-th tile of the current 32
+    int my_page = -1;
+    auto fetch_pages = [&](int from) {   // from: a tile, a multiple of 32
+      const int i = from + lane, p = p0 + i / SUB * kBlock + i % SUB * 16;
+      my_page = p < end ? (int)kv_page(c, w, seq, p) : -1;
+      if (p < end && my_page < 0) record_status(ICX_DEVICE_BAD_PAGE);
+    };
+    // there[stage]: bit s: tile s of the stage has a page and positions
+    uint32_t there = 0;
+    auto advance = [&](int i) {
+      if (i >= tiles || !ok) return;
+      const int st = i % C::kStages, first = i * SUB;
+      if ((first & 31) == 0) fetch_pages(first);
+      const int page = __shfl_sync(0xffffffffu, my_page, (first + my_sub) & 31);
+      const uint32_t pages = __ballot_sync(0xffffffffu, my_page >= 0) >> (first & 31) & ((1u << SUB) - 1);
+      there = (there & ~(((1u << SUB) - 1) << (st * SUB))) | pages << (st * SUB);
+      if (pages == 0) return;
+      uint64_t* bar = &full[warp][st];
+      if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)__popc(pages) * C::kTile);
+      __syncwarp();
+      if (lane < 4 * SUB && page >= 0) {
+        const int off = (p0 + my_sub * 16) & ((1 << c.page_shift) - 1);   // p0 of every step: kBlock apart
+        const int in_page = (off + i * kBlock) & ((1 << c.page_shift) - 1);
+        bulk_load(ring + st * C::kStage + my_dst, my_src + page * my_page_bytes + in_page * my_row, my_bytes, bar);
       }
     };
 
-    auto process = [&](int stage, int pos) {
-      const bool edge = pos + 16 > see_all;
-      const uint8_t* kc = ring + stage * C::kStage;
-      const uint32_t* kprm = reinterpret_cast<const uint32_t*>(kc + C::kCodes);
-      const uint8_t* vc = kc + C::kCodes + C::kParams;
-      const uint32_t* vprm = reinterpret_cast<const uint32_t*>(vc + C::kCodes);
-      uint32_t kw[2][KW];
+    // One step: SUB tiles of 16 positions.  EDGE: some row does not see some of
+    // them, or a tile has no page.
+    auto process = [&](auto edge_tag, int stage, int pos, uint32_t pages) {
+      constexpr bool EDGE = decltype(edge_tag)::value;
+      const uint8_t* base = ring + stage * C::kStage;
+      // -- scores: positions g, g + 8 of each tile (rows) x columns 2t, 2t+1
+      float s[SUB][NT][4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int at = row_position(g) + 8 * h;
+      for (int u = 0; u < SUB; ++u) {
+        const uint8_t* kc = base + u * C::kTile;
+        const uint32_t* kprm = reinterpret_cast<const uint32_t*>(kc + C::kCodes);
+        uint32_t kw[2][KW], kp[2][G];
 #pragma unroll
-        for (int i = 0; i < KW; i += 4) {
+        for (int h = 0; h < 2; ++h) {
+          const int at = g + 8 * h;
           if constexpr (KW >= 4) {
-            const uint4 u = *reinterpret_cast<const uint4*>(kc + at * C::ROW + k_word_at<C::ROW>(at, t, i));
-            kw[h][i] = u.x;
-            kw[h][i + 1] = u.y;
-            kw[h][i + 2] = u.z;
-            kw[h][i + 3] = u.w;
-          } else {
-            load_words(reinterpret_cast<const uint32_t*>(kc + at * C::ROW + k_word_at<C::ROW>(at, t, i)), kw[h]);
-          }
-        }
-      }
-      uint32_t kp[2][G];
-      load_words(kprm + row_position(g) * G, kp[0]);
-      load_words(kprm + (row_position(g) + 8) * G, kp[1]);
-      // -- scores: positions pos + g, pos + g + 8 (rows) x columns 2t, 2t+1
-      float s[NT][4] = {};
 #pragma unroll
-      for (int k = 0; k < G; ++k) {
-        float acc[NT][4] = {};
-#pragma unroll
-        for (int js = 0; js < SG; ++js) {
-          const int j = k * SG + js;
-          uint32_t A[4];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (BITS == 4) {
-              const uint32_t mask = (j & 1) ? 0x00f000f0u : 0x000f000fu;
-              const uint32_t word = kw[h][j >> 1];
-              A[h] = word & mask;
-              A[2 + h] = (word >> 8) & mask;
-            } else {
-              const uint32_t word = kw[h][j];
-              A[h] = word & 0x00ff00ffu;
-              A[2 + h] = (word >> 8) & 0x00ff00ffu;
+            for (int i = 0; i < KW; i += 4) {
+              const uint4 x = *reinterpret_cast<const uint4*>(kc + at * ROW + k_word_at<ROW>(at, t, i));
+              kw[h][i] = x.x;
+              kw[h][i + 1] = x.y;
+              kw[h][i + 2] = x.z;
+              kw[h][i + 3] = x.w;
             }
+          } else {
+            load_words(reinterpret_cast<const uint32_t*>(kc + at * ROW + k_word_at<ROW>(at, t, 0)), kw[h]);
           }
+          load_words(kprm + at * G, kp[h]);
+        }
 #pragma unroll
-          for (int x = 0; x < NT; ++x) {
+        for (int x = 0; x < NT; ++x)
 #pragma unroll
-            for (int i = 0; i < QP; ++i) {
-              if constexpr (C::kQReg) {
-                mma_f16(acc[x], A, qr[j][i][0], qr[j][i][1]);
+          for (int i = 0; i < 4; ++i) s[u][x][i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < G; ++k) {
+          float acc[NT][4] = {};
+#pragma unroll
+          for (int js = 0; js < SG; ++js) {
+            const int j = k * SG + js;
+            uint32_t A[4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (BITS == 4) {
+                const uint32_t mask = (j & 1) ? 0x00f000f0u : 0x000f000fu;
+                const uint32_t word = kw[h][j >> 1];
+                A[h] = word & mask;
+                A[2 + h] = (word >> 8) & mask;
               } else {
-                const uint2 b = q_smem[((x * KS + j) * QP + i) * 32];
-                mma_f16(acc[x], A, b.x, b.y);
+                const uint32_t word = kw[h][j];
+                A[h] = word & 0x00ff00ffu;
+                A[2 + h] = (word >> 8) & 0x00ff00ffu;
               }
             }
+#pragma unroll
+            for (int x = 0; x < NT; ++x)
+#pragma unroll
+              for (int i = 0; i < QP; ++i) {
+                if constexpr (C::kQReg) {
+                  mma_f16(acc[x], A, qr[j][i][0], qr[j][i][1]);
+                } else {
+                  const uint2 b = q_smem[((x * KS + j) * QP + i) * 32];
+                  mma_f16(acc[x], A, b.x, b.y);
+                }
+              }
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float sc = param_scale(kp[h][k]), lo = param_low(kp[h][k]);
+#pragma unroll
+            for (int x = 0; x < NT; ++x)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                float& v = s[u][x][2 * h + i];
+                v = k == 0 ? lo * qsum[x][k][i] : fmaf(lo, qsum[x][k][i], v);
+                v = fmaf(sc, acc[x][2 * h + i], v);
+              }
           }
         }
+        if (EDGE) {
 #pragma unroll
-        for (int x = 0; x < NT; ++x)
+          for (int x = 0; x < NT; ++x)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t p = kp[i >> 1][k];
-            s[x][i] = fmaf(param_scale(p), acc[x][i] * qf[x][i & 1], s[x][i]);
-            s[x][i] = fmaf(param_low(p), qsum[x][k][i & 1], s[x][i]);
-          }
-      }
-      if (edge) {
-#pragma unroll
-        for (int x = 0; x < NT; ++x)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (pos + row_position(g) + 8 * (i >> 1) >= see[x][i & 1]) s[x][i] = -INFINITY;
+            for (int i = 0; i < 4; ++i)
+              if (!(pages >> u & 1u) || pos + 16 * u + g + 8 * (i >> 1) >= see[x][i & 1]) s[u][x][i] = -INFINITY;
+        }
       }
       // -- the reference follows the scores in steps of at least 8
       bool move = false;
+      float top[NT][2];
 #pragma unroll
       for (int x = 0; x < NT; ++x)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) move |= fmaxf(s[x][h], s[x][2 + h]) > m[x][h] + 8.0f;
+        for (int h = 0; h < 2; ++h) {
+          top[x][h] = fmaxf(s[0][x][h], s[0][x][2 + h]);
+#pragma unroll
+          for (int u = 1; u < SUB; ++u) top[x][h] = fmaxf(top[x][h], fmaxf(s[u][x][h], s[u][x][2 + h]));
+          move |= top[x][h] > m[x][h] + step[x][h];
+        }
       if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
         for (int x = 0; x < NT; ++x)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float top = fmaxf(s[x][h], s[x][2 + h]);
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            top = fmaxf(top, m[x][h]);
-            const float f = ex2(m[x][h] - top);
-            m[x][h] = top;
+            float v = top[x][h];
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+            v = fmaxf(v, m[x][h]);
+            const float f = ex2((m[x][h] - v) * qf[x][h]);
+            m[x][h] = v;
             l[x][h] *= f;
 #pragma unroll
             for (int k = 0; k < G; ++k) vlo[x][k][h] *= f;
@@ -471,31 +528,42 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
 #pragma unroll
       for (int x = 0; x < NT; ++x)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[x][i] = ex2(s[x][i] - m[x][i & 1]);
-          l[x][i & 1] += s[x][i];
+        for (int h = 0; h < 2; ++h) {
+          const float mf = fmaxf(m[x][h] * qf[x][h], -3e38f);   // finite before the first score
+#pragma unroll
+          for (int u = 0; u < SUB; ++u)
+#pragma unroll
+            for (int i = h; i < 4; i += 2) {
+              s[u][x][i] = ex2(fmaf(s[u][x][i], qf[x][h], -mf));
+              l[x][h] += s[u][x][i];
+            }
         }
       // -- the scale of w s follows the largest s
       bool grow = false;
-      uint32_t vp[2][G];
-      load_words(vprm + row_position(g) * G, vp[0]);
-      load_words(vprm + (row_position(g) + 8) * G, vp[1]);
+      uint32_t vp[SUB][2][G];
 #pragma unroll
-      for (int k = 0; k < G; ++k)
+      for (int u = 0; u < SUB; ++u)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          // positions behind the last hold whatever the page held before
-          if (edge && pos + row_position(g) + 8 * h >= see_any) vp[h][k] = 0u;
-          grow |= param_scale(vp[h][k]) > vmax[k];
+          load_words(reinterpret_cast<const uint32_t*>(base + u * C::kTile + 2 * C::kCodes + C::kParams) + (g + 8 * h) * G,
+                     vp[u][h]);
+#pragma unroll
+          for (int k = 0; k < G; ++k) {
+            // positions behind the last hold whatever the page held before
+            if (EDGE && (!(pages >> u & 1u) || pos + 16 * u + g + 8 * h >= see_any)) vp[u][h][k] = 0u;
+            grow |= param_scale(vp[u][h][k]) > vmax[k];
+          }
         }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int k = 0; k < G; ++k) {
-          float top = fmaxf(vmax[k], fmaxf(param_scale(vp[0][k]), param_scale(vp[1][k])));
-          top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-          if (!(top > vmax[k])) continue;
-          // top in [2^(E-1), 2^E): 2^(5-E) leaves it below 2^5, with room for 4 times as much
-          const int E = min(max((int)(__float_as_uint(top) >> 23) - 126, -90), 128);
+          float v = vmax[k];
+#pragma unroll
+          for (int u = 0; u < SUB; ++u) v = fmaxf(v, fmaxf(param_scale(vp[u][0][k]), param_scale(vp[u][1][k])));
+          v = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
+          if (!(v > vmax[k])) continue;
+          // v in [2^(E-1), 2^E): 2^(5-E) leaves it below 2^5, with room for 4 times as much
+          const int E = min(max((int)(__float_as_uint(v) >> 23) - 126, -90), 128);
           const float down = __uint_as_float((uint32_t)(5 - E + 127) << 23);
           const float f = vmax[k] > 0.0f ? down / vdown[k] : 0.0f;
           vmax[k] = __uint_as_float((uint32_t)(min(E + 2, 127) + 127) << 23);
@@ -508,110 +576,88 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
               for (int q = 0; q < 4; ++q) o[x][k * (GROUP / 16) + i][q] *= f;
         }
       }
-      // -- output: rows are dimensions, the contraction runs over the positions;
-      // contraction indices 2t, 2t+1, 2t+8, 2t+9 are the score rows of that name
-      uint32_t vw[4][VW];
+      // -- output: rows are dimensions, the contraction runs over the positions
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int at = row_position(2 * t + (i & 1)) + 8 * (i >> 1);
+      for (int u = 0; u < SUB; ++u) {
+        uint32_t ph[G][NT][2], pl[C::PLO ? G : 1][C::PLO ? NT : 1][2];
 #pragma unroll
-        for (int j = 0; j < VW; j += 4) {
-          const uint32_t* p = reinterpret_cast<const uint32_t*>(vc + at * C::ROW + v_word_at<C::ROW>(at, g, j));
-          if constexpr (VW >= 4) {
-            const uint4 u = *reinterpret_cast<const uint4*>(p);
-            vw[i][j] = u.x;
-            vw[i][j + 1] = u.y;
-            vw[i][j + 2] = u.z;
-            vw[i][j + 3] = u.w;
-          } else {
-            load_words(p, vw[i]);
-          }
-        }
-      }
+        for (int k = 0; k < G; ++k)
 #pragma unroll
-      for (int k = 0; k < G; ++k) {
-        uint32_t ph[NT][2], pl[C::PLO ? NT : 1][2];
+          for (int h = 0; h < 2; ++h) {
+            const float sv = param_scale(vp[u][h][k]) * vdown[k], lo = param_low(vp[u][h][k]);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float sv = param_scale(vp[h][k]) * vdown[k], lo = param_low(vp[h][k]);
-#pragma unroll
-          for (int x = 0; x < NT; ++x) {
-            float p0 = s[x][2 * h], p1 = s[x][2 * h + 1];
-            float w0 = p0 * sv, w1 = p1 * sv, z0 = p0 * lo, z1 = p1 * lo;
-            if (edge) {   // a position that a row does not see gives it nothing, NaN or not
-              const int at = pos + row_position(g) + 8 * h;
-              if (at >= see[x][0]) w0 = z0 = 0.0f;
-              if (at >= see[x][1]) w1 = z1 = 0.0f;
-            }
-            vlo[x][k][0] += z0;
-            vlo[x][k][1] += z1;
-            const uint32_t hi = pack_f16(w0, w1);
-            ph[x][h] = transpose_8x8(hi);
-            if constexpr (C::PLO) {
-              const float2 f = unpack_f16(hi);
-              pl[x][h] = transpose_8x8(pack_f16(w0 - f.x, w1 - f.y));
+            for (int x = 0; x < NT; ++x) {
+              const float e0 = s[u][x][2 * h], e1 = s[u][x][2 * h + 1];
+              float w0 = e0 * sv, w1 = e1 * sv;
+              if (EDGE) {   // a position that a row does not see gives it nothing, NaN or not
+                const int at = pos + 16 * u + g + 8 * h;
+                if (at >= see[x][0]) w0 = 0.0f;
+                else vlo[x][k][0] = fmaf(e0, lo, vlo[x][k][0]);
+                if (at >= see[x][1]) w1 = 0.0f;
+                else vlo[x][k][1] = fmaf(e1, lo, vlo[x][k][1]);
+              } else {
+                vlo[x][k][0] = fmaf(e0, lo, vlo[x][k][0]);
+                vlo[x][k][1] = fmaf(e1, lo, vlo[x][k][1]);
+              }
+              const uint32_t hi = pack_f16(w0, w1);
+              ph[k][x][h] = transpose_8x8(hi);
+              if constexpr (C::PLO) {
+                const float2 f = unpack_f16(hi);
+                pl[k][x][h] = transpose_8x8(pack_f16(w0 - f.x, w1 - f.y));
+              }
             }
           }
-        }
+        // lane's row: position lane % 16, piece lane / 16 of a pair
+        const int vr = lane & 15;
+        const uint32_t v_at = smem_addr(base + u * C::kTile + C::kCodes + C::kParams) + vr * ROW;
+        const int v_x = (lane >> 4) ^ v_swizzle<ROW>(vr);
 #pragma unroll
-        for (int i = 0; i < GROUP / 16; ++i) {
-          const int mt = k * (GROUP / 16) + i;
-          uint32_t A[4];
+        for (int pp = 0; pp < ROW / 16; pp += 2) {
+          uint32_t r[4];   // pieces pp and pp + 1: positions 2t, 2t+1 and 2t+8, 2t+9
+          load_transposed(v_at + ((v_x ^ pp) << 4), r);
+          constexpr int kPerPiece = 8 / BITS;   // row tiles
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {   // positions 2t, 2t+1 and 2t+8, 2t+9
+          for (int q = 0; q < 2 * kPerPiece; ++q) {
+            const int mt = pp * kPerPiece + q, k = mt / (GROUP / 16);
+            const uint32_t lo8 = r[q / kPerPiece * 2], hi8 = r[q / kPerPiece * 2 + 1];
+            uint32_t A[4];
             if (BITS == 4) {
-              const uint32_t pair = __byte_perm(vw[2 * h][mt >> 2], vw[2 * h + 1][mt >> 2],
-                                                (mt & 2) ? 0x7632 : 0x5410) >> (8 * (mt & 1));
-              A[2 * h] = pair & 0x000f000fu;
-              A[2 * h + 1] = pair & 0x00f000f0u;
+              const uint32_t a0 = (q & 1) ? lo8 >> 8 : lo8, a1 = (q & 1) ? hi8 >> 8 : hi8;
+              A[0] = a0 & 0x000f000fu;
+              A[1] = a0 & 0x00f000f0u;
+              A[2] = a1 & 0x000f000fu;
+              A[3] = a1 & 0x00f000f0u;
             } else {
-              const uint32_t pair = __byte_perm(vw[2 * h][mt >> 1], vw[2 * h + 1][mt >> 1],
-                                                (mt & 1) ? 0x7632 : 0x5410);
-              A[2 * h] = pair & 0x00ff00ffu;
-              A[2 * h + 1] = (pair >> 8) & 0x00ff00ffu;
+              A[0] = lo8 & 0x00ff00ffu;
+              A[1] = (lo8 >> 8) & 0x00ff00ffu;
+              A[2] = hi8 & 0x00ff00ffu;
+              A[3] = (hi8 >> 8) & 0x00ff00ffu;
             }
-          }
 #pragma unroll
-          for (int x = 0; x < NT; ++x) {
-            mma_f16(o[x][mt], A, ph[x][0], ph[x][1]);
-            if constexpr (C::PLO) mma_f16(o[x][mt], A, pl[x][0], pl[x][1]);
+            for (int x = 0; x < NT; ++x) {
+              mma_f16(o[x][mt], A, ph[k][x][0], ph[k][x][1]);
+              if constexpr (C::PLO) mma_f16(o[x][mt], A, pl[k][x][0], pl[k][x][1]);
+            }
           }
         }
       }
     };
 
     // ------------------------------------------------------ the positions
-    const int end = min(block1 * kAttBlock, see_any);
-    const int p0 = block0 * kAttBlock + warp * 16;
-    const int tiles = p0 < end ? (end - p0 + kAttBlock - 1) / kAttBlock : 0;
-    uint32_t bad = 0;   // stages whose tile has no page
-    // lane i holds the page of this warp's tile (32 n + i)
-    int my_page = -1;
-    auto fetch_pages = [&](int from) {
-      const int p = p0 + (from + lane) * kAttBlock;
-      my_page = from + lane < tiles ? (int)kv_page(c, w, seq, p) : -1;
-      if (from + lane < tiles && my_page < 0) record_status(ICX_DEVICE_BAD_PAGE);
-    };
-    // pages are taken in order, and the ring holds the next kStages - 1 tiles
-    auto advance = [&](int i) {
-      if (i >= tiles || !ok) return;
-      if ((i & 31) == 0) fetch_pages(i);
-      const int page = __shfl_sync(0xffffffffu, my_page, i & 31);
-      if (page >= 0) load(i % C::kStages, page, p0 + i * kAttBlock);
-      else bad |= 1u << (i % C::kStages);
-    };
+    // the ring holds the next kStages - 1 steps
     for (int i = 0; i < C::kStages - 1; ++i) advance(i);
     for (int i = 0; i < tiles; ++i) {
       const int stage = i % C::kStages;
       __syncwarp();   // every lane is done with the stage that is filled next
       advance(i + C::kStages - 1);
-      if (bad >> stage & 1) {
-        bad &= ~(1u << stage);
-        continue;
-      }
+      const uint32_t pages = there >> (stage * SUB) & ((1u << SUB) - 1);
+      if (pages == 0) continue;
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][stage], phase >> stage & 1, ICX_DEVICE_TIMEOUT_CACHE));
       phase ^= 1u << stage;
-      if (ok) process(stage, p0 + i * kAttBlock);
+      const int pos = p0 + i * kBlock;
+      if (!ok) continue;
+      if (pos + 16 * SUB > see_all || pages != (1u << SUB) - 1) process(std::true_type{}, stage, pos, pages);
+      else process(std::false_type{}, stage, pos, pages);
     }
 
     // --------------------------------------------- join lanes, then warps
@@ -635,6 +681,10 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l[x][h] += __shfl_xor_sync(0xffffffffu, l[x][h], d);
       }
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) m[x][h] = fmaxf(m[x][h] * qf[x][h], kNoScore);   // in powers of two from here
     __syncthreads();   // the ring is free
 #pragma unroll
     for (int half = kAttWarps / 2; half >= 1; half >>= 1) {

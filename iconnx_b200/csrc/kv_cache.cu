@@ -166,8 +166,7 @@ __device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c
 
 // One block of 64 dimensions: eight lanes (l = 0..7) of eight consecutive
 // dimensions.  Lane l holds step / row tile j = l / 2 of the block, quarters
-// 2 (l & 1) and 2 (l & 1) + 1 of it (K), or thread chunks g = 4 (l & 1) .. + 3
-// (V).  The shuffles stay inside the eight lanes; all 32 lanes take part.
+// 2 (l & 1) and 2 (l & 1) + 1 of it (K), or g = 4 (l & 1) .. + 3 (V).  The shuffles stay inside the eight lanes; all 32 lanes take part.
 template <int BITS, int D>
 __device__ __forceinline__ void store_block(uint8_t* row, int token, int which, int block, int l,
                                             const uint32_t (&c)[8], bool valid) {
@@ -189,23 +188,15 @@ __device__ __forceinline__ void store_block(uint8_t* row, int token, int which, 
       put(k_word_at<ROW>(token, 2 * odd + 1, block * 4 + j), b);
     }
   } else if (BITS == 4) {
-    // byte i: chunk 4 odd + i, codes 2j and 2j+1; a 4 x 4 byte transposition
-    // over the lanes j leaves lane j with the word of chunk 4 odd + j
-    uint32_t u = low_bytes(c[0], c[2], c[4], c[6]) | (low_bytes(c[1], c[3], c[5], c[7]) << 4);
-    uint32_t v = __shfl_xor_sync(0xffffffffu, u, 2);
-    u = (j & 1) ? __byte_perm(v, u, 0x7351) : __byte_perm(u, v, 0x6240);
-    v = __shfl_xor_sync(0xffffffffu, u, 4);
-    u = (j & 2) ? __byte_perm(v, u, 0x7632) : __byte_perm(u, v, 0x5410);
-    put(v_word_at<ROW>(token, 4 * odd + j, block), u);
-  } else {
-    // half words of chunks 4 odd + {0,1} and {2,3}; lanes j and j ^ 1 exchange
-    // so that each holds whole words of two chunks
-    const uint32_t a = low_bytes(c[0], c[1], c[2], c[3]), b = low_bytes(c[4], c[5], c[6], c[7]);
-    const uint32_t other = __shfl_xor_sync(0xffffffffu, (j & 1) ? a : b, 2);
-    const uint32_t lo = (j & 1) ? other : a, hi = (j & 1) ? b : other;
-    const int g = 4 * odd + 2 * (j & 1), w = block * 2 + (j >> 1);
-    put(v_word_at<ROW>(token, g, w), __byte_perm(lo, hi, 0x5410));
-    put(v_word_at<ROW>(token, g + 1, w), __byte_perm(lo, hi, 0x7632));
+    // byte i: g = 4 odd + i, tile j; lanes j and j ^ 1 hold the two tiles of a
+    // piece and exchange so that each stores the half words of two g
+    const uint32_t u = low_bytes(c[0], c[2], c[4], c[6]) | (low_bytes(c[1], c[3], c[5], c[7]) << 4);
+    const uint32_t v = __shfl_xor_sync(0xffffffffu, u, 2);
+    put(((block * 2 + (j >> 1)) ^ v_swizzle<ROW>(token)) * 16 + 8 * odd + 4 * (j & 1),
+        (j & 1) ? __byte_perm(v, u, 0x7362) : __byte_perm(u, v, 0x5140));
+  } else if (valid) {
+    *reinterpret_cast<uint2*>(row + ((block * 4 + j) ^ v_swizzle<ROW>(token)) * 16 + 8 * odd) =
+        make_uint2(low_bytes(c[0], c[1], c[2], c[3]), low_bytes(c[4], c[5], c[6], c[7]));
   }
 }
 
@@ -222,11 +213,11 @@ __device__ __forceinline__ void load_block_words(const uint8_t* row, int token, 
     w[0] = get(k_word_at<ROW>(token, 2 * odd, n));
     w[1] = get(k_word_at<ROW>(token, 2 * odd + 1, n));
   } else if (BITS == 4) {
-    w[0] = get(v_word_at<ROW>(token, 4 * odd + j, block));
+    w[0] = get(((block * 2 + (j >> 1)) ^ v_swizzle<ROW>(token)) * 16 + 8 * odd + 4 * (j & 1));
   } else {
-    const int g = 4 * odd + 2 * (j & 1), n = block * 2 + (j >> 1);
-    w[0] = get(v_word_at<ROW>(token, g, n));
-    w[1] = get(v_word_at<ROW>(token, g + 1, n));
+    const uint2 u = *reinterpret_cast<const uint2*>(row + ((block * 4 + j) ^ v_swizzle<ROW>(token)) * 16 + 8 * odd);
+    w[0] = u.x;
+    w[1] = u.y;
   }
 }
 // Eight codes, each on the bits of 2^23 (2^23 + code as an f32).
@@ -249,11 +240,8 @@ __device__ __forceinline__ void block_codes(int which, int l, const uint32_t (&w
       c[4 * h + 3] = code_at(u, 3);
     }
   } else if (BITS == 4) {
-    uint32_t u = w[0];
-    uint32_t v = __shfl_xor_sync(0xffffffffu, u, 2);
-    u = (j & 1) ? __byte_perm(v, u, 0x7351) : __byte_perm(u, v, 0x6240);
-    v = __shfl_xor_sync(0xffffffffu, u, 4);
-    u = (j & 2) ? __byte_perm(v, u, 0x7632) : __byte_perm(u, v, 0x5410);
+    const uint32_t v = __shfl_xor_sync(0xffffffffu, w[0], 2);
+    const uint32_t u = (j & 1) ? __byte_perm(v, w[0], 0x7531) : __byte_perm(w[0], v, 0x6420);
     const uint32_t even = u & 0x0f0f0f0fu, odd = (u >> 4) & 0x0f0f0f0fu;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -261,13 +249,10 @@ __device__ __forceinline__ void block_codes(int which, int l, const uint32_t (&w
       c[2 * i + 1] = code_at(odd, i);
     }
   } else {
-    const uint32_t lo = __byte_perm(w[0], w[1], 0x5410), hi = __byte_perm(w[0], w[1], 0x7632);
-    const uint32_t other = __shfl_xor_sync(0xffffffffu, (j & 1) ? lo : hi, 2);
-    const uint32_t a = (j & 1) ? other : lo, b = (j & 1) ? hi : other;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      c[i] = code_at(a, i);
-      c[4 + i] = code_at(b, i);
+      c[i] = code_at(w[0], i);
+      c[4 + i] = code_at(w[1], i);
     }
   }
 }

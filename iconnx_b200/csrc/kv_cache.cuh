@@ -5,9 +5,8 @@
 // token of the page), so 16 consecutive tokens are one contiguous piece that a
 // bulk copy brings to shared memory as it stands.  Inside a row the codes are
 // ordered for the attention's matrix instructions (m16n8k16, thread (g, t) of
-// a warp: g = lane / 4, t = lane % 4): what a thread needs is consecutive, and
-// the places are exchanged by token so that a warp's reads meet no shared
-// memory bank twice.
+// a warp: g = lane / 4, t = lane % 4), and 16-byte pieces are exchanged by
+// token so that a warp's reads meet no shared memory bank twice.
 //
 //   K is the left operand of the scores (rows = tokens, contraction over the
 //   dimensions).  Step j of the contraction covers dimensions 16j .. 16j+15,
@@ -20,12 +19,13 @@
 //     8 bits: word j of a chunk holds step j; dimension i stands in byte
 //             {0, 2, 1, 3}[i].
 //   V is the left operand of the output (rows = dimensions, contraction over
-//   the tokens).  Row tile m covers dimensions 16m .. 16m+15, of which thread
-//   g holds 16m + 2g + {0,1}.  The row is eight chunks, one per g; dimension
-//   16m + 2g + h is code 2m + h of chunk g, in order of the bits.  Chunks of
-//   32 bytes are cut into two pieces, first all first ones.  Chunk g stands at
-//   place g ^ 2h (16-byte pieces) or g ^ 4 (h & 1) (8 bytes), h = bits 1 and 2
-//   of the token.
+//   the tokens), read by transposing 8 x 8 half words.  Row tile m covers
+//   dimensions 16m .. 16m+15, of which thread g holds 16m + 2g + {0,1}.
+//   A 16-byte piece is one half word per g:
+//     4 bits: piece p holds tiles 2p and 2p+1: (tile 2p: dimensions 2g, 2g+1;
+//             tile 2p+1: the same), four nibbles from the low bits up.
+//     8 bits: piece p holds tile p, two bytes.
+//   Piece p stands at place p ^ v_swizzle(token).
 #pragma once
 
 #include "floats.cuh"
@@ -81,8 +81,8 @@ __device__ __forceinline__ int64_t kv_row(const KvView& c, int64_t page, int hea
   return (((page * c.heads) + head) << c.page_shift) + (p & ((1 << c.page_shift) - 1));
 }
 
-// Byte where word w of K chunk t stands in the row of a token, and word w of
-// V chunk g.  ROW = bytes per row.
+// Byte where word w of K chunk t stands in the row of a token.  ROW = bytes per
+// row.
 template <int ROW>
 __device__ __forceinline__ int k_word_at(int token, int t, int w) {
   if (ROW == 32) return t * 8 + w * 4;
@@ -90,11 +90,8 @@ __device__ __forceinline__ int k_word_at(int token, int t, int w) {
   return piece * 64 + t * 16 + (w & 3) * 4;
 }
 template <int ROW>
-__device__ __forceinline__ int v_word_at(int token, int g, int w) {
-  const int h = (token >> 1) & 3;
-  if (ROW == 32) return g * 4;
-  if (ROW == 64) return (g ^ (4 * (h & 1))) * 8 + w * 4;
-  return (w >> 2) * 128 + (g ^ (2 * h)) * 16 + (w & 3) * 4;
+__device__ __forceinline__ int v_swizzle(int token) {
+  return ROW == 32 ? (token >> 2) & 1 : ROW == 64 ? (token >> 1) & 3 : token & 7;
 }
 
 }  // namespace icx

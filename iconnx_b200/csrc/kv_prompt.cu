@@ -160,8 +160,8 @@ __global__ void __launch_bounds__(kPrThreads, 2)
             }
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            const int piece = 4 * half + x, at = BITS == 4 ? k : 2 * k;
-            *reinterpret_cast<uint4*>(vr + ((piece ^ (key & 7)) << 4)) = spread<BITS>(raw.v[x][at], raw.v[x][BITS == 4 ? at : at + 1]);
+            const int piece = 4 * half + x;
+            *reinterpret_cast<uint4*>(vr + ((piece ^ (key & 7)) << 4)) = spread<BITS>(raw.v[k][BITS / 4 * x], raw.v[k][BITS == 4 ? x : 2 * x + 1]);
           }
         }
         const uint32_t holes = __ballot_sync(0xffffffffu, hole);   // bit: two lanes per position
@@ -407,25 +407,24 @@ __global__ void __launch_bounds__(kPrThreads, 2)
 #pragma unroll
           for (int kk = 1; kk < G; ++kk) low = k == kk ? vlo[kk] : low;
 #pragma unroll 1
-          for (int n = 0; n < 2; ++n) {   // pieces g = 4 n .. 4 n + 3
+          for (int n = 0; n < 2; ++n) {   // dimensions 32 n .. 32 n + 31 of the group
             uint32_t x[32];
             if (tiles > 0) {
               tmem_ld_32x32b_x32(t_o + (uint32_t)(k * kPrGroup + 32 * n), x);
               tmem_ld_wait_regs(x);
             }
-            // dimensions 16 m + 8 n .. + 7: 2 g + h of the four pieces
             float y[4][8];
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                const float o = tiles > 0 ? __uint_as_float(x[8 * g + i]) : 0.0f;
-                y[v_tile<BITS>(i)][2 * g + v_half(i)] =
-                    l != 0.0f ? fmaf(o * (times16<BITS>(i) ? 1048576.0f : 16777216.0f), up, low) * inv : 0.0f;
+                const float o = tiles > 0 ? __uint_as_float(x[8 * j + i]) : 0.0f;
+                const int d = v_dim<BITS>(j, i);
+                y[d >> 3][d & 7] = l != 0.0f ? fmaf(o * (times16<BITS>(i) ? 1048576.0f : 16777216.0f), up, low) * inv : 0.0f;
               }
             if (mine)
 #pragma unroll
-              for (int mt = 0; mt < 4; ++mt) store_f32<T, 8>(out + k * kPrGroup + 16 * mt + 8 * n, y[mt]);
+              for (int j = 0; j < 4; ++j) store_f32<T, 8>(out + k * kPrGroup + 32 * n + 8 * j, y[j]);
           }
         }
       }

@@ -42,12 +42,13 @@ template <int BITS>
 __host__ __device__ constexpr int k_dim(int r) {
   return BITS == 4 ? (r & 1) + 2 * (r >> 2) : ((r >> 1) & 1) * 2 + (r & 1);
 }
-// V: piece g, r-th value: dimension 16 m + 2 g + h of the group.
+// V: a group's pieces 4 n .. 4 n + 3 are its dimensions 32 n .. 32 n + 31; the
+// r-th value of the j-th of them is dimension 32 n + v_dim(j, r).
 template <int BITS>
-__host__ __device__ constexpr int v_tile(int r) {
-  return BITS == 4 ? 2 * (r & 1) + (r >> 2) : (r & 1) + 2 * (r >> 2);
+__host__ __device__ constexpr int v_dim(int j, int r) {
+  const int pair = ((r & 1) << 1) | ((r >> 1) & 1);   // {0, 2, 1, 3}
+  return BITS == 4 ? 16 * (r >> 2) + 4 * j + pair : 16 * (j >> 1) + 8 * (j & 1) + 4 * (r >> 2) + pair;
 }
-__host__ __device__ constexpr int v_half(int r) { return (r >> 1) & 1; }
 // 4 bits: these values are sixteen times their code
 template <int BITS>
 __host__ __device__ constexpr bool times16(int r) {
@@ -95,32 +96,40 @@ __device__ __forceinline__ void find_row_tile(const KvView& c, const KvTokens& w
   }
 }
 
-// The codes of one position: words of K chunks 2 half, 2 half + 1 and of V
-// chunks 4 half .. 4 half + 3.
+// Half the codes of one position: words of K chunks 2 half, 2 half + 1, and the
+// V words of each group's dimensions 32 half .. 32 half + 31.
 template <int D, int BITS>
 struct RawCodes {
-  static constexpr int ROW = D * BITS / 8, KW = D * BITS / 128, VW = KW / 2;
-  uint32_t k[2][KW], v[4][VW];
-  __device__ __forceinline__ void load(const KvView& c, int64_t row, int pos, int half) {
-    load_k(c, row, pos, half);
-    load_v(c, row, pos, half);
+  static constexpr int ROW = D * BITS / 8, KW = D * BITS / 128, VW = BITS, G = D / 64;
+  uint32_t k[2][KW], v[G][VW];
+  __device__ __forceinline__ void load(const KvView& c, int64_t row, int token, int half) {
+    load_k(c, row, token, half);
+    load_v(c, row, token, half);
   }
-  __device__ __forceinline__ void load_v(const KvView& c, int64_t row, int pos, int half) {
+  __device__ __forceinline__ void load_v(const KvView& c, int64_t row, int token, int half) {
     const uint8_t* vr = c.codes[1] + row * ROW;
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
-      load_words(reinterpret_cast<const uint32_t*>(vr + v_word_at<ROW>(pos, 4 * half + x, 0)), v[x]);
+    for (int x = 0; x < G; ++x)
+#pragma unroll
+      for (int n = 0; n < VW / 4; ++n) {
+        const int piece = BITS == 4 ? 2 * x + half : 4 * x + 2 * half + n;
+        const uint4 u = *reinterpret_cast<const uint4*>(vr + ((piece ^ v_swizzle<ROW>(token)) << 4));
+        v[x][4 * n] = u.x;
+        v[x][4 * n + 1] = u.y;
+        v[x][4 * n + 2] = u.z;
+        v[x][4 * n + 3] = u.w;
+      }
   }
-  __device__ __forceinline__ void load_k(const KvView& c, int64_t row, int pos, int half) {
+  __device__ __forceinline__ void load_k(const KvView& c, int64_t row, int token, int half) {
     const uint8_t* kr = c.codes[0] + row * ROW;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       if constexpr (KW < 4) {
-        load_words(reinterpret_cast<const uint32_t*>(kr + k_word_at<ROW>(pos, 2 * half + x, 0)), k[x]);
+        load_words(reinterpret_cast<const uint32_t*>(kr + k_word_at<ROW>(token, 2 * half + x, 0)), k[x]);
       } else {
 #pragma unroll
         for (int n = 0; n < KW; n += 4) {
-          const uint4 u = *reinterpret_cast<const uint4*>(kr + k_word_at<ROW>(pos, 2 * half + x, n));
+          const uint4 u = *reinterpret_cast<const uint4*>(kr + k_word_at<ROW>(token, 2 * half + x, n));
           k[x][n] = u.x;
           k[x][n + 1] = u.y;
           k[x][n + 2] = u.z;

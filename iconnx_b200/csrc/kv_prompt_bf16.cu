@@ -242,23 +242,25 @@ __global__ void __launch_bounds__(kB16Threads, 2)
         const int64_t page = pos < see_any ? kv_page(c, w, seq, pos) : -1;
         row_next = page >= 0 ? kv_row(c, page, head, pos) : -1;
       };
-      auto fetch_k = [&](int i) {
+      // (a tile is a multiple of 16 positions: the swizzle of the thread's row
+      // is the same in all of them)
+      auto fetch_k = [&]() {
         if (row_next < 0) return;
-        raw.load_k(c, row_next, i * kB16Keys + key, half);
+        raw.load_k(c, row_next, key, half);
         load_words(c.params[0] + row_next * G, kp);
         load_words(c.params[1] + row_next * G, vp);
       };
-      auto fetch_v = [&](int i) {
-        if (row >= 0) raw.load_v(c, row, i * kB16Keys + key, half);
+      auto fetch_v = [&]() {
+        if (row >= 0) raw.load_v(c, row, key, half);
       };
       const float k_down = power_of_two(-k_exp), v_down = power_of_two(-v_exp);
       const float k_up24 = k_down * 16777216.0f, v_up24 = v_down * 16777216.0f;
       bool ok = true;
       if (tiles > 0) {
         find(0);
-        fetch_k(0);
+        fetch_k();
         row = row_next;
-        fetch_v(0);
+        fetch_v();
         if (tiles > 1) find(1);
       }
       for (int i = 0; i < tiles; ++i) {
@@ -283,7 +285,7 @@ __global__ void __launch_bounds__(kB16Threads, 2)
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&k_full[st]);
-        if (i + 1 < tiles) fetch_k(i + 1);
+        if (i + 1 < tiles) fetch_k();
         if (ok) ok = wait_warp(&v_empty[st], ((i >> 1) & 1) ^ 1, ICX_DEVICE_TIMEOUT_PRODUCER);
 #pragma unroll
         for (int k = 0; k < G; ++k) {
@@ -291,16 +293,16 @@ __global__ void __launch_bounds__(kB16Threads, 2)
           uint8_t* vr = s_v(st) + k * kB16Keys * 128 + key * 128;
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            const int piece = 4 * half + x, at = BITS == 4 ? k : 2 * k;
+            const int piece = 4 * half + x;
             *reinterpret_cast<uint4*>(vr + ((piece ^ (key & 7)) << 4)) =
-                dequantize<BITS>(raw.v[x][at], raw.v[x][BITS == 4 ? at : at + 1], g);
+                dequantize<BITS>(raw.v[k][BITS / 4 * x], raw.v[k][BITS == 4 ? x : 2 * x + 1], g);
           }
         }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&v_full[st]);
         row = row_next;
-        if (i + 1 < tiles) fetch_v(i + 1);
+        if (i + 1 < tiles) fetch_v();
         if (i + 2 < tiles) find(i + 2);
       }
     } else {
@@ -428,23 +430,24 @@ __global__ void __launch_bounds__(kB16Threads, 2)
 #pragma unroll
           for (int kk = 1; kk < G; ++kk) bad = k == kk ? vnan[kk] : bad;
 #pragma unroll 1
-          for (int n = 0; n < 2; ++n) {   // pieces g = 4 n .. 4 n + 3
+          for (int n = 0; n < 2; ++n) {   // dimensions 32 n .. 32 n + 31 of the group
             uint32_t x[32];
             if (tiles > 0) {
               tmem_ld_32x32b_x32(t_o + t_lane + (uint32_t)(k * kPrGroup + 32 * n), x);
               tmem_ld_wait_regs(x);
             }
-            float y[4][8];   // dimensions 16 m + 8 n .. + 7: 2 g + h of the four pieces
+            float y[4][8];
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const float o = tiles > 0 ? __uint_as_float(x[8 * g + j]) : 0.0f;
-                y[v_tile<BITS>(j)][2 * g + v_half(j)] = bad ? NAN : l != 0.0f ? o * inv * up : 0.0f;
+              for (int e = 0; e < 8; ++e) {
+                const float o = tiles > 0 ? __uint_as_float(x[8 * j + e]) : 0.0f;
+                const int d = v_dim<BITS>(j, e);
+                y[d >> 3][d & 7] = bad ? NAN : l != 0.0f ? o * inv * up : 0.0f;
               }
             if (mine)
 #pragma unroll
-              for (int mt = 0; mt < 4; ++mt) store_f32<T, 8>(out + k * kPrGroup + 16 * mt + 8 * n, y[mt]);
+              for (int j = 0; j < 4; ++j) store_f32<T, 8>(out + k * kPrGroup + 32 * n + 8 * j, y[j]);
           }
         }
       }
