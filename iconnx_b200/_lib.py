@@ -61,7 +61,7 @@ PROTOTYPES = {
     "icx_matmul_integer_scaled": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _sz, _vp, _vp, _vp, _i, _vp]),
     "icx_kv_cache_append": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i64, _i64, _i64, _i64, _vp, _vp]),
     "icx_kv_cache_read": (_i, [_vp, _vp, _vp, _i, _vp, _vp]),
-    "icx_kv_cache_attention_workspace_bytes": (_sz, [_vp, _vp, _i]),
+    "icx_kv_cache_attention_workspace_bytes": (_sz, [_vp, _vp, _i, _i]),
     "icx_kv_cache_attention": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i64, _i64, ctypes.c_float, _vp, _vp,
                                     _sz]),
     "icx_engine_create": (_vp, [_i]),

@@ -6,23 +6,28 @@
 
 namespace icx {
 
-AttendPlan plan_attend(const KvView& c, const KvTokens& w, int q_heads) {
+AttendPlan plan_attend(const KvView& c, const KvTokens& w, int q_heads, int type) {
   AttendPlan p{};
   const int share = q_heads / c.heads;
   // rows that share one read of the cache: as many as the average sequence
-  // has, up to what the registers hold
+  // has, up to what the registers (and, for two f16 parts of 256 dimensions of
+  // q per warp, shared memory) hold
   const int64_t rows = (w.tokens + w.batch - 1) / w.batch * share;
-  p.nt = rows <= 8 ? 1 : rows <= 16 || c.dim == 256 ? 2 : 4;
-  const int R = 8 * p.nt;
-  const int block = att_block(c.dim, c.bits, R);
-  const int64_t blocks = (((int64_t)w.width << c.page_shift) + block - 1) / block;
-  const int64_t units = (w.tokens * share / R + w.batch) * c.heads * (blocks > 1 ? blocks : 1);
-  const int64_t resident = (int64_t)sm_count() * (c.dim * p.nt <= 128 ? 2 : 1);
-  p.ctas = (int)(units < resident ? units : resident);
-  p.split = blocks > 1;
+  const int most = c.dim == 256 ? (type == ICX_F32 ? 1 : 2) : 4;
+  p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+  if (p.nt > most) p.nt = most;
+  const int R = 8 * p.nt, step = att_step(c.dim, c.bits, R);
+  const int64_t reach = (int64_t)w.width << c.page_shift;
+  // four steps are over before a second launch would be
+  p.split = reach > 4 * step;
+  p.unit = p.split ? step : 4 * step;
+  const int64_t blocks = reach > p.unit ? (reach + p.unit - 1) / p.unit : 1;
+  const int64_t units = (w.tokens * share / R + w.batch) * c.heads * blocks;
+  const int64_t resident = (int64_t)sm_count() * att_resident(c.dim, p.nt, (int)float_bytes(type)), want = (units + kAttWarps - 1) / kAttWarps;
+  p.ctas = (int)(want < resident ? want : resident);
   if (p.split) {
     p.prefix_bytes = ((size_t)(w.batch + 1) * 8 + 255) & ~size_t(255);
-    p.bytes = p.prefix_bytes + (size_t)p.ctas * 2 * R * (c.dim + 2) * 4;
+    p.bytes = p.prefix_bytes + (size_t)p.ctas * kAttWarps * 2 * R * (c.dim + 2) * 4;
   }
   return p;
 }
@@ -32,13 +37,14 @@ AttendPlan plan_attend(const KvView& c, const KvTokens& w, int q_heads) {
 using namespace icx;
 
 extern "C" size_t icx_kv_cache_attention_workspace_bytes(const icx_kv_cache* cache, const icx_kv_tokens* where,
-                                                         int q_heads) {
+                                                         int q_heads, int type) {
   KvView c;
   KvTokens w;
   if (kv_views("KvCacheAttention", cache, where, &c, &w) || w.tokens == 0 || w.batch == 0 || q_heads < 1 ||
       q_heads % c.heads)
     return 0;
-  return plan_attend(c, w, q_heads).bytes;
+  if (!is_float_type(type)) return 0;
+  return prompt_preferred(c, w, q_heads, type) ? 0 : plan_attend(c, w, q_heads, type).bytes;
 }
 
 extern "C" int icx_kv_cache_attention(void* stream, const icx_kv_cache* cache, const icx_kv_tokens* where,
@@ -60,7 +66,7 @@ extern "C" int icx_kv_cache_attention(void* stream, const icx_kv_cache* cache, c
   ICX_REQUIRE(d_q && d_out, "KvCacheAttention: null operand");
   ICX_REQUIRE((reinterpret_cast<uintptr_t>(d_out) & 15) == 0, "KvCacheAttention: out must be 16-byte aligned");
   const bool prompt = prompt_preferred(c, w, q_heads, type);
-  const AttendPlan p = prompt ? AttendPlan{} : plan_attend(c, w, q_heads);
+  const AttendPlan p = prompt ? AttendPlan{} : plan_attend(c, w, q_heads, type);
   if (p.bytes > 0 && (!d_workspace || workspace_bytes < p.bytes)) {
     set_error("KvCacheAttention: workspace %zu bytes < %zu required", d_workspace ? workspace_bytes : 0, p.bytes);
     return ICX_ERR_WORKSPACE;
@@ -76,6 +82,7 @@ extern "C" int icx_kv_cache_attention(void* stream, const icx_kv_cache* cache, c
   a.scale = scale;
   a.out = d_out;
   a.split = p.split;
+  a.unit = p.unit;
   a.prefix = static_cast<int64_t*>(d_workspace);
   a.partial = reinterpret_cast<float*>(static_cast<char*>(d_workspace) + p.prefix_bytes);
   cudaStream_t s = as_stream(stream);

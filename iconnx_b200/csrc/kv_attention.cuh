@@ -26,13 +26,14 @@
 // nothing.  Each lane adds its own positions' weights; lanes are joined once
 // per run of positions.
 //
-// Work: a unit is a block of positions (16 or 32 per warp) of one (sequence, K/V
-// head, tile of query rows); each CTA takes an equal, contiguous share of all units, found on the
+// Work: a unit is 16 or 32 positions of one (sequence, K/V head, tile of query
+// rows); each warp takes an equal, contiguous share of all units, found on the
 // device from seq_lens and cu_tokens, so ragged batches balance and a captured
-// call can be replayed with other lengths.  Eight warps of a CTA take
-// the block's positions in turn and are joined through shared memory; rows whose units went
-// to several CTAs leave (m, l, o) in the workspace for the join kernel.  All
-// joins run in a fixed order, so equal calls give equal results.
+// call can be replayed with other lengths.  Warps meet nowhere: one that runs
+// into another sequence or head starts on it while the other fifteen of the SM
+// keep its pipes busy.  Rows whose units went to several warps leave (m, l, o)
+// in the workspace for the join kernel.  All joins run in a fixed order, so
+// equal calls give equal results.
 #pragma once
 
 #include <type_traits>
@@ -48,10 +49,14 @@ constexpr int kAttWarps = 8;
 // Tiles of 16 positions that a warp takes at once: two where codes and sums are
 // small enough, which halves what a step costs beside its arithmetic.
 __host__ __device__ constexpr int att_subtiles(int dim, int bits, int R) { return dim * bits <= 512 && R <= 8 ? 2 : 1; }
-__host__ __device__ constexpr int att_block(int dim, int bits, int R) {
-  return 16 * kAttWarps * att_subtiles(dim, bits, R);
-}
+__host__ __device__ constexpr int att_step(int dim, int bits, int R) { return 16 * att_subtiles(dim, bits, R); }
 constexpr float kNoScore = -1.7e38f;        // m before the first score
+
+// CTAs per SM: two where 128 registers hold the sums, and shared memory two
+// rings beside their queries.
+__host__ __device__ constexpr int att_resident(int dim, int nt, int q_bytes) {
+  return dim * nt <= 128 && !(q_bytes == 4 && dim == 128) ? 2 : 1;
+}
 
 struct AttendArgs {
   const void* q;
@@ -61,8 +66,9 @@ struct AttendArgs {
   float scale;      // of the scores, times log2(e)
   void* out;
   int64_t* prefix;  // workspace: units before each sequence [batch + 1]
-  float* partial;   // workspace: two slots per CTA of R x (D + 2) floats
-  int split;        // rows may go to several CTAs
+  float* partial;   // workspace: two slots per warp of R x (D + 2) floats
+  int split;        // rows may go to several warps
+  int unit;         // positions per unit
 };
 
 // Units of a sequence: its row tiles x K/V heads x blocks of positions.
@@ -71,8 +77,8 @@ struct SeqUnits {
   int64_t units;
 };
 
-__device__ __forceinline__ SeqUnits seq_units(const KvView& c, const KvTokens& w, int share, int R, int b) {
-  const int block = att_block(c.dim, c.bits, R);
+__device__ __forceinline__ SeqUnits seq_units(const KvView& c, const KvTokens& w, int share, int R, int b,
+                                              int unit = 1 << 30) {
   SeqUnits u;
   u.from = b;
   u.n = 1;
@@ -87,7 +93,7 @@ __device__ __forceinline__ SeqUnits seq_units(const KvView& c, const KvTokens& w
   u.rows = u.n * share;
   u.tiles = (u.rows + R - 1) / R;
   const int reach = (int)min((int64_t)u.len, (int64_t)w.width << c.page_shift);
-  u.blocks = max(1, (reach + block - 1) / block);
+  u.blocks = max(1, (int)(((int64_t)reach + unit - 1) / unit));
   u.units = (int64_t)u.tiles * c.heads * u.blocks;
   return u;
 }
@@ -165,8 +171,7 @@ struct AttConfig {
   static constexpr bool PLO = !std::is_same<T, __nv_bfloat16>::value;
   static constexpr int R = 8 * NT;
   static constexpr int G = D / GROUP;
-  // two CTAs per SM where 128 registers hold the sums
-  static constexpr int kMinBlocks = D * NT <= 128 ? 2 : 1;
+  static constexpr int kMinBlocks = att_resident(D, NT, sizeof(T));
   // q stays in registers where it takes at most 16
   static constexpr bool kQReg = NT == 1 && (D / 16) * 2 * (QLO ? 2 : 1) <= 16;
   static constexpr int kRowFloats = D + 2;
@@ -175,14 +180,13 @@ struct AttConfig {
   static constexpr int ROW = D * BITS / 8, SUB = att_subtiles(D, BITS, R);
   static constexpr int kCodes = 16 * ROW, kParams = 16 * G * 4;
   static constexpr int kTile = 2 * (kCodes + kParams), kStage = SUB * kTile;
-  static constexpr int kFit = (kMinBlocks == 2 ? 80 : 160) * 1024 / (kAttWarps * kStage);
+  // a warp's query operand
+  static constexpr int kQBytes = kQReg ? 0 : NT * (D / 16) * (QLO ? 2 : 1) * 32 * 8;
+  static constexpr int kFit = ((kMinBlocks == 2 ? 108 : 220) * 1024 / kAttWarps - kQBytes) / kStage;
   static constexpr int kStages = kFit > 4 ? 4 : kFit < 2 ? 2 : kFit;
   static constexpr int kRing = kAttWarps * kStages * kStage;
-  // joining the warps: half of them put down R rows at a time, over the ring
-  static constexpr int kJoin = (kAttWarps / 2) * R * kRowFloats * 4;
-  static constexpr int kQOffset = kRing > kJoin ? kRing : kJoin;
-  static constexpr int kQBytes = kQReg ? 0 : NT * (D / 16) * (QLO ? 2 : 1) * 32 * 8;
-  static constexpr int kSmem = kQOffset + kQBytes;
+  static constexpr int kSmem = kRing + kAttWarps * kQBytes;
+  static_assert(kSmem * kMinBlocks <= 224 * 1024, "shared memory");
 };
 
 template <typename T, int D, int BITS, int GROUP, int NT>
@@ -192,11 +196,9 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
   using C = AttConfig<T, D, BITS, GROUP, NT>;
   constexpr int G = C::G, R = C::R, KS = D / 16, SG = GROUP / 16, MT = D / 16;
   constexpr int KW = D * BITS / 128;   // words of a K chunk
-  constexpr int ROW = C::ROW, SUB = C::SUB, kBlock = att_block(D, BITS, R);
+  constexpr int ROW = C::ROW, SUB = C::SUB, kStep = att_step(D, BITS, R);
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t full[kAttWarps][C::kStages];
-  __shared__ int64_t s_prefix, s_total;
-  __shared__ int s_seq;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int share = a.q_heads / c.heads;
@@ -205,56 +207,46 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
   pdl_wait();
   pdl_trigger();
 
-  // this CTA's units [u0, u1) of all
-  if (warp == 0) {
-    int64_t total = 0;
-    for (int b = lane; b < w.batch; b += 32) total += seq_units(c, w, share, R, b).units;
+  // this warp's units [u0, u1) of all
+  const int64_t me = (int64_t)blockIdx.x * kAttWarps + warp, warps = (int64_t)gridDim.x * kAttWarps;
+  int64_t total = 0;
+  for (int b = lane; b < w.batch; b += 32) total += seq_units(c, w, share, R, b, a.unit).units;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const int64_t first = total * blockIdx.x / gridDim.x;
-    const bool write = a.split && blockIdx.x == 0;
-    int64_t before = 0;
-    int seq = w.batch;
-    int64_t at = 0;
-    for (int b0 = 0; b0 < w.batch; b0 += 32) {
-      const int b = b0 + lane;
-      const int64_t n = b < w.batch ? seq_units(c, w, share, R, b).units : 0;
-      int64_t inc = n;
+  for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  const int64_t u0 = total * me / warps, u1 = total * (me + 1) / warps;
+  const bool write = a.split && me == 0;   // the first warp leaves the prefix sums
+  int seq = w.batch;
+  int64_t base = 0, before = 0;
+  for (int b0 = 0; b0 < w.batch; b0 += 32) {
+    const int b = b0 + lane;
+    const int64_t n = b < w.batch ? seq_units(c, w, share, R, b, a.unit).units : 0;
+    int64_t inc = n;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += x;
-      }
-      if (write && b < w.batch) a.prefix[b + 1] = before + inc;
-      const uint32_t hit = __ballot_sync(0xffffffffu, before + inc > first);
-      if (hit && seq == w.batch) {
-        const int l = __ffs(hit) - 1;
-        seq = b0 + l;
-        at = before + __shfl_sync(0xffffffffu, inc - n, l);
-        if (!write) break;
-      }
-      before += __shfl_sync(0xffffffffu, inc, 31);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += x;
     }
-    if (lane == 0) {
-      if (write) a.prefix[0] = 0;
-      s_total = total;
-      s_seq = seq;
-      s_prefix = at;
+    if (write && b < w.batch) a.prefix[b + 1] = before + inc;
+    const uint32_t hit = __ballot_sync(0xffffffffu, before + inc > u0);
+    if (hit && seq == w.batch) {
+      const int l = __ffs(hit) - 1;
+      seq = b0 + l;
+      base = before + __shfl_sync(0xffffffffu, inc - n, l);
+      if (!write) break;
     }
+    before += __shfl_sync(0xffffffffu, inc, 31);
   }
-  __syncthreads();
-  const int64_t u0 = s_total * blockIdx.x / gridDim.x, u1 = s_total * (blockIdx.x + 1) / gridDim.x;
-  int seq = s_seq;
-  int64_t base = s_prefix;
+  if (write && lane == 0) a.prefix[0] = 0;
   if (u0 >= u1) return;
-  SeqUnits su = seq_units(c, w, share, R, seq);
+  SeqUnits su = seq_units(c, w, share, R, seq, a.unit);
+  __syncwarp();
   uint32_t phase = 0;   // parity of each stage's barrier
   bool ok = true;       // false once a bounded wait gave up
 
   for (int64_t u = u0; u < u1;) {
     while (u >= base + su.units) {
       base += su.units;
-      su = seq_units(c, w, share, R, ++seq);
+      su = seq_units(c, w, share, R, ++seq, a.unit);
     }
     const int64_t in = u - base;
     const int block0 = (int)(in % su.blocks);
@@ -269,14 +261,58 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
     const int reach = (int)min((int64_t)su.len, (int64_t)w.width << c.page_shift);
     const int see_any = (int)max((int64_t)0, min(first_pos + (r0 + nrows - 1) / share + 1, (int64_t)reach));
     const int see_all = (int)max((int64_t)0, min(first_pos + r0 / share + 1, (int64_t)reach));
-    if (threadIdx.x == 0 && su.len > reach) record_status(ICX_DEVICE_BAD_PAGE);
+    if (lane == 0 && su.len > reach) record_status(ICX_DEVICE_BAD_PAGE);
+
+    // ------------------------------------------------------- codes on their way
+    uint8_t* ring = smem + warp * C::kStages * C::kStage;
+    const int end = (int)min((int64_t)block1 * a.unit, (int64_t)see_any);
+    const int p0 = block0 * a.unit;
+    const int tiles = p0 < end ? (end - p0 + kStep - 1) / kStep : 0;   // steps of SUB tiles
+    // lane i < 4 SUB brings piece i % 4 (K codes, K parameters, V codes, V
+    // parameters) of tile i / 4
+    const int my_piece = lane & 3, my_sub = (lane >> 2) & (SUB - 1);
+    const uint32_t my_bytes = (my_piece & 1) ? C::kParams : C::kCodes;
+    const int64_t my_row = (my_piece & 1) ? G * 4 : ROW;
+    const uint8_t* my_src = ((my_piece & 1) ? reinterpret_cast<const uint8_t*>(c.params[my_piece >> 1]) : c.codes[my_piece >> 1]) +
+                            ((int64_t)head << c.page_shift) * my_row;
+    const int64_t my_page_bytes = ((int64_t)c.heads << c.page_shift) * my_row;
+    const int my_dst = my_sub * C::kTile + (my_piece >> 1) * (C::kCodes + C::kParams) + (my_piece & 1) * C::kCodes;
+    // lane i holds the page of this warp's i-th tile of the current 32
+    int my_page = -1;
+    auto fetch_pages = [&](int from) {   // from: a tile, a multiple of 32
+      const int i = from + lane, p = p0 + i / SUB * kStep + i % SUB * 16;
+      my_page = p < end ? (int)kv_page(c, w, seq, p) : -1;
+      if (p < end && my_page < 0) record_status(ICX_DEVICE_BAD_PAGE);
+    };
+    // there[stage]: bit s: tile s of the stage has a page and positions
+    uint32_t there = 0;
+    auto advance = [&](int i) {
+      if (i >= tiles || !ok) return;
+      const int st = i % C::kStages, first = i * SUB;
+      if ((first & 31) == 0) fetch_pages(first);
+      const int page = __shfl_sync(0xffffffffu, my_page, (first + my_sub) & 31);
+      const uint32_t pages = __ballot_sync(0xffffffffu, my_page >= 0) >> (first & 31) & ((1u << SUB) - 1);
+      there = (there & ~(((1u << SUB) - 1) << (st * SUB))) | pages << (st * SUB);
+      if (pages == 0) return;
+      uint64_t* bar = &full[warp][st];
+      if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)__popc(pages) * C::kTile);
+      __syncwarp();
+      if (lane < 4 * SUB && page >= 0) {
+        const int off = (p0 + my_sub * 16) & ((1 << c.page_shift) - 1);   // p0 of every step: kStep apart
+        const int in_page = (off + i * kStep) & ((1 << c.page_shift) - 1);
+        bulk_load(ring + st * C::kStage + my_dst, my_src + page * my_page_bytes + in_page * my_row, my_bytes, bar);
+      }
+    };
+
+    // the ring holds the next kStages - 1 steps
+    for (int i = 0; i < C::kStages - 1; ++i) advance(i);
 
     // ------------------------------------------------------ query operand
     // column g of tile x is row r0 + 8 x + g; step j's contraction index of
     // this thread is dimensions 16 j + 4 t + {0,1} and {2,3}
     constexpr int QP = C::QLO ? 2 : 1;   // f16 parts of q
     uint32_t qr[C::kQReg ? KS : 1][QP][2];
-    uint2* q_smem = reinterpret_cast<uint2*>(smem + C::kQOffset) + lane;   // [NT][KS][QP][32]
+    uint2* q_smem = reinterpret_cast<uint2*>(smem + C::kRing + warp * C::kQBytes) + lane;   // [NT][KS][QP][32], own lane's
     float qsum[NT][G][2], qf[NT][2], step[NT][2];   // per column 2t and 2t+1: sums by group, score factor, 8 / factor
     int see[NT][2];                    // positions that row sees
 #pragma unroll
@@ -319,7 +355,7 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
           if constexpr (C::kQReg) {
             qr[j][i][0] = part[i][0];
             qr[j][i][1] = part[i][1];
-          } else if (warp == 0) {
+          } else {
             q_smem[((x * KS + j) * QP + i) * 32] = make_uint2(part[i][0], part[i][1]);
           }
         }
@@ -344,7 +380,6 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
       }
     }
 
-    if (!C::kQReg) __syncthreads();
     // -------------------------------------------------------- running sums
     float o[NT][MT][4] = {};
     float m[NT][2], l[NT][2], vlo[NT][G][2];
@@ -364,46 +399,6 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
       vmax[k] = 0.0f;
       vdown[k] = 0.0f;
     }
-
-    uint8_t* ring = smem + warp * C::kStages * C::kStage;
-    const int end = min(block1 * kBlock, see_any);
-    const int p0 = block0 * kBlock + warp * 16 * SUB;
-    const int tiles = p0 < end ? (end - p0 + kBlock - 1) / kBlock : 0;   // steps of SUB tiles
-    // lane i < 4 SUB brings piece i % 4 (K codes, K parameters, V codes, V
-    // parameters) of tile i / 4
-    const int my_piece = lane & 3, my_sub = (lane >> 2) & (SUB - 1);
-    const uint32_t my_bytes = (my_piece & 1) ? C::kParams : C::kCodes;
-    const int64_t my_row = (my_piece & 1) ? G * 4 : ROW;
-    const uint8_t* my_src = ((my_piece & 1) ? reinterpret_cast<const uint8_t*>(c.params[my_piece >> 1]) : c.codes[my_piece >> 1]) +
-                            ((int64_t)head << c.page_shift) * my_row;
-    const int64_t my_page_bytes = ((int64_t)c.heads << c.page_shift) * my_row;
-    const int my_dst = my_sub * C::kTile + (my_piece >> 1) * (C::kCodes + C::kParams) + (my_piece & 1) * C::kCodes;
-    // lane i holds the page of this warp's i-th tile of the current 32
-    int my_page = -1;
-    auto fetch_pages = [&](int from) {   // from: a tile, a multiple of 32
-      const int i = from + lane, p = p0 + i / SUB * kBlock + i % SUB * 16;
-      my_page = p < end ? (int)kv_page(c, w, seq, p) : -1;
-      if (p < end && my_page < 0) record_status(ICX_DEVICE_BAD_PAGE);
-    };
-    // there[stage]: bit s: tile s of the stage has a page and positions
-    uint32_t there = 0;
-    auto advance = [&](int i) {
-      if (i >= tiles || !ok) return;
-      const int st = i % C::kStages, first = i * SUB;
-      if ((first & 31) == 0) fetch_pages(first);
-      const int page = __shfl_sync(0xffffffffu, my_page, (first + my_sub) & 31);
-      const uint32_t pages = __ballot_sync(0xffffffffu, my_page >= 0) >> (first & 31) & ((1u << SUB) - 1);
-      there = (there & ~(((1u << SUB) - 1) << (st * SUB))) | pages << (st * SUB);
-      if (pages == 0) return;
-      uint64_t* bar = &full[warp][st];
-      if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)__popc(pages) * C::kTile);
-      __syncwarp();
-      if (lane < 4 * SUB && page >= 0) {
-        const int off = (p0 + my_sub * 16) & ((1 << c.page_shift) - 1);   // p0 of every step: kBlock apart
-        const int in_page = (off + i * kBlock) & ((1 << c.page_shift) - 1);
-        bulk_load(ring + st * C::kStage + my_dst, my_src + page * my_page_bytes + in_page * my_row, my_bytes, bar);
-      }
-    };
 
     // One step: SUB tiles of 16 positions.  EDGE: some row does not see some of
     // them, or a tile has no page.
@@ -644,8 +639,6 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
     };
 
     // ------------------------------------------------------ the positions
-    // the ring holds the next kStages - 1 steps
-    for (int i = 0; i < C::kStages - 1; ++i) advance(i);
     for (int i = 0; i < tiles; ++i) {
       const int stage = i % C::kStages;
       __syncwarp();   // every lane is done with the stage that is filled next
@@ -654,17 +647,27 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
       if (pages == 0) continue;
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][stage], phase >> stage & 1, ICX_DEVICE_TIMEOUT_CACHE));
       phase ^= 1u << stage;
-      const int pos = p0 + i * kBlock;
+      const int pos = p0 + i * kStep;
       if (!ok) continue;
       if (pos + 16 * SUB > see_all || pages != (1u << SUB) - 1) process(std::true_type{}, stage, pos, pages);
       else process(std::false_type{}, stage, pos, pages);
     }
 
-    // --------------------------------------------- join lanes, then warps
+    // ---------------------------------------------- join lanes, and write
+    const bool whole = block0 == 0 && block1 == su.blocks;
+    float* slot = a.partial + (me * 2 + (block0 == 0 ? 1 : 0)) * R * C::kRowFloats;
 #pragma unroll
     for (int x = 0; x < NT; ++x)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        m[x][h] = fmaxf(m[x][h] * qf[x][h], kNoScore);   // in powers of two from here
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[x][h] += __shfl_xor_sync(0xffffffffu, l[x][h], d);
+        const float inv = !whole ? 1.0f : l[x][h] != 0.0f ? 1.0f / l[x][h] : 0.0f;
+        const int r = r0 + 8 * x + 2 * t + h;
+        T* out = static_cast<T*>(a.out) +
+                 ((int64_t)(row_base + r / share) * a.q_heads + head * share + r % share) * D + 2 * g;
+        float* part = slot + (r - r0) * C::kRowFloats + 2 * g;
 #pragma unroll
         for (int k = 0; k < G; ++k) {
 #pragma unroll
@@ -673,138 +676,105 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
           const float up = vdown[k] > 0.0f ? 1.0f / vdown[k] : 0.0f;
 #pragma unroll
           for (int i = 0; i < GROUP / 16; ++i) {
-            float* ot = o[x][k * (GROUP / 16) + i];
-            ot[h] = fmaf(ot[h] * 16777216.0f, up, vlo[x][k][h]);
-            ot[2 + h] = fmaf(ot[2 + h] * (BITS == 4 ? 1048576.0f : 16777216.0f), up, vlo[x][k][h]);
+            const int mt = k * (GROUP / 16) + i;
+            const float v[2] = {fmaf(o[x][mt][h] * 16777216.0f, up, vlo[x][k][h]) * inv,
+                                fmaf(o[x][mt][2 + h] * (BITS == 4 ? 1048576.0f : 16777216.0f), up, vlo[x][k][h]) * inv};
+            if (r >= su.rows) continue;
+            if (whole) store_f32<T, 2>(out + 16 * mt, v);
+            else *reinterpret_cast<float2*>(part + 16 * mt) = make_float2(v[0], v[1]);
           }
         }
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) l[x][h] += __shfl_xor_sync(0xffffffffu, l[x][h], d);
+        if (!whole && g == 0 && r < su.rows) *reinterpret_cast<float2*>(part + D) = make_float2(m[x][h], l[x][h]);
       }
-#pragma unroll
-    for (int x = 0; x < NT; ++x)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) m[x][h] = fmaxf(m[x][h] * qf[x][h], kNoScore);   // in powers of two from here
-    __syncthreads();   // the ring is free
-#pragma unroll
-    for (int half = kAttWarps / 2; half >= 1; half >>= 1) {
-      float* mine = reinterpret_cast<float*>(smem) + (size_t)(warp % half) * R * C::kRowFloats;
-      if (warp >= half && warp < 2 * half) {
-#pragma unroll
-        for (int x = 0; x < NT; ++x)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float* row = mine + (8 * x + 2 * t + h) * C::kRowFloats;
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-              *reinterpret_cast<float2*>(row + 16 * i + 2 * g) = make_float2(o[x][i][h], o[x][i][2 + h]);
-            if (g == 0) *reinterpret_cast<float2*>(row + D) = make_float2(m[x][h], l[x][h]);
-          }
-      }
-      __syncthreads();
-      if (warp < half) {
-#pragma unroll
-        for (int x = 0; x < NT; ++x)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float* row = mine + (8 * x + 2 * t + h) * C::kRowFloats;
-            const float2 ml = *reinterpret_cast<const float2*>(row + D);
-            const float top = fmaxf(m[x][h], ml.x);
-            const float fa = ex2(m[x][h] - top), fb = ex2(ml.x - top);
-            m[x][h] = top;
-            l[x][h] = l[x][h] * fa + ml.y * fb;
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-              const float2 v = *reinterpret_cast<const float2*>(row + 16 * i + 2 * g);
-              o[x][i][h] = o[x][i][h] * fa + v.x * fb;
-              o[x][i][2 + h] = o[x][i][2 + h] * fa + v.y * fb;
-            }
-          }
-      }
-      __syncthreads();
-    }
-    fence_proxy_async_smem();   // before the next bulk copies over what was written here
-    if (warp == 0) {
-      const bool whole = block0 == 0 && block1 == su.blocks;
-      float* slot = a.partial + ((int64_t)blockIdx.x * 2 + (block0 == 0 ? 1 : 0)) * R * C::kRowFloats;
-#pragma unroll
-      for (int x = 0; x < NT; ++x)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = r0 + 8 * x + 2 * t + h;
-          if (r >= su.rows) continue;
-          if (whole) {
-            const float inv = l[x][h] != 0.0f ? 1.0f / l[x][h] : 0.0f;
-            T* out = static_cast<T*>(a.out) +
-                     ((int64_t)(row_base + r / share) * a.q_heads + head * share + r % share) * D;
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-              const float v[2] = {o[x][i][h] * inv, o[x][i][2 + h] * inv};
-              store_f32<T, 2>(out + 16 * i + 2 * g, v);
-            }
-          } else {
-            float* row = slot + (r - r0) * C::kRowFloats;
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-              *reinterpret_cast<float2*>(row + 16 * i + 2 * g) = make_float2(o[x][i][h], o[x][i][2 + h]);
-            if (g == 0) *reinterpret_cast<float2*>(row + D) = make_float2(m[x][h], l[x][h]);
-          }
-        }
-    }
   }
 }
 
-// Joins the rows whose units went to several CTAs: one warp per (token, query
-// head), the CTAs in order.
+// Joins the rows whose units went to several warps: `per_row` (1 or 8) warps per
+// (token, query head), each taking every per_row-th part, then in order.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) kv_attend_join_kernel(const KvView c, const KvTokens w, const AttendArgs a,
-                                                             int R, int ctas) {
+__global__ void __launch_bounds__(256)
+    kv_attend_join_kernel(const __grid_constant__ KvView c, const __grid_constant__ KvTokens w,
+                          const __grid_constant__ AttendArgs a, int R, int warps, int per_row) {
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (item >= w.tokens * a.q_heads) return;
+  constexpr int E = D / 32;
+  __shared__ float s_o[8][D + 2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int mine = warp % per_row;
+  const int64_t item = (int64_t)blockIdx.x * (8 / per_row) + warp / per_row;
   const int share = a.q_heads / c.heads;
   const int64_t token = item / a.q_heads;
   const int hq = (int)(item % a.q_heads);
-  const int b = kv_sequence(w, token);
-  if (b < 0) return;
-  const SeqUnits su = seq_units(c, w, share, R, b);
-  const int64_t row = token - su.from;
-  const int r = (int)row * share + hq % share;
-  const int64_t total = a.prefix[w.batch];
-  const int64_t s0 = a.prefix[b] + ((int64_t)(hq / share) * su.tiles + r / R) * su.blocks, s1 = s0 + su.blocks;
-  if (total <= 0) return;
-  // the CTA that holds unit s is the last with total * cta / ctas <= s
-  const int first = (int)(((s0 + 1) * ctas - 1) / total), last = (int)((s1 * ctas - 1) / total);
-  if (first == last) return;   // written whole
-  constexpr int E = D / 32;
-  float m = kNoScore, l = 0.0f, o[E] = {};
-  for (int i = first; i <= last; ++i) {
-    if (total * i / ctas == total * (i + 1) / ctas) continue;   // more CTAs than units: this one had none
-    const float* p = a.partial + (((int64_t)i * 2 + (i == first ? 1 : 0)) * R + r % R) * (D + 2);
-    const float mi = p[D], li = p[D + 1];
-    const float top = fmaxf(m, mi), fa = ex2(m - top), fb = ex2(mi - top);
-    m = top;
-    l = l * fa + li * fb;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = o[e] * fa + p[lane + 32 * e] * fb;
+  const int b = item < w.tokens * a.q_heads ? kv_sequence(w, token) : -1;
+  int first = 0, last = 0, r = 0;
+  int64_t total = 0;
+  if (b >= 0) {
+    const SeqUnits su = seq_units(c, w, share, R, b, a.unit);
+    r = (int)(token - su.from) * share + hq % share;
+    total = a.prefix[w.batch];
+    const int64_t s0 = a.prefix[b] + ((int64_t)(hq / share) * su.tiles + r / R) * su.blocks, s1 = s0 + su.blocks;
+    // the warp that holds unit s is the last with total * warp / warps <= s
+    if (total > 0) {
+      first = (int)(((s0 + 1) * warps - 1) / total);
+      last = (int)((s1 * warps - 1) / total);
+    }
   }
-  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+  // first == last: written whole, or nothing there
+  float m = kNoScore, l = 0.0f, o[E] = {};
+  if (first < last) {
+    for (int i = first + mine; i <= last; i += per_row) {
+      if (total * i / warps == total * (i + 1) / warps) continue;   // more warps than units: this one had none
+      const float* p = a.partial + (((int64_t)i * 2 + (i == first ? 1 : 0)) * R + r % R) * (D + 2);
+      const float2 ml = *reinterpret_cast<const float2*>(p + D);
+      const float top = fmaxf(m, ml.x), fa = ex2(m - top), fb = ex2(ml.x - top);
+      m = top;
+      l = l * fa + ml.y * fb;
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    static_cast<T*>(a.out)[(token * a.q_heads + hq) * D + lane + 32 * e] = from_f32<T>(o[e] * inv);
+      for (int e = 0; e < E; e += 2) {
+        const float2 v = *reinterpret_cast<const float2*>(p + lane * E + e);
+        o[e] = o[e] * fa + v.x * fb;
+        o[e + 1] = o[e + 1] * fa + v.y * fb;
+      }
+    }
+  }
+  if (per_row > 1) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) s_o[warp][lane * E + e] = o[e];
+    if (lane == 0) {
+      s_o[warp][D] = m;
+      s_o[warp][D + 1] = l;
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    for (int i = 1; i < per_row; ++i) {
+      const float mi = s_o[i][D], li = s_o[i][D + 1];
+      const float top = fmaxf(m, mi), fa = ex2(m - top), fb = ex2(mi - top);
+      m = top;
+      l = l * fa + li * fb;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = o[e] * fa + s_o[i][lane * E + e] * fb;
+    }
+  }
+  if (first == last) return;
+  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+  T* out = static_cast<T*>(a.out) + (token * a.q_heads + hq) * D + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; e += 2) {
+    const float v[2] = {o[e] * inv, o[e + 1] * inv};
+    store_f32<T, 2>(out + e, v);
+  }
 }
 
 // Which kernel, on how many CTAs.
 struct AttendPlan {
   int nt;      // query rows per tile / 8
   int ctas;
+  int unit;    // positions per unit
   bool split;
   size_t prefix_bytes, bytes;   // workspace
 };
 
-AttendPlan plan_attend(const KvView& c, const KvTokens& w, int q_heads);
+AttendPlan plan_attend(const KvView& c, const KvTokens& w, int q_heads, int type);
 
 // Many rows per sequence: the tensor-memory kernel (kv_prompt.cu).
 bool prompt_preferred(const KvView& c, const KvTokens& w, int q_heads, int type);
@@ -828,17 +798,22 @@ int launch_attend_rows(cudaStream_t s, const KvView& c, const KvTokens& w, const
   if (C::kSmem > 40 * 1024)   // beside the static part
     ICX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
   ICX_CUDA(launch_pdl(kern, dim3(p.ctas), dim3(32 * kAttWarps), C::kSmem, s, c, w, a));
-  if (p.split)
-    ICX_CUDA(launch_pdl(kv_attend_join_kernel<T, D>, dim3((unsigned)((w.tokens * a.q_heads + 7) / 8)), dim3(256), 0,
-                        s, c, w, a, C::R, p.ctas));
+  if (p.split) {
+    // few rows have many parts each
+    const int64_t rows = w.tokens * a.q_heads;
+    const int per_row = rows <= 1024 ? 8 : 1;
+    ICX_CUDA(launch_pdl(kv_attend_join_kernel<T, D>, dim3((unsigned)((rows * per_row + 7) / 8)), dim3(256), 0, s, c, w, a,
+                        C::R, p.ctas * kAttWarps, per_row));
+  }
   return ICX_OK;
 }
 
 template <typename T, int D, int BITS, int GROUP>
 int launch_attend_nt(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a, const AttendPlan& p) {
+  constexpr int kMost = D == 256 ? (sizeof(T) == 4 ? 1 : 2) : 4;   // as plan_attend
   if (p.nt == 1) return launch_attend_rows<T, D, BITS, GROUP, 1>(s, c, w, a, p);
-  if (p.nt == 2 || D == 256) return launch_attend_rows<T, D, BITS, GROUP, 2>(s, c, w, a, p);
-  return launch_attend_rows<T, D, BITS, GROUP, D == 256 ? 2 : 4>(s, c, w, a, p);
+  if (p.nt == 2) return launch_attend_rows<T, D, BITS, GROUP, kMost < 2 ? 1 : 2>(s, c, w, a, p);
+  return launch_attend_rows<T, D, BITS, GROUP, kMost>(s, c, w, a, p);
 }
 
 template <typename T, int D>

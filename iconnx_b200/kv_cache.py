@@ -206,7 +206,7 @@ def gpu_kv_cache_attention(cache: KvCache, q: torch.Tensor, page_table: torch.Te
     else:
         out = _new_rows(out, q.shape, q.dtype, cache.device, f"{what}: out")
     L = _lib.load()
-    size = L.icx_kv_cache_attention_workspace_bytes(cache._ref, ctypes.byref(arg), heads)
+    size = L.icx_kv_cache_attention_workspace_bytes(cache._ref, ctypes.byref(arg), heads, t)
     ws = q.new_empty(size, dtype=torch.uint8) if size else None
     _on(cache.device, L.icx_kv_cache_attention, cache._ref, ctypes.byref(arg),
         q.data_ptr(), t, heads, q.stride(0), q.stride(1), scale, out.data_ptr(), _ptr(ws), size)

@@ -350,7 +350,8 @@ ICX_API int icx_kv_cache_read(void* stream, const icx_kv_cache* cache, const icx
  * zeros.  Positions without a usable page take no part.
  * Scores, softmax statistics and sums are f32. */
 ICX_API size_t icx_kv_cache_attention_workspace_bytes(const icx_kv_cache* cache,
-                                                      const icx_kv_tokens* where, int q_heads);
+                                                      const icx_kv_tokens* where, int q_heads,
+                                                      int type);
 
 ICX_API int icx_kv_cache_attention(void* stream, const icx_kv_cache* cache,
                                    const icx_kv_tokens* where, const void* d_q, int type,
