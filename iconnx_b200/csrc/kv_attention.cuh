@@ -284,28 +284,30 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
       my_page = p < end ? (int)kv_page(c, w, seq, p) : -1;
       if (p < end && my_page < 0) record_status(ICX_DEVICE_BAD_PAGE);
     };
-    // there[stage]: bit s: tile s of the stage has a page and positions
+    // bits SUB st ..: which tiles of stage st have a page and positions
     uint32_t there = 0;
-    auto advance = [&](int i) {
-      if (i >= tiles || !ok) return;
-      const int st = i % C::kStages, first = i * SUB;
-      if ((first & 31) == 0) fetch_pages(first);
-      const int page = __shfl_sync(0xffffffffu, my_page, (first + my_sub) & 31);
-      const uint32_t pages = __ballot_sync(0xffffffffu, my_page >= 0) >> (first & 31) & ((1u << SUB) - 1);
-      there = (there & ~(((1u << SUB) - 1) << (st * SUB))) | pages << (st * SUB);
-      if (pages == 0) return;
-      uint64_t* bar = &full[warp][st];
-      if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)__popc(pages) * C::kTile);
-      __syncwarp();
-      if (lane < 4 * SUB && page >= 0) {
-        const int off = (p0 + my_sub * 16) & ((1 << c.page_shift) - 1);   // p0 of every step: kStep apart
-        const int in_page = (off + i * kStep) & ((1 << c.page_shift) - 1);
-        bulk_load(ring + st * C::kStage + my_dst, my_src + page * my_page_bytes + in_page * my_row, my_bytes, bar);
+    int filled = 0, fill = 0;   // steps brought so far, and the next one's stage
+    auto advance = [&]() {
+      if (filled >= tiles || !ok) return;
+      const int first = filled * SUB & 31;
+      if (first == 0) fetch_pages(filled * SUB);
+      const int page = __shfl_sync(0xffffffffu, my_page, first + my_sub);
+      const uint32_t pages = __ballot_sync(0xffffffffu, my_page >= 0) >> first & ((1u << SUB) - 1);
+      there = (there & ~(((1u << SUB) - 1) << (fill * SUB))) | pages << (fill * SUB);
+      if (pages != 0) {
+        uint64_t* bar = &full[warp][fill];
+        if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)__popc(pages) * C::kTile);
+        __syncwarp();
+        if (lane < 4 * SUB && page >= 0) {
+          const int in_page = (p0 + my_sub * 16 + filled * kStep) & ((1 << c.page_shift) - 1);
+          bulk_load(ring + fill * C::kStage + my_dst, my_src + page * my_page_bytes + in_page * my_row, my_bytes, bar);
+        }
       }
+      ++filled;
+      fill = fill + 1 == C::kStages ? 0 : fill + 1;
     };
-
     // the ring holds the next kStages - 1 steps
-    for (int i = 0; i < C::kStages - 1; ++i) advance(i);
+    for (int i = 0; i < C::kStages - 1; ++i) advance();
 
     // ------------------------------------------------------ query operand
     // column g of tile x is row r0 + 8 x + g; step j's contraction index of
@@ -639,18 +641,20 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
     };
 
     // ------------------------------------------------------ the positions
-    for (int i = 0; i < tiles; ++i) {
-      const int stage = i % C::kStages;
+    int stage = 0;
+    for (int pos = p0; pos < p0 + tiles * kStep; pos += kStep) {
       __syncwarp();   // every lane is done with the stage that is filled next
-      advance(i + C::kStages - 1);
+      advance();
       const uint32_t pages = there >> (stage * SUB) & ((1u << SUB) - 1);
-      if (pages == 0) continue;
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][stage], phase >> stage & 1, ICX_DEVICE_TIMEOUT_CACHE));
-      phase ^= 1u << stage;
-      const int pos = p0 + i * kStep;
-      if (!ok) continue;
-      if (pos + 16 * SUB > see_all || pages != (1u << SUB) - 1) process(std::true_type{}, stage, pos, pages);
-      else process(std::false_type{}, stage, pos, pages);
+      if (pages != 0) {
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][stage], phase >> stage & 1, ICX_DEVICE_TIMEOUT_CACHE));
+        phase ^= 1u << stage;
+        if (ok) {
+          if (pos + 16 * SUB > see_all || pages != (1u << SUB) - 1) process(std::true_type{}, stage, pos, pages);
+          else process(std::false_type{}, stage, pos, pages);
+        }
+      }
+      stage = stage + 1 == C::kStages ? 0 : stage + 1;
     }
 
     // ---------------------------------------------- join lanes, and write

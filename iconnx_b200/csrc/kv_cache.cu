@@ -138,16 +138,26 @@ __device__ __forceinline__ void group_codes(const float (&x)[8], float lo, float
       code[k + 1] = __float_as_uint(r1);
       worst = fmaxf(worst, fmaxf(fabsf(u0 - c[k]), fabsf(u1 - c[k + 1])));
     }
+    // One at a time, by its index: in 16-bit types such values are exact ties
+    // more often than not, one in a few hundred.
+    uint32_t near = 0;
     if (worst > 0.4998f) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {   // few lanes have one, and seldom the same: a branch for each
-        const float u = (x[k] - lo) * inv;
-        const bool near = fabsf(u - c[k]) > 0.4998f;
-        if (__any_sync(__activemask(), near)) {
-          if (near) c[k] = fminf(code_near_half(x[k], lo, s, u), (float)((1 << BITS) - 1));
-          code[k] = __float_as_uint(c[k] + kRound);
+      for (int k = 0; k < 8; ++k) near |= fabsf((x[k] - lo) * inv - c[k]) > 0.4998f ? 1u << k : 0u;
+    }
+    while (near) {
+      const int at = __ffs(near) - 1;
+      near &= near - 1;
+      float xv = x[0];
+#pragma unroll
+      for (int k = 1; k < 8; ++k) xv = at == k ? x[k] : xv;
+      const float n = fminf(code_near_half(xv, lo, s, (xv - lo) * inv), (float)((1 << BITS) - 1));
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (at == k) {
+          c[k] = n;
+          code[k] = __float_as_uint(n + kRound);
         }
-      }
     }
   } else {
     constexpr float L = (float)((1 << BITS) - 1);

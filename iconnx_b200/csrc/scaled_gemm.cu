@@ -257,12 +257,54 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     int acc = 0, buf = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
+    // The residual's box into the places its outputs will take; the box's store
+    // of two boxes ago has been read out.
+    auto put_residual = [&](uint8_t* box, int mrow0, int nb) {
+      if (!residual || mrow0 >= p.M) return;
+      if (tma_store && lane == 0) bulk_wait_read<1>();
+      __syncwarp();
+      if (vec_residual && nb + CB <= p.N) {
+        uint4 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int rr = (lane >> 3) + 4 * i;
+          v[i] = make_uint4(0, 0, 0, 0);
+          if (mrow0 + rr < p.M)
+            v[i] = __ldg(reinterpret_cast<const uint4*>(residual + (size_t)(mrow0 + rr) * p.N + nb) + (lane & 7));
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int rr = (lane >> 3) + 4 * i;
+          *reinterpret_cast<uint4*>(box + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4)) = v[i];
+        }
+      } else {
+        for (int r0 = 0; r0 < 32; r0 += 16) {   // sixteen rows in flight
+          T v[16][CB / 32];
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+#pragma unroll
+            for (int x = 0; x < CB / 32; ++x) {
+              const int mm = mrow0 + r0 + i, n = nb + x * 32 + lane;
+              v[i][x] = mm < p.M && n < p.N ? residual[(size_t)mm * p.N + n] : from_f32<T>(0.0f);
+            }
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+#pragma unroll
+            for (int x = 0; x < CB / 32; ++x) {
+              const int rr = r0 + i, c = x * 32 + lane;
+              *reinterpret_cast<T*>(box + rr * 128 + (((c / kPiece) ^ (rr & 7)) << 4) + c % kPiece * sizeof(T)) = v[i][x];
+            }
+        }
+      }
+    };
     for (int t = tile0; t < ntiles; t += tstep) {
       int m0, n0;
       tile_at(t, m0, n0);
       const int mrow0 = m0 + quad * 32, m = mrow0 + lane;
       const float sa = m < p.M ? __ldg(p.q_scale + m) : 0.0f;
       const int nboxes = (min(BN, p.N - n0) + CB - 1) / CB;
+      // the first box's residual arrives while the products run
+      if (part < nboxes) put_residual(box0 + buf * 4096, mrow0, n0 + part * CB);
       if (ok) ok = mbar_wait_warp(&tfull[acc], acc_phase, ICX_DEVICE_TIMEOUT_EPILOGUE);
       tc_fence_after();
       const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN);
@@ -273,36 +315,14 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         uint8_t* row = box + lane * 128;
         uint32_t r[32];
         tmem_ld_32x32b_x32(trow + (uint32_t)(bx * CB), r);
-        // the box's store of two boxes ago has been read out
-        if (tma_store && lane == 0) bulk_wait_read<1>();
+        if (bx != part) put_residual(box, mrow0, nb);
+        if (tma_store && !residual && lane == 0) bulk_wait_read<1>();
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < CB / 32; ++i) {
           const int c = i * 32 + lane, n = nb + c;
           ops[c] = n < p.N ? __ldg(p.w_scale + n) : 0.0f;
           ops[CB + c] = p.bias && n < p.N ? __ldg(p.bias + n) : 0.0f;
-        }
-        if (residual && rows_here) {
-          // the residual's box, into the places its outputs will take
-          if (vec_residual && nb + CB <= p.N) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int rr = (lane >> 3) + 4 * i, c = lane & 7;
-              uint4 v = make_uint4(0, 0, 0, 0);
-              if (mrow0 + rr < p.M)
-                v = __ldg(reinterpret_cast<const uint4*>(residual + (size_t)(mrow0 + rr) * p.N + nb) + c);
-              *reinterpret_cast<uint4*>(box + rr * 128 + ((c ^ (rr & 7)) << 4)) = v;
-            }
-          } else {
-            for (int rr = 0; rr < 32 && mrow0 + rr < p.M; ++rr)
-#pragma unroll
-              for (int i = 0; i < CB / 32; ++i) {
-                const int c = i * 32 + lane;
-                if (nb + c < p.N)
-                  *reinterpret_cast<T*>(box + rr * 128 + (((c / kPiece) ^ (rr & 7)) << 4) + c % kPiece * sizeof(T)) =
-                      residual[(size_t)(mrow0 + rr) * p.N + nb + c];
-              }
-          }
         }
         __syncwarp();
 #pragma unroll
