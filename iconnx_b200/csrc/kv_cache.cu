@@ -6,6 +6,8 @@
 // together from lanes of one such eighth.
 #include "kv_cache.cuh"
 
+#include <type_traits>
+
 #include "capi.cuh"
 #include "common.cuh"
 
@@ -114,14 +116,12 @@ __device__ __forceinline__ float code_near_half(float x, float lo, float s, floa
   return d > e ? k + 1.0f : d < e ? k : 2.0f * rintf(0.5f * k + 0.25f);
 }
 
-// The codes, each on the bits of kRound (the code in the low byte), and as
-// floats.
+// The codes, each on the bits of kRound (the code in the low byte).
 constexpr float kRound = 12582912.0f;   // 1.5 * 2^23: adding it rounds to an integer (half to even)
 
 // Scales whose reciprocal or range may not be finite take the 64-bit quotient.
 template <int BITS>
-__device__ __forceinline__ void group_codes(const float (&x)[8], float lo, float s, bool finite, uint32_t (&code)[8],
-                                            float (&c)[8]) {
+__device__ __forceinline__ void group_codes(const float (&x)[8], float lo, float s, bool finite, uint32_t (&code)[8]) {
   if (finite && s >= 1e-36f && s <= 1e36f && lo > -3e38f) {
     // here lo <= x <= lo + L s, so that the quotient needs no clamp
     float inv, worst = 0.0f;
@@ -130,20 +130,21 @@ __device__ __forceinline__ void group_codes(const float (&x)[8], float lo, float
 #pragma unroll
     for (int k = 0; k < 8; k += 2) {
       const F2 u = f2_mul(f2_add(f2(x[k], x[k + 1]), lo2), inv2), r = f2_add(u, up), n = f2_add(r, down);
-      float r0, r1, u0, u1;
+      float r0, r1, u0, u1, n0, n1;
       f2_split(r, r0, r1);
       f2_split(u, u0, u1);
-      f2_split(n, c[k], c[k + 1]);
+      f2_split(n, n0, n1);
       code[k] = __float_as_uint(r0);
       code[k + 1] = __float_as_uint(r1);
-      worst = fmaxf(worst, fmaxf(fabsf(u0 - c[k]), fabsf(u1 - c[k + 1])));
+      worst = fmaxf(worst, fmaxf(fabsf(u0 - n0), fabsf(u1 - n1)));
     }
     // One at a time, by its index: in 16-bit types such values are exact ties
     // more often than not, one in a few hundred.
     uint32_t near = 0;
     if (worst > 0.4998f) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) near |= fabsf((x[k] - lo) * inv - c[k]) > 0.4998f ? 1u << k : 0u;
+      for (int k = 0; k < 8; ++k)
+        near |= fabsf((x[k] - lo) * inv - (__uint_as_float(code[k]) - kRound)) > 0.4998f ? 1u << k : 0u;
     }
     while (near) {
       const int at = __ffs(near) - 1;
@@ -151,21 +152,17 @@ __device__ __forceinline__ void group_codes(const float (&x)[8], float lo, float
       float xv = x[0];
 #pragma unroll
       for (int k = 1; k < 8; ++k) xv = at == k ? x[k] : xv;
-      const float n = fminf(code_near_half(xv, lo, s, (xv - lo) * inv), (float)((1 << BITS) - 1));
+      const uint32_t n = __float_as_uint(
+          fminf(code_near_half(xv, lo, s, (xv - lo) * inv), (float)((1 << BITS) - 1)) + kRound);
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (at == k) {
-          c[k] = n;
-          code[k] = __float_as_uint(n + kRound);
-        }
+      for (int k = 0; k < 8; ++k) code[k] = at == k ? n : code[k];
     }
   } else {
     constexpr float L = (float)((1 << BITS) - 1);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      c[k] = finite && s > 0.0f ? (float)fmin(fmax(rint(((double)x[k] - (double)lo) / (double)s), 0.0), (double)L) : 0.0f;
-      code[k] = __float_as_uint(c[k] + kRound);
-    }
+    for (int k = 0; k < 8; ++k)
+      code[k] = __float_as_uint(
+          kRound + (finite && s > 0.0f ? (float)fmin(fmax(rint(((double)x[k] - (double)lo) / (double)s), 0.0), (double)L) : 0.0f));
   }
 }
 
@@ -298,16 +295,17 @@ struct WarpPart {
 
 struct Parts {
   int run, parts, per;
-  int64_t items;
+  unsigned items;
 };
 
-__device__ __forceinline__ WarpPart warp_part(const KvView& c, const KvTokens& w, const Parts& n, int64_t item,
+__device__ __forceinline__ WarpPart warp_part(const KvView& c, const KvTokens& w, const Parts& n, unsigned item,
                                               int blocks) {
   WarpPart p;
   const int lane = threadIdx.x & 31;
-  const int part = (int)(item % n.parts);
-  p.which = (int)((item / n.parts) & 1);
-  p.token0 = item / (2 * n.parts) * n.run;
+  const unsigned side = item / (unsigned)n.parts;
+  const int part = (int)(item - side * (unsigned)n.parts);
+  p.which = (int)(side & 1);
+  p.token0 = (int64_t)(side >> 1) * n.run;
   p.tokens = (int)min((int64_t)n.run, w.tokens - p.token0);
   p.from = part * n.per;
   p.to = min(p.from + n.per, blocks);
@@ -329,15 +327,64 @@ __device__ __forceinline__ WarpPart warp_part(const KvView& c, const KvTokens& w
   return p;
 }
 
+// Eight values, and the smallest and largest of them (NaN if one is).
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8], bool vec) {
-  if (sizeof(T) == 2) {
-    load_f32<T, 8>(p, x, vec);
+__device__ __forceinline__ void load8(const T* p, float (&x)[8], bool vec, float& mn, float& mx) {
+  if constexpr (sizeof(T) == 2) {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    Vec<T, 8> v;
+    if (vec) {
+      v = *reinterpret_cast<const Vec<T, 8>*>(p);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v.v[i] = p[i];
+    }
+    const T2* w = reinterpret_cast<const T2*>(&v);
+    const T2 lo = __hmin2_nan(__hmin2_nan(w[0], w[1]), __hmin2_nan(w[2], w[3]));
+    const T2 hi = __hmax2_nan(__hmax2_nan(w[0], w[1]), __hmax2_nan(w[2], w[3]));
+    mn = min_nan(to_f32(lo.x), to_f32(lo.y));
+    mx = max_nan(to_f32(hi.x), to_f32(hi.y));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_f32(v.v[i]);
   } else {
     load_f32<T, 4>(p, *reinterpret_cast<float(*)[4]>(&x[0]), vec);
     load_f32<T, 4>(p + 4, *reinterpret_cast<float(*)[4]>(&x[4]), vec);
+    mn = mx = x[0];
+#pragma unroll
+    for (int k = 1; k < 8; ++k) {
+      mn = min_nan(mn, x[k]);
+      mx = max_nan(mx, x[k]);
+    }
   }
 }
+
+// Over the four or eight lanes of a group.  16-bit types: both ends in one
+// word, the larger negated, so that one minimum serves both.
+template <typename T>
+__device__ __forceinline__ void group_range(float& mn, float& mx, bool eight) {
+  if constexpr (sizeof(T) == 2) {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    T2 v;
+    v.x = from_f32<T>(mn);   // exact: values of the type
+    v.y = from_f32<T>(-mx);
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+      if (o == 4 && !eight) break;
+      uint32_t u = __shfl_xor_sync(0xffffffffu, *reinterpret_cast<uint32_t*>(&v), o);
+      v = __hmin2_nan(v, *reinterpret_cast<T2*>(&u));
+    }
+    mn = to_f32(v.x);
+    mx = -to_f32(v.y);
+  } else {
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+      if (o == 4 && !eight) break;
+      mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+      mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    }
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
   if (sizeof(T) == 2) {
@@ -355,7 +402,7 @@ __global__ void __launch_bounds__(128, 8)
   pdl_wait();
   pdl_trigger();
   constexpr int kPerHead = D / 64, ROW = D * BITS / 8;
-  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const unsigned item = blockIdx.x * 4 + (threadIdx.x >> 5);
   if (item >= n.items) return;
   const WarpPart p = warp_part(c, w, n, item, c.heads * kPerHead);
   const int l = threadIdx.x & 7, sub = (threadIdx.x >> 3) & 3;
@@ -376,35 +423,23 @@ __global__ void __launch_bounds__(128, 8)
       const int pos = __shfl_sync(0xffffffffu, p.pos, i);
       const int64_t row0 = __shfl_sync(0xffffffffu, p.row0, i);
       if (pos < 0) continue;
-      float x[8];
-      load8<T>(x_at, x, vec);
-      float mn = x[0], mx = x[0];
-#pragma unroll
-      for (int k = 1; k < 8; ++k) {
-        mn = min_nan(mn, x[k]);
-        mx = max_nan(mx, x[k]);
-      }
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) {
-        if (o == 4 && c.group == 32) break;
-        mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-        mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      }
+      float x[8], mn, mx;
+      load8<T>(x_at, x, vec, mn, mx);
+      group_range<T>(mn, mx, c.group == 64);
       const bool finite = fabsf(mn) < INFINITY && fabsf(mx) < INFINITY;
       const uint32_t prm = finite ? group_params<BITS>(mn, mx) : 0x7fc07fc0u;
       const float s = param_scale(prm), lo = param_low(prm);
       uint32_t code[8];
-      float v[8];
-      group_codes<BITS>(x, lo, s, finite, code, v);
+      group_codes<BITS>(x, lo, s, finite, code);
       store_block<BITS, D>(codes + row0 * ROW, pos, p.which, block, l, code, valid);
       if (valid && store_group) params[row0 * D >> c.group_shift] = prm;
       if (values) {
 #pragma unroll
         for (int k = 0; k < 8; k += 2) {
-          const F2 y = f2_fma(f2(v[k], v[k + 1]), f2(s, s), f2(lo, lo));
-          f2_split(y, v[k], v[k + 1]);
+          const F2 q = f2_add(f2(__uint_as_float(code[k]), __uint_as_float(code[k + 1])), f2(-kRound, -kRound));
+          f2_split(f2_fma(q, f2(s, s), f2(lo, lo)), x[k], x[k + 1]);
         }
-        store8<T>(v_at, v);
+        store8<T>(v_at, x);
       }
     }
   }
@@ -417,7 +452,7 @@ __global__ void __launch_bounds__(128, 8)
   pdl_wait();
   pdl_trigger();
   constexpr int kPerHead = D / 64, ROW = D * BITS / 8, U = 4;   // tokens in flight
-  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const unsigned item = blockIdx.x * 4 + (threadIdx.x >> 5);
   if (item >= n.items) return;
   const WarpPart p = warp_part(c, w, n, item, c.heads * kPerHead);
   T* out = p.which ? v_out : k_out;
@@ -461,17 +496,17 @@ __global__ void __launch_bounds__(128, 8)
 }
 
 // Enough warps to fill the GPU: with few tokens their heads are divided (down
-// to four blocks per warp), with many a warp takes up to four tokens.
+// to four blocks per warp), with many a warp takes up to eight tokens.
 static Parts make_parts(const KvView& c, const KvTokens& w) {
   const int blocks = c.heads * (c.dim / 64), fours = (blocks + 3) / 4;
-  constexpr int64_t kWarps = 148 * 48;
+  constexpr int64_t kWarps = 148 * 32;
   Parts n{1, 1, 0, 0};
   while (n.parts < fours && w.tokens * 2 * n.parts < kWarps) ++n.parts;
   n.per = (fours + n.parts - 1) / n.parts * 4;
   n.parts = (blocks + n.per - 1) / n.per;
   if (n.parts == 1)
-    while (n.run < 4 && w.tokens * 2 / (n.run * 2) >= kWarps) n.run *= 2;
-  n.items = (w.tokens + n.run - 1) / n.run * 2 * n.parts;
+    while (n.run < 8 && w.tokens * 2 / (n.run * 2) >= kWarps) n.run *= 2;
+  n.items = (unsigned)((w.tokens + n.run - 1) / n.run * 2 * n.parts);   // tokens < 2^31, and parts > 1 for few
   return n;
 }
 
