@@ -76,29 +76,18 @@ __device__ __forceinline__ uint32_t bf16_up(float x) {     // finite x >= 0
 // is taken instead if it is already enough: below * L is exact, and with the
 // difference rounded up, "difference <= below * L" decides exactly (an f32 is
 // not below the exact difference if and only if it is not below that
-// difference rounded up).  Ranges that pass f32 are done in 64 bits.
-template <int BITS>
-__device__ __noinline__ uint32_t group_params_wide(float mn, float mx) {
-  constexpr int L = (1 << BITS) - 1;
-  const uint32_t lo = bf16_down(mn);
-  // (not negative: a maximum below the lowest finite bf16 gives s = 0)
-  const double range = fmax((double)mx - (double)__uint_as_float(lo << 16), 0.0);
-  uint32_t s = bf16_up(__double2float_ru(range * ((1.0 + 1e-15) / L)));
-  if (s > 0) {
-    const double below = (double)__uint_as_float((s - 1) << 16);
-    if (range <= below * L) --s;
-  }
-  return s | (lo << 16);
-}
-
+// difference rounded up).  Ranges that may pass f32 are taken at a sixteenth.
 template <int BITS>
 __device__ __forceinline__ uint32_t group_params(float mn, float mx) {
   constexpr int L = (1 << BITS) - 1;
-  if (fmaxf(fabsf(mn), fabsf(mx)) > 1e38f) return group_params_wide<BITS>(mn, mx);
+  const bool wide = fmaxf(fabsf(mn), fabsf(mx)) > 1e38f;
+  const float z = wide ? 0.0625f : 1.0f;
   const uint32_t lo = bf16_down(mn);
-  const float range = __fsub_ru(mx, __uint_as_float(lo << 16));
+  // (not negative: a maximum below the lowest finite bf16 gives s = 0)
+  const float range = fmaxf(__fsub_ru(mx * z, __uint_as_float(lo << 16) * z), 0.0f);
   uint32_t s = bf16_up(__fmul_ru(range, (float)((1.0 + 1e-6) / L)));
   if (s > 0 && range <= __uint_as_float((s - 1) << 16) * (float)L) --s;
+  if (wide && s > 0) s += 4 << 7;   // times 16
   return s | (lo << 16);
 }
 
@@ -116,53 +105,62 @@ __device__ __forceinline__ float code_near_half(float x, float lo, float s, floa
   return d > e ? k + 1.0f : d < e ? k : 2.0f * rintf(0.5f * k + 0.25f);
 }
 
-// The codes, each on the bits of kRound (the code in the low byte).
+// The codes, each on the bits of kRound (the code in the low byte).  x is used
+// up.  Where the reciprocal of the scale or the range might not be finite (or
+// normal), all are scaled by a power of two first: |lo| is below 2^33 s, so
+// that nothing overflows.
 constexpr float kRound = 12582912.0f;   // 1.5 * 2^23: adding it rounds to an integer (half to even)
 
-// Scales whose reciprocal or range may not be finite take the 64-bit quotient.
 template <int BITS>
-__device__ __forceinline__ void group_codes(const float (&x)[8], float lo, float s, bool finite, uint32_t (&code)[8]) {
-  if (finite && s >= 1e-36f && s <= 1e36f && lo > -3e38f) {
-    // here lo <= x <= lo + L s, so that the quotient needs no clamp
-    float inv, worst = 0.0f;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
-    const F2 lo2 = f2(-lo, -lo), inv2 = f2(inv, inv), up = f2(kRound, kRound), down = f2(-kRound, -kRound);
+__device__ __forceinline__ void group_codes(float (&x)[8], float lo, float s, bool finite, uint32_t (&code)[8]) {
+  if (!(finite && s > 0.0f)) {
 #pragma unroll
-    for (int k = 0; k < 8; k += 2) {
-      const F2 u = f2_mul(f2_add(f2(x[k], x[k + 1]), lo2), inv2), r = f2_add(u, up), n = f2_add(r, down);
-      float r0, r1, u0, u1, n0, n1;
-      f2_split(r, r0, r1);
-      f2_split(u, u0, u1);
-      f2_split(n, n0, n1);
-      code[k] = __float_as_uint(r0);
-      code[k + 1] = __float_as_uint(r1);
-      worst = fmaxf(worst, fmaxf(fabsf(u0 - n0), fabsf(u1 - n1)));
-    }
-    // One at a time, by its index: in 16-bit types such values are exact ties
-    // more often than not, one in a few hundred.
-    uint32_t near = 0;
-    if (worst > 0.4998f) {
+    for (int k = 0; k < 8; ++k) code[k] = __float_as_uint(kRound);
+    return;
+  }
+  if (s < 1e-36f || s > 1e36f) {
+    const float z = s < 1.0f ? 1.2676506e30f : 0.0625f;   // 2^100, 2^-4
+    s *= z;
+    lo *= z;
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        near |= fabsf((x[k] - lo) * inv - (__uint_as_float(code[k]) - kRound)) > 0.4998f ? 1u << k : 0u;
-    }
-    while (near) {
-      const int at = __ffs(near) - 1;
-      near &= near - 1;
-      float xv = x[0];
+    for (int k = 0; k < 8; ++k) x[k] *= z;
+  }
+  // lo <= x <= lo + L s, so that the quotient needs no clamp, unless lo itself
+  // was clamped to the lowest finite bf16
 #pragma unroll
-      for (int k = 1; k < 8; ++k) xv = at == k ? x[k] : xv;
-      const uint32_t n = __float_as_uint(
-          fminf(code_near_half(xv, lo, s, (xv - lo) * inv), (float)((1 << BITS) - 1)) + kRound);
+  for (int k = 0; k < 8; ++k) x[k] = fmaxf(x[k], lo);
+  float inv, worst = 0.0f;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  const F2 lo2 = f2(-lo, -lo), inv2 = f2(inv, inv), up = f2(kRound, kRound), down = f2(-kRound, -kRound);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) code[k] = at == k ? n : code[k];
-    }
-  } else {
-    constexpr float L = (float)((1 << BITS) - 1);
+  for (int k = 0; k < 8; k += 2) {
+    const F2 u = f2_mul(f2_add(f2(x[k], x[k + 1]), lo2), inv2), r = f2_add(u, up), n = f2_add(r, down);
+    float r0, r1, u0, u1, n0, n1;
+    f2_split(r, r0, r1);
+    f2_split(u, u0, u1);
+    f2_split(n, n0, n1);
+    code[k] = __float_as_uint(r0);
+    code[k + 1] = __float_as_uint(r1);
+    worst = fmaxf(worst, fmaxf(fabsf(u0 - n0), fabsf(u1 - n1)));
+  }
+  // One at a time, by its index: in 16-bit types such values are exact ties
+  // more often than not, one in a few hundred.
+  uint32_t near = 0;
+  if (worst > 0.4998f) {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      code[k] = __float_as_uint(
-          kRound + (finite && s > 0.0f ? (float)fmin(fmax(rint(((double)x[k] - (double)lo) / (double)s), 0.0), (double)L) : 0.0f));
+      near |= fabsf((x[k] - lo) * inv - (__uint_as_float(code[k]) - kRound)) > 0.4998f ? 1u << k : 0u;
+  }
+  while (near) {
+    const int at = __ffs(near) - 1;
+    near &= near - 1;
+    float xv = x[0];
+#pragma unroll
+    for (int k = 1; k < 8; ++k) xv = at == k ? x[k] : xv;
+    const uint32_t n =
+        __float_as_uint(fminf(code_near_half(xv, lo, s, (xv - lo) * inv), (float)((1 << BITS) - 1)) + kRound);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) code[k] = at == k ? n : code[k];
   }
 }
 
