@@ -131,17 +131,11 @@ __device__ __forceinline__ void group_codes(float (&x)[8], float lo, float s, bo
   for (int k = 0; k < 8; ++k) x[k] = fmaxf(x[k], lo);
   float inv, worst = 0.0f;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
-  const F2 lo2 = f2(-lo, -lo), inv2 = f2(inv, inv), up = f2(kRound, kRound), down = f2(-kRound, -kRound);
 #pragma unroll
-  for (int k = 0; k < 8; k += 2) {
-    const F2 u = f2_mul(f2_add(f2(x[k], x[k + 1]), lo2), inv2), r = f2_add(u, up), n = f2_add(r, down);
-    float r0, r1, u0, u1, n0, n1;
-    f2_split(r, r0, r1);
-    f2_split(u, u0, u1);
-    f2_split(n, n0, n1);
-    code[k] = __float_as_uint(r0);
-    code[k + 1] = __float_as_uint(r1);
-    worst = fmaxf(worst, fmaxf(fabsf(u0 - n0), fabsf(u1 - n1)));
+  for (int k = 0; k < 8; ++k) {
+    const float u = (x[k] - lo) * inv, r = __fadd_rn(u, kRound);
+    worst = fmaxf(worst, fabsf(u - __fsub_rn(r, kRound)));
+    code[k] = __float_as_uint(r);
   }
   // One at a time, by its index: in 16-bit types such values are exact ties
   // more often than not, one in a few hundred.
@@ -433,10 +427,7 @@ __global__ void __launch_bounds__(128, 8)
       if (valid && store_group) params[row0 * D >> c.group_shift] = prm;
       if (values) {
 #pragma unroll
-        for (int k = 0; k < 8; k += 2) {
-          const F2 q = f2_add(f2(__uint_as_float(code[k]), __uint_as_float(code[k + 1])), f2(-kRound, -kRound));
-          f2_split(f2_fma(q, f2(s, s), f2(lo, lo)), x[k], x[k + 1]);
-        }
+        for (int k = 0; k < 8; ++k) x[k] = fmaf(__uint_as_float(code[k]) - kRound, s, lo);
         store8<T>(v_at, x);
       }
     }
@@ -483,10 +474,7 @@ __global__ void __launch_bounds__(128, 8)
         const float s = param_scale(prm[i]), lo = param_low(prm[i]);
         float v[8];
 #pragma unroll
-        for (int k = 0; k < 8; k += 2) {
-          const F2 q = f2_add(f2(__uint_as_float(code[k]), __uint_as_float(code[k + 1])), f2(-8388608.0f, -8388608.0f));
-          f2_split(f2_fma(q, f2(s, s), f2(lo, lo)), v[k], v[k + 1]);
-        }
+        for (int k = 0; k < 8; ++k) v[k] = fmaf(__uint_as_float(code[k]) - 8388608.0f, s, lo);
         if (valid) store8<T>(out_at + i * step, v);
       }
     }
