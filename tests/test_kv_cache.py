@@ -347,6 +347,59 @@ def test_attention_many_rows(dim):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim,bits,share", [(64, 4, 2), (64, 8, 4), (128, 4, 8), (128, 8, 1)])
+def test_attention_prompt_chunks(dim, bits, share, dtype):
+    """Prompt chunks in the 16-bit types: tiles that end inside a page, chunks of
+    every alignment, a sequence whose first rows see almost nothing."""
+    lens = [129, 64, 200, 1, 333]
+    c = Case(lens, 2, dim, bits, 64, 16, dtype, seed=dim + bits)
+    check_attention(c, [129, 63, 70, 1, 130], 2 * share, dtype, seed=share, pad=2)
+    check_attention(c, [129, 64, 200, 1, 333], 2 * share, dtype, -0.05, seed=share + 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_prompt_chunks_with_missing_pages_and_nan(dtype):
+    """Rows meet neither the positions of a missing page nor a NaN they do not see."""
+    c = Case([150], 1, 128, 4, 64, 16, dtype, seed=21)
+    q = torch.randn(100, 4, 128).to(dtype)
+    lens, cu = i32([150]), i32([0, 100])
+    table = c.table.clone()
+    table[0, 2] = -1
+    out = f64(gpu_kv_cache_attention(c.cache, q.to(DEV), table, lens, cu))
+    assert status() == _lib.ICX_DEVICE_BAD_PAGE
+    keep = [p for p in range(150) if not 32 <= p < 48]
+    k, v = (x[keep] for x in c.sequence(0))
+    want = ref.attention(f64(q), k, v, 128 ** -0.5)
+    tol = ref.attention_tolerance(f64(q), k, v, 128 ** -0.5, dtype, want)
+    assert (np.abs(out - want) <= tol).all()
+    # position 120's V is NaN in the first group: rows from 70 on, dimensions 0..63
+    bad = c.v[120:121].clone()
+    bad[..., 5] = float("nan")
+    gpu_kv_cache_append(c.cache, c.k[120:121].to(DEV), bad.to(DEV), c.table, i32([121]), i32([0, 1]))
+    out = gpu_kv_cache_attention(c.cache, q.to(DEV), c.table, lens, cu)
+    nan = out.isnan()
+    assert nan[70:, :, :64].all() and not nan[:70].any() and not nan[..., 64:].any()
+    # and with a NaN K, every dimension of the rows that see it
+    gpu_kv_cache_append(c.cache, bad.to(DEV), c.v[120:121].to(DEV), c.table, i32([121]), i32([0, 1]))
+    nan = gpu_kv_cache_attention(c.cache, q.to(DEV), c.table, lens, cu).isnan()
+    assert nan[70:].all() and not nan[:70].any()
+    assert status() == 0
+
+
+@pytest.mark.gpu
+def test_prompt_chunk_values_of_unequal_size():
+    """V groups and K scales of very different sizes in one prompt chunk."""
+    c = Case([300], 1, 128, 4, 64, 16, torch.bfloat16, seed=22)
+    k = (c.k * torch.linspace(0.1, 2.0, 300)[:, None, None]).bfloat16()
+    v = (c.v * torch.pow(10.0, torch.arange(300) % 5 - 4.0)[:, None, None]).bfloat16()
+    gpu_kv_cache_append(c.cache, k.to(DEV), v.to(DEV), c.table, i32([300]), i32([0, 300]))
+    c.kv = [ref.cached_values(f64(x), 4, 64) for x in (k, v)]
+    check_attention(c, [200], 4, torch.bfloat16, seed=8)
+
+
+@pytest.mark.gpu
 def test_attention_scales_and_strong_scores():
     """Scores of order 100 (one position takes all), scale 0, negative scale, tiny and huge q."""
     for spread, q_scale, scale in ((4.0, 4.0, 0.5), (1.0, 1.0, 0.0), (1.0, 1.0, -0.3), (1.0, 1e-6, None),
