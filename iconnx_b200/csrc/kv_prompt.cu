@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(kPrThreads, 2)
   }
   pdl_wait();
   pdl_trigger();
-  if (warp == 0) find_row_tile(c, w, share, blockIdx.x, &s_seq, &s_tile);
+  if (warp == 0) find_row_tile(c, w, share, kPrRows, blockIdx.x, &s_seq, &s_tile);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

@@ -69,13 +69,13 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int co
 
 // The want-th row tile of the batch, the last tiles of a sequence (the longest)
 // first; *seq = -1 if there is none.  One warp.
-__device__ __forceinline__ void find_row_tile(const KvView& c, const KvTokens& w, int share, int want, int* seq_out,
-                                              int* tile_out) {
+__device__ __forceinline__ void find_row_tile(const KvView& c, const KvTokens& w, int share, int rows, int want,
+                                              int* seq_out, int* tile_out) {
   const int lane = threadIdx.x & 31;
   int before = 0, seq = -1, tile = 0;
   for (int b0 = 0; b0 < w.batch && seq < 0; b0 += 32) {
     const int b = b0 + lane;
-    const int n = b < w.batch ? seq_units(c, w, share, kPrRows, b).tiles : 0;
+    const int n = b < w.batch ? seq_units(c, w, share, rows, b).tiles : 0;
     int inc = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {

@@ -13,37 +13,42 @@
 // the value times 2^-E.  The CTA looks over the scales of all its positions
 // first (a sixteenth of the cache) to choose E for K and for V.
 //
-// A CTA takes 128 query rows of one (sequence, K/V head), 48 positions at a
-// time, two CTAs per SM:
-//   warps 0..3  softmax, thread = row.  Two score accumulators, so the next
-//               tile's scores are computed meanwhile; the weights go back over
-//               the accumulator they came from, as the left operand of the
-//               output product.
-//   warps 4..6  bring codes and scales from the pages, dequantise and store
-//               (K and V apart, two stages each).
-//   warp 7      issues the products: the output's of tile i and the scores' of
-//               tile i + 2 when tile i's weights are there.
-// (48 positions rather than 64: three warps fill them, the fourth of that
-// group is free to issue, and a row's scores stay in 128 registers.)
+// A CTA (one per SM) takes 256 query rows of one (sequence, K/V head) as two
+// tiles of 128, 48 positions at a time, so that what is dequantised serves both;
+// 128 rows where there are too few rows to fill the GPU otherwise:
+//   warps 0..7   softmax, thread = row.  Two score accumulators per row tile, so
+//                the next tile's scores are computed meanwhile; the weights go
+//                back over the accumulator they came from, as the left operand
+//                of the output product.
+//   warps 8..13  bring codes and scales from the pages, dequantise and store,
+//                three warps for even tiles of positions and three for odd ones
+//                (K and V apart, four stages each).
+//   warps 14, 15 issue the products of a row tile each: the output's of tile i
+//                and the scores' of tile i + 2 when tile i's weights are there.
+// (48 positions rather than 64: three warps fill them, two threads to each, and
+// a row's scores stay in 128 registers.)
 // Rows that do not see a position must not meet its NaN: a V group that holds
 // one is stored as zeros, and the rows that see it end as NaN.  That and pages
 // that are missing are found in the first look; only then do the softmax warps
 // ask for them, tile by tile.
 #include "kv_prompt.cuh"
+#include "tmap.cuh"
 
 namespace icx {
 
 constexpr int kB16Keys = 48;   // positions per tile: what three warps dequantise, two threads to each
-constexpr int kB16Threads = 256;
+constexpr int kB16Threads = 512, kB16Stages = 4;
 constexpr int kB16Cols = 64;   // tensor memory columns of an accumulator
 
 template <int D>
 struct PromptB16Config {
   static constexpr int G = D / kPrGroup;
-  static constexpr int kQ = G * kPrRows * 128;
+  static constexpr int kQ = G * kPrRows * 128;        // of a row tile
   static constexpr int kTile = G * kB16Keys * 128;    // K or V of a stage
-  static constexpr int kSmem = 1024 + kQ + 4 * kTile;
-  static constexpr int kTmemCols = 256;               // two score accumulators, D columns of output
+  static constexpr int kSmem = 1024 + 2 * kQ + 2 * kB16Stages * kTile;
+  // per row tile two score accumulators, then per row tile the output
+  static constexpr int kTmemCols = 512;
+  static constexpr int kOutCol = 4 * kB16Cols;
 };
 
 
@@ -87,20 +92,21 @@ __device__ __forceinline__ uint4 dequantize(uint32_t w0, uint32_t w1, const Grou
 }
 
 template <int D, int BITS>
-__global__ void __launch_bounds__(kB16Threads, 2)
+__global__ void __launch_bounds__(kB16Threads, 1)
     kv_prompt_bf16_kernel(const __grid_constant__ KvView c, const __grid_constant__ KvTokens w,
-                          const __grid_constant__ AttendArgs a) {
+                          const __grid_constant__ AttendArgs a, int rows_per_cta) {
   using T = __nv_bfloat16;
   using C = PromptB16Config<D>;
   constexpr int G = C::G;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* s_q = smem;
-  auto s_k = [&](int n) { return smem + C::kQ + n * C::kTile; };
-  auto s_v = [&](int n) { return smem + C::kQ + (2 + n) * C::kTile; };
-  __shared__ __align__(8) uint64_t bars[14];
-  uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6, *s_full = bars + 8,
-           *p_full = bars + 10, *q_full = bars + 12, *o_full = bars + 13;
+  auto s_k = [&](int n) { return smem + 2 * C::kQ + n * C::kTile; };
+  auto s_v = [&](int n) { return smem + 2 * C::kQ + (kB16Stages + n) * C::kTile; };
+  __shared__ __align__(8) uint64_t bars[4 * kB16Stages + 10];
+  uint64_t *k_full = bars, *k_empty = k_full + kB16Stages, *v_full = k_empty + kB16Stages, *v_empty = v_full + kB16Stages;
+  uint64_t *s_full = v_empty + kB16Stages, *p_full = s_full + 4;   // [row tile][accumulator]
+  uint64_t *q_full = p_full + 4, *o_full = q_full + 1;
   __shared__ uint32_t s_look[5];   // largest s and |lo| of K, of V; whether anything is special
   __shared__ uint32_t tmem_slot;
   __shared__ int s_seq, s_tile;
@@ -109,37 +115,39 @@ __global__ void __launch_bounds__(kB16Threads, 2)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 5; ++i) s_look[i] = 0u;
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kB16Stages; ++i) {
       mbar_init(&k_full[i], 3);    // one arrival per warp
       mbar_init(&v_full[i], 3);
-      mbar_init(&k_empty[i], 1);
-      mbar_init(&v_empty[i], 1);
+      mbar_init(&k_empty[i], 2);   // one per row tile
+      mbar_init(&v_empty[i], 2);
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
     }
-    mbar_init(q_full, 4);
-    mbar_init(o_full, 1);
+    mbar_init(q_full, 8);
+    mbar_init(o_full, 2);
     fence_barrier_init();
   }
-  if (warp == 7) {
+  if (warp == 14) {
     tmem_alloc(&tmem_slot, C::kTmemCols);
     tmem_relinquish();
   }
   pdl_wait();
   pdl_trigger();
-  if (warp == 0) find_row_tile(c, w, share, blockIdx.x, &s_seq, &s_tile);
+  if (warp == 0) find_row_tile(c, w, share, rows_per_cta, blockIdx.x, &s_seq, &s_tile);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   const int seq = s_seq, head = blockIdx.y;
   if (seq >= 0) {
-    const SeqUnits su = seq_units(c, w, share, kPrRows, seq);
-    const int r0 = s_tile * kPrRows, nrows = min(kPrRows, su.rows - r0);
+    const SeqUnits su = seq_units(c, w, share, rows_per_cta, seq);
+    const int r0 = s_tile * rows_per_cta, nrows = min(rows_per_cta, su.rows - r0);
+    const int row_tiles = nrows > kPrRows ? 2 : 1;
     const int64_t first_pos = (int64_t)su.len - su.n;
     const int reach = (int)min((int64_t)su.len, (int64_t)w.width << c.page_shift);
     const int see_any = (int)max((int64_t)0, min(first_pos + (r0 + nrows - 1) / share + 1, (int64_t)reach));
-    const int see_all = (int)max((int64_t)0, min(first_pos + r0 / share + 1, (int64_t)reach));
     const int tiles = (see_any + kB16Keys - 1) / kB16Keys;
     if (threadIdx.x == 0 && su.len > reach) record_status(ICX_DEVICE_BAD_PAGE);
 
@@ -182,56 +190,60 @@ __global__ void __launch_bounds__(kB16Threads, 2)
     const int k_exp = unit_for(s_look[0], s_look[1]), v_exp = unit_for(s_look[2], s_look[3]);
     const bool special = s_look[4] != 0u;
 
-    if (warp == 7) {
+    if (warp >= 14) {
       // ---------------------------------------------------------- products
-      if (elect_one()) {
+      const int h = warp - 14;   // row tile
+      if (h < row_tiles && elect_one()) {
         constexpr uint32_t id_s = prompt_idesc(kB16Keys, false), id_o = prompt_idesc(kPrGroup, true);
-        const uint32_t t_o = tmem + 2 * kB16Cols;
+        const uint64_t q_desc = smem_desc_k128(smem_addr(s_q + h * C::kQ));
+        const uint64_t k_desc = smem_desc_k128(smem_addr(s_k(0))), v_desc = smem_desc_k128(smem_addr(s_v(0)));
+        const uint32_t t_acc = tmem + (uint32_t)(2 * h * kB16Cols), t_out = tmem + (uint32_t)(C::kOutCol + h * 128);
+        // a stage is free when both row tiles' products have read it
+        auto done = [&](uint64_t* bar) {
+          mma_commit(bar);
+          if (row_tiles == 1) mma_commit(bar);
+        };
         // scores of tile i into accumulator i & 1 (its weights of two tiles ago
         // have been issued to the output product before)
-        auto issue_scores = [&](int i) {
-          const int st = i & 1;
-          if (!mbar_wait(&k_full[st], (i >> 1) & 1, ICX_DEVICE_TIMEOUT_MMA)) return false;
+        auto scores = [&](int i) {
+          const int st = i % kB16Stages;
+          if (!mbar_wait(&k_full[st], (uint32_t)(i / kB16Stages & 1), ICX_DEVICE_TIMEOUT_MMA)) return false;
           tc_fence_after();
+          const uint64_t kb = k_desc + (uint64_t)(st * (C::kTile >> 4));
 #pragma unroll
-          for (int k = 0; k < G; ++k) {
-            const uint64_t qa = smem_desc_k128(smem_addr(s_q + k * kPrRows * 128));
-            const uint64_t kb = smem_desc_k128(smem_addr(s_k(st) + k * kB16Keys * 128));
+          for (int k = 0; k < G; ++k)
 #pragma unroll
             for (int n = 0; n < kPrGroup / 16; ++n)
-              mma_f16_ss(tmem + (uint32_t)(st * kB16Cols), qa + (uint64_t)(n * 2), kb + (uint64_t)(n * 2), id_s,
-                         k > 0 || n > 0);
-          }
-          mma_commit(&s_full[st]);
-          mma_commit(&k_empty[st]);
+              mma_f16_ss(t_acc + (uint32_t)((i & 1) * kB16Cols), q_desc + (uint64_t)(k * (kPrRows * 128 >> 4) + n * 2),
+                         kb + (uint64_t)(k * (kB16Keys * 128 >> 4) + n * 2), id_s, k > 0 || n > 0);
+          mma_commit(&s_full[2 * h + (i & 1)]);
+          done(&k_empty[st]);
           return true;
         };
         bool ok = tiles > 0 && mbar_wait(q_full, 0, ICX_DEVICE_TIMEOUT_MMA);
-        if (ok) ok = issue_scores(0);
-        if (ok && tiles > 1) ok = issue_scores(1);
+        for (int i = 0; i < 2 && i < tiles && ok; ++i) ok = scores(i);
         for (int i = 0; i < tiles && ok; ++i) {
-          const int st = i & 1;
-          ok = mbar_wait(&v_full[st], (i >> 1) & 1, ICX_DEVICE_TIMEOUT_MMA) &&
-               mbar_wait(&p_full[st], (i >> 1) & 1, ICX_DEVICE_TIMEOUT_MMA);
+          const int st = i % kB16Stages;
+          ok = mbar_wait(&v_full[st], (uint32_t)(i / kB16Stages & 1), ICX_DEVICE_TIMEOUT_MMA) &&
+               mbar_wait(&p_full[2 * h + (i & 1)], (i >> 1) & 1, ICX_DEVICE_TIMEOUT_MMA);
           if (!ok) break;
           tc_fence_after();
+          const uint64_t vb = v_desc + (uint64_t)(st * (C::kTile >> 4));
 #pragma unroll
-          for (int k = 0; k < G; ++k) {
-            const uint64_t b = smem_desc_k128(smem_addr(s_v(st) + k * kB16Keys * 128));
+          for (int k = 0; k < G; ++k)
 #pragma unroll
             for (int n = 0; n < kB16Keys / 16; ++n)
-              mma_f16_ts(t_o + (uint32_t)(k * kPrGroup), tmem + (uint32_t)(st * kB16Cols + n * 8), b + (uint64_t)(n * 128),
-                         id_o, i > 0 || n > 0);
-          }
-          mma_commit(&v_empty[st]);
-          if (i + 2 < tiles) ok = issue_scores(i + 2);
-          if (i + 1 == tiles) mma_commit(o_full);
+              mma_f16_ts(t_out + (uint32_t)(k * kPrGroup), t_acc + (uint32_t)((i & 1) * kB16Cols + n * 8),
+                         vb + (uint64_t)(k * (kB16Keys * 128 >> 4) + n * 128), id_o, i > 0 || n > 0);
+          done(&v_empty[st]);
+          if (i + 2 < tiles) ok = scores(i + 2);
+          if (ok && i + 1 == tiles) done(o_full);
         }
       }
       __syncwarp();
-    } else if (warp >= 4) {
+    } else if (warp >= 8) {
       // ------------------------------------------------------ dequantising
-      const int p = threadIdx.x - 128, key = p >> 1, half = p & 1;
+      const int set = (warp - 8) / 3, p = threadIdx.x - 256 - set * 96, key = p >> 1, half = p & 1;   // set: tiles set, set + 2, ..
       // the next tile's K codes and scales are fetched when this one's are
       // stored, its V codes likewise
       RawCodes<D, BITS> raw;
@@ -256,19 +268,20 @@ __global__ void __launch_bounds__(kB16Threads, 2)
       const float k_down = power_of_two(-k_exp), v_down = power_of_two(-v_exp);
       const float k_up24 = k_down * 16777216.0f, v_up24 = v_down * 16777216.0f;
       bool ok = true;
-      if (tiles > 0) {
-        find(0);
+      if (set < tiles) {
+        find(set);
         fetch_k();
         row = row_next;
         fetch_v();
-        if (tiles > 1) find(1);
+        if (set + 2 < tiles) find(set + 2);
       }
-      for (int i = 0; i < tiles; ++i) {
-        const int st = i & 1;
+      for (int i = set; i < tiles; i += 2) {
+        const int st = i % kB16Stages;
+        const uint32_t free = (uint32_t)(i / kB16Stages & 1) ^ 1;
         uint32_t vq[G];
 #pragma unroll
         for (int k = 0; k < G; ++k) vq[k] = vp[k];
-        if (ok) ok = wait_warp(&k_empty[st], ((i >> 1) & 1) ^ 1, ICX_DEVICE_TIMEOUT_PRODUCER);
+        if (ok) ok = wait_warp(&k_empty[st], free, ICX_DEVICE_TIMEOUT_PRODUCER);
 #pragma unroll
         for (int k = 0; k < G; ++k) {
           const GroupF16 g(kp[k], k_up24, k_down, row < 0);
@@ -285,8 +298,8 @@ __global__ void __launch_bounds__(kB16Threads, 2)
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&k_full[st]);
-        if (i + 1 < tiles) fetch_k();
-        if (ok) ok = wait_warp(&v_empty[st], ((i >> 1) & 1) ^ 1, ICX_DEVICE_TIMEOUT_PRODUCER);
+        if (i + 2 < tiles) fetch_k();
+        if (ok) ok = wait_warp(&v_empty[st], free, ICX_DEVICE_TIMEOUT_PRODUCER);
 #pragma unroll
         for (int k = 0; k < G; ++k) {
           const GroupF16 g(vq[k], v_up24, v_down, row < 0 || isnan(param_scale(vq[k])));
@@ -302,20 +315,23 @@ __global__ void __launch_bounds__(kB16Threads, 2)
         __syncwarp();
         if (lane == 0) mbar_arrive(&v_full[st]);
         row = row_next;
-        if (i + 1 < tiles) fetch_v();
-        if (i + 2 < tiles) find(i + 2);
+        if (i + 2 < tiles) fetch_v();
+        if (i + 4 < tiles) find(i + 4);
       }
     } else {
       // ---------------------------------------------------------- softmax
-      const int row = threadIdx.x, r = r0 + row;   // this thread's row = TMEM lane
-      const bool mine = r < su.rows;
+      const int row = threadIdx.x, r = r0 + row;   // this thread's row = TMEM lane of its row tile
+      const bool mine = row < nrows;
       const int see = mine ? (int)max((int64_t)0, min(first_pos + r / share + 1, (int64_t)reach)) : 0;
-      const uint32_t t_lane = (uint32_t)(warp * 32) << 16, t_o = tmem + 2 * kB16Cols;
+      const int h = warp >> 2;                     // row tile
+      const uint32_t t_lane = (uint32_t)((warp & 3) * 32) << 16, t_o = tmem + (uint32_t)(C::kOutCol + h * 128);
+      // positions that every row of the tile sees
+      const int see_all = (int)max((int64_t)0, min(first_pos + (r0 + h * kPrRows) / share + 1, (int64_t)reach));
       bool ok = true;
       const T* q = static_cast<const T*>(a.q) + (int64_t)(su.from + (mine ? r / share : 0)) * a.q_token_stride +
                    (int64_t)(head * share + (mine ? r % share : 0)) * a.q_head_stride;
       float f, qsum[G];
-      put_query<T, G, BITS, false>(a, q, mine, row, s_q, &f, qsum);
+      put_query<T, G, BITS, false>(a, q, mine, row & (kPrRows - 1), s_q + h * C::kQ, &f, qsum);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
@@ -324,12 +340,12 @@ __global__ void __launch_bounds__(kB16Threads, 2)
       bool vnan[G];
 #pragma unroll
       for (int k = 0; k < G; ++k) vnan[k] = false;
-      for (int i = 0; i < tiles && ok; ++i) {
+      for (int i = 0; i < tiles && ok && h < row_tiles; ++i) {
         const int st = i & 1;
-        ok = wait_warp(&s_full[st], (i >> 1) & 1, ICX_DEVICE_TIMEOUT_EPILOGUE);
+        ok = wait_warp(&s_full[2 * h + st], (i >> 1) & 1, ICX_DEVICE_TIMEOUT_EPILOGUE);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t t_s = tmem + t_lane + (uint32_t)(st * kB16Cols);
+        const uint32_t t_s = tmem + t_lane + (uint32_t)((2 * h + st) * kB16Cols);
         uint32_t x0[32], x1[16];
         tmem_ld_32x32b_x32(t_s, x0);
         tmem_ld_32x32b_x16(t_s + 32, x1);
@@ -372,7 +388,7 @@ __global__ void __launch_bounds__(kB16Threads, 2)
           l *= alpha;
           if (i > 0) {
             // the output so far: its last product has to be there
-            ok = wait_warp(&v_empty[(i - 1) & 1], ((i - 1) >> 1) & 1, ICX_DEVICE_TIMEOUT_EPILOGUE);
+            ok = wait_warp(&v_empty[(i - 1) % kB16Stages], (uint32_t)((i - 1) / kB16Stages & 1), ICX_DEVICE_TIMEOUT_EPILOGUE);
             if (!ok) break;
             tc_fence_after();
 #pragma unroll 1
@@ -414,7 +430,7 @@ __global__ void __launch_bounds__(kB16Threads, 2)
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[st]);
+        if (lane == 0) mbar_arrive(&p_full[2 * h + st]);
       }
       // ----------------------------------------------------------- output
       if (tiles > 0 && ok) ok = wait_warp(o_full, 0, ICX_DEVICE_TIMEOUT_EPILOGUE);
@@ -423,7 +439,7 @@ __global__ void __launch_bounds__(kB16Threads, 2)
       const float up = power_of_two(v_exp);
       T* out = static_cast<T*>(a.out) +
                ((int64_t)(su.from + (mine ? r / share : 0)) * a.q_heads + head * share + (mine ? r % share : 0)) * D;
-      if (ok) {
+      if (ok && h < row_tiles) {
 #pragma unroll 1
         for (int k = 0; k < G; ++k) {
           bool bad = vnan[0];
@@ -456,7 +472,7 @@ __global__ void __launch_bounds__(kB16Threads, 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 7) tmem_dealloc(tmem, C::kTmemCols);
+  if (warp == 14) tmem_dealloc(tmem, C::kTmemCols);
 }
 
 template <int D, int BITS>
@@ -465,8 +481,11 @@ static int launch_kernel(cudaStream_t s, const KvView& c, const KvTokens& w, con
   auto kern = kv_prompt_bf16_kernel<D, BITS>;
   ICX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
   const int64_t share = a.q_heads / c.heads;
-  const dim3 grid((unsigned)(w.tokens * share / kPrRows + w.batch), (unsigned)c.heads);   // at most so many row tiles
-  ICX_CUDA(launch_pdl(kern, grid, dim3(kB16Threads), C::kSmem, s, c, w, a));
+  // at most so many row tiles; twice the rows per CTA if they still fill the GPU
+  const auto tiles = [&](int rows) { return w.tokens * share / rows + w.batch; };
+  const int rows = (tiles(2 * kPrRows) - w.batch / 2) * c.heads >= sm_count() ? 2 * kPrRows : kPrRows;
+  const dim3 grid((unsigned)tiles(rows), (unsigned)c.heads);
+  ICX_CUDA(launch_pdl(kern, grid, dim3(kB16Threads), C::kSmem, s, c, w, a, rows));
   return ICX_OK;
 }
 
