@@ -8,6 +8,10 @@ namespace icx {
 
 AttendPlan plan_attend(const KvView& c, const KvTokens& w, int q_heads, int type) {
   AttendPlan p{};
+  if (prompt_preferred(c, w, q_heads, type)) {
+    p.bytes = plan_prompt(c, w, q_heads, type).bytes;
+    return p;
+  }
   const int share = q_heads / c.heads;
   // rows that share one read of the cache: as many as the average sequence
   // has, up to what the registers (and, for two f16 parts of 256 dimensions of
@@ -44,7 +48,7 @@ extern "C" size_t icx_kv_cache_attention_workspace_bytes(const icx_kv_cache* cac
       q_heads % c.heads)
     return 0;
   if (!is_float_type(type)) return 0;
-  return prompt_preferred(c, w, q_heads, type) ? 0 : plan_attend(c, w, q_heads, type).bytes;
+  return plan_attend(c, w, q_heads, type).bytes;
 }
 
 extern "C" int icx_kv_cache_attention(void* stream, const icx_kv_cache* cache, const icx_kv_tokens* where,
@@ -66,7 +70,7 @@ extern "C" int icx_kv_cache_attention(void* stream, const icx_kv_cache* cache, c
   ICX_REQUIRE(d_q && d_out, "KvCacheAttention: null operand");
   ICX_REQUIRE((reinterpret_cast<uintptr_t>(d_out) & 15) == 0, "KvCacheAttention: out must be 16-byte aligned");
   const bool prompt = prompt_preferred(c, w, q_heads, type);
-  const AttendPlan p = prompt ? AttendPlan{} : plan_attend(c, w, q_heads, type);
+  const AttendPlan p = plan_attend(c, w, q_heads, type);
   if (p.bytes > 0 && (!d_workspace || workspace_bytes < p.bytes)) {
     set_error("KvCacheAttention: workspace %zu bytes < %zu required", d_workspace ? workspace_bytes : 0, p.bytes);
     return ICX_ERR_WORKSPACE;

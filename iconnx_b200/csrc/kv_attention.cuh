@@ -784,6 +784,13 @@ AttendPlan plan_attend(const KvView& c, const KvTokens& w, int q_heads, int type
 bool prompt_preferred(const KvView& c, const KvTokens& w, int q_heads, int type);
 int launch_prompt(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a, int type);
 
+// Rows per CTA, shares of the positions, and the workspace these need.
+struct PromptPlan {
+  int rows, splits;
+  size_t bytes;
+};
+PromptPlan plan_prompt(const KvView& c, const KvTokens& w, int q_heads, int type);
+
 template <typename T>
 int launch_attend(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a, const AttendPlan& p);
 

@@ -25,6 +25,7 @@
 // Bound by the softmax warps (about ten instructions per score, pairs of f32 in
 // one) beside the tensor cores.
 #include "kv_prompt.cuh"
+#include "tmap.cuh"
 
 namespace icx {
 
@@ -43,7 +44,7 @@ struct PromptConfig {
 template <typename T, int D, int BITS>
 __global__ void __launch_bounds__(kPrThreads, 2)
     kv_prompt_kernel(const __grid_constant__ KvView c, const __grid_constant__ KvTokens w,
-                     const __grid_constant__ AttendArgs a) {
+                     const __grid_constant__ AttendArgs a, int splits) {
   using C = PromptConfig<D>;
   constexpr int G = C::G;
   constexpr bool PLO = true;   // w s as two f16: an f16 output has as many bits as one
@@ -92,7 +93,8 @@ __global__ void __launch_bounds__(kPrThreads, 2)
     const int reach = (int)min((int64_t)su.len, (int64_t)w.width << c.page_shift);
     const int see_any = (int)max((int64_t)0, min(first_pos + (r0 + nrows - 1) / share + 1, (int64_t)reach));
     const int see_all = (int)max((int64_t)0, min(first_pos + r0 / share + 1, (int64_t)reach));
-    const int tiles = (see_any + kPrKeys - 1) / kPrKeys;
+    const PromptShare part(see_any, kPrKeys, splits);
+    const int tiles = part.tiles, p0 = part.first, p_end = part.end;
     if (threadIdx.x == 0 && su.len > reach) record_status(ICX_DEVICE_BAD_PAGE);
 
     if (warp >= 4) {
@@ -103,16 +105,16 @@ __global__ void __launch_bounds__(kPrThreads, 2)
       uint32_t kp[2][G], vp[2][G];   // warp 4: parameters of positions lane, lane + 32
       bool pvalid[2] = {false, false};
       auto fetch = [&](int i) {
-        const int pos = i * kPrKeys + key;
-        const int64_t page = pos < see_any ? kv_page(c, w, seq, pos) : -1;
-        hole = pos < see_any && page < 0;
+        const int pos = p0 + i * kPrKeys + key;
+        const int64_t page = pos < p_end ? kv_page(c, w, seq, pos) : -1;
+        hole = pos < p_end && page < 0;
         if (hole && half == 0) record_status(ICX_DEVICE_BAD_PAGE);
         if (page >= 0) raw.load(c, kv_row(c, page, head, pos), pos, half);
         if (warp == 4) {
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const int pp = i * kPrKeys + lane + 32 * x;
-            const int64_t pg = pp < see_any ? kv_page(c, w, seq, pp) : -1;
+            const int pp = p0 + i * kPrKeys + lane + 32 * x;
+            const int64_t pg = pp < p_end ? kv_page(c, w, seq, pp) : -1;
             pvalid[x] = pg >= 0;
             if (pvalid[x]) {
               const int64_t row = kv_row(c, pg, head, pp) * G;
@@ -266,7 +268,7 @@ __global__ void __launch_bounds__(kPrThreads, 2)
         tc_fence_after();
         const float* prm = s_p(st);
         const uint4 holes = *reinterpret_cast<const uint4*>(s_fix + 4 + 4 * st);
-        const bool edge = (i + 1) * kPrKeys > see_all || (holes.x | holes.y | holes.z | holes.w) != 0;
+        const bool edge = p0 + (i + 1) * kPrKeys > see_all || (holes.x | holes.y | holes.z | holes.w) != 0;
         // -- scores (in units of 1 / f)
         float s[kPrKeys];
 #pragma unroll
@@ -299,7 +301,7 @@ __global__ void __launch_bounds__(kPrThreads, 2)
           const uint32_t hw[4] = {holes.x, holes.y, holes.z, holes.w};
 #pragma unroll
           for (int j = 0; j < kPrKeys; ++j)
-            if (i * kPrKeys + j >= see || (hw[j >> 4] >> (2 * (j & 15)) & 1u)) s[j] = -INFINITY;
+            if (p0 + i * kPrKeys + j >= see || (hw[j >> 4] >> (2 * (j & 15)) & 1u)) s[j] = -INFINITY;
         }
         // -- the reference, and the output's factors when it or the scale of w s moves
         float top = s[0];
@@ -396,8 +398,8 @@ __global__ void __launch_bounds__(kPrThreads, 2)
       if (tiles > 0 && ok) ok = wait_warp(o_full, 0, ICX_DEVICE_TIMEOUT_EPILOGUE);
       tc_fence_after();
       const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-      T* out = static_cast<T*>(a.out) +
-               ((int64_t)(su.from + (mine ? r / share : 0)) * a.q_heads + head * share + (mine ? r % share : 0)) * D;
+      const int64_t out_row = (int64_t)(su.from + (mine ? r / share : 0)) * a.q_heads + head * share + (mine ? r % share : 0);
+      const PromptOut<T, D> out(a, w, splits, out_row);
       if (ok) {
 #pragma unroll 1
         for (int k = 0; k < G; ++k) {
@@ -422,11 +424,10 @@ __global__ void __launch_bounds__(kPrThreads, 2)
                 const int d = v_dim<BITS>(j, i);
                 y[d >> 3][d & 7] = l != 0.0f ? fmaf(o * (times16<BITS>(i) ? 1048576.0f : 16777216.0f), up, low) * inv : 0.0f;
               }
-            if (mine)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) store_f32<T, 8>(out + k * kPrGroup + 32 * n + 8 * j, y[j]);
+            if (mine) out.put(k * kPrGroup + 32 * n, y);
           }
         }
+        if (mine) out.put_weight(fmaxf(m * f, -3e38f), l);
       }
     }
   }
@@ -437,20 +438,18 @@ __global__ void __launch_bounds__(kPrThreads, 2)
 }
 
 template <typename T, int D, int BITS>
-static int launch_prompt_kernel(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a) {
+static int launch_prompt_kernel(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a, const PromptPlan& p) {
   using C = PromptConfig<D>;
   auto kern = kv_prompt_kernel<T, D, BITS>;
   ICX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
-  const int64_t share = a.q_heads / c.heads;
-  const dim3 grid((unsigned)(w.tokens * share / kPrRows + w.batch), (unsigned)c.heads);   // at most so many row tiles
-  ICX_CUDA(launch_pdl(kern, grid, dim3(kPrThreads), C::kSmem, s, c, w, a));
-  return ICX_OK;
+  ICX_CUDA(launch_pdl(kern, prompt_grid(c, w, a, p), dim3(kPrThreads), C::kSmem, s, c, w, a, p.splits));
+  return launch_prompt_join<T, D>(s, w, a, p);
 }
 
-static int launch_prompt_f16(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a) {
+static int launch_prompt_f16(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a, const PromptPlan& p) {
   using T = __half;
-  if (c.dim == 64) return c.bits == 4 ? launch_prompt_kernel<T, 64, 4>(s, c, w, a) : launch_prompt_kernel<T, 64, 8>(s, c, w, a);
-  return c.bits == 4 ? launch_prompt_kernel<T, 128, 4>(s, c, w, a) : launch_prompt_kernel<T, 128, 8>(s, c, w, a);
+  if (c.dim == 64) return c.bits == 4 ? launch_prompt_kernel<T, 64, 4>(s, c, w, a, p) : launch_prompt_kernel<T, 64, 8>(s, c, w, a, p);
+  return c.bits == 4 ? launch_prompt_kernel<T, 128, 4>(s, c, w, a, p) : launch_prompt_kernel<T, 128, 8>(s, c, w, a, p);
 }
 
 bool prompt_preferred(const KvView& c, const KvTokens& w, int q_heads, int type) {
@@ -459,8 +458,34 @@ bool prompt_preferred(const KvView& c, const KvTokens& w, int q_heads, int type)
   return rows >= 64;
 }
 
+PromptPlan plan_prompt(const KvView& c, const KvTokens& w, int q_heads, int type) {
+  PromptPlan p{kPrRows, 1, 0};
+  const int64_t share = q_heads / c.heads;
+  // about so many row tiles; bf16 takes twice the rows per CTA if they still
+  // fill the GPU
+  const auto tiles = [&](int rows) { return (w.tokens * share + rows - 1) / rows * c.heads; };
+  if (type == ICX_BF16 && tiles(2 * kPrRows) >= sm_count()) p.rows = 2 * kPrRows;
+  // Positions in shares where that fills the GPU (128 tokens of one sequence of
+  // 32,000, 8 K/V heads of 4 query heads: PLACEHOLDER).  A CTA's start and end cost about
+  // what `own` positions cost, and its number of positions is at most the page
+  // table's (the host does not know more).
+  const double own = type == ICX_BF16 ? 900 : 300, reach = (double)((int64_t)w.width << c.page_shift);
+  const int64_t n = tiles(p.rows), at_once = (int64_t)sm_count() * (type == ICX_BF16 ? 1 : 2);
+  double best = 0;
+  for (int x = 1; x <= 32 && (x == 1 || n * x <= 2 * at_once); ++x) {
+    const double time = (double)((n * x + at_once - 1) / at_once) * (reach / x + own);
+    if (x == 1 || time < 0.9 * best) {
+      best = time;
+      p.splits = x;
+    }
+  }
+  if (p.splits > 1) p.bytes = (size_t)p.splits * w.tokens * q_heads * (c.dim + 2) * 4;
+  return p;
+}
+
 int launch_prompt(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a, int type) {
-  return type == ICX_F16 ? launch_prompt_f16(s, c, w, a) : launch_prompt_bf16(s, c, w, a);
+  const PromptPlan p = plan_prompt(c, w, a.q_heads, type);
+  return type == ICX_F16 ? launch_prompt_f16(s, c, w, a, p) : launch_prompt_bf16(s, c, w, a, p);
 }
 
 }  // namespace icx

@@ -192,6 +192,87 @@ __device__ __forceinline__ void put_query(const AttendArgs& a, const T* q, bool 
   }
 }
 
-int launch_prompt_bf16(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a);
+// A CTA's share of the positions below `see`: whole tiles of `keys`.
+struct PromptShare {
+  int first, end, tiles;
+  __device__ __forceinline__ PromptShare(int see, int keys, int splits) {
+    const int all = (see + keys - 1) / keys, t0 = (int)((int64_t)all * blockIdx.z / splits);
+    tiles = (int)((int64_t)all * (blockIdx.z + 1) / splits) - t0;
+    first = t0 * keys;
+    end = min(see, first + tiles * keys);
+  }
+};
+
+// A row's output, or with several shares its part in the workspace: the values
+// over the share's own weights, the reference of its scores and the sum of its
+// weights, at [share][token][query head].
+template <typename T, int D>
+struct PromptOut {
+  T* out;
+  float* part;
+  __device__ __forceinline__ PromptOut(const AttendArgs& a, const KvTokens& w, int splits, int64_t row) {
+    out = static_cast<T*>(a.out) + row * D;
+    part = splits > 1 ? a.partial + ((int64_t)blockIdx.z * w.tokens * a.q_heads + row) * (D + 2) : nullptr;
+  }
+  __device__ __forceinline__ void put(int d, const float (&y)[4][8]) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (!part) {
+        store_f32<T, 8>(out + d + 8 * j, y[j]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) *reinterpret_cast<float2*>(part + d + 8 * j + e) = make_float2(y[j][e], y[j][e + 1]);
+      }
+    }
+  }
+  __device__ __forceinline__ void put_weight(float m, float l) const {
+    if (part) *reinterpret_cast<float2*>(part + D) = make_float2(m, l);
+  }
+};
+
+// Joins the shares of a (token, query head), in their order.  One warp each.
+template <typename T, int D>
+__global__ void __launch_bounds__(256)
+    kv_prompt_join_kernel(const __grid_constant__ KvTokens w, const __grid_constant__ AttendArgs a, int splits) {
+  pdl_wait();
+  pdl_trigger();
+  constexpr int E = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int64_t rows = w.tokens * a.q_heads, row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= rows || kv_sequence(w, row / a.q_heads) < 0) return;
+  auto part = [&](int z) { return a.partial + (z * rows + row) * (D + 2); };
+  float top = kNoScore, l = 0.0f, o[E] = {};
+  for (int z = 0; z < splits; ++z) top = fmaxf(top, part(z)[D]);
+  auto weight = [&](int z) {
+    const float2 ml = *reinterpret_cast<const float2*>(part(z) + D);
+    return ml.y * ex2(ml.x - top);
+  };
+  for (int z = 0; z < splits; ++z) l += weight(z);
+  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+  for (int z = 0; z < splits; ++z) {
+    const float f = weight(z) * inv;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      const float2 v = *reinterpret_cast<const float2*>(part(z) + lane * E + e);
+      o[e] = fmaf(v.x, f, o[e]);
+      o[e + 1] = fmaf(v.y, f, o[e + 1]);
+    }
+  }
+  store_f32<T, E>(static_cast<T*>(a.out) + row * D + lane * E, o);
+}
+
+inline dim3 prompt_grid(const KvView& c, const KvTokens& w, const AttendArgs& a, const PromptPlan& p) {
+  // at most so many row tiles
+  return dim3((unsigned)(w.tokens * (a.q_heads / c.heads) / p.rows + w.batch), (unsigned)c.heads, (unsigned)p.splits);
+}
+template <typename T, int D>
+static int launch_prompt_join(cudaStream_t s, const KvTokens& w, const AttendArgs& a, const PromptPlan& p) {
+  if (p.splits == 1) return ICX_OK;
+  ICX_CUDA(launch_pdl(kv_prompt_join_kernel<T, D>, dim3((unsigned)((w.tokens * a.q_heads + 7) / 8)), dim3(256), 0, s, w, a,
+                      p.splits));
+  return ICX_OK;
+}
+
+int launch_prompt_bf16(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a, const PromptPlan& p);
 
 }  // namespace icx

@@ -8,10 +8,14 @@
 // the softmax warps with about five instructions per score, against ten in
 // kv_prompt.cu, whose operands are exact and which f16 outputs take.
 //
-// Dequantising is one fused multiply-add per pair: a code in the low bits of a
-// half word is the f16 number code * 2^-24, so code * (s 2^24 2^-E) + lo 2^-E is
+// Dequantising is three instructions per pair: a code put into the low bits of
+// 1024 (f16) less 1024 is the code as a number, and code * (s 2^-E) + lo 2^-E is
 // the value times 2^-E.  The CTA looks over the scales of all its positions
-// first (a sixteenth of the cache) to choose E for K and for V.
+// first (a sixteenth of the cache) to choose E for K and for V; scales 2^20 times
+// smaller than the largest of the CTA's positions keep their 11 bits.
+// (A code in the low bits of a half word is also the f16 number code * 2^-24,
+// which saves the subtraction, but then s 2^24 2^-E has to fit f16: a scale
+// 2^15 below the largest was off by half its step.)
 //
 // A CTA (one per SM) takes 256 query rows of one (sequence, K/V head) as two
 // tiles of 128, 48 positions at a time, so that what is dequantised serves both;
@@ -58,34 +62,37 @@ __device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t taddr, const uint32_t
                : "memory");
 }
 
-// E for groups with scales up to s_top and low ends up to lo_top: s 2^24 2^-E and
-// lo 2^-E stay below 2^15 (and codes x scale mostly in f16's normal range).
+// E for groups with scales up to s_top and low ends up to lo_top: codes x s 2^-E
+// and lo 2^-E stay below 2^14 each, their sum below 2^15.
+template <int BITS>
 __device__ __forceinline__ int unit_for(uint32_t s_top, uint32_t lo_top) {
   const int s = (int)(s_top >> 23) - 126, lo = (int)(lo_top >> 23) - 126;   // below 2^s, 2^lo
-  return min(max(max(s + 9, lo - 15), -100), 120);
+  return min(max(max(s + BITS - 14, lo - 14), -100), 120);
 }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
-// Scale (for codes that count 2^-24, and for those that count 2^-20) and low
-// end of a group in f16.
+// Scale (of codes, and of sixteen times codes) and low end of a group in f16.
 struct GroupF16 {
   __half2 s, s16, lo;
-  __device__ __forceinline__ GroupF16(uint32_t p, float up24, float down, bool zero) {
-    const float a = zero ? 0.0f : param_scale(p) * up24, b = zero ? 0.0f : param_low(p) * down;
+  __device__ __forceinline__ GroupF16(uint32_t p, float down, bool zero) {
+    const float a = zero ? 0.0f : param_scale(p) * down, b = zero ? 0.0f : param_low(p) * down;
     s = __float2half2_rn(a);
     s16 = __float2half2_rn(a * 0.0625f);
     lo = __float2half2_rn(b);
   }
 };
 
-// Eight dequantised values of a 16-byte piece, one rounding each.
+// Eight dequantised values of a 16-byte piece, one rounding each (beside the scale's).
 template <int BITS>
 __device__ __forceinline__ uint4 dequantize(uint32_t w0, uint32_t w1, const GroupF16& g) {
   uint4 u = spread<BITS>(w0, w1);
   uint32_t* v = reinterpret_cast<uint32_t*>(&u);
+  const __half2 k1024 = __float2half2_rn(1024.0f);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&v[i]), times16<BITS>(2 * i) ? g.s16 : g.s, g.lo);
+    const uint32_t x = v[i] | 0x64006400u;   // 1024 + code
+    const __half2 code = __hsub2(*reinterpret_cast<const __half2*>(&x), k1024);
+    const __half2 y = __hfma2(code, times16<BITS>(2 * i) ? g.s16 : g.s, g.lo);
     v[i] = *reinterpret_cast<const uint32_t*>(&y);
   }
   return u;
@@ -94,7 +101,7 @@ __device__ __forceinline__ uint4 dequantize(uint32_t w0, uint32_t w1, const Grou
 template <int D, int BITS>
 __global__ void __launch_bounds__(kB16Threads, 1)
     kv_prompt_bf16_kernel(const __grid_constant__ KvView c, const __grid_constant__ KvTokens w,
-                          const __grid_constant__ AttendArgs a, int rows_per_cta) {
+                          const __grid_constant__ AttendArgs a, int rows_per_cta, int splits) {
   using T = __nv_bfloat16;
   using C = PromptB16Config<D>;
   constexpr int G = C::G;
@@ -148,14 +155,15 @@ __global__ void __launch_bounds__(kB16Threads, 1)
     const int64_t first_pos = (int64_t)su.len - su.n;
     const int reach = (int)min((int64_t)su.len, (int64_t)w.width << c.page_shift);
     const int see_any = (int)max((int64_t)0, min(first_pos + (r0 + nrows - 1) / share + 1, (int64_t)reach));
-    const int tiles = (see_any + kB16Keys - 1) / kB16Keys;
+    const PromptShare part(see_any, kB16Keys, splits);
+    const int tiles = part.tiles, p0 = part.first, p_end = part.end;
     if (threadIdx.x == 0 && su.len > reach) record_status(ICX_DEVICE_BAD_PAGE);
 
     // the first look
     {
       uint32_t top[4] = {0, 0, 0, 0}, special = 0;
 #pragma unroll 4
-      for (int pos = threadIdx.x; pos < see_any; pos += kB16Threads) {
+      for (int pos = p0 + threadIdx.x; pos < p_end; pos += kB16Threads) {
         const int64_t page = kv_page(c, w, seq, pos);
         if (page < 0) {
           special = 1;
@@ -187,7 +195,7 @@ __global__ void __launch_bounds__(kB16Threads, 1)
       if (special) s_look[4] = 1u;
       __syncthreads();
     }
-    const int k_exp = unit_for(s_look[0], s_look[1]), v_exp = unit_for(s_look[2], s_look[3]);
+    const int k_exp = unit_for<BITS>(s_look[0], s_look[1]), v_exp = unit_for<BITS>(s_look[2], s_look[3]);
     const bool special = s_look[4] != 0u;
 
     if (warp >= 14) {
@@ -250,8 +258,8 @@ __global__ void __launch_bounds__(kB16Threads, 1)
       uint32_t kp[G], vp[G];
       int64_t row = -1, row_next = -1;   // cache row of this thread's position, or -1
       auto find = [&](int i) {
-        const int pos = i * kB16Keys + key;
-        const int64_t page = pos < see_any ? kv_page(c, w, seq, pos) : -1;
+        const int pos = p0 + i * kB16Keys + key;
+        const int64_t page = pos < p_end ? kv_page(c, w, seq, pos) : -1;
         row_next = page >= 0 ? kv_row(c, page, head, pos) : -1;
       };
       // (a tile is a multiple of 16 positions: the swizzle of the thread's row
@@ -266,7 +274,6 @@ __global__ void __launch_bounds__(kB16Threads, 1)
         if (row >= 0) raw.load_v(c, row, key, half);
       };
       const float k_down = power_of_two(-k_exp), v_down = power_of_two(-v_exp);
-      const float k_up24 = k_down * 16777216.0f, v_up24 = v_down * 16777216.0f;
       bool ok = true;
       if (set < tiles) {
         find(set);
@@ -284,7 +291,7 @@ __global__ void __launch_bounds__(kB16Threads, 1)
         if (ok) ok = wait_warp(&k_empty[st], free, ICX_DEVICE_TIMEOUT_PRODUCER);
 #pragma unroll
         for (int k = 0; k < G; ++k) {
-          const GroupF16 g(kp[k], k_up24, k_down, row < 0);
+          const GroupF16 g(kp[k], k_down, row < 0);
           uint8_t* kr = s_k(st) + k * kB16Keys * 128 + key * 128;
 #pragma unroll
           for (int x = 0; x < 2; ++x)
@@ -302,7 +309,7 @@ __global__ void __launch_bounds__(kB16Threads, 1)
         if (ok) ok = wait_warp(&v_empty[st], free, ICX_DEVICE_TIMEOUT_PRODUCER);
 #pragma unroll
         for (int k = 0; k < G; ++k) {
-          const GroupF16 g(vq[k], v_up24, v_down, row < 0 || isnan(param_scale(vq[k])));
+          const GroupF16 g(vq[k], v_down, row < 0 || isnan(param_scale(vq[k])));
           uint8_t* vr = s_v(st) + k * kB16Keys * 128 + key * 128;
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
@@ -354,15 +361,15 @@ __global__ void __launch_bounds__(kB16Threads, 1)
         float s[kB16Keys];
 #pragma unroll
         for (int j = 0; j < kB16Keys; ++j) s[j] = __uint_as_float(j < 32 ? x0[j & 31] : x1[j & 15]);
-        if ((i + 1) * kB16Keys > see_all) {
+        if (p0 + (i + 1) * kB16Keys > see_all) {
 #pragma unroll
           for (int j = 0; j < kB16Keys; ++j)
-            if (i * kB16Keys + j >= see) s[j] = -INFINITY;
+            if (p0 + i * kB16Keys + j >= see) s[j] = -INFINITY;
         }
         if (special) {
 #pragma unroll
           for (int j = 0; j < kB16Keys; ++j) {
-            const int pos = i * kB16Keys + j;
+            const int pos = p0 + i * kB16Keys + j;
             if (pos >= see) continue;
             const int64_t page = kv_page(c, w, seq, pos);
             if (page < 0) {
@@ -437,8 +444,8 @@ __global__ void __launch_bounds__(kB16Threads, 1)
       tc_fence_after();
       const float inv = l != 0.0f ? 1.0f / l : 0.0f;
       const float up = power_of_two(v_exp);
-      T* out = static_cast<T*>(a.out) +
-               ((int64_t)(su.from + (mine ? r / share : 0)) * a.q_heads + head * share + (mine ? r % share : 0)) * D;
+      const int64_t out_row = (int64_t)(su.from + (mine ? r / share : 0)) * a.q_heads + head * share + (mine ? r % share : 0);
+      const PromptOut<T, D> out(a, w, splits, out_row);
       if (ok && h < row_tiles) {
 #pragma unroll 1
         for (int k = 0; k < G; ++k) {
@@ -461,11 +468,10 @@ __global__ void __launch_bounds__(kB16Threads, 1)
                 const int d = v_dim<BITS>(j, e);
                 y[d >> 3][d & 7] = bad ? NAN : l != 0.0f ? o * inv * up : 0.0f;
               }
-            if (mine)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) store_f32<T, 8>(out + k * kPrGroup + 32 * n + 8 * j, y[j]);
+            if (mine) out.put(k * kPrGroup + 32 * n, y);
           }
         }
+        if (mine) out.put_weight(m, l);
       }
     }
   }
@@ -476,22 +482,17 @@ __global__ void __launch_bounds__(kB16Threads, 1)
 }
 
 template <int D, int BITS>
-static int launch_kernel(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a) {
+static int launch_kernel(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a, const PromptPlan& p) {
   using C = PromptB16Config<D>;
   auto kern = kv_prompt_bf16_kernel<D, BITS>;
   ICX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
-  const int64_t share = a.q_heads / c.heads;
-  // at most so many row tiles; twice the rows per CTA if they still fill the GPU
-  const auto tiles = [&](int rows) { return w.tokens * share / rows + w.batch; };
-  const int rows = (tiles(2 * kPrRows) - w.batch / 2) * c.heads >= sm_count() ? 2 * kPrRows : kPrRows;
-  const dim3 grid((unsigned)tiles(rows), (unsigned)c.heads);
-  ICX_CUDA(launch_pdl(kern, grid, dim3(kB16Threads), C::kSmem, s, c, w, a, rows));
-  return ICX_OK;
+  ICX_CUDA(launch_pdl(kern, prompt_grid(c, w, a, p), dim3(kB16Threads), C::kSmem, s, c, w, a, p.rows, p.splits));
+  return launch_prompt_join<__nv_bfloat16, D>(s, w, a, p);
 }
 
-int launch_prompt_bf16(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a) {
-  if (c.dim == 64) return c.bits == 4 ? launch_kernel<64, 4>(s, c, w, a) : launch_kernel<64, 8>(s, c, w, a);
-  return c.bits == 4 ? launch_kernel<128, 4>(s, c, w, a) : launch_kernel<128, 8>(s, c, w, a);
+int launch_prompt_bf16(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a, const PromptPlan& p) {
+  if (c.dim == 64) return c.bits == 4 ? launch_kernel<64, 4>(s, c, w, a, p) : launch_kernel<64, 8>(s, c, w, a, p);
+  return c.bits == 4 ? launch_kernel<128, 4>(s, c, w, a, p) : launch_kernel<128, 8>(s, c, w, a, p);
 }
 
 }  // namespace icx

@@ -400,6 +400,54 @@ def test_prompt_chunk_values_of_unequal_size():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 8])
+def test_prompt_rows_beside_much_larger_values_they_do_not_see(bits):
+    """A position 2^18 times as large as the others leaves the rows before it as exact."""
+    c = Case([180], 1, 128, bits, 64, 16, torch.bfloat16, seed=24)
+    v = c.v.clone()
+    v[150] *= 2.0 ** 18
+    gpu_kv_cache_append(c.cache, c.k.to(DEV), v.to(DEV), c.table, i32([180]), i32([0, 180]))
+    c.kv[1] = ref.cached_values(f64(v), bits, 64)
+    check_attention(c, [130], 4, torch.bfloat16, seed=9)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim,bits,share", [(64, 8, 4), (128, 4, 4), (128, 8, 8)])
+def test_prompt_chunks_on_long_prefixes(dim, bits, share, dtype):
+    """Few rows and many positions, which are read in shares: some shares of the
+    shorter sequences hold nothing, and the first rows of one see few positions."""
+    lens = [2900, 70, 0, 1000]
+    c = Case(lens, 2, dim, bits, 64, 16, dtype, seed=dim + bits + 1, width_extra=60)
+    check_attention(c, [65, 70, 0, 129], 2 * share, dtype, seed=share + 2, pad=1)
+    check_attention(c, [20, 20, 0, 300], 2 * share, dtype, seed=share + 3, q_scale=6.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_prompt_shares_with_missing_pages_and_nan(dtype):
+    c = Case([2000], 1, 128, 4, 64, 16, dtype, seed=25)
+    q = torch.randn(100, 4, 128).to(dtype)
+    lens, cu = i32([2000]), i32([0, 100])
+    table = c.table.clone()
+    table[0, 3:90] = -1     # more than the first share
+    out = f64(gpu_kv_cache_attention(c.cache, q.to(DEV), table, lens, cu))
+    assert status() == _lib.ICX_DEVICE_BAD_PAGE
+    k, v = (np.delete(x, np.s_[48:1440], 0) for x in c.sequence(0))
+    want = ref.attention(f64(q), k, v, 128 ** -0.5)
+    tol = ref.attention_tolerance(f64(q), k, v, 128 ** -0.5, dtype, want)
+    assert (np.abs(out - want) <= tol).all()
+    out = gpu_kv_cache_attention(c.cache, q.to(DEV), torch.full_like(table, -1), lens, cu)
+    assert status() == _lib.ICX_DEVICE_BAD_PAGE and (out == 0).all()
+    bad = c.v[1950:1951].clone()
+    bad[..., 70] = float("nan")
+    gpu_kv_cache_append(c.cache, c.k[1950:1951].to(DEV), bad.to(DEV), c.table, i32([1951]), i32([0, 1]))
+    nan = gpu_kv_cache_attention(c.cache, q.to(DEV), c.table, lens, cu).isnan()
+    assert nan[50:, :, 64:].all() and not nan[:50].any() and not nan[..., :64].any()
+    assert status() == 0
+
+
+@pytest.mark.gpu
 def test_attention_scales_and_strong_scores():
     """Scores of order 100 (one position takes all), scale 0, negative scale, tiny and huge q."""
     for spread, q_scale, scale in ((4.0, 4.0, 0.5), (1.0, 1.0, 0.0), (1.0, 1.0, -0.3), (1.0, 1e-6, None),
