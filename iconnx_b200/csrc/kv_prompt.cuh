@@ -148,30 +148,48 @@ struct RawCodes {
 template <typename T, int G, int BITS, bool CODES>
 __device__ __forceinline__ void put_query(const AttendArgs& a, const T* q, bool mine, int row, uint8_t* s_q, float* f,
                                           float (&sum)[G]) {
+  // A group is fetched with eight 16-byte loads at once: with nearly all of the
+  // SM's memory shared there is no L1 that would keep a row, and a warp's load
+  // touches 32 of them (8-byte loads: PLACEHOLDER).
+  Vec<T, 8> u[kPrGroup / 8];
+  const bool wide = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
+  auto fetch = [&](int k) {
+    if (wide) {
+#pragma unroll
+      for (int i = 0; i < kPrGroup / 8; ++i) u[i] = *reinterpret_cast<const Vec<T, 8>*>(q + k * kPrGroup + 8 * i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPrGroup / 8; ++i)
+#pragma unroll
+        for (int x = 0; x < 8; ++x) u[i].v[x] = q[k * kPrGroup + 8 * i + x];
+    }
+  };
   float peak = 0.0f;
+#pragma unroll 1
+  for (int k = 0; k < G; ++k) {
+    fetch(k);
 #pragma unroll
-  for (int d = 0; d < G * kPrGroup; d += 4) {
-    float v[4];
-    load_f32<T, 4>(q + d, v, a.q_vec);
+    for (int i = 0; i < kPrGroup / 8; ++i)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) peak = fmaxf(peak, fabsf(v[i]));
+      for (int x = 0; x < 8; ++x) peak = fmaxf(peak, fabsf(to_f32(u[i].v[x])));
   }
   const int e = mine && peak > 0.0f ? max(-60, min(120, 14 - (int)((__float_as_uint(peak) >> 23) & 255) + 127)) : 0;
   const float up = mine && a.scale != 0.0f ? copysignf(__uint_as_float((uint32_t)(e + 127) << 23), a.scale) : 0.0f;
   *f = a.scale != 0.0f ? fabsf(a.scale) * (CODES ? 16777216.0f : 1.0f) * __uint_as_float((uint32_t)(127 - e) << 23) : 1.0f;
 #pragma unroll 1
-  for (int k = 0; k < G; ++k) {
+  for (int k = G - 1; k >= 0; --k) {   // the last group is there
+    if (k < G - 1) fetch(k);
     float total = 0.0f;
-#pragma unroll 1
+#pragma unroll
     for (int t = 0; t < 4; ++t) {
       // step j's dimensions 16 j + 4 t .. + 3 of the group
       float v[4][4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        load_f32<T, 4>(q + k * kPrGroup + 16 * j + 4 * t, v[j], a.q_vec);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          v[j][i] = up != 0.0f ? v[j][i] * up : 0.0f;
+          const int d = 16 * j + 4 * t + i;
+          v[j][i] = up != 0.0f ? to_f32(u[d >> 3].v[d & 7]) * up : 0.0f;
           total += v[j][i];
         }
       }
