@@ -466,9 +466,11 @@ PromptPlan plan_prompt(const KvView& c, const KvTokens& w, int q_heads, int type
   const auto tiles = [&](int rows) { return (w.tokens * share + rows - 1) / rows * c.heads; };
   if (type == ICX_BF16 && tiles(2 * kPrRows) >= sm_count()) p.rows = 2 * kPrRows;
   // Positions in shares where that fills the GPU (128 tokens of one sequence of
-  // 32,000, 8 K/V heads of 4 query heads: PLACEHOLDER).  A CTA's start and end cost about
-  // what `own` positions cost, and its number of positions is at most the page
-  // table's (the host does not know more).
+  // 32,000, 8 K/V heads of 4 query heads of 128, 4 bits: f16 2040 -> 328 us in 9
+  // shares).  A CTA's start and end cost about what `own` positions cost, and its
+  // number of positions is at most the page table's (the host does not know more).
+  // Two sequences with 1024 rows each keep whole rows: four shares, which would
+  // even out the last wave of CTAs, took 367 us instead of 258.
   const double own = type == ICX_BF16 ? 900 : 300, reach = (double)((int64_t)w.width << c.page_shift);
   const int64_t n = tiles(p.rows), at_once = (int64_t)sm_count() * (type == ICX_BF16 ? 1 : 2);
   double best = 0;

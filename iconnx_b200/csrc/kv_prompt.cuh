@@ -150,7 +150,8 @@ __device__ __forceinline__ void put_query(const AttendArgs& a, const T* q, bool 
                                           float (&sum)[G]) {
   // A group is fetched with eight 16-byte loads at once: with nearly all of the
   // SM's memory shared there is no L1 that would keep a row, and a warp's load
-  // touches 32 of them (8-byte loads: PLACEHOLDER).
+  // touches 32 of them (all of it in 8-byte loads: 265 us instead of 250 where
+  // kv_prompt_bf16.cu states 250).
   Vec<T, 8> u[kPrGroup / 8];
   const bool wide = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
   auto fetch = [&](int k) {

@@ -676,7 +676,8 @@ extern "C" int icx_matmul_integer_scaled(void* stream, const int8_t* d_q, const 
   ICX_REQUIRE(is_float_type(out_type), "MatMulIntegerScaled: output must be Float32, Float16 or BFloat16");
   ICX_REQUIRE(K <= ICX_SCALED_MAX_K, "MatMulIntegerScaled: K %zu above %d, where the s32 sum could wrap", K,
               ICX_SCALED_MAX_K);
-  ICX_REQUIRE(M < (1ull << 22) && N < (1ull << 22), "MatMulIntegerScaled: shape too large");
+  ICX_REQUIRE(M <= 65535ull * 64 && N < (1ull << 22),   // tiles of 64 tokens in grid.y
+              "MatMulIntegerScaled: shape too large");
   if (M == 0 || N == 0) return ICX_OK;
   ICX_REQUIRE(d_out && d_q_scale && d_w_scale && (K == 0 || (d_q && d_wt)),
               "MatMulIntegerScaled: null operand");

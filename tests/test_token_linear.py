@@ -49,6 +49,7 @@ def test_product_refusals_before_any_launch():
     assert call(t=2) == -1 and b"output must be" in L.icx_last_error()
     assert call(K=_lib.ICX_SCALED_MAX_K + 1) == -1 and b"could wrap" in L.icx_last_error()
     assert call(M=1 << 22) == -1 and b"too large" in L.icx_last_error()
+    assert call(M=65535 * 64 + 1) == -1 and b"too large" in L.icx_last_error()
     assert call(q=None) == -1 and b"null" in L.icx_last_error()
     assert call(out=None) == -1 and b"null" in L.icx_last_error()
     assert call(M=0, q=None, out=None) == 0
