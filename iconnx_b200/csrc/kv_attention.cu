@@ -13,15 +13,15 @@ AttendPlan plan_attend(const KvView& c, const KvTokens& w, int q_heads, int type
     return p;
   }
   const int share = q_heads / c.heads;
-  // rows that share one read of the cache: as many as the average sequence
-  // has, up to what the registers (and, for two f16 parts of 256 dimensions of
-  // q per warp, shared memory) hold
   const int64_t rows = (w.tokens + w.batch - 1) / w.batch * share;
-  const int most = c.dim == 256 ? (type == ICX_F32 ? 1 : 2) : 4;
-  p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
-  if (p.nt > most) p.nt = most;
-  const int R = 8 * p.nt, step = att_step(c.dim, c.bits, R);
   const int64_t reach = (int64_t)w.width << c.page_shift;
+  p.nt = 1;
+  if (type == ICX_F32 && att_most_nt<float>(c.dim) == 2 && rows > 8) {
+    // steps per warp with one tile of 8 rows: from 64 on, two
+    const int64_t steps = (w.tokens * share / 8 + w.batch) * c.heads * (reach / att_step(c.dim, c.bits, 8) + 1);
+    if (steps >= 64ll * sm_count() * kAttWarps * att_resident(c.dim, 1, 4)) p.nt = 2;
+  }
+  const int R = 8 * p.nt, step = att_step(c.dim, c.bits, R);
   // four steps are over before a second launch would be
   p.split = reach > 4 * step;
   p.unit = p.split ? step : 4 * step;

@@ -58,6 +58,17 @@ __host__ __device__ constexpr int att_resident(int dim, int nt, int q_bytes) {
   return dim * nt <= 128 && !(q_bytes == 4 && dim == 128) ? 2 : 1;
 }
 
+// 8 or 16 query rows per tile.  16 read the cache half as often but take twice
+// the registers and instructions, which a warp with few steps has to fetch: they
+// pay for long runs in f32 alone (64 rows of one sequence of 16,000, 8 K/V heads
+// of 4 query heads of 128, 4 bits: 198 -> 168 us), not in 16 bits (4 rows of 64
+// sequences of up to 8,000, bf16: 184 -> 199 us) nor in short runs (5 rows of 6
+// sequences of up to 5,300, bf16: 27 -> 29 us; 32 rows per tile: 48 us).
+template <typename T>
+constexpr int att_most_nt(int dim) {
+  return sizeof(T) == 4 && dim <= 128 ? 2 : 1;
+}
+
 struct AttendArgs {
   const void* q;
   int64_t q_token_stride, q_head_stride;
@@ -96,6 +107,11 @@ __device__ __forceinline__ SeqUnits seq_units(const KvView& c, const KvTokens& w
   u.blocks = max(1, (int)(((int64_t)reach + unit - 1) / unit));
   u.units = (int64_t)u.tiles * c.heads * u.blocks;
   return u;
+}
+
+// How many of the warps get units: all of them, or one per unit.
+__device__ __forceinline__ int64_t working_warps(int64_t total, int64_t warps) {
+  return max(min(warps, total), (int64_t)1);
 }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -208,12 +224,14 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
   pdl_trigger();
 
   // this warp's units [u0, u1) of all
-  const int64_t me = (int64_t)blockIdx.x * kAttWarps + warp, warps = (int64_t)gridDim.x * kAttWarps;
   int64_t total = 0;
   for (int b = lane; b < w.batch; b += 32) total += seq_units(c, w, share, R, b, a.unit).units;
 #pragma unroll
   for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  const int64_t u0 = total * me / warps, u1 = total * (me + 1) / warps;
+  const int64_t all = (int64_t)gridDim.x * kAttWarps, warps = working_warps(total, all);
+  // few working warps: one per CTA first
+  const int64_t me = warps < all ? (int64_t)warp * gridDim.x + blockIdx.x : (int64_t)blockIdx.x * kAttWarps + warp;
+  const int64_t u0 = min(total * me / warps, total), u1 = min(total * (me + 1) / warps, total);
   const bool write = a.split && me == 0;   // the first warp leaves the prefix sums
   int seq = w.batch;
   int64_t base = 0, before = 0;
@@ -711,33 +729,47 @@ __global__ void __launch_bounds__(256)
   const int hq = (int)(item % a.q_heads);
   const int b = item < w.tokens * a.q_heads ? kv_sequence(w, token) : -1;
   int first = 0, last = 0, r = 0;
-  int64_t total = 0;
   if (b >= 0) {
     const SeqUnits su = seq_units(c, w, share, R, b, a.unit);
     r = (int)(token - su.from) * share + hq % share;
-    total = a.prefix[w.batch];
+    const int64_t total = a.prefix[w.batch], working = working_warps(total, warps);
     const int64_t s0 = a.prefix[b] + ((int64_t)(hq / share) * su.tiles + r / R) * su.blocks, s1 = s0 + su.blocks;
-    // the warp that holds unit s is the last with total * warp / warps <= s
+    // the warp that holds unit s is the last with total * warp / working <= s
     if (total > 0) {
-      first = (int)(((s0 + 1) * warps - 1) / total);
-      last = (int)((s1 * warps - 1) / total);
+      first = (int)(((s0 + 1) * working - 1) / total);
+      last = (int)((s1 * working - 1) / total);
     }
   }
   // first == last: written whole, or nothing there
   float m = kNoScore, l = 0.0f, o[E] = {};
   if (first < last) {
-    for (int i = first + mine; i <= last; i += per_row) {
-      if (total * i / warps == total * (i + 1) / warps) continue;   // more warps than units: this one had none
-      const float* p = a.partial + (((int64_t)i * 2 + (i == first ? 1 : 0)) * R + r % R) * (D + 2);
-      const float2 ml = *reinterpret_cast<const float2*>(p + D);
-      const float top = fmaxf(m, ml.x), fa = ex2(m - top), fb = ex2(ml.x - top);
-      m = top;
-      l = l * fa + ml.y * fb;
+    auto part = [&](int i) { return a.partial + (((int64_t)i * 2 + (i == first ? 1 : 0)) * R + r % R) * (D + 2); };
+    // 32 parts at a time: a lane each for their factors, then all lanes for each
+    for (int i0 = first + mine; i0 <= last; i0 += 32 * per_row) {
+      const int n = min(32, (last - i0) / per_row + 1);
+      float2 ml = make_float2(kNoScore, 0.0f);
+      if (lane < n) ml = *reinterpret_cast<const float2*>(part(i0 + lane * per_row) + D);
+      float top = fmaxf(m, ml.x);
 #pragma unroll
-      for (int e = 0; e < E; e += 2) {
-        const float2 v = *reinterpret_cast<const float2*>(p + lane * E + e);
-        o[e] = o[e] * fa + v.x * fb;
-        o[e + 1] = o[e + 1] * fa + v.y * fb;
+      for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      const float moved = ex2(m - top), f = ex2(ml.x - top);
+      float sum = ml.y * f;
+#pragma unroll
+      for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      m = top;
+      l = l * moved + sum;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] *= moved;
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) {
+        const float fj = __shfl_sync(0xffffffffu, f, j);
+        const float* p = part(i0 + j * per_row) + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          const float2 v = *reinterpret_cast<const float2*>(p + e);
+          o[e] = fmaf(v.x, fj, o[e]);
+          o[e + 1] = fmaf(v.y, fj, o[e + 1]);
+        }
       }
     }
   }
@@ -821,10 +853,9 @@ int launch_attend_rows(cudaStream_t s, const KvView& c, const KvTokens& w, const
 
 template <typename T, int D, int BITS, int GROUP>
 int launch_attend_nt(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a, const AttendPlan& p) {
-  constexpr int kMost = D == 256 ? (sizeof(T) == 4 ? 1 : 2) : 4;   // as plan_attend
-  if (p.nt == 1) return launch_attend_rows<T, D, BITS, GROUP, 1>(s, c, w, a, p);
-  if (p.nt == 2) return launch_attend_rows<T, D, BITS, GROUP, kMost < 2 ? 1 : 2>(s, c, w, a, p);
-  return launch_attend_rows<T, D, BITS, GROUP, kMost>(s, c, w, a, p);
+  if constexpr (att_most_nt<T>(D) == 2)
+    if (p.nt == 2) return launch_attend_rows<T, D, BITS, GROUP, 2>(s, c, w, a, p);
+  return launch_attend_rows<T, D, BITS, GROUP, 1>(s, c, w, a, p);
 }
 
 template <typename T, int D>
