@@ -1,9 +1,10 @@
 // Attention of few query rows over the quantised K/V cache (decoding).
 //
-// Bound: the cache is read once, 4 D / 32 .. bytes per position with some tens
-// of operations per byte, so HBM sets the floor and the instruction issue rate
-// comes next.  Codes are therefore never dequantised: with K[p] = c s + lo per
-// group of dimensions,
+// The cache is read once, D bits / 4 + 8 D / group bytes per position and K/V
+// head (144 for 128 dimensions of 4 bits in groups of 64), so HBM sets the floor;
+// what bounds the kernel at 4 bits is the issue of about 340 instructions per 16
+// positions, half of them of the integer pipe.  Codes are therefore never
+// dequantised: with K[p] = c s + lo per group of dimensions,
 //     q . K[p] = sum_groups  s (q . c) + lo sum(q)
 //     sum_p w_p V[p] = sum_p (w_p s_p) c_p + sum_p w_p lo_p
 // and the two contractions run on m16n8k16 matrix instructions whose left
@@ -34,6 +35,11 @@
 // keep its pipes busy.  Rows whose units went to several warps leave (m, l, o)
 // in the workspace for the join kernel.  All joins run in a fixed order, so
 // equal calls give equal results.
+//
+// Measured: 64 sequences of up to 16,000 positions, one token, 8 K/V heads of 4
+// query heads of 128, bf16: 4 bits 198 us (3.8 TB/s; floor 118 us at 6.46 TB/s),
+// 8 bits 254 us (5.7 TB/s; floor 222).  One sequence of 500, 12 heads of 64, f32,
+// 8 bits: 12 us for both launches, latency.
 #pragma once
 
 #include <type_traits>
@@ -181,9 +187,27 @@ __device__ __forceinline__ void load_transposed(uint32_t addr, uint32_t (&r)[4])
                : "memory");
 }
 
+// Two codes as f16 for a matrix operand: as they stand (subnormals), or as numbers
+// around zero: 1024 + code less 1024 + middle.  HIGH: in bits 4..7, sixteen times.
+template <bool CENTRE, int BITS, bool HIGH>
+__device__ __forceinline__ uint32_t code_operand(uint32_t codes) {
+  if constexpr (!CENTRE) return codes;
+  constexpr uint32_t zero = BITS == 4 && !HIGH ? 0x64086408u : 0x64806480u;   // 1032, 1152
+  uint32_t x = codes | 0x64006400u;
+  const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&zero));
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+
 template <typename T, int D, int BITS, int GROUP, int NT>
 struct AttConfig {
   static constexpr bool QLO = sizeof(T) == 4;
+  // f32: codes as f16 integers less kMiddle (one more instruction per operand
+  // word), so that the two parts of a sum, s c and lo, do not cancel: with K and V
+  // around zero they are some forty times the output (error 3.4e-6 of it without).
+  // A code counts 1 then, not 2^-24.
+  static constexpr bool CENTRE = sizeof(T) == 4;
+  static constexpr float kMiddle = CENTRE ? (float)(1 << (BITS - 1)) : 0.0f;
+  static constexpr float kUnit = CENTRE ? 1.0f : 16777216.0f;
   static constexpr bool PLO = !std::is_same<T, __nv_bfloat16>::value;
   static constexpr int R = 8 * NT;
   static constexpr int G = D / GROUP;
@@ -351,7 +375,7 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
       peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
       peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
       // 2^e with peak * 2^e in [2^14, 2^15)
-      const int e = peak > 0.0f ? max(-60, min(120, 14 - (int)((__float_as_uint(peak) >> 23) & 255) + 127)) : 0;
+      const int e = peak > 0.0f ? max(-60, min(C::CENTRE ? 96 : 120, 14 - (int)((__float_as_uint(peak) >> 23) & 255) + 127)) : 0;
       // scores are held in units of 1 / f, f > 0: a negative scale turns q round
       const float up = a.scale != 0.0f ? copysignf(__uint_as_float((uint32_t)(e + 127) << 23), a.scale) : 0.0f;
       float sums[G] = {};
@@ -380,7 +404,7 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
           }
         }
       }
-      const float f = a.scale != 0.0f ? fabsf(a.scale) * 16777216.0f * __uint_as_float((uint32_t)(127 - e) << 23) : 1.0f;
+      const float f = a.scale != 0.0f ? fabsf(a.scale) * C::kUnit * __uint_as_float((uint32_t)(127 - e) << 23) : 1.0f;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int from = (2 * t + h) * 4;   // a lane that holds column 2t + h
@@ -394,7 +418,7 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
         float s = sums[k];
         s += __shfl_xor_sync(0xffffffffu, s, 1);
         s += __shfl_xor_sync(0xffffffffu, s, 2);
-        s *= 5.9604644775390625e-8f;   // a code counts 2^-24
+        s *= 1.0f / C::kUnit;   // in units of a code
         qsum[x][k][0] = __shfl_sync(0xffffffffu, s, 8 * t);
         qsum[x][k][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
       }
@@ -463,14 +487,18 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               if (BITS == 4) {
-                const uint32_t mask = (j & 1) ? 0x00f000f0u : 0x000f000fu;
                 const uint32_t word = kw[h][j >> 1];
-                A[h] = word & mask;
-                A[2 + h] = (word >> 8) & mask;
+                if (j & 1) {
+                  A[h] = code_operand<C::CENTRE, 4, true>(word & 0x00f000f0u);
+                  A[2 + h] = code_operand<C::CENTRE, 4, true>((word >> 8) & 0x00f000f0u);
+                } else {
+                  A[h] = code_operand<C::CENTRE, 4, false>(word & 0x000f000fu);
+                  A[2 + h] = code_operand<C::CENTRE, 4, false>((word >> 8) & 0x000f000fu);
+                }
               } else {
                 const uint32_t word = kw[h][j];
-                A[h] = word & 0x00ff00ffu;
-                A[2 + h] = (word >> 8) & 0x00ff00ffu;
+                A[h] = code_operand<C::CENTRE, 8, false>(word & 0x00ff00ffu);
+                A[2 + h] = code_operand<C::CENTRE, 8, false>((word >> 8) & 0x00ff00ffu);
               }
             }
 #pragma unroll
@@ -487,7 +515,7 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
           }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float sc = param_scale(kp[h][k]), lo = param_low(kp[h][k]);
+            const float sc = param_scale(kp[h][k]), lo = C::CENTRE ? fmaf(C::kMiddle, sc, param_low(kp[h][k])) : param_low(kp[h][k]);
 #pragma unroll
             for (int x = 0; x < NT; ++x)
 #pragma unroll
@@ -599,7 +627,8 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
         for (int k = 0; k < G; ++k)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float sv = param_scale(vp[u][h][k]) * vdown[k], lo = param_low(vp[u][h][k]);
+            const float sv = param_scale(vp[u][h][k]) * vdown[k];
+            const float lo = C::CENTRE ? fmaf(C::kMiddle, param_scale(vp[u][h][k]), param_low(vp[u][h][k])) : param_low(vp[u][h][k]);
 #pragma unroll
             for (int x = 0; x < NT; ++x) {
               const float e0 = s[u][x][2 * h], e1 = s[u][x][2 * h + 1];
@@ -638,15 +667,15 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
             uint32_t A[4];
             if (BITS == 4) {
               const uint32_t a0 = (q & 1) ? lo8 >> 8 : lo8, a1 = (q & 1) ? hi8 >> 8 : hi8;
-              A[0] = a0 & 0x000f000fu;
-              A[1] = a0 & 0x00f000f0u;
-              A[2] = a1 & 0x000f000fu;
-              A[3] = a1 & 0x00f000f0u;
+              A[0] = code_operand<C::CENTRE, 4, false>(a0 & 0x000f000fu);
+              A[1] = code_operand<C::CENTRE, 4, true>(a0 & 0x00f000f0u);
+              A[2] = code_operand<C::CENTRE, 4, false>(a1 & 0x000f000fu);
+              A[3] = code_operand<C::CENTRE, 4, true>(a1 & 0x00f000f0u);
             } else {
-              A[0] = lo8 & 0x00ff00ffu;
-              A[1] = (lo8 >> 8) & 0x00ff00ffu;
-              A[2] = hi8 & 0x00ff00ffu;
-              A[3] = (hi8 >> 8) & 0x00ff00ffu;
+              A[0] = code_operand<C::CENTRE, 8, false>(lo8 & 0x00ff00ffu);
+              A[1] = code_operand<C::CENTRE, 8, false>((lo8 >> 8) & 0x00ff00ffu);
+              A[2] = code_operand<C::CENTRE, 8, false>(hi8 & 0x00ff00ffu);
+              A[3] = code_operand<C::CENTRE, 8, false>((hi8 >> 8) & 0x00ff00ffu);
             }
 #pragma unroll
             for (int x = 0; x < NT; ++x) {
@@ -699,8 +728,8 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
 #pragma unroll
           for (int i = 0; i < GROUP / 16; ++i) {
             const int mt = k * (GROUP / 16) + i;
-            const float v[2] = {fmaf(o[x][mt][h] * 16777216.0f, up, vlo[x][k][h]) * inv,
-                                fmaf(o[x][mt][2 + h] * (BITS == 4 ? 1048576.0f : 16777216.0f), up, vlo[x][k][h]) * inv};
+            const float v[2] = {fmaf(o[x][mt][h] * C::kUnit, up, vlo[x][k][h]) * inv,
+                                fmaf(o[x][mt][2 + h] * (BITS == 4 ? C::kUnit * 0.0625f : C::kUnit), up, vlo[x][k][h]) * inv};
             if (r >= su.rows) continue;
             if (whole) store_f32<T, 2>(out + 16 * mt, v);
             else *reinterpret_cast<float2*>(part + 16 * mt) = make_float2(v[0], v[1]);

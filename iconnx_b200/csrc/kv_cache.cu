@@ -1,6 +1,10 @@
 // Quantised K/V cache: append (quantise) and read (dequantise).
 //
-// Bound by HBM.  Eight lanes take 64 dimensions of one (token, head) of K or V,
+// HBM sets the floor, the issue of about 350 (append) and 110 (read) instructions
+// per 256 values the time: 7 f16 prompts of up to 3,000 tokens into 8 bits, 8 heads
+// of 128, 56 us (2.4 TB/s; floor 21); 6 sequences of up to 8,100 read from 4 bits
+// to bf16, 39 us (4.1 TB/s; floor 25); a decode step's append or read 2.6 to 2.8.
+// Eight lanes take 64 dimensions of one (token, head) of K or V,
 // eight consecutive ones (one or two 16-byte accesses) per lane, so a
 // quantisation group is 4 or 8 lanes and every code word of the layout is put
 // together from lanes of one such eighth.

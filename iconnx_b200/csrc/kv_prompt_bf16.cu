@@ -31,6 +31,11 @@
 //                and the scores' of tile i + 2 when tile i's weights are there.
 // (48 positions rather than 64: three warps fill them, two threads to each, and
 // a row's scores stay in 128 registers.)
+//
+// Measured: 1024 tokens of each of 2 sequences of up to 6,000, 8 K/V heads of 4
+// query heads of 128, 4 bits: 250 us (floor 73 at 1.72 PFLOP/s).  128 rows per
+// CTA 284 us, one warp issuing for both row tiles 296.  About 18 us are a CTA's
+// start and end, and 1.5 waves of CTAs leave a quarter of the SMs' time unused.
 // Rows that do not see a position must not meet its NaN: a V group that holds
 // one is stored as zeros, and the rows that see it end as NaN.  That and pages
 // that are missing are found in the first look; only then do the softmax warps

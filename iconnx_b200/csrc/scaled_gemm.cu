@@ -6,15 +6,17 @@
 //
 //   scaled_rows_kernel    many tokens: 128 (one CTA) or 256 (a CTA pair,
 //                         cta_group::2) tokens x 128 / 256 channels per tile,
-//                         persistent, bound by the tensor cores.
+//                         persistent, bound by the tensor cores (8192 tokens,
+//                         K = 4096, N = 14336: 310 us, 3.1 POPS).
 //   scaled_stream_kernel  up to 128 tokens: the weight is the 128-row operand
 //                         and the tokens the narrow one, so that nothing is
 //                         padded to 128 tokens; bound by reading the weight
 //                         once, which all SMs share by splitting K over the
 //                         CTAs of a cluster, summed in s32 through distributed
-//                         shared memory (exact, so in any order).
+//                         shared memory (exact, so in any order).  4 tokens,
+//                         K = N = 4096: 5.7 us, 2.9 TB/s, latency.
 //   scaled_tile_kernel    any K and alignment (TMA needs K % 16 == 0 and
-//                         16-byte bases): dp4a on 64 x 64 tiles.
+//                         16-byte bases): mma.sync on 64 x 64 tiles.
 #include <type_traits>
 
 #include "capi.cuh"
@@ -42,43 +44,129 @@ __device__ __forceinline__ float scaled_value(int acc, float sa, float sw, float
 }
 
 // ------------------------------------------------- any K and any alignment
+// 64 tokens x 64 channels per CTA, 128 bytes of K per step, on m16n8k32 matrix
+// instructions.  A row may start at any byte, so it is fetched as the aligned
+// words that hold it and shifted into place; the next step's words are on their
+// way meanwhile.  Where the tiles are few, the CTAs of a cluster (up to eight)
+// share out K and sum in s32 through distributed shared memory.  Bound by the
+// instructions of the shifts (8 tokens, K = 7425, N = 7424: 89 us, 205 us with
+// byte loads and dp4a; 5288 tokens, K = 7816, N = 64: 76 us, 227).
+constexpr int kAnyTile = 64, kAnyStep = 128, kAnyRow = kAnyStep / 4 + 4;   // words of a row in shared memory, padded
+
+// The aligned words that hold bytes [at, at + 64) of [from, to), zero outside;
+// *shift tells where they start.
+__device__ __forceinline__ void fetch_any(const int8_t* from, const int8_t* to, const int8_t* at, bool there,
+                                          uint32_t (&w)[17], int* shift) {
+  const int8_t* a = reinterpret_cast<const int8_t*>(reinterpret_cast<uintptr_t>(at) & ~uintptr_t(3));
+  *shift = (int)(at - a) * 8;
+  if (there && a >= from && a + 68 <= to) {
+#pragma unroll
+    for (int i = 0; i < 17; ++i) w[i] = *reinterpret_cast<const uint32_t*>(a + 4 * i);
+  } else {   // a row that does not exist, or the operand's first or last bytes
+#pragma unroll 1
+    for (int i = 0; i < 17; ++i) {
+      uint32_t x = 0;
+      if (there)
+        for (int b = 0; b < 4; ++b)
+          if (a + 4 * i + b >= from && a + 4 * i + b < to) x |= (uint32_t)(uint8_t)a[4 * i + b] << (8 * b);
+#pragma unroll
+      for (int n = 0; n < 17; ++n) w[n] = n == i ? x : w[n];
+    }
+  }
+}
+
+__device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
 template <typename T>
-__global__ void __launch_bounds__(256) scaled_tile_kernel(const ScaledArgs p) {
+__global__ void __launch_bounds__(256) scaled_tile_kernel(const ScaledArgs p, int split) {
+  __shared__ __align__(16) uint32_t s_ab[2][2 * kAnyTile][kAnyRow];   // rows: tokens, then channels
+  const int rank = split > 1 ? (int)cluster_ctarank() : 0;
+  const int m0 = blockIdx.y * kAnyTile, n0 = (int)(blockIdx.x / split) * kAnyTile;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int wm = (warp & 1) * 32, wn = kAnyTile + (warp >> 1) * 16;   // this warp's tokens and channels
+  // this thread brings half a row per step
+  const int row = threadIdx.x >> 1, half = threadIdx.x & 1;
+  const bool token = row < kAnyTile;
+  const int index = token ? m0 + row : n0 + row - kAnyTile;
+  const bool there = index < (token ? p.M : p.N);
+  const int8_t* from = token ? p.q : p.wt;
+  const int8_t* to = from + (size_t)(token ? p.M : p.N) * p.K;
+  const int8_t* src = from + (size_t)(there ? index : 0) * p.K + half * 64;
+  const int steps = (p.K + kAnyStep - 1) / kAnyStep;
+  const int k0 = steps * rank / split, k1 = steps * (rank + 1) / split;
   pdl_wait();
   pdl_trigger();
-  __shared__ int sa[64][17], sb[64][17];   // 64 rows of 64 bytes, padded
-  const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  int acc[4][4] = {};
-  for (int k0 = 0; k0 < p.K; k0 += 64) {
-    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-      const int r = i >> 6, c = i & 63;
-      const bool kv = k0 + c < p.K;
-      reinterpret_cast<int8_t*>(&sa[r][0])[c] =
-          kv && m0 + r < p.M ? p.q[(size_t)(m0 + r) * p.K + k0 + c] : (int8_t)0;
-      reinterpret_cast<int8_t*>(&sb[r][0])[c] =
-          kv && n0 + r < p.N ? p.wt[(size_t)(n0 + r) * p.K + k0 + c] : (int8_t)0;
+  int acc[2][2][4] = {};
+  uint32_t w[17];
+  int shift = 0;
+  if (k0 < k1) fetch_any(from, to, src + k0 * kAnyStep, there, w, &shift);
+  for (int k = k0; k < k1; ++k) {
+    uint32_t(*ab)[kAnyRow] = s_ab[(k - k0) & 1];
+    // bytes of K that this half row has: what lies behind them meets zeros of q
+    const int left = p.K - k * kAnyStep - half * 64;
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      uint32_t v[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        v[x] = __funnelshift_r(w[i + x], w[i + x + 1], shift);
+        const int n = left - 4 * (i + x);
+        if (token && n < 4) v[x] &= n <= 0 ? 0u : (1u << (8 * n)) - 1u;
+      }
+      *reinterpret_cast<uint4*>(&ab[row][half * 16 + i]) = make_uint4(v[0], v[1], v[2], v[3]);
     }
-    __syncthreads();
+    __syncthreads();   // the other buffer is free then, too: all have passed its products
+    if (k + 1 < k1) fetch_any(from, to, src + (k + 1) * kAnyStep, there, w, &shift);
 #pragma unroll
-    for (int k = 0; k < 16; ++k)
+    for (int kk = 0; kk < kAnyStep / 4; kk += 8) {
+      uint32_t b[2][2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int j = 0; j < 2; ++j) {
+        b[j][0] = ab[wn + 8 * j + g][kk + t];
+        b[j][1] = ab[wn + 8 * j + g][kk + t + 4];
+      }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(sa[ty + 16 * i][k], sb[tx + 16 * j][k], acc[i][j]);
-    __syncthreads();
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t a0 = ab[wm + 16 * i + g][kk + t], a1 = ab[wm + 16 * i + g + 8][kk + t];
+        const uint32_t a2 = ab[wm + 16 * i + g][kk + t + 4], a3 = ab[wm + 16 * i + g + 8][kk + t + 4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+              : "+r"(acc[i][j][0]), "+r"(acc[i][j][1]), "+r"(acc[i][j][2]), "+r"(acc[i][j][3])
+              : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[j][0]), "r"(b[j][1]));
+      }
+    }
   }
+  // sums into shared memory; each CTA of the cluster finishes its share of the tokens
+  __syncthreads();
+  int* sums = reinterpret_cast<int*>(&s_ab[0][0][0]);
+  constexpr int kSumRow = kAnyTile + 8;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-      if (m >= p.M || n >= p.N) continue;
-      const size_t o = (size_t)m * p.N + n;
-      float v = scaled_value(acc[i][j], p.q_scale[m], p.w_scale[n], p.bias ? p.bias[n] : 0.0f);
-      if (p.residual) v += to_f32(static_cast<const T*>(p.residual)[o]);
-      static_cast<T*>(p.out)[o] = from_f32<T>(v);
-    }
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<int2*>(&sums[(wm + 16 * i + 8 * h + g) * kSumRow + wn - kAnyTile + 8 * j + 2 * t]) =
+            make_int2(acc[i][j][2 * h], acc[i][j][2 * h + 1]);
+  if (split > 1) cluster_sync();
+  else __syncthreads();
+  for (int i = threadIdx.x; i < kAnyTile / split * kAnyTile; i += 256) {
+    const int r = rank + i / kAnyTile * split, m = m0 + r, n = n0 + i % kAnyTile;
+    if (m >= p.M || n >= p.N) continue;
+    const int* at = sums + r * kSumRow + i % kAnyTile;
+    int sum = split > 1 ? 0 : *at;
+    for (int z = 0; split > 1 && z < split; ++z) sum += ld_cluster_s32(cluster_addr(at, (uint32_t)z));
+    const size_t o = (size_t)m * p.N + n;
+    float v = scaled_value(sum, p.q_scale[m], p.w_scale[n], p.bias ? p.bias[n] : 0.0f);
+    if (p.residual) v += to_f32(static_cast<const T*>(p.residual)[o]);
+    static_cast<T*>(p.out)[o] = from_f32<T>(v);
+  }
+  if (split > 1) cluster_sync();   // no CTA leaves while another reads its sums
 }
 
 constexpr int kRows = 128;    // rows of the wide operand per CTA
@@ -417,12 +505,6 @@ struct StreamConfig {
   static_assert(TOK * kRows * 4 <= kStages * kStageBytes, "sums over the ring");
 };
 
-__device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
-  int v;
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
-}
-
 template <typename T, int TOK>
 __global__ void __launch_bounds__(kStreamThreads, 1)
     scaled_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmQ,
@@ -644,8 +726,12 @@ static int launch_stream(cudaStream_t s, const ScaledArgs& p) {
 template <typename T>
 static int launch_scaled(cudaStream_t s, const ScaledArgs& p) {
   if (p.K == 0 || p.K % 16 != 0 || !aligned16(p.q) || !aligned16(p.wt)) {
-    const dim3 grid((unsigned)((p.N + 63) / 64), (unsigned)((p.M + 63) / 64));
-    ICX_CUDA(launch_pdl(scaled_tile_kernel<T>, grid, dim3(256), 0, s, p));
+    const unsigned tn = (unsigned)((p.N + kAnyTile - 1) / kAnyTile), tm = (unsigned)((p.M + kAnyTile - 1) / kAnyTile);
+    // K in shares while that leaves three CTAs per SM or fewer, of two steps or more
+    const int steps = (p.K + kAnyStep - 1) / kAnyStep;
+    int split = 1;
+    while (split < 8 && (int64_t)tn * tm * split * 2 <= 3 * sm_count() && steps / (split * 2) >= 2) split *= 2;
+    ICX_CUDA(launch_pdl_cluster(scaled_tile_kernel<T>, dim3(tn * split, tm), dim3(256), 0, s, (unsigned)split, p, split));
     return ICX_OK;
   }
   if (p.M <= 16) return launch_stream<T, 16>(s, p);

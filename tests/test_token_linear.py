@@ -207,6 +207,36 @@ def test_product_largest_sum_is_exact(M):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N", [(1, 127, 1), (2, 129, 63), (3, 1633, 130), (5, 2049, 64), (63, 4099, 65),
+                                   (64, 255, 700), (130, 1031, 200), (1000, 515, 129), (8, 7425, 520)])
+def test_product_any_k(M, K, N):
+    """Rows that start at every byte, and K shared out between CTAs."""
+    check_product(M, K, N, torch.float32, True, True, seed=M + K)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("at", [1, 2, 3, 8])
+def test_product_operands_at_any_byte(at):
+    """q and the weight inside larger buffers whose bytes around them must not count."""
+    M, K, N = 6, 640, 70
+    q, sa, w, sw, _, _ = product_case(M, K, N, torch.float32, False, False, seed=at)
+    buf = torch.full((M * K + 32,), 99, dtype=torch.int8, device=DEV)
+    view = buf[at:at + M * K].view(M, K)
+    view.copy_(q)
+    L, out = _lib.load(), torch.empty(M, N, device=DEV)
+    wt = torch.full((N * K + 32,), 77, dtype=torch.int8, device=DEV)
+    wt[at:at + N * K].view(N, K).copy_(w.t())
+    ptr = lambda t, d=0: ctypes.c_void_p(t.data_ptr() + d)
+    csa, csw = sa.to(DEV), sw.to(DEV)
+    assert L.icx_matmul_integer_scaled(None, ptr(buf, at), ptr(csa), ptr(wt, at), M, K, N, ptr(csw), None, None,
+                                       _lib.ICX_F32, ptr(out)) == 0
+    torch.cuda.synchronize()
+    acc, want = ref.scaled_product(q.numpy(), sa.numpy(), w.numpy(), sw.numpy(), None, None)
+    tol = 5 * 2.0 ** -24 * np.abs(acc * f64(sa)[:, None] * f64(sw))
+    assert (np.abs(f64(out) - want) <= ref.rounding(want, tol, torch.float32)).all()
+
+
+@pytest.mark.gpu
 def test_product_large_tiles_and_leading_axes():
     check_product(1500, 768, 2304, torch.bfloat16, True, True, seed=1)
     check_product(8320, 1600, 520, torch.float16, seed=2)
