@@ -8,13 +8,13 @@
 //                         cta_group::2) tokens x 128 / 256 channels per tile,
 //                         persistent, bound by the tensor cores (8192 tokens,
 //                         K = 4096, N = 14336: 310 us, 3.1 POPS).
-//   scaled_stream_kernel  up to 128 tokens: the weight is the 128-row operand
-//                         and the tokens the narrow one, so that nothing is
-//                         padded to 128 tokens; bound by reading the weight
+//   scaled_stream_kernel  up to 32 tokens, and up to 128 where K is long: the
+//                         weight is the 128-row operand and the tokens the
+//                         narrow one, so that nothing is padded to 128 tokens; bound by reading the weight
 //                         once, which all SMs share by splitting K over the
 //                         CTAs of a cluster, summed in s32 through distributed
 //                         shared memory (exact, so in any order).  4 tokens,
-//                         K = N = 4096: 5.7 us, 2.9 TB/s, latency.
+//                         K = N = 4096: 5.9 us, 2.8 TB/s, latency.
 //   scaled_tile_kernel    any K and alignment (TMA needs K % 16 == 0 and
 //                         16-byte bases): mma.sync on 64 x 64 tiles.
 #include <type_traits>
@@ -78,6 +78,15 @@ __device__ __forceinline__ void fetch_any(const int8_t* from, const int8_t* to, 
 __device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
   int v;
   asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ int4 ld_cluster_s32x4(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
 
@@ -598,20 +607,37 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   else __syncthreads();
   if (ok) {
     const int m_from = p.M * rank / split, m_to = p.M * (rank + 1) / split;
-    for (int i = threadIdx.x; i < (m_to - m_from) * kRows; i += kStreamThreads) {
-      const int m = m_from + i / kRows, c = i % kRows, n = n0 + c;
-      int acc = 0;
-      if (split > 1) {
-        for (int r = 0; r < split; ++r)
-          if (nk * (r + 1) / split > nk * r / split) acc += ld_cluster_s32(cluster_addr(sums + m * kRows + c, (uint32_t)r));
-      } else {
-        acc = sums[m * kRows + c];
+    // four channels per thread (every CTA of the cluster has steps: nk >= split)
+#pragma unroll 2
+    for (int i = threadIdx.x; i < (m_to - m_from) * (kRows / 4); i += kStreamThreads) {
+      const int m = m_from + i / (kRows / 4), c = i % (kRows / 4) * 4, n = n0 + c;
+      if (n >= p.N) continue;
+      int4 acc = *reinterpret_cast<const int4*>(sums + m * kRows + c);
+      for (int x = 1; x < split; ++x) {   // the others', in any order: s32 sums are exact
+        const int4 y = ld_cluster_s32x4(cluster_addr(sums + m * kRows + c, (uint32_t)((rank + x) & (split - 1))));
+        acc.x += y.x;
+        acc.y += y.y;
+        acc.z += y.z;
+        acc.w += y.w;
       }
-      if (n < p.N) {
-        float v = scaled_value(acc, __ldg(p.q_scale + m), __ldg(p.w_scale + n), p.bias ? __ldg(p.bias + n) : 0.0f);
-        const size_t o = (size_t)m * p.N + n;
-        if (p.residual) v += to_f32(static_cast<const T*>(p.residual)[o]);
-        static_cast<T*>(p.out)[o] = from_f32<T>(v);
+      const int sum[4] = {acc.x, acc.y, acc.z, acc.w};
+      const float sa = __ldg(p.q_scale + m);
+      const size_t o = (size_t)m * p.N + n;
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = 0.0f;
+        if (n + e >= p.N) continue;
+        v[e] = scaled_value(sum[e], sa, __ldg(p.w_scale + n + e), p.bias ? __ldg(p.bias + n + e) : 0.0f);
+        if (p.residual) v[e] += to_f32(static_cast<const T*>(p.residual)[o + e]);
+      }
+      T* out = static_cast<T*>(p.out) + o;
+      if ((reinterpret_cast<uintptr_t>(out) & (4 * sizeof(T) - 1)) == 0 && n + 4 <= p.N) {
+        store_f32<T, 4>(out, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n + e < p.N) out[e] = from_f32<T>(v[e]);
       }
     }
   }
@@ -704,6 +730,15 @@ static int launch_rows(cudaStream_t s, const ScaledArgs& p, int units) {
   return ICX_OK;
 }
 
+// CTAs that share out K for a tile of channels: while the SMs are not all busy
+// and a CTA keeps at least four steps.
+static int stream_split(const ScaledArgs& p) {
+  const int tiles = (p.N + kRows - 1) / kRows, nk = (p.K + kStep - 1) / kStep, sms = sm_count();
+  int split = 1;
+  while (split < 8 && tiles * split * 2 <= sms && nk / (split * 2) >= 4) split *= 2;
+  return split;
+}
+
 template <typename T, int TOK>
 static int launch_stream(cudaStream_t s, const ScaledArgs& p) {
   using C = StreamConfig<TOK>;
@@ -714,10 +749,7 @@ static int launch_stream(cudaStream_t s, const ScaledArgs& p) {
   rc = make_tmap(&tq, p.q, p.M, p.K, TOK);
   if (rc) return rc;
   ICX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
-  // split K while the SMs are not all busy and a CTA keeps at least four steps
-  const int tiles = (p.N + kRows - 1) / kRows, nk = (p.K + kStep - 1) / kStep, sms = sm_count();
-  int split = 1;
-  while (split < 8 && tiles * split * 2 <= sms && nk / (split * 2) >= 4) split *= 2;
+  const int tiles = (p.N + kRows - 1) / kRows, split = stream_split(p);
   ICX_CUDA(launch_pdl_cluster(kern, dim3((unsigned)(tiles * split)), dim3(kStreamThreads), C::kSmem, s,
                               (unsigned)split, tw, tq, p, split));
   return ICX_OK;
@@ -736,8 +768,12 @@ static int launch_scaled(cudaStream_t s, const ScaledArgs& p) {
   }
   if (p.M <= 16) return launch_stream<T, 16>(s, p);
   if (p.M <= 32) return launch_stream<T, 32>(s, p);
-  if (p.M <= 64) return launch_stream<T, 64>(s, p);
-  if (p.M <= 128) return launch_stream<T, 128>(s, p);
+  // 33 to 128 tokens: the other way round where K is short or hardly shared out
+  // (K, N; rows / stream, us: 128 tokens 1472, 768: 6.9 / 10.0; 4096, 14336: 18.2 /
+  // 20.9; 8192, 1024: 15.4 / 8.4; 100 tokens 4096, 4096: 11.1 / 9.2; 64 tokens 768,
+  // 768: 5.2 / 6.9; 4096, 4096: 10.5 / 7.3)
+  if (p.M <= 64 && p.K > 8 * kStep) return launch_stream<T, 64>(s, p);
+  if (p.M > 64 && p.M <= 128 && stream_split(p) >= 4) return launch_stream<T, 128>(s, p);
   const int sms = sm_count();
   const long nm = (p.M + kRows - 1) / kRows;
   const int pairs = p.M >= 1024 && p.N > 128 ? max_pairs<T, 256>() : 0;
