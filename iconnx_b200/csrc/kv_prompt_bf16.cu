@@ -47,6 +47,7 @@ namespace icx {
 
 constexpr int kB16Keys = 48;   // positions per tile: what three warps dequantise, two threads to each
 constexpr int kB16Threads = 512, kB16Stages = 4;
+constexpr float kWeightUp = 7.0f;   // scores pass the reference by 8 at most
 constexpr int kB16Cols = 64;   // tensor memory columns of an accumulator
 
 template <int D>
@@ -414,8 +415,9 @@ __global__ void __launch_bounds__(kB16Threads, 1)
             }
           }
         }
-        const float m_use = fmaxf(m, -3e38f);
-        const F2 f_2 = f2(ft, ft), m_2 = f2(-m_use, -m_use);
+        // weights 2^7 times as large, up to 2^15: f16 keeps those 2^-39 of that
+        const float m_use = kWeightUp - fmaxf(m, -3e38f);
+        const F2 f_2 = f2(ft, ft), m_2 = f2(m_use, m_use);
         F2 l_a = f2(0.0f, 0.0f), l_b = f2(0.0f, 0.0f);
 #pragma unroll
         for (int n = 0; n < kB16Keys; n += 16) {

@@ -189,7 +189,11 @@ def gpu_kv_cache_attention(cache: KvCache, q: torch.Tensor, page_table: torch.Te
     ``scale`` (default 1 / sqrt(head_dim)) multiplies the scores.  Returns q's
     shape and type, contiguous.  A token without any position gives zeros;
     rows outside ``cu_tokens`` are left as they were in ``out`` (undefined in a
-    fresh tensor).  Scores, softmax statistics and sums are f32.
+    fresh tensor).  Scores, softmax statistics and sums are f32.  BFloat16
+    prompt chunks (64 rows of a K/V head per sequence or more, group 64,
+    head_dim up to 128) meet K, V and the weights as f16, K and V in units of
+    the largest of the positions a block of rows reads: values 2^20 times
+    smaller keep their bits, still smaller ones lose them.
     """
     what = "KvCacheAttention"
     q = _rows(q, None, cache.head_dim, cache.device, f"{what}: q")

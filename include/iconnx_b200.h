@@ -276,7 +276,7 @@ ICX_API int icx_quantize_per_token(void* stream, const void* d_x, int x_type, si
  *              [+ bias[n]] [+ residual[m,n]]
  * The sum is exact in s32 (K <= ICX_SCALED_MAX_K, so it cannot wrap); the
  * rest is f32, rounded once to out_type.  bias: f32 [N] or NULL; residual:
- * out_type [M, N] or NULL. */
+ * out_type [M, N] or NULL.  M <= 4194240, N < 2^22. */
 #define ICX_SCALED_MAX_K 131071
 ICX_API int icx_matmul_integer_scaled(void* stream, const int8_t* d_q, const float* d_q_scale,
                                       const int8_t* d_wt, size_t M, size_t K, size_t N,
@@ -348,7 +348,9 @@ ICX_API int icx_kv_cache_read(void* stream, const icx_kv_cache* cache, const icx
  * contiguous), q_heads a multiple of kv_heads (consecutive query heads share
  * a kv head); out: contiguous, of q's type.  A row without any position gives
  * zeros.  Positions without a usable page take no part.
- * Scores, softmax statistics and sums are f32. */
+ * Scores, softmax statistics and sums are f32; where an output is bf16 and a
+ * sequence has many rows, K, V and the weights are rounded to f16.  The
+ * workspace depends on the shapes alone. */
 ICX_API size_t icx_kv_cache_attention_workspace_bytes(const icx_kv_cache* cache,
                                                       const icx_kv_tokens* where, int q_heads,
                                                       int type);

@@ -400,6 +400,31 @@ def test_prompt_chunk_values_of_unequal_size():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_prompt_output_of_small_weights(dtype):
+    """One position holds nearly all the weight and no value; what the others
+    (2^-20 of its weight each) give is as exact as an output should be."""
+    n, D = 600, 64
+    c = Case([n], 1, D, 8, 64, 16, dtype, seed=26)
+    g = torch.Generator().manual_seed(27)
+    k = torch.randn(n, 1, D, generator=g) * 0.01
+    v = 1.0 + 0.1 * torch.rand(n, 1, D, generator=g)
+    k[0], v[0] = 1.0, 0.0
+    k, v = k.to(dtype), v.to(dtype)
+    gpu_kv_cache_append(c.cache, k.to(DEV), v.to(DEV), c.table, i32([n]), i32([0, n]))
+    kc, vc = (ref.cached_values(f64(x), 8, 64) for x in (k, v))
+    q = (torch.full((80, 2, D), 20 * np.log(2.0) / (D * D ** -0.5)) + 0.01 * torch.randn(80, 2, D, generator=g)).to(dtype)
+    out = f64(gpu_kv_cache_attention(c.cache, q.to(DEV), c.table, i32([n]), i32([0, 80])))
+    want = ref.attention(f64(q), kc, vc, D ** -0.5)
+    assert 1e-4 < want.min() and want.max() < 1e-3
+    # every value is positive, so relative errors do not grow in the sum: the
+    # output's half step (f16: in its subnormals' 2^-25 besides), a weight and a
+    # value to f16 (2^-12 each), K and q as there is nothing to cancel: |S| 2^-11
+    tol = np.abs(want) * (torch.finfo(dtype).eps / 2 + 2 * 2.0 ** -12 + 14 * 2.0 ** -11) + 2.0 ** -25
+    assert (np.abs(out - want) <= tol).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("bits", [4, 8])
 def test_prompt_rows_beside_much_larger_values_they_do_not_see(bits):
     """A position 2^18 times as large as the others leaves the rows before it as exact."""
