@@ -2,6 +2,7 @@
 // error text and CUDA-call checking.  No entry point throws across the ABI.
 #pragma once
 
+#include <atomic>
 #include <cuda_runtime.h>
 #include <cstdarg>
 #include <cstdio>
@@ -57,6 +58,22 @@ inline cudaError_t launch_pdl_cluster(void (*kern)(KArgs...), dim3 grid, dim3 bl
   cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
 }
+
+// Allows a kernel its dynamic shared memory, once per device: a static of the
+// function that launches the kernel.
+struct SharedMemoryOnce {
+  std::atomic<unsigned long long> done{0};
+  template <typename... KArgs>
+  cudaError_t allow(void (*kern)(KArgs...), int bytes) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    const unsigned long long bit = device < 64 ? 1ull << device : 0ull;
+    if (e != cudaSuccess || (done.load(std::memory_order_relaxed) & bit)) return e;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+  }
+};
 
 }  // namespace icx
 

@@ -22,14 +22,26 @@ AttendPlan plan_attend(const KvView& c, const KvTokens& w, int q_heads, int type
     if (steps >= 64ll * sm_count() * kAttWarps * att_resident(c.dim, 1, 4)) p.nt = 2;
   }
   const int R = 8 * p.nt, step = att_step(c.dim, c.bits, R);
-  // four steps are over before a second launch would be
-  p.split = reach > 4 * step;
-  p.unit = p.split ? step : 4 * step;
+  const int64_t runs = (w.tokens * share / R + w.batch) * c.heads;   // row tiles
+  const int64_t resident = (int64_t)sm_count() * att_resident(c.dim, p.nt, (int)float_bytes(type));
+  // Up to four steps per warp of a CTA, or in one warp, are over before a second
+  // launch would be; many row tiles are shared out evenly instead.
+  if (reach <= step || (reach <= 4 * step && runs > resident)) {
+    p.split = kSplitNone;
+    p.unit = 4 * step;
+  } else if (reach <= 4 * kAttWarps * step && runs <= 2 * resident) {
+    p.split = kSplitCta;
+    p.unit = 1 << 30;
+    p.ctas = (int)runs;
+    return p;
+  } else {
+    p.split = kSplitAny;
+    p.unit = step;
+  }
   const int64_t blocks = reach > p.unit ? (reach + p.unit - 1) / p.unit : 1;
-  const int64_t units = (w.tokens * share / R + w.batch) * c.heads * blocks;
-  const int64_t resident = (int64_t)sm_count() * att_resident(c.dim, p.nt, (int)float_bytes(type)), want = (units + kAttWarps - 1) / kAttWarps;
+  const int64_t want = (runs * blocks + kAttWarps - 1) / kAttWarps;
   p.ctas = (int)(want < resident ? want : resident);
-  if (p.split) {
+  if (p.split == kSplitAny) {
     p.prefix_bytes = ((size_t)(w.batch + 1) * 8 + 255) & ~size_t(255);
     p.bytes = p.prefix_bytes + (size_t)p.ctas * kAttWarps * 2 * R * (c.dim + 2) * 4;
   }

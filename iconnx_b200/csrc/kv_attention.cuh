@@ -39,7 +39,7 @@
 // Measured: 64 sequences of up to 16,000 positions, one token, 8 K/V heads of 4
 // query heads of 128, bf16: 4 bits 198 us (3.8 TB/s; floor 118 us at 6.46 TB/s),
 // 8 bits 254 us (5.7 TB/s; floor 222).  One sequence of 500, 12 heads of 64, f32,
-// 8 bits: 12 us for both launches, latency.
+// 8 bits: 10 us, latency.
 #pragma once
 
 #include <type_traits>
@@ -75,6 +75,13 @@ constexpr int att_most_nt(int dim) {
   return sizeof(T) == 4 && dim <= 128 ? 2 : 1;
 }
 
+// What a row's positions are shared out to: one warp; any warps, which leave
+// their parts in the workspace; the warps of one CTA, which join in shared memory
+// (one launch, no workspace: 1 token on 500 positions, 12 heads of 64, f32: 12.5 -> 10.0
+// us; 16 sequences of up to 500, 8 K/V heads of 4 query heads of 128, bf16: 18.6 ->
+// 13.8).
+enum AttendSplit { kSplitNone, kSplitAny, kSplitCta };
+
 struct AttendArgs {
   const void* q;
   int64_t q_token_stride, q_head_stride;
@@ -84,7 +91,7 @@ struct AttendArgs {
   void* out;
   int64_t* prefix;  // workspace: units before each sequence [batch + 1]
   float* partial;   // workspace: two slots per warp of R x (D + 2) floats
-  int split;        // rows may go to several warps
+  int split;        // AttendSplit
   int unit;         // positions per unit
 };
 
@@ -255,8 +262,10 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
   const int64_t all = (int64_t)gridDim.x * kAttWarps, warps = working_warps(total, all);
   // few working warps: one per CTA first
   const int64_t me = warps < all ? (int64_t)warp * gridDim.x + blockIdx.x : (int64_t)blockIdx.x * kAttWarps + warp;
-  const int64_t u0 = min(total * me / warps, total), u1 = min(total * (me + 1) / warps, total);
-  const bool write = a.split && me == 0;   // the first warp leaves the prefix sums
+  const bool cta = a.split == kSplitCta;   // a unit (row tile) per CTA
+  const int64_t u0 = cta ? min((int64_t)blockIdx.x, total) : min(total * me / warps, total);
+  const int64_t u1 = cta ? min((int64_t)blockIdx.x + 1, total) : min(total * (me + 1) / warps, total);
+  const bool write = a.split == kSplitAny && me == 0;   // the first warp leaves the prefix sums
   int seq = w.batch;
   int64_t base = 0, before = 0;
   for (int b0 = 0; b0 < w.batch; b0 += 32) {
@@ -307,8 +316,12 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
 
     // ------------------------------------------------------- codes on their way
     uint8_t* ring = smem + warp * C::kStages * C::kStage;
-    const int end = (int)min((int64_t)block1 * a.unit, (int64_t)see_any);
-    const int p0 = block0 * a.unit;
+    int end = (int)min((int64_t)block1 * a.unit, (int64_t)see_any), p0 = block0 * a.unit;
+    if (cta) {
+      const int steps = (end + kStep - 1) / kStep;
+      p0 = steps * warp / kAttWarps * kStep;
+      end = min(end, steps * (warp + 1) / kAttWarps * kStep);
+    }
     const int tiles = p0 < end ? (end - p0 + kStep - 1) / kStep : 0;   // steps of SUB tiles
     // lane i < 4 SUB brings piece i % 4 (K codes, K parameters, V codes, V
     // parameters) of tile i / 4
@@ -705,8 +718,10 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
     }
 
     // ---------------------------------------------- join lanes, and write
-    const bool whole = block0 == 0 && block1 == su.blocks;
-    float* slot = a.partial + (me * 2 + (block0 == 0 ? 1 : 0)) * R * C::kRowFloats;
+    const bool whole = !cta && block0 == 0 && block1 == su.blocks;
+    static_assert(C::kStages * C::kStage >= R * C::kRowFloats * 4, "a warp's ring holds its part");
+    float* slot = cta ? reinterpret_cast<float*>(ring) : a.partial + (me * 2 + (block0 == 0 ? 1 : 0)) * R * C::kRowFloats;
+    __syncwarp();   // the ring has been read by all lanes
 #pragma unroll
     for (int x = 0; x < NT; ++x)
 #pragma unroll
@@ -737,6 +752,29 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
         }
         if (!whole && g == 0 && r < su.rows) *reinterpret_cast<float2*>(part + D) = make_float2(m[x][h], l[x][h]);
       }
+    if (cta) {   // the only pass of this loop, in all warps
+      __syncthreads();
+      for (int i = threadIdx.x; i < nrows * (D / 2); i += 32 * kAttWarps) {
+        const int row = i / (D / 2), d = i % (D / 2) * 2;
+        auto at = [&](int z) { return reinterpret_cast<const float*>(smem + z * C::kStages * C::kStage) + row * C::kRowFloats; };
+        float top = kNoScore, sum = 0.0f, v[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int z = 0; z < kAttWarps; ++z) top = fmaxf(top, at(z)[D]);
+#pragma unroll
+        for (int z = 0; z < kAttWarps; ++z) {
+          const float2 ml = *reinterpret_cast<const float2*>(at(z) + D), y = *reinterpret_cast<const float2*>(at(z) + d);
+          const float f = ex2(ml.x - top);
+          sum = fmaf(ml.y, f, sum);
+          v[0] = fmaf(y.x, f, v[0]);
+          v[1] = fmaf(y.y, f, v[1]);
+        }
+        const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+        v[0] *= inv;
+        v[1] *= inv;
+        const int r = r0 + row;
+        store_f32<T, 2>(static_cast<T*>(a.out) + ((int64_t)(row_base + r / share) * a.q_heads + head * share + r % share) * D + d, v);
+      }
+    }
   }
 }
 
@@ -835,7 +873,7 @@ struct AttendPlan {
   int nt;      // query rows per tile / 8
   int ctas;
   int unit;    // positions per unit
-  bool split;
+  int split;   // AttendSplit
   size_t prefix_bytes, bytes;   // workspace
 };
 
@@ -867,10 +905,11 @@ int launch_attend_rows(cudaStream_t s, const KvView& c, const KvTokens& w, const
                        const AttendPlan& p) {
   using C = AttConfig<T, D, BITS, GROUP, NT>;
   auto kern = kv_attend_rows_kernel<T, D, BITS, GROUP, NT>;
+  static SharedMemoryOnce once;
   if (C::kSmem > 40 * 1024)   // beside the static part
-    ICX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    ICX_CUDA(once.allow(kern, C::kSmem));
   ICX_CUDA(launch_pdl(kern, dim3(p.ctas), dim3(32 * kAttWarps), C::kSmem, s, c, w, a));
-  if (p.split) {
+  if (p.split == kSplitAny) {
     // few rows have many parts each
     const int64_t rows = w.tokens * a.q_heads;
     const int per_row = rows <= 1024 ? 8 : 1;

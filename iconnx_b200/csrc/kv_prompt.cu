@@ -443,7 +443,8 @@ template <typename T, int D, int BITS>
 static int launch_prompt_kernel(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a, const PromptPlan& p) {
   using C = PromptConfig<D>;
   auto kern = kv_prompt_kernel<T, D, BITS>;
-  ICX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+  static SharedMemoryOnce once;
+  ICX_CUDA(once.allow(kern, C::kSmem));
   ICX_CUDA(launch_pdl(kern, prompt_grid(c, w, a, p), dim3(kPrThreads), C::kSmem, s, c, w, a, p.splits));
   return launch_prompt_join<T, D>(s, w, a, p);
 }

@@ -492,7 +492,8 @@ template <int D, int BITS>
 static int launch_kernel(cudaStream_t s, const KvView& c, const KvTokens& w, const AttendArgs& a, const PromptPlan& p) {
   using C = PromptB16Config<D>;
   auto kern = kv_prompt_bf16_kernel<D, BITS>;
-  ICX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+  static SharedMemoryOnce once;
+  ICX_CUDA(once.allow(kern, C::kSmem));
   ICX_CUDA(launch_pdl(kern, prompt_grid(c, w, a, p), dim3(kB16Threads), C::kSmem, s, c, w, a, p.rows, p.splits));
   return launch_prompt_join<__nv_bfloat16, D>(s, w, a, p);
 }

@@ -719,7 +719,8 @@ static int launch_rows(cudaStream_t s, const ScaledArgs& p, int units) {
     if (rc) return rc;
   }
   const int vec_residual = pitch16 && p.residual && aligned16(p.residual);
-  ICX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+  static SharedMemoryOnce once;
+  ICX_CUDA(once.allow(kern, C::kSmem));
   const long tiles = (long)((p.M + kRows * CG - 1) / (kRows * CG)) * ((p.N + BN - 1) / BN);
   const unsigned grid = (unsigned)(tiles < units ? tiles : units) * CG;
   if (CG == 2)
@@ -748,7 +749,8 @@ static int launch_stream(cudaStream_t s, const ScaledArgs& p) {
   if (rc) return rc;
   rc = make_tmap(&tq, p.q, p.M, p.K, TOK);
   if (rc) return rc;
-  ICX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+  static SharedMemoryOnce once;
+  ICX_CUDA(once.allow(kern, C::kSmem));
   const int tiles = (p.N + kRows - 1) / kRows, split = stream_split(p);
   ICX_CUDA(launch_pdl_cluster(kern, dim3((unsigned)(tiles * split)), dim3(kStreamThreads), C::kSmem, s,
                               (unsigned)split, tw, tq, p, split));

@@ -326,6 +326,26 @@ def test_attention_several_tokens(dim, bits, share, news, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_many_short_sequences(dtype):
+    """More row tiles than CTAs at once, each within one warp."""
+    lens = [(37 * b) % 61 for b in range(160)]
+    c = Case(lens, 2, 128, 8, 64, 16, dtype, seed=31, width_extra=0)
+    check_attention(c, [1] * 160, 4, dtype, seed=6)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,bits", [(64, 4), (64, 8), (128, 4), (256, 8)])
+def test_attention_row_tile_per_cta(dim, bits, dtype):
+    """Row tiles whose positions the warps of one CTA share: from none and one up."""
+    lens = [440, 0, 1, 17, 130, 300]
+    c = Case(lens, 2, dim, bits, 32, 16, dtype, seed=32 + dim)
+    check_attention(c, [1] * 6, 6, dtype, seed=7)
+    check_attention(c, [3, 0, 1, 5, 2, 9], 10, dtype, seed=8, pad=2)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("page", [16, 64, 1024])
 def test_attention_long_and_ragged(page):
     """Long sequences beside short ones: work split over the positions and joined."""
