@@ -30,9 +30,9 @@
 // Work: a unit is 16 or 32 positions of one (sequence, K/V head, tile of query
 // rows); each warp takes an equal, contiguous share of all units, found on the
 // device from seq_lens and cu_tokens, so ragged batches balance and a captured
-// call can be replayed with other lengths.  Warps meet nowhere: one that runs
-// into another sequence or head starts on it while the other fifteen of the SM
-// keep its pipes busy.  Rows whose units went to several warps leave (m, l, o)
+// call can be replayed with other lengths.  Warps meet nowhere (but at the end of
+// the short form, kSplitCta): one that runs into another sequence or head starts
+// on it while the other fifteen of the SM keep its pipes busy.  Rows whose units went to several warps leave (m, l, o)
 // in the workspace for the join kernel.  All joins run in a fixed order, so
 // equal calls give equal results.
 //
