@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     // The residual's box into the places its outputs will take; the box's store
     // of two boxes ago has been read out.
     auto put_residual = [&](uint8_t* box, int mrow0, int nb) {
-      if (!residual || mrow0 >= p.M) return;
+      if (!residual) return;
       if (tma_store && lane == 0) bulk_wait_read<1>();
       __syncwarp();
       if (vec_residual && nb + CB <= p.N) {
@@ -400,13 +400,15 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
       const int mrow0 = m0 + quad * 32, m = mrow0 + lane;
       const float sa = m < p.M ? __ldg(p.q_scale + m) : 0.0f;
       const int nboxes = (min(BN, p.N - n0) + CB - 1) / CB;
+      // A warp whose 32 tokens all lie behind the last leaves its boxes alone: they
+      // may still be on their way out with the tile before.
+      const bool rows_here = mrow0 < p.M;
       // the first box's residual arrives while the products run
-      if (part < nboxes) put_residual(box0 + buf * 4096, mrow0, n0 + part * CB);
+      if (rows_here && part < nboxes) put_residual(box0 + buf * 4096, mrow0, n0 + part * CB);
       if (ok) ok = mbar_wait_warp(&tfull[acc], acc_phase, ICX_DEVICE_TIMEOUT_EPILOGUE);
       tc_fence_after();
       const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN);
-      const bool rows_here = mrow0 < p.M;
-      for (int bx = part; ok && bx < nboxes; bx += kRowsEpi / 4) {
+      for (int bx = part; ok && rows_here && bx < nboxes; bx += kRowsEpi / 4) {
         const int nb = n0 + bx * CB;
         uint8_t* box = box0 + buf * 4096;
         uint8_t* row = box + lane * 128;
@@ -455,7 +457,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            if (rows_here) tma_store_2d(&tmOut, box, nb, mrow0);
+            tma_store_2d(&tmOut, box, nb, mrow0);
             bulk_commit();
           }
           buf ^= 1;

@@ -245,6 +245,26 @@ def test_product_large_tiles_and_leading_axes():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N", [(8320, 8192), (300, 14336), (1500, 6144)])
+def test_product_residual_where_a_warp_has_no_rows(M, N, dtype):
+    """More tiles than CTAs, and a last token tile that leaves some warps (8320: a
+    whole CTA of a pair) without a token: what the tile before still has to
+    store must not be touched.  Integers, so that f32 and bf16 hold every sum."""
+    K, top = 64, 100
+    g = torch.Generator(DEV).manual_seed(M)
+    q = torch.randint(-1, 2, (M, K), generator=g, device=DEV, dtype=torch.int8)
+    w = torch.randint(-1, 2, (K, N), generator=g, device=DEV, dtype=torch.int8)
+    r = torch.randint(-top, top + 1, (M, N), generator=g, device=DEV).to(dtype)
+    one, pw = torch.ones(M, device=DEV), ops.prepare_weight(w)
+    # at most 64 + 100: exact in every type
+    want = ((q.float() @ w.float()) + r.float()).to(dtype)
+    for _ in range(20):
+        out = ops.gpu_matmul_integer_scaled(q, one, pw, torch.ones(N, device=DEV), residual=r, out_dtype=dtype)
+        assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
 def test_product_empties_and_nan_rows():
     w = ops.prepare_weight(torch.ones(32, 5, dtype=torch.int8, device=DEV))
     ws, bias = torch.ones(5, device=DEV), torch.arange(5.0, device=DEV)
