@@ -116,10 +116,10 @@ __global__ void __launch_bounds__(kB16Threads, 1)
   uint8_t* s_q = smem;
   auto s_k = [&](int n) { return smem + 2 * C::kQ + n * C::kTile; };
   auto s_v = [&](int n) { return smem + 2 * C::kQ + (kB16Stages + n) * C::kTile; };
-  __shared__ __align__(8) uint64_t bars[4 * kB16Stages + 10];
+  __shared__ __align__(8) uint64_t bars[4 * kB16Stages + 14];
   uint64_t *k_full = bars, *k_empty = k_full + kB16Stages, *v_full = k_empty + kB16Stages, *v_empty = v_full + kB16Stages;
   uint64_t *s_full = v_empty + kB16Stages, *p_full = s_full + 4;   // [row tile][accumulator]
-  uint64_t *q_full = p_full + 4, *o_full = q_full + 1;
+  uint64_t *q_full = p_full + 4, *o_full = q_full + 1, *o_done = o_full + 1;   // o_done: as s_full
   __shared__ uint32_t s_look[5];   // largest s and |lo| of K, of V; whether anything is special
   __shared__ uint32_t tmem_slot;
   __shared__ int s_seq, s_tile;
@@ -137,6 +137,7 @@ __global__ void __launch_bounds__(kB16Threads, 1)
     for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
+      mbar_init(&o_done[i], 1);
     }
     mbar_init(q_full, 8);
     mbar_init(o_full, 2);
@@ -250,6 +251,7 @@ __global__ void __launch_bounds__(kB16Threads, 1)
               mma_f16_ts(t_out + (uint32_t)(k * kPrGroup), t_acc + (uint32_t)((i & 1) * kB16Cols + n * 8),
                          vb + (uint64_t)(k * (kB16Keys * 128 >> 4) + n * 128), id_o, i > 0 || n > 0);
           done(&v_empty[st]);
+          mma_commit(&o_done[2 * h + (i & 1)]);
           if (i + 2 < tiles) ok = scores(i + 2);
           if (ok && i + 1 == tiles) done(o_full);
         }
@@ -400,8 +402,12 @@ __global__ void __launch_bounds__(kB16Threads, 1)
           m = nm;
           l *= alpha;
           if (i > 0) {
-            // the output so far: its last product has to be there
-            ok = wait_warp(&v_empty[(i - 1) % kB16Stages], (uint32_t)((i - 1) / kB16Stages & 1), ICX_DEVICE_TIMEOUT_EPILOGUE);
+            // The output so far: this row tile's product of tile i - 1 has to be
+            // there.  The barrier's phase before belongs to tile i - 3, whose product
+            // the scores of tile i come behind.  (The stages' barriers do not serve:
+            // they count the other row tile too, which may be five tiles behind, and
+            // then the phase before lets this wait pass.)
+            ok = wait_warp(&o_done[2 * h + (st ^ 1)], (uint32_t)((i - 1) >> 1 & 1), ICX_DEVICE_TIMEOUT_EPILOGUE);
             if (!ok) break;
             tc_fence_after();
 #pragma unroll 1

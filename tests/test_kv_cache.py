@@ -492,6 +492,67 @@ def test_prompt_shares_with_missing_pages_and_nan(dtype):
     assert status() == 0
 
 
+def bounded_attention(q, k, v, scale, dtype, operand):
+    """(want, bound of |out - want|) of q [n, heads, D], the last n of k, v [len,
+    kv_heads, D], all f64 on the GPU.  With r the half step of the operands that K,
+    V and the weights pass through (f16: 2^-11; 0 where they keep f32's bits) and
+    32-bit sums of D products, a score is off by e = (r + D 2^-24) sum |q k| scale
+    and its weight by exp(e) - 1; a weight and a value are off by r, an exponential
+    by 2^-20, and n weighted values in 32 bits by n 2^-24 of their largest sum."""
+    n, hq, D = q.shape
+    length, hk = k.shape[:2]
+    q, k, v = q.transpose(0, 1), *(x.transpose(0, 1).repeat_interleave(hq // hk, 0) for x in (k, v))
+    s = q @ k.transpose(1, 2) * scale
+    last = torch.arange(length - n, length, device=q.device)[:, None]
+    s.masked_fill_(torch.arange(length, device=q.device) > last, -torch.inf)
+    p = torch.softmax(s, -1)
+    want = p @ v
+    e = torch.expm1((operand + D * 2.0 ** -24) * (q.abs() @ k.abs().transpose(1, 2)) * abs(scale))
+    e = p * (e + operand + 2.0 ** -20)
+    off = e.sum(-1, keepdim=True)
+    assert off.max() < 0.5
+    far = p @ v.abs() * (operand + length * 2.0 ** -24)
+    tol = (e @ v.abs() + off * want.abs() + far) / (1 - off) + v.abs().max() * length * 2.0 ** -39
+    want, tol = (x.transpose(0, 1).cpu().numpy() for x in (want, tol))
+    return want, ref.rounding(want, tol, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim,bits,tokens", [(64, 4, 1200), (64, 8, 1217), (128, 4, 1217), (128, 8, 1200)])
+def test_prompt_rows_that_fill_the_gpu(dim, bits, tokens, dtype):
+    """Enough rows for 256 per CTA in bf16 (the last ones over and under 128), whose
+    scores grow along the positions: every 32 tokens (128 rows) at another rate, so
+    that the reference moves in every tile of some rows and late and seldom in the
+    rows beside them."""
+    heads, share, page, prefix = 8, 4, 16, 150
+    lens, news = [tokens + prefix, 70], [tokens, 20]
+    g = torch.Generator(DEV).manual_seed(dim + bits)
+    cache = KvCache(100, page, heads, dim, bits, 64, DEV)
+    need = -(-lens[0] // page)
+    order = torch.randperm(100, generator=g, device=DEV).int()
+    table = torch.full((2, need), -1, dtype=torch.int32, device=DEV)
+    table[0], table[1, :5] = order[:need], order[need:need + 5]
+    k, v = torch.randn(2, sum(lens), heads, dim, generator=g, device=DEV)
+    k[:lens[0], :, 0] = torch.linspace(0, 10, lens[0], device=DEV)[:, None]
+    gpu_kv_cache_append(cache, k.to(dtype), v.to(dtype), table, i32(lens), i32(ends(lens)))
+    kc, vc = (x.double() for x in gpu_kv_cache_read(cache, table, i32(lens), i32(ends(lens)), tokens=sum(lens)))
+    # powers of two of weight over the whole sequence: 200, 40, -90 (the first position leads), 10
+    rate = torch.tensor([200.0, 40.0, -90.0, 10.0], device=DEV) * np.log(2.0) * dim ** 0.5 / 10
+    q = 0.5 * torch.randn(sum(news), heads * share, dim, generator=g, device=DEV)
+    q[:tokens, :, 0] = rate[torch.arange(tokens, device=DEV) // 32 % 4][:, None]
+    q = q.to(dtype)
+    out = gpu_kv_cache_attention(cache, q, table, i32(lens), i32(ends(news)))
+    for _ in range(8):
+        assert torch.equal(gpu_kv_cache_attention(cache, q, table, i32(lens), i32(ends(news))), out)
+    for a, n, la, ln in ((0, news[0], 0, lens[0]), (news[0], news[1], lens[0], lens[1])):
+        want, tol = bounded_attention(q[a:a + n].double(), kc[la:la + ln], vc[la:la + ln], dim ** -0.5, dtype,
+                                      2.0 ** -11 if dtype == torch.bfloat16 else 0.0)
+        off = np.abs(f64(out[a:a + n]) - want)
+        assert (off <= tol).all(), (off / tol).max()
+    assert status() == 0
+
+
 @pytest.mark.gpu
 def test_attention_scales_and_strong_scores():
     """Scores of order 100 (one position takes all), scale 0, negative scale, tiny and huge q."""
