@@ -18,8 +18,13 @@
 // Right operands: q is scaled per row by a power of two into f16's range and
 // split into f16 + f16 where it has more than 11 bits (f32 input); w s is scaled
 // per group by a power of two that follows the largest s met so far, and split
-// into f16 + f16 unless the output is bf16, whose 8 bits one f16 (11 bits)
-// does not disturb.  Everything summed is f32.
+// into f16 + f16 for every output type: what is rounded there is w s c, and the
+// value is what w lo leaves of it, so that beside one strong dimension in a group
+// (-50 among values of order 1) a single f16 was off by several steps of bf16.
+// The split keeps 22 bits of the largest s's weights, and of smaller ones what
+// lies above 2^-25 in its units: an s 2^-13 of the largest keeps about 17 bits, one
+// of 2^-20 about 10, beside the weighted low ends, which are f32.  Everything
+// summed is f32.
 //
 // Softmax: one pass.  Weights are taken relative to a reference m that only
 // moves (rescaling the sums) when a score passes m + 8, so that most tiles
@@ -37,9 +42,9 @@
 // equal calls give equal results.
 //
 // Measured: 64 sequences of up to 16,000 positions, one token, 8 K/V heads of 4
-// query heads of 128, bf16: 4 bits 198 us (3.8 TB/s; floor 118 us at 6.46 TB/s),
-// 8 bits 254 us (5.7 TB/s; floor 222).  One sequence of 500, 12 heads of 64, f32,
-// 8 bits: 10 us, latency.
+// query heads of 128, bf16: 4 bits 212 us (3.6 TB/s; floor 118 us at 6.46 TB/s),
+// 8 bits 278 us (5.2 TB/s; floor 222); with one f16 for w s 197 and 263.  One
+// sequence of 500, 12 heads of 64, f32, 8 bits: 10 us, latency.
 #pragma once
 
 #include <type_traits>
@@ -215,7 +220,6 @@ struct AttConfig {
   static constexpr bool CENTRE = sizeof(T) == 4;
   static constexpr float kMiddle = CENTRE ? (float)(1 << (BITS - 1)) : 0.0f;
   static constexpr float kUnit = CENTRE ? 1.0f : 16777216.0f;
-  static constexpr bool PLO = !std::is_same<T, __nv_bfloat16>::value;
   static constexpr int R = 8 * NT;
   static constexpr int G = D / GROUP;
   static constexpr int kMinBlocks = att_resident(D, NT, sizeof(T));
@@ -635,7 +639,7 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
       // -- output: rows are dimensions, the contraction runs over the positions
 #pragma unroll
       for (int u = 0; u < SUB; ++u) {
-        uint32_t ph[G][NT][2], pl[C::PLO ? G : 1][C::PLO ? NT : 1][2];
+        uint32_t ph[G][NT][2], pl[G][NT][2];
 #pragma unroll
         for (int k = 0; k < G; ++k)
 #pragma unroll
@@ -658,10 +662,8 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
               }
               const uint32_t hi = pack_f16(w0, w1);
               ph[k][x][h] = transpose_8x8(hi);
-              if constexpr (C::PLO) {
-                const float2 f = unpack_f16(hi);
-                pl[k][x][h] = transpose_8x8(pack_f16(w0 - f.x, w1 - f.y));
-              }
+              const float2 f = unpack_f16(hi);
+              pl[k][x][h] = transpose_8x8(pack_f16(w0 - f.x, w1 - f.y));
             }
           }
         // lane's row: position lane % 16, piece lane / 16 of a pair
@@ -693,7 +695,7 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
 #pragma unroll
             for (int x = 0; x < NT; ++x) {
               mma_f16(o[x][mt], A, ph[k][x][0], ph[k][x][1]);
-              if constexpr (C::PLO) mma_f16(o[x][mt], A, pl[k][x][0], pl[k][x][1]);
+              mma_f16(o[x][mt], A, pl[k][x][0], pl[k][x][1]);
             }
           }
         }

@@ -492,13 +492,15 @@ def test_prompt_shares_with_missing_pages_and_nan(dtype):
     assert status() == 0
 
 
-def bounded_attention(q, k, v, scale, dtype, operand):
+def bounded_attention(q, k, v, scale, dtype, operand, parts=None):
     """(want, bound of |out - want|) of q [n, heads, D], the last n of k, v [len,
     kv_heads, D], all f64 on the GPU.  With r the half step of the operands that K,
     V and the weights pass through (f16: 2^-11; 0 where they keep f32's bits) and
     32-bit sums of D products, a score is off by e = (r + D 2^-24) sum |q k| scale
     and its weight by exp(e) - 1; a weight and a value are off by r, an exponential
-    by 2^-20, and n weighted values in 32 bits by n 2^-24 of their largest sum."""
+    by 2^-20, and n weighted values in 32 bits by n 2^-24 of their largest sum
+    (parts: what is summed in a value's place, where that is larger: its scaled
+    code and its group's low end, with weights split at 2^-22)."""
     n, hq, D = q.shape
     length, hk = k.shape[:2]
     q, k, v = q.transpose(0, 1), *(x.transpose(0, 1).repeat_interleave(hq // hk, 0) for x in (k, v))
@@ -512,6 +514,8 @@ def bounded_attention(q, k, v, scale, dtype, operand):
     off = e.sum(-1, keepdim=True)
     assert off.max() < 0.5
     far = p @ v.abs() * (operand + length * 2.0 ** -24)
+    if parts is not None:
+        far += p @ parts.transpose(0, 1).repeat_interleave(hq // hk, 0) * (2.0 ** -22 + length * 2.0 ** -24)
     tol = (e @ v.abs() + off * want.abs() + far) / (1 - off) + v.abs().max() * length * 2.0 ** -39
     want, tol = (x.transpose(0, 1).cpu().numpy() for x in (want, tol))
     return want, ref.rounding(want, tol, dtype)
@@ -550,6 +554,33 @@ def test_prompt_rows_that_fill_the_gpu(dim, bits, tokens, dtype):
                                       2.0 ** -11 if dtype == torch.bfloat16 else 0.0)
         off = np.abs(f64(out[a:a + n]) - want)
         assert (off <= tol).all(), (off / tol).max()
+    assert status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,bits,group", [(64, 8, 64), (128, 4, 64), (128, 8, 32), (256, 8, 64)])
+def test_attention_beside_a_strong_dimension(dim, bits, group, dtype):
+    """One dimension of -50 in each group of V: the group's low end is far from the
+    other values, which keep their bits all the same."""
+    lens, heads, share = [40, 7, 33], 2, 3
+    g = torch.Generator(DEV).manual_seed(dim + bits)
+    cache = KvCache(16, 16, heads, dim, bits, group, DEV)
+    table = torch.randperm(16, generator=g, device=DEV).int()[:9].view(3, 3)
+    k, v = torch.randn(2, sum(lens), heads, dim, generator=g, device=DEV)
+    v[..., 5::group] = -50
+    gpu_kv_cache_append(cache, k.to(dtype), v.to(dtype), table, i32(lens), i32(ends(lens)))
+    kc, vc = (x.double() for x in gpu_kv_cache_read(cache, table, i32(lens), i32(ends(lens)), tokens=sum(lens)))
+    low = vc.unflatten(-1, (-1, group)).amin(-1).repeat_interleave(group, -1)
+    for news in ([1, 1, 1], [5, 7, 2]):
+        q = (2 * torch.randn(sum(news), heads * share, dim, generator=g, device=DEV)).to(dtype)
+        out = gpu_kv_cache_attention(cache, q, table, i32(lens), i32(ends(news)))
+        for b, n in enumerate(news):
+            a, la, le = ends(news)[b], ends(lens)[b], ends(lens)[b + 1]
+            want, tol = bounded_attention(q[a:a + n].double(), kc[la:le], vc[la:le], dim ** -0.5, dtype, 0.0,
+                                          low[la:le].abs() + (vc - low)[la:le])
+            off = np.abs(f64(out[a:a + n]) - want)
+            assert (off <= tol).all(), (off / tol).max()
     assert status() == 0
 
 
