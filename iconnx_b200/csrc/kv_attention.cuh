@@ -23,8 +23,16 @@
 // (-50 among values of order 1) a single f16 was off by several steps of bf16.
 // The split keeps 22 bits of the largest s's weights, and of smaller ones what
 // lies above 2^-25 in its units: an s 2^-13 of the largest keeps about 17 bits, one
-// of 2^-20 about 10, beside the weighted low ends, which are f32.  Everything
-// summed is f32.
+// of 2^-20 about 10, beside the weighted low ends, which are f32.
+//
+// Sums: f32, but matrix units cut off what falls below an f32 sum's last bit
+// instead of rounding it, and sums of codes only grow, so that over a warp's share
+// of thousands of positions they drifted (9 tokens of each of 115 sequences of up
+// to 10,500: f16 outputs off by 1.28e-3 of their norm, where their own rounding is
+// 2.07e-4; f32 2.6e-5).  So matrix units sum pieces of 8 steps, and the pieces are
+// added in rounded f32 (2.30e-4; 1.3e-6; pieces of 4: 2.26e-4, 1.0e-6).  Earlier
+// pieces stand in shared memory, whose third ring stage was worth nothing; in local
+// memory, which misses L1, pieces of 8 cost 92 us where they cost 8 now.
 //
 // Softmax: one pass.  Weights are taken relative to a reference m that only
 // moves (rescaling the sums) when a score passes m + 8, so that most tiles
@@ -42,9 +50,9 @@
 // equal calls give equal results.
 //
 // Measured: 64 sequences of up to 16,000 positions, one token, 8 K/V heads of 4
-// query heads of 128, bf16: 4 bits 212 us (3.6 TB/s; floor 118 us at 6.46 TB/s),
-// 8 bits 278 us (5.2 TB/s; floor 222); with one f16 for w s 197 and 263.  One
-// sequence of 500, 12 heads of 64, f32, 8 bits: 10 us, latency.
+// query heads of 128, bf16: 4 bits 220 us (3.5 TB/s; floor 118 us at 6.46 TB/s),
+// 8 bits 292 us (4.9 TB/s; floor 222); 212 and 278 in one sum, 197 and 263 with one
+// f16 for w s besides.  One sequence of 500, 12 heads of 64, f32, 8 bits: 10 us, latency.
 #pragma once
 
 #include <type_traits>
@@ -233,10 +241,18 @@ struct AttConfig {
   static constexpr int kTile = 2 * (kCodes + kParams), kStage = SUB * kTile;
   // a warp's query operand
   static constexpr int kQBytes = kQReg ? 0 : NT * (D / 16) * (QLO ? 2 : 1) * 32 * 8;
-  static constexpr int kFit = ((kMinBlocks == 2 ? 108 : 220) * 1024 / kAttWarps - kQBytes) / kStage;
+  // a warp's sums of earlier pieces, in shared memory where that leaves two
+  // stages (not beside 256 dimensions of 8 bits: local memory and larger pieces;
+  // 32 sequences of up to 16,000, 8 K/V heads of 4 query heads: 236 -> 272 us)
+  static constexpr int kRoom = (kMinBlocks == 2 ? 108 : 220) * 1024 / kAttWarps - kQBytes;
+  static constexpr bool kSharedSums = kRoom - R * D * 4 >= 2 * kStage;
+  static constexpr int kSumBytes = kSharedSums ? R * D * 4 : 0;
+  static constexpr int kPiece = kSharedSums ? 8 : 32;   // steps
+  static constexpr int kFit = (kRoom - kSumBytes) / kStage;
   static constexpr int kStages = kFit > 4 ? 4 : kFit < 2 ? 2 : kFit;
   static constexpr int kRing = kAttWarps * kStages * kStage;
-  static constexpr int kSmem = kRing + kAttWarps * kQBytes;
+  static constexpr int kSums = kRing + kAttWarps * kQBytes;   // where the sums stand
+  static constexpr int kSmem = kSums + kAttWarps * kSumBytes;
   static_assert(kSmem * kMinBlocks <= 224 * 1024, "shared memory");
 };
 
@@ -444,6 +460,15 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
     // -------------------------------------------------------- running sums
     float o[NT][MT][4] = {};
     float m[NT][2], l[NT][2], vlo[NT][G][2];
+    float4 local_sums[C::kSharedSums ? 1 : NT * MT];
+    // the sums of the pieces before this one, [NT][MT], own lane's
+    constexpr int kNext = C::kSharedSums ? 32 : 1;
+    float4* sums = C::kSharedSums ? reinterpret_cast<float4*>(smem + C::kSums + warp * C::kSumBytes) + lane : local_sums;
+    bool pieces = false;   // whether there are any
+    auto scale_sums = [&](int i, int n, float f0, float f1) {   // columns 2t and 2t + 1
+#pragma unroll 1
+      for (float4* v = sums + i * kNext; n > 0; --n, v += kNext) *v = make_float4(v->x * f0, v->y * f1, v->z * f0, v->w * f1);
+    };
 #pragma unroll
     for (int x = 0; x < NT; ++x)
 #pragma unroll
@@ -565,7 +590,8 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
         }
       if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
-        for (int x = 0; x < NT; ++x)
+        for (int x = 0; x < NT; ++x) {
+          float moved[2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float v = top[x][h];
@@ -575,6 +601,7 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
             v = fmaxf(v, m[x][h]);
             const float f = ex2((m[x][h] - v) * qf[x][h]);
             m[x][h] = v;
+            moved[h] = f;
             l[x][h] *= f;
 #pragma unroll
             for (int k = 0; k < G; ++k) vlo[x][k][h] *= f;
@@ -584,6 +611,8 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
               o[x][i][2 + h] *= f;
             }
           }
+          if (pieces) scale_sums(x * MT, MT, moved[0], moved[1]);
+        }
       }
 #pragma unroll
       for (int x = 0; x < NT; ++x)
@@ -634,6 +663,9 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
             for (int i = 0; i < GROUP / 16; ++i)
 #pragma unroll
               for (int q = 0; q < 4; ++q) o[x][k * (GROUP / 16) + i][q] *= f;
+          if (pieces)
+#pragma unroll
+            for (int x = 0; x < NT; ++x) scale_sums(x * MT + k * (GROUP / 16), GROUP / 16, f, f);
         }
       }
       // -- output: rows are dimensions, the contraction runs over the positions
@@ -717,6 +749,32 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
         }
       }
       stage = stage + 1 == C::kStages ? 0 : stage + 1;
+      if (((pos - p0) / kStep & (C::kPiece - 1)) == C::kPiece - 1) {   // the end of a piece
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            float(&v)[4] = o[x][i];
+            float4& sum = sums[(x * MT + i) * kNext];
+            if (pieces) sum = make_float4(sum.x + v[0], sum.y + v[1], sum.z + v[2], sum.w + v[3]);
+            else sum = make_float4(v[0], v[1], v[2], v[3]);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = 0.0f;
+          }
+        pieces = true;
+      }
+    }
+    if (pieces) {
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const float4 sum = sums[(x * MT + i) * kNext];
+          o[x][i][0] += sum.x;
+          o[x][i][1] += sum.y;
+          o[x][i][2] += sum.z;
+          o[x][i][3] += sum.w;
+        }
     }
 
     // ---------------------------------------------- join lanes, and write

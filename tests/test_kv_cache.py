@@ -585,6 +585,46 @@ def test_attention_beside_a_strong_dimension(dim, bits, group, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,bits,group,news,batch", [(64, 4, 64, 1, 600), (128, 8, 32, 1, 300), (64, 8, 64, 9, 100),
+                                                       (256, 4, 64, 1, 300), (256, 8, 64, 1, 300)])
+def test_attention_sums_of_long_sequences(dim, bits, group, news, batch, dtype):
+    """Many sequences over the pages of one (a warp's share is thousands of
+    positions), values around zero whose average is small beside them: matrix units
+    cut what falls off the end of a sum, always towards zero, so that one sum over
+    a whole share would drift by its number of products."""
+    length, heads, share, page = 12000, 4, 4, 64
+    g = torch.Generator(DEV).manual_seed(dim + bits)
+    need = -(-length // page)
+    cache = KvCache(need, page, heads, dim, bits, group, DEV)
+    table = torch.randperm(need, generator=g, device=DEV).int()[None]
+    k, v = torch.randn(2, length, heads, dim, generator=g, device=DEV)
+    gpu_kv_cache_append(cache, k.to(dtype), v.to(dtype), table, i32([length]), i32([0, length]))
+    kc, vc = (x.double() for x in gpu_kv_cache_read(cache, table, i32([length]), i32([0, length]), tokens=length))
+    q = torch.randn(batch * news, heads * share, dim, generator=g, device=DEV).to(dtype)
+    out = gpu_kv_cache_attention(cache, q, table.expand(batch, -1), i32([length] * batch),
+                                 i32(ends([news] * batch)))
+    low = vc.unflatten(-1, (-1, group)).amin(-1).repeat_interleave(group, -1)
+    parts = (low.abs() + (vc - low)).mean(0).amax()
+    drift = []
+    for b in range(0, batch, 7):
+        want, tol = bounded_attention(q[b * news:(b + 1) * news].double(), kc, vc, dim ** -0.5, dtype, 0.0,
+                                      low.abs() + (vc - low))
+        off = f64(out[b * news:(b + 1) * news]) - want
+        assert (np.abs(off) <= tol).all(), (np.abs(off) / tol).max()
+        drift.append(off.mean())
+    # At most 64 products (32 steps of two parts) in a piece, each cutting up to
+    # 2^-23 of the piece's sum and so 2^-24 of it on average over its growth (which
+    # the last of them sees whole: 64 2^-24), and rounding errors, which have no
+    # side: half a step of outputs up to 2^-2 (of 2^-24 parts in f32), averaged
+    n = batch // 7 * news * heads * share * dim
+    side = max(2.0 ** -2 * ref.HALF_STEP[dtype], parts.item() * length ** 0.5 * 2.0 ** -24)
+    limit = 64 * 2.0 ** -24 * parts.item() + 5 * side / n ** 0.5
+    assert abs(np.mean(drift)) <= limit, (np.mean(drift), limit)
+    assert status() == 0
+
+
+@pytest.mark.gpu
 def test_attention_scales_and_strong_scores():
     """Scores of order 100 (one position takes all), scale 0, negative scale, tiny and huge q."""
     for spread, q_scale, scale in ((4.0, 4.0, 0.5), (1.0, 1.0, 0.0), (1.0, 1.0, -0.3), (1.0, 1e-6, None),
