@@ -10,6 +10,14 @@
 // memory, scaled and joined in registers.  w s is rounded to two f16 (an f16
 // output has as many bits as one; bf16 outputs take kv_prompt_bf16.cu).
 //
+// Matrix units cut off what falls below an f32 sum's last bit instead of rounding
+// it, and sums of codes only grow: in one sum over 16,000 positions they drifted by
+// 2.2e-3 of the output's norm (8 bits: 3.6e-3), where f16's rounding is 2.1e-4.  So
+// tensor memory sums pieces of 8 tiles, which the softmax warps add in rounded f32
+// (3.0e-4; 3.1e-4; pieces of 16: 4.0e-4 and 5.8e-4).  128 rows' earlier pieces are
+// 64 KB, which neither tensor nor shared memory has left: they stand in local
+// memory, and cost 821 -> 916 us where 916 is stated below (pieces of 16: 899).
+//
 // A CTA takes 128 query rows of one (sequence, K/V head), 64 positions at a
 // time; two CTAs share an SM, so that one's softmax runs beside the other's
 // matrix instructions:
@@ -24,12 +32,14 @@
 //               stands, position by position: MN-major).
 // Bound by the softmax warps (about ten instructions per score, pairs of f32 in
 // one) beside the tensor cores.  1024 tokens of each of 2 sequences of up to 6,000,
-// 8 K/V heads of 4 query heads of 128, 4 bits: 820 us (floor 73 at 1.72 PFLOP/s,
+// 8 K/V heads of 4 query heads of 128, 4 bits: 916 us (floor 73 at 1.72 PFLOP/s,
 // with one f16 for each operand).
 #include "kv_prompt.cuh"
 #include "tmap.cuh"
 
 namespace icx {
+
+constexpr int kPrPiece = 8;   // tiles whose products are summed in tensor memory
 
 template <int D>
 struct PromptConfig {
@@ -142,7 +152,7 @@ __global__ void __launch_bounds__(kPrThreads, 2)
 #pragma unroll
             for (int n = 0; n < kPrKeys / 16; ++n)
               mma_f16_ts(t_o + k * kPrGroup, t_s + (lo * G + k) * (kPrKeys / 2) + n * 8, b + (uint64_t)(n * 128), id_o,
-                         i > 0 || lo > 0 || n > 0);
+                         i % kPrPiece > 0 || lo > 0 || n > 0);
         }
       };
       bool ok = true;
@@ -261,6 +271,11 @@ __global__ void __launch_bounds__(kPrThreads, 2)
       float m = kNoScore, l = 0.0f, vlo[G];
 #pragma unroll
       for (int k = 0; k < G; ++k) vlo[k] = 0.0f;
+      // the output's sums of the pieces before this one, times kept_by
+      alignas(16) float kept[D];   // (local memory: 128 rows take 64 KB)
+      float kept_by[G];
+#pragma unroll
+      for (int k = 0; k < G; ++k) kept_by[k] = 1.0f;
       bool ok = true;
       for (int i = 0; i < tiles; ++i) {
         const int st = i & 1;
@@ -319,7 +334,10 @@ __global__ void __launch_bounds__(kPrThreads, 2)
           m = nm;
           l *= alpha;
 #pragma unroll
-          for (int k = 0; k < G; ++k) vlo[k] *= alpha;
+          for (int k = 0; k < G; ++k) {
+            vlo[k] *= alpha;
+            kept_by[k] *= alpha * s_fix[st * 2 + k];
+          }
           if (i > 0) {   // before the first tile's product there is no output
 #pragma unroll 1
             for (int n = 0; n < D; n += 32) {
@@ -331,6 +349,26 @@ __global__ void __launch_bounds__(kPrThreads, 2)
               for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * g);
               tmem_st_32x32b_x32(t_o + (uint32_t)n, x);
             }
+          }
+        }
+        // -- the end of a piece: the next product starts its sum anew
+        if (i > 0 && i % kPrPiece == 0) {
+#pragma unroll
+          for (int k = 0; k < G; ++k) {
+#pragma unroll 1
+            for (int n = k * kPrGroup; n < (k + 1) * kPrGroup; n += 16) {
+              uint32_t x[16];
+              tmem_ld_32x32b_x16(t_o + (uint32_t)n, x);
+              tmem_ld_wait_regs16(x);
+#pragma unroll
+              for (int j = 0; j < 16; j += 4) {
+                float4* sum = reinterpret_cast<float4*>(kept + n + j);
+                const float4 old = i > kPrPiece ? *sum : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                *sum = make_float4(fmaf(old.x, kept_by[k], __uint_as_float(x[j])), fmaf(old.y, kept_by[k], __uint_as_float(x[j + 1])),
+                                   fmaf(old.z, kept_by[k], __uint_as_float(x[j + 2])), fmaf(old.w, kept_by[k], __uint_as_float(x[j + 3])));
+              }
+            }
+            kept_by[k] = 1.0f;
           }
         }
         // -- weights, and w s as the left operand over the accumulators
@@ -407,15 +445,23 @@ __global__ void __launch_bounds__(kPrThreads, 2)
         for (int k = 0; k < G; ++k) {
           const float vd = tiles > 0 ? s_fix[12 + ((tiles - 1) & 1) * 2 + k] : 0.0f;
           const float up = vd > 0.0f ? 1.0f / vd : 0.0f;
-          float low = vlo[0];
+          float low = vlo[0], by = kept_by[0];
 #pragma unroll
-          for (int kk = 1; kk < G; ++kk) low = k == kk ? vlo[kk] : low;
+          for (int kk = 1; kk < G; ++kk) {
+            low = k == kk ? vlo[kk] : low;
+            by = k == kk ? kept_by[kk] : by;
+          }
 #pragma unroll 1
           for (int n = 0; n < 2; ++n) {   // dimensions 32 n .. 32 n + 31 of the group
             uint32_t x[32];
             if (tiles > 0) {
               tmem_ld_32x32b_x32(t_o + (uint32_t)(k * kPrGroup + 32 * n), x);
               tmem_ld_wait_regs(x);
+            }
+            if (tiles > kPrPiece) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                x[j] = __float_as_uint(fmaf(kept[k * kPrGroup + 32 * n + j], by, __uint_as_float(x[j])));
             }
             float y[4][8];
 #pragma unroll

@@ -589,10 +589,22 @@ def test_attention_beside_a_strong_dimension(dim, bits, group, dtype):
 @pytest.mark.parametrize("dim,bits,group,news,batch", [(64, 4, 64, 1, 600), (128, 8, 32, 1, 300), (64, 8, 64, 9, 100),
                                                        (256, 4, 64, 1, 300), (256, 8, 64, 1, 300)])
 def test_attention_sums_of_long_sequences(dim, bits, group, news, batch, dtype):
-    """Many sequences over the pages of one (a warp's share is thousands of
-    positions), values around zero whose average is small beside them: matrix units
-    cut what falls off the end of a sum, always towards zero, so that one sum over
-    a whole share would drift by its number of products."""
+    """Many sequences over the pages of one: a warp's share is thousands of positions."""
+    check_long_sums(dim, bits, group, news, batch, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim,bits", [(64, 4), (64, 8), (128, 4), (128, 8)])
+def test_prompt_sums_of_long_sequences(dim, bits, dtype):
+    """Enough rows that each reads its thousands of positions in one share."""
+    check_long_sums(dim, bits, 64, 400, 12, dtype, 2.0 ** -11 if dtype == torch.bfloat16 else 0.0)
+
+
+def check_long_sums(dim, bits, group, news, batch, dtype, operand=0.0):
+    """Values around zero whose average is small beside them: matrix units cut what
+    falls off the end of a sum, always towards zero, so that one sum over all the
+    positions would drift by its number of products."""
     length, heads, share, page = 12000, 4, 4, 64
     g = torch.Generator(DEV).manual_seed(dim + bits)
     need = -(-length // page)
@@ -608,16 +620,17 @@ def test_attention_sums_of_long_sequences(dim, bits, group, news, batch, dtype):
     parts = (low.abs() + (vc - low)).mean(0).amax()
     drift = []
     for b in range(0, batch, 7):
-        want, tol = bounded_attention(q[b * news:(b + 1) * news].double(), kc, vc, dim ** -0.5, dtype, 0.0,
+        want, tol = bounded_attention(q[b * news:(b + 1) * news].double(), kc, vc, dim ** -0.5, dtype, operand,
                                       low.abs() + (vc - low))
         off = f64(out[b * news:(b + 1) * news]) - want
         assert (np.abs(off) <= tol).all(), (np.abs(off) / tol).max()
         drift.append(off.mean())
-    # At most 64 products (32 steps of two parts) in a piece, each cutting up to
-    # 2^-23 of the piece's sum and so 2^-24 of it on average over its growth (which
-    # the last of them sees whole: 64 2^-24), and rounding errors, which have no
-    # side: half a step of outputs up to 2^-2 (of 2^-24 parts in f32), averaged
-    n = batch // 7 * news * heads * share * dim
+    # At most 64 products (32 steps of two parts; 8 tiles of 64 positions in two
+    # parts) in a piece, each cutting up to 2^-23 of the piece's sum and so 2^-24 of
+    # it on average over its growth (which the last of them sees whole: 64 2^-24),
+    # and rounding errors, which have no side: half a step of outputs up to 2^-2 (of
+    # 2^-24 parts in f32), averaged
+    n = len(drift) * news * heads * share * dim
     side = max(2.0 ** -2 * ref.HALF_STEP[dtype], parts.item() * length ** 0.5 * 2.0 ** -24)
     limit = 64 * 2.0 ** -24 * parts.item() + 5 * side / n ** 0.5
     assert abs(np.mean(drift)) <= limit, (np.mean(drift), limit)
