@@ -37,8 +37,11 @@ __device__ __forceinline__ uint32_t smem_addr(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
 
+// The first code stays, but a bad page (a caller's mistake, nothing touched)
+// gives way to a wait that gave up, whose results are not whole.
 __device__ __forceinline__ void record_status(int code) {
-  atomicCAS(&g_icx_device_status, 0, code);
+  if (atomicCAS(&g_icx_device_status, 0, code) == ICX_DEVICE_BAD_PAGE)
+    atomicCAS(&g_icx_device_status, ICX_DEVICE_BAD_PAGE, code);
 }
 
 // ----------------------------------------------------------------- mbarrier

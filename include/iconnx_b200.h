@@ -79,8 +79,10 @@ ICX_API const char* icx_last_error(void);
 /* Library version string. */
 ICX_API const char* icx_version(void);
 
-/* Reads and clears the device-side status word of `device` (0 = no kernel
- * gave up on a bounded wait since the last call). */
+/* Reads and clears the device-side status word of `device`: 0 where no kernel
+ * has recorded anything since the last call, else the first code recorded, but
+ * an ICX_DEVICE_TIMEOUT_* (a kernel gave up on a bounded wait, and its results
+ * are not whole) before ICX_DEVICE_BAD_PAGE. */
 ICX_API int icx_device_status(int device, int* status_out);
 
 /* Self-test of the kernels' failure handling (no reference counterpart; the

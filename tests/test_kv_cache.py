@@ -276,6 +276,28 @@ def test_unusable_pages_are_skipped_and_noted():
         assert (np.abs(got[b] - want[0]) <= tol[0]).all()
 
 
+@pytest.mark.gpu
+def test_a_bad_page_does_not_hide_a_wait_that_gave_up():
+    L, timeout = _lib.load(), 0x1ff
+    c = KvCache(4, 16, 2, 64, device=DEV)
+    k = torch.zeros(1, 2, 64, device=DEV)
+
+    def bad_page():
+        gpu_kv_cache_append(c, k, k, i32([[-1]]), i32([1]))
+
+    def wait():   # a bounded wait that nothing ends, 1 ms
+        assert L.icx_selftest_bounded_wait(torch.cuda.current_stream(DEV).cuda_stream, 1_000_000) == 0
+
+    status()
+    for steps, want in (((bad_page,), _lib.ICX_DEVICE_BAD_PAGE), ((bad_page, wait), timeout), ((wait, bad_page), timeout),
+                        ((bad_page, wait, bad_page), timeout)):
+        for step in steps:
+            step()
+        torch.cuda.synchronize()
+        assert status() == want
+        assert status() == 0
+
+
 # --------------------------------------------------------------- attention
 def check_attention(c, news, q_heads, dtype, scale=None, seed=0, q_scale=1.0, pad=0):
     lens, D = c.lens, c.cache.head_dim
