@@ -674,14 +674,15 @@ static int make_out_map(CUtensorMap* map, void* out, int M, int N) {
   return ICX_OK;
 }
 
-// CTA pairs of a kernel that can be resident at once (per device).
+// CTA pairs of a kernel that can be resident at once (per device; callers on
+// several threads store the same number).
 template <typename T, int BN>
 static int max_pairs() {
-  static int cached[64] = {};
+  static std::atomic<int> cached[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return 0;
-  if (cached[dev]) return cached[dev];
+  if (const int known = cached[dev].load(std::memory_order_relaxed)) return known;
   using C = RowsConfig<BN, 2>;
   auto kern = scaled_rows_kernel<T, BN, 2>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess) return 0;
@@ -701,7 +702,7 @@ static int max_pairs() {
     cudaGetLastError();
     return 0;
   }
-  cached[dev] = n;
+  cached[dev].store(n, std::memory_order_relaxed);
   return n;
 }
 

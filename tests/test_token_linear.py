@@ -2,6 +2,7 @@
 implementation.  Codes and scales are bit-exact; the product's tolerance is
 derived from its roundings."""
 import ctypes
+from concurrent.futures import ThreadPoolExecutor
 
 import numpy as np
 import pytest
@@ -304,6 +305,27 @@ def test_unaligned_operands():
         a, b = ops.gpu_quantize_per_token(x.to(dt)), ops.gpu_quantize_per_token(
             torch.cat([torch.zeros(1, device=DEV, dtype=dt), x.to(dt).flatten()])[1:].view(3, 70))
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.gpu
+def test_calls_from_several_threads():
+    """The first calls that need a kernel's limits, from threads at once."""
+    M, K, N = 2048, 64, 512
+    g = torch.Generator(DEV).manual_seed(3)
+    q = torch.randint(-9, 10, (M, K), generator=g, device=DEV, dtype=torch.int8)
+    w = torch.randint(-9, 10, (K, N), generator=g, device=DEV, dtype=torch.int8)
+    pw, one, ws = ops.prepare_weight(w), torch.ones(M, device=DEV), torch.ones(N, device=DEV)
+    want = q.float() @ w.float()   # at most 64 * 81
+    torch.cuda.synchronize()
+
+    def call(i):
+        with torch.cuda.stream(torch.cuda.Stream(DEV)):
+            out = ops.gpu_matmul_integer_scaled(q, one, pw, ws, out_dtype=TYPES[i % 2])
+            torch.cuda.current_stream(DEV).synchronize()
+            return torch.equal(out.float(), want.to(TYPES[i % 2]).float())
+
+    with ThreadPoolExecutor(8) as pool:
+        assert all(pool.map(call, range(32)))
 
 
 @pytest.mark.gpu
