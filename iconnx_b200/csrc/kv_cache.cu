@@ -34,7 +34,9 @@ int kv_views(const char* what, const icx_kv_cache* c, const icx_kv_tokens* w, Kv
   ICX_REQUIRE(w->batch >= 0 && w->batch < (1 << 20) && w->table_width >= 0 && w->tokens >= 0 &&
                   w->tokens < (1ll << 31),
               "%s: batch, table width or tokens out of range", what);
-  ICX_REQUIRE((int64_t)w->table_width << shift < (1ll << 31), "%s: page table row beyond 2^31 positions", what);
+  // kernels look up to 1024 positions ahead of the last in 32 bits
+  ICX_REQUIRE((int64_t)w->table_width << shift <= (1ll << 31) - 4096,
+              "%s: page table row beyond 2^31 - 4096 positions", what);
   ICX_REQUIRE(w->d_cu_tokens || w->tokens == w->batch,
               "%s: without cu_tokens there is one token per sequence (%lld tokens, batch %d)", what,
               (long long)w->tokens, w->batch);

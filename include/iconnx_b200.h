@@ -316,7 +316,8 @@ typedef struct icx_kv_cache {
  * cu_tokens[b+1]-1 of the packed operands and stand at its last positions.
  * d_cu_tokens (s32 [batch + 1]) may be NULL: one token per sequence.  Rows
  * outside [cu_tokens[0], cu_tokens[batch]) are left as they were.  All
- * index arrays are s32 on the device; page_table is [batch, table_width]. */
+ * index arrays are s32 on the device; page_table is [batch, table_width], and
+ * table_width * page_size at most 2^31 - 4096. */
 typedef struct icx_kv_tokens {
   const int32_t* d_page_table;
   const int32_t* d_seq_lens;

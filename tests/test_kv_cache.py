@@ -90,6 +90,20 @@ def test_refusals_before_any_launch(over, text):
         assert re.search(text, L.icx_last_error()), L.icx_last_error()
 
 
+@pytest.mark.parametrize("page", [16, 64, 1024])
+def test_page_tables_whose_last_positions_pass_32_bits_are_refused(page):
+    L, p = _lib.load(), ctypes.c_void_p(64)
+    for width in ((1 << 31) // page, (1 << 31) // page - 1, ((1 << 31) - 4096) // page + 1):
+        c, w = (ctypes.byref(a) for a in c_args(page_size=page, table_width=width))
+        for rc in (L.icx_kv_cache_append(None, c, w, p, p, 3, 64, 64, 64, 64, None, None),
+                   L.icx_kv_cache_read(None, c, w, 3, p, p),
+                   L.icx_kv_cache_attention(None, c, w, p, 3, 2, 128, 64, 1.0, p, None, 0)):
+            assert rc == -1 and b"2^31 - 4096" in L.icx_last_error()
+    # the widest table, of an empty call
+    c, w = (ctypes.byref(a) for a in c_args(page_size=page, table_width=((1 << 31) - 4096) // page, tokens=0, batch=0))
+    assert L.icx_kv_cache_read(None, c, w, 3, p, p) == 0
+
+
 def test_operand_refusals_before_any_launch():
     L = _lib.load()
     p = ctypes.c_void_p(64)
