@@ -42,6 +42,8 @@ class KvCache:
     over 2^bits - 1 rounded up, and codes are rounded half to even.  A group
     with a NaN or an infinity reads back as NaN.  ``page_size`` is a power of
     two in 16..1024, ``head_dim`` 64, 128 or 256.  A new pool is all zeros.
+    ``k_codes``, ``v_codes``, ``k_params`` and ``v_params`` are its buffers, to be
+    copied from and into (saving and restoring a pool), not to be replaced.
     """
 
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, bits: int = 4,
@@ -66,14 +68,19 @@ class KvCache:
         rows = (pages, kv_heads, page_size)
         codes = (*rows, head_dim * bits // 8)
         params = (*rows, head_dim // group)
-        self.k_codes = torch.zeros(codes, dtype=torch.uint8, device=device)
-        self.v_codes = torch.zeros(codes, dtype=torch.uint8, device=device)
-        self.k_params = torch.zeros(params, dtype=torch.int32, device=device)
-        self.v_params = torch.zeros(params, dtype=torch.int32, device=device)
-        self.device = self.k_codes.device
-        self._arg = KvCacheArg(self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.k_params.data_ptr(),
-                               self.v_params.data_ptr(), pages, page_size, kv_heads, head_dim, bits, group)
+        self._buffers = [torch.zeros(shape, dtype=dtype, device=device)
+                         for shape, dtype in ((codes, torch.uint8),) * 2 + ((params, torch.int32),) * 2]
+        self.device = self._buffers[0].device
+        self._arg = KvCacheArg(*(t.data_ptr() for t in self._buffers), pages, page_size, kv_heads, head_dim, bits,
+                               group)
         self._ref = ctypes.byref(self._arg)
+
+    # The calls take the buffers' addresses from _arg, so they stay the same
+    # tensors for the pool's life.
+    k_codes = property(lambda self: self._buffers[0])
+    v_codes = property(lambda self: self._buffers[1])
+    k_params = property(lambda self: self._buffers[2])
+    v_params = property(lambda self: self._buffers[3])
 
 
 def _index(t, shape, device, what: str) -> torch.Tensor:

@@ -127,6 +127,27 @@ def test_operand_refusals_before_any_launch():
             KvCache(**(dict(pages=4, page_size=16, kv_heads=2, head_dim=64) | kw))
 
 
+@pytest.mark.parametrize("name", ["k_codes", "v_codes", "k_params", "v_params"])
+def test_buffers_of_a_pool_cannot_be_replaced(name):
+    """The calls keep their addresses: another tensor would not be used, and the
+    one it replaces would be freed under them."""
+    cache = object.__new__(KvCache)
+    with pytest.raises(AttributeError):
+        setattr(cache, name, torch.zeros(1))
+
+
+@pytest.mark.gpu
+def test_restored_pool_reads_the_same():
+    c = Case([50, 20], seed=41)
+    args = c.table, i32(c.lens), i32(ends(c.lens))
+    want = gpu_kv_cache_read(c.cache, *args, tokens=70)
+    other = KvCache(c.cache.pages, 16, 2, 64, 4, 64, DEV)
+    for name in ("k_codes", "v_codes", "k_params", "v_params"):
+        getattr(other, name).copy_(getattr(c.cache, name))
+    got = gpu_kv_cache_read(other, *args, tokens=70)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 @pytest.mark.gpu
 def test_python_refusals():
     c = KvCache(4, 16, 2, 64, device=DEV)
