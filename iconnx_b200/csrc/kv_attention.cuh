@@ -207,6 +207,13 @@ __device__ __forceinline__ void load_transposed(uint32_t addr, uint32_t (&r)[4])
                : "memory");
 }
 
+// The factor from products of a row scaled by 2^e with codes that count 1 / unit
+// to scores in powers of two: above 0, which a masked score's -infinity must not
+// meet (below f32's normal numbers all weights are equal anyway).
+__device__ __forceinline__ float score_factor(float scale, float unit, int e) {
+  return scale != 0.0f ? fmaxf(fabsf(scale) * unit * __uint_as_float((uint32_t)(127 - e) << 23), 1.17549435e-38f) : 1.0f;
+}
+
 // Two codes as f16 for a matrix operand: as they stand (subnormals), or as numbers
 // around zero: 1024 + code less 1024 + middle.  HIGH: in bits 4..7, sixteen times.
 template <bool CENTRE, int BITS, bool HIGH>
@@ -437,7 +444,7 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
           }
         }
       }
-      const float f = a.scale != 0.0f ? fabsf(a.scale) * C::kUnit * __uint_as_float((uint32_t)(127 - e) << 23) : 1.0f;
+      const float f = score_factor(a.scale, C::kUnit, e);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int from = (2 * t + h) * 4;   // a lane that holds column 2t + h

@@ -176,7 +176,7 @@ __device__ __forceinline__ void put_query(const AttendArgs& a, const T* q, bool 
   }
   const int e = mine && peak > 0.0f ? max(-60, min(120, 14 - (int)((__float_as_uint(peak) >> 23) & 255) + 127)) : 0;
   const float up = mine && a.scale != 0.0f ? copysignf(__uint_as_float((uint32_t)(e + 127) << 23), a.scale) : 0.0f;
-  *f = a.scale != 0.0f ? fabsf(a.scale) * (CODES ? 16777216.0f : 1.0f) * __uint_as_float((uint32_t)(127 - e) << 23) : 1.0f;
+  *f = score_factor(a.scale, CODES ? 16777216.0f : 1.0f, e);
 #pragma unroll 1
   for (int k = G - 1; k >= 0; --k) {   // the last group is there
     if (k < G - 1) fetch(k);

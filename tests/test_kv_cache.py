@@ -704,6 +704,17 @@ def test_attention_scales_and_strong_scores():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("q_scale,scale", [(1.0, 1e-44), (1e-30, 1e-25)])
+def test_attention_of_scores_that_vanish(q_scale, scale, dtype):
+    """A scale and queries so small that their product is below f32: the average
+    of the positions that a row sees."""
+    c = Case([77, 400, 3], 2, 128, 4, 64, 16, dtype, seed=34)
+    check_attention(c, [1, 1, 1], 4, dtype, scale, seed=5, q_scale=q_scale)
+    check_attention(c, [70, 130, 3], 4, dtype, scale, seed=6, q_scale=q_scale)
+
+
+@pytest.mark.gpu
 def test_attention_values_of_unequal_size():
     """Values whose groups differ by many orders of magnitude, token by token."""
     c = Case([90], 1, 128, 4, 64, 16, torch.float32, seed=12)
