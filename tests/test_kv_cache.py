@@ -705,6 +705,39 @@ def test_attention_scales_and_strong_scores():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("prompt,others", [(400, 63), (1500, 40)])
+def test_attention_of_a_prompt_beside_decoding_sequences(prompt, others, dtype):
+    """One call for a prompt chunk and sequences of one token: of 6 and of 38 tokens on
+    average, so that with four query heads for a K/V head the one takes the kernel for
+    few rows and the other, in 16 bits, that for prompts."""
+    heads, share, dim, page = 2, 4, 128, 32
+    g = torch.Generator(DEV).manual_seed(prompt)
+    lens = [(prompt + 300) if b == others // 2 else 1 + (b * 97) % 900 for b in range(others + 1)]
+    news = [prompt if b == others // 2 else 1 for b in range(others + 1)]
+    need = [-(-n // page) for n in lens]
+    order = torch.randperm(sum(need), generator=g, device=DEV).int()
+    table = torch.full((others + 1, max(need)), -1, dtype=torch.int32, device=DEV)
+    for b, n in enumerate(need):
+        table[b, :n] = order[ends(need)[b]:ends(need)[b + 1]]
+    cache = KvCache(sum(need), page, heads, dim, 4, 64, DEV)
+    k, v = torch.randn(2, sum(lens), heads, dim, generator=g, device=DEV)
+    gpu_kv_cache_append(cache, k.to(dtype), v.to(dtype), table, i32(lens), i32(ends(lens)))
+    kc, vc = (x.double() for x in gpu_kv_cache_read(cache, table, i32(lens), i32(ends(lens)), tokens=sum(lens)))
+    low = vc.unflatten(-1, (-1, 64)).amin(-1).repeat_interleave(64, -1)
+    q = torch.randn(sum(news), heads * share, dim, generator=g, device=DEV).to(dtype)
+    out = gpu_kv_cache_attention(cache, q, table, i32(lens), i32(ends(news)))
+    rounded = dtype == torch.bfloat16 and sum(news) // (others + 1) * share >= 64
+    for b, n in enumerate(news):
+        a, la, le = ends(news)[b], ends(lens)[b], ends(lens)[b + 1]
+        want, tol = bounded_attention(q[a:a + n].double(), kc[la:le], vc[la:le], dim ** -0.5, dtype,
+                                      2.0 ** -11 if rounded else 0.0, low[la:le].abs() + (vc - low)[la:le])
+        off = np.abs(f64(out[a:a + n]) - want)
+        assert (off <= tol).all(), (b, (off / tol).max())
+    assert status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("q_scale,scale", [(1.0, 1e-44), (1e-30, 1e-25)])
 def test_attention_of_scores_that_vanish(q_scale, scale, dtype):
     """A scale and queries so small that their product is below f32: the average
