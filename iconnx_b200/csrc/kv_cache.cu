@@ -14,6 +14,7 @@
 
 #include "capi.cuh"
 #include "common.cuh"
+#include "tmap.cuh"
 
 namespace icx {
 
@@ -491,13 +492,13 @@ __global__ void __launch_bounds__(128, 8)
 // to four blocks per warp), with many a warp takes up to eight tokens.
 static Parts make_parts(const KvView& c, const KvTokens& w) {
   const int blocks = c.heads * (c.dim / 64), fours = (blocks + 3) / 4;
-  constexpr int64_t kWarps = 148 * 32;
+  const int64_t warps = (int64_t)sm_count() * 32;
   Parts n{1, 1, 0, 0};
-  while (n.parts < fours && w.tokens * 2 * n.parts < kWarps) ++n.parts;
+  while (n.parts < fours && w.tokens * 2 * n.parts < warps) ++n.parts;
   n.per = (fours + n.parts - 1) / n.parts * 4;
   n.parts = (blocks + n.per - 1) / n.per;
   if (n.parts == 1)
-    while (n.run < 8 && w.tokens * 2 / (n.run * 2) >= kWarps) n.run *= 2;
+    while (n.run < 8 && w.tokens * 2 / (n.run * 2) >= warps) n.run *= 2;
   n.items = (unsigned)((w.tokens + n.run - 1) / n.run * 2 * n.parts);   // tokens < 2^31, and parts > 1 for few
   return n;
 }
