@@ -1,10 +1,13 @@
 // Attention of few query rows over the quantised K/V cache (decoding).
 //
 // The cache is read once, D bits / 4 + 8 D / group bytes per position and K/V
-// head (144 for 128 dimensions of 4 bits in groups of 64), so HBM sets the floor;
-// what bounds the kernel at 4 bits is the issue of about 340 instructions per 16
-// positions, half of them of the integer pipe.  Codes are therefore never
-// dequantised: with K[p] = c s + lo per group of dimensions,
+// head (144 for 128 dimensions of 4 bits in groups of 64), so HBM sets the floor.
+// At 4 bits a warp takes about 450 instructions for 16 positions, and at 128
+// registers an SM holds 16 warps: an instruction issues in 53% of the cycles, with
+// one of a scheduler's four warps ready and most others waiting for the result
+// before (integer pipe 50% busy, matrix pipe 23%, HBM 35%): too few warps for so
+// many dependent instructions.  Codes are therefore never dequantised: with
+// K[p] = c s + lo per group of dimensions,
 //     q . K[p] = sum_groups  s (q . c) + lo sum(q)
 //     sum_p w_p V[p] = sum_p (w_p s_p) c_p + sum_p w_p lo_p
 // and the two contractions run on m16n8k16 matrix instructions whose left
@@ -79,10 +82,9 @@ __host__ __device__ constexpr int att_resident(int dim, int nt, int q_bytes) {
 
 // 8 or 16 query rows per tile.  16 read the cache half as often but take twice
 // the registers and instructions, which a warp with few steps has to fetch: they
-// pay for long runs in f32 alone (64 rows of one sequence of 16,000, 8 K/V heads
-// of 4 query heads of 128, 4 bits: 198 -> 168 us), not in 16 bits (4 rows of 64
-// sequences of up to 8,000, bf16: 184 -> 199 us) nor in short runs (5 rows of 6
-// sequences of up to 5,300, bf16: 27 -> 29 us; 32 rows per tile: 48 us).
+// pay for long runs in f32 alone (4 tokens of each of 64 sequences of up to 8,000, 8
+// K/V heads of 4 query heads of 128, 4 bits: 277 -> 263 us), not in 16 bits (bf16:
+// 203 -> 226 us) nor in short runs (6 sequences of up to 5,300, bf16: 42 -> 44 us).
 template <typename T>
 constexpr int att_most_nt(int dim) {
   return sizeof(T) == 4 && dim <= 128 ? 2 : 1;
@@ -92,7 +94,7 @@ constexpr int att_most_nt(int dim) {
 // their parts in the workspace; the warps of one CTA, which join in shared memory
 // (one launch, no workspace: 1 token on 500 positions, 12 heads of 64, f32: 12.5 -> 10.0
 // us; 16 sequences of up to 500, 8 K/V heads of 4 query heads of 128, bf16: 18.6 ->
-// 13.8).
+// 13.8, and 14.4 since w s is two f16).
 enum AttendSplit { kSplitNone, kSplitAny, kSplitCta };
 
 struct AttendArgs {
@@ -231,7 +233,9 @@ struct AttConfig {
   // f32: codes as f16 integers less kMiddle (one more instruction per operand
   // word), so that the two parts of a sum, s c and lo, do not cancel: with K and V
   // around zero they are some forty times the output (error 3.4e-6 of it without).
-  // A code counts 1 then, not 2^-24.
+  // A code counts 1 then, not 2^-24.  16-bit outputs, with half steps of 2^-11 and
+  // 2^-8, go without (64 sequences of up to 16,000 as above, before the pieces: 212
+  // -> 265 us with it).
   static constexpr bool CENTRE = sizeof(T) == 4;
   static constexpr float kMiddle = CENTRE ? (float)(1 << (BITS - 1)) : 0.0f;
   static constexpr float kUnit = CENTRE ? 1.0f : 16777216.0f;

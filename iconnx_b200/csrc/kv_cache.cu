@@ -1,9 +1,13 @@
 // Quantised K/V cache: append (quantise) and read (dequantise).
 //
-// HBM sets the floor, the issue of about 350 (append) and 110 (read) instructions
-// per 256 values the time: 7 f16 prompts of up to 3,000 tokens into 8 bits, 8 heads
-// of 128, 56 us (2.4 TB/s; floor 21); 6 sequences of up to 8,100 read from 4 bits
-// to bf16, 39 us (4.1 TB/s; floor 25); a decode step's append or read 2.6 to 2.8.
+// HBM sets the floor: 7 f16 prompts of up to 3,000 tokens into 8 bits, 8 heads of
+// 128, 57 us (2.4 TB/s; floor 21; f32 58, floor 38); 6 sequences of up to 8,100 read
+// from 4 bits to bf16 or f16, 40 us (4.0 TB/s; floor 25), to f32 60 (floor 44); a
+// decode step's append or read 2.6 to 2.8.  What lies between: about 350 (append)
+// and 107 (read) instructions per 256 values, of which one issues in 63% and 64% of
+// the cycles (integer pipe 53% and 62%), while three warps wait for memory per
+// instruction: lookups, then one token's values (append) or four tokens' codes
+// (read) in flight.  Nothing is full.
 // Eight lanes take 64 dimensions of one (token, head) of K or V,
 // eight consecutive ones (one or two 16-byte accesses) per lane, so a
 // quantisation group is 4 or 8 lanes and every code word of the layout is put

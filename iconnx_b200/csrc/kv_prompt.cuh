@@ -151,7 +151,7 @@ __device__ __forceinline__ void put_query(const AttendArgs& a, const T* q, bool 
   // A group is fetched with eight 16-byte loads at once: with nearly all of the
   // SM's memory shared there is no L1 that would keep a row, and a warp's load
   // touches 32 of them (all of it in 8-byte loads: 265 us instead of 250 where
-  // kv_prompt_bf16.cu states 250).
+  // kv_prompt_bf16.cu states 253 now).
   Vec<T, 8> u[kPrGroup / 8];
   const bool wide = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
   auto fetch = [&](int k) {

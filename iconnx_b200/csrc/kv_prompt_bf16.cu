@@ -2,17 +2,25 @@
 // chunks), on the 5th-generation tensor cores.
 //
 // A bf16 output has 8 significant bits, so here K and V are dequantised to f16
-// (11 bits: half a step is 2^-12, an eighth of the output's) on their way into
+// (11 bits: half a step is 2^-11, an eighth of the output's 2^-8) on their way into
 // shared memory, scaled by powers of two into f16's range, and the weights are
 // rounded to one f16.  Scores, their maximum and all sums stay f32.  That leaves
 // the softmax warps with about five instructions per score, against ten in
 // kv_prompt.cu, whose operands are exact and which f16 outputs take.
+// What it costs: a score is off by up to 2^-11 of scale * sum |q k|, its weight by
+// that part of itself, and a value by 2^-11 of itself (chunks of 400 tokens on up to
+// 9,000 positions: error 1.68e-3 of the output's norm, 1.66e-3 of which is bf16's
+// own rounding).  Sums need no pieces here: they are of values, not of codes
+// that only grow, and what matrix units cut off (up to 2^-23 of the sum per product,
+// 16,000 positions are 1,000 products) stays far below 2^-8 of the output.
 //
 // Dequantising is three instructions per pair: a code put into the low bits of
 // 1024 (f16) less 1024 is the code as a number, and code * (s 2^-E) + lo 2^-E is
 // the value times 2^-E.  The CTA looks over the scales of all its positions
 // first (a sixteenth of the cache) to choose E for K and for V; scales 2^20 times
-// smaller than the largest of the CTA's positions keep their 11 bits.
+// smaller than the largest of the CTA's positions keep their 11 bits.  (Those are
+// the positions that the last of its rows sees: beyond that factor a row's bits
+// depend on positions that it may not see itself.)
 // (A code in the low bits of a half word is also the f16 number code * 2^-24,
 // which saves the subtraction, but then s 2^24 2^-E has to fit f16: a scale
 // 2^15 below the largest was off by half its step.)
@@ -33,8 +41,8 @@
 // a row's scores stay in 128 registers.)
 //
 // Measured: 1024 tokens of each of 2 sequences of up to 6,000, 8 K/V heads of 4
-// query heads of 128, 4 bits: 250 us (floor 73 at 1.72 PFLOP/s).  128 rows per
-// CTA 284 us, one warp issuing for both row tiles 296.  About 18 us are a CTA's
+// query heads of 128, 4 bits: 253 us (floor 73 at 1.72 PFLOP/s).  128 rows per
+// CTA 284 us, one warp issuing for both row tiles 296 (beside 250 at the time).  About 18 us are a CTA's
 // start and end, and 1.5 waves of CTAs leave a quarter of the SMs' time unused.
 // Rows that do not see a position must not meet its NaN: a V group that holds
 // one is stored as zeros, and the rows that see it end as NaN.  That and pages

@@ -196,11 +196,22 @@ def gpu_kv_cache_attention(cache: KvCache, q: torch.Tensor, page_table: torch.Te
     ``scale`` (default 1 / sqrt(head_dim)) multiplies the scores.  Returns q's
     shape and type, contiguous.  A token without any position gives zeros;
     rows outside ``cu_tokens`` are left as they were in ``out`` (undefined in a
-    fresh tensor).  Scores, softmax statistics and sums are f32.  BFloat16
-    prompt chunks (64 rows of a K/V head per sequence or more, group 64,
-    head_dim up to 128) meet K, V and the weights as f16, K and V in units of
-    the largest of the positions a block of rows reads: values 2^20 times
-    smaller keep their bits, still smaller ones lose them.
+    fresh tensor).  Scores, softmax statistics and sums are f32.
+
+    Which kernel runs follows the rows per K/V head and sequence on average
+    over the call, ``tokens // batch * (q_heads // kv_heads)``: from 64 on, 16-bit
+    queries with group 64 and head_dim up to 128 take those for prompt chunks, all
+    else the one for few rows, which reads the cache once per 8 (16) rows.  A call
+    that mixes a long chunk with many single tokens is right either way, but two
+    calls, one for each, suit them better.
+
+    BFloat16 prompt chunks meet K, V and the weights as f16 (2^-11 of a value),
+    K and V in units of the largest of the positions a block of rows reads: values
+    2^20 times smaller keep their bits, still smaller ones lose them.  Elsewhere
+    the weights times the scales of V carry 22 bits where the scale is near the
+    largest met, about 17 at 2^-13 of it and 10 at 2^-20.  Queries of 2^75 and
+    more, and scores beyond 2^20, are more than f32 can tell apart: such rows may
+    come out as NaN.
     """
     what = "KvCacheAttention"
     q = _rows(q, None, cache.head_dim, cache.device, f"{what}: q")

@@ -351,9 +351,15 @@ ICX_API int icx_kv_cache_read(void* stream, const icx_kv_cache* cache, const icx
  * contiguous), q_heads a multiple of kv_heads (consecutive query heads share
  * a kv head); out: contiguous, of q's type.  A row without any position gives
  * zeros.  Positions without a usable page take no part.
- * Scores, softmax statistics and sums are f32; where an output is bf16 and a
- * sequence has many rows, K, V and the weights are rounded to f16.  The
- * workspace depends on the shapes alone. */
+ * Scores, softmax statistics and sums are f32.  Calls with 64 rows per K/V head
+ * and sequence or more on average (tokens / batch * (q_heads / kv_heads)), of a
+ * 16-bit type, group 64 and head_dim up to 128, take kernels for prompt chunks;
+ * there bf16 rounds K, V and the weights to f16, K and V in units of the largest
+ * of the positions that a block of rows reads (values 2^20 times smaller keep
+ * their bits).  Elsewhere weights times scales of V carry 22 bits where the scale
+ * is near the largest met, about 17 at 2^-13 of it and 10 at 2^-20.  Queries of
+ * 2^75 and more, and scores beyond 2^20, are more than f32 can tell apart: such
+ * rows may come out as NaN.  The workspace depends on the shapes alone. */
 ICX_API size_t icx_kv_cache_attention_workspace_bytes(const icx_kv_cache* cache,
                                                       const icx_kv_tokens* where, int q_heads,
                                                       int type);
