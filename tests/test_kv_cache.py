@@ -615,6 +615,73 @@ def test_prompt_rows_that_fill_the_gpu(dim, bits, tokens, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_prompt_rows_that_fill_the_gpu_with_missing_pages_and_nan(dtype):
+    tokens, heads, share, dim, page = 1200, 8, 4, 64, 32
+    g = torch.Generator(DEV).manual_seed(51)
+    need = -(-tokens // page)
+    cache = KvCache(need, page, heads, dim, 8, 64, DEV)
+    table = torch.randperm(need, generator=g, device=DEV).int()[None]
+    lens, cu = i32([tokens]), i32([0, tokens])
+    k, v = (x.to(dtype) for x in torch.randn(2, tokens, heads, dim, generator=g, device=DEV))
+    v[700, 3, 9] = float("nan")    # rows from 700 on, K/V head 3
+    k[900, 5, 1] = float("inf")    # rows from 900 on, K/V head 5
+    gpu_kv_cache_append(cache, k, v, table, lens, cu)
+    kc, vc = (x.double() for x in gpu_kv_cache_read(cache, table, lens, cu, tokens=tokens))
+    q = torch.randn(tokens, heads * share, dim, generator=g, device=DEV).to(dtype)
+    gone = table.clone()
+    gone[0, 3:5], gone[0, 20] = -1, need
+    out = gpu_kv_cache_attention(cache, q, gone, lens, cu)
+    assert status() == _lib.ICX_DEVICE_BAD_PAGE
+    nan = torch.zeros(out.shape, dtype=torch.bool, device=DEV)
+    nan[700:, 3 * share:4 * share] = True
+    nan[900:, 5 * share:6 * share] = True
+    assert torch.equal(out.isnan(), nan)
+    # the missing positions as zero weight: K that no row can prefer
+    mask = torch.zeros(tokens, device=DEV, dtype=torch.bool)
+    mask[96:160], mask[640:672] = True, True
+    keep = torch.arange(tokens, device=DEV)[~mask]
+    for row in (95, 96, 130, 160, 641, 699, 1199):   # each row over what it sees
+        seen = keep[keep <= row]
+        fine = [h for h in range(heads * share) if not nan[row, h, 0]]
+        kr, vr = (x[seen].repeat_interleave(share, 1)[:, fine] for x in (kc, vc))
+        want, tol = bounded_attention(q[row:row + 1, fine].double(), kr, vr, dim ** -0.5, dtype, 2.0 ** -11)
+        assert (np.abs(f64(out[row:row + 1, fine]) - want) <= tol).all(), row
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_prompt_chunks_captured_and_replayed_with_other_lengths(dtype):
+    """Few rows on a wide table (positions in shares) and many rows."""
+    for tokens, width, batch in ((130, 120, 2), (1300, 90, 2)):
+        heads, share, dim, page = 8, 4, 64, 16
+        g = torch.Generator(DEV).manual_seed(tokens)
+        pool = width * batch
+        cache = KvCache(pool, page, heads, dim, 4, 64, DEV)
+        table = torch.randperm(pool, generator=g, device=DEV).int().view(batch, width)
+        full = i32([width * page] * batch)
+        k, v = (x.to(dtype) for x in torch.randn(2, pool * page, heads, dim, generator=g, device=DEV))
+        gpu_kv_cache_append(cache, k, v, table, full, i32(ends([width * page] * batch)))
+        q = torch.randn(tokens, heads * share, dim, generator=g, device=DEV).to(dtype)
+        lens, cu = i32([0] * batch), i32([0] * (batch + 1))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = gpu_kv_cache_attention(cache, q, table, lens, cu)
+        half = tokens // 2
+        for ln, c in (([width * page, half], [0, half, tokens]), ([half + 1, 5], [0, 1, 6]),
+                      ([tokens - 3, width * page], [0, tokens - 2, tokens]), ([0, 0], [0, half, tokens]),
+                      ([1, width * page], [0, 0, tokens])):
+            lens.copy_(i32(ln))
+            cu.copy_(i32(c))
+            out.fill_(3.0)
+            graph.replay()
+            want = gpu_kv_cache_attention(cache, q, table, lens, cu, out=torch.full_like(out, 3.0))
+            assert torch.equal(out, want), (tokens, ln, c)
+            assert (out[c[-1]:] == 3.0).all()
+    assert status() == 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("dim,bits,group", [(64, 8, 64), (128, 4, 64), (128, 8, 32), (256, 8, 64)])
 def test_attention_beside_a_strong_dimension(dim, bits, group, dtype):
