@@ -5,6 +5,7 @@
 namespace icx {
 
 __device__ int g_icx_device_status = 0;
+__device__ int g_icx_device_bad_page = 0;
 
 static thread_local std::string t_last_error;
 
@@ -55,16 +56,20 @@ extern "C" int icx_device_status(int device, int* status_out) {
   int prev = 0;
   ICX_CUDA(cudaGetDevice(&prev));
   ICX_CUDA(cudaSetDevice(device));
-  int v = 0, zero = 0;
+  int v = 0, bad_page = 0, zero = 0;
   cudaError_t e =
       cudaMemcpyFromSymbol(&v, icx::g_icx_device_status, sizeof(int));
   if (e == cudaSuccess)
     e = cudaMemcpyToSymbol(icx::g_icx_device_status, &zero, sizeof(int));
+  if (e == cudaSuccess)
+    e = cudaMemcpyFromSymbol(&bad_page, icx::g_icx_device_bad_page, sizeof(int));
+  if (e == cudaSuccess)
+    e = cudaMemcpyToSymbol(icx::g_icx_device_bad_page, &zero, sizeof(int));
   cudaSetDevice(prev);
   if (e != cudaSuccess) {
     icx::set_error("icx_device_status: %s", cudaGetErrorString(e));
     return ICX_ERR_CUDA;
   }
-  *status_out = v;
+  *status_out = v != 0 ? v : bad_page ? ICX_DEVICE_BAD_PAGE : 0;
   return ICX_OK;
 }

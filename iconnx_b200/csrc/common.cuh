@@ -22,6 +22,9 @@ namespace icx {
 // Device-side status word written by bounded waits that give up
 // (ICX_DEVICE_TIMEOUT_*).  Read back with icx_device_status().
 extern __device__ int g_icx_device_status;
+// Whether a cache operator met a position without a usable page: a word of its
+// own, so that a caller's mistake does not hide a wait that gave up.
+extern __device__ int g_icx_device_bad_page;
 
 // Wall-clock bound of every spin-wait: 2 seconds, far beyond any legitimate
 // wait in these kernels (a whole GEMM takes milliseconds).
@@ -37,12 +40,11 @@ __device__ __forceinline__ uint32_t smem_addr(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
 
-// The first code stays, but a bad page (a caller's mistake, nothing touched)
-// gives way to a wait that gave up, whose results are not whole.
 __device__ __forceinline__ void record_status(int code) {
-  if (atomicCAS(&g_icx_device_status, 0, code) == ICX_DEVICE_BAD_PAGE)
-    atomicCAS(&g_icx_device_status, ICX_DEVICE_BAD_PAGE, code);
+  atomicCAS(&g_icx_device_status, 0, code);
 }
+
+__device__ __forceinline__ void record_bad_page() { g_icx_device_bad_page = 1; }
 
 // ----------------------------------------------------------------- mbarrier
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {

@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
     const int reach = (int)min((int64_t)su.len, (int64_t)w.width << c.page_shift);
     const int see_any = (int)max((int64_t)0, min(first_pos + (r0 + nrows - 1) / share + 1, (int64_t)reach));
     const int see_all = (int)max((int64_t)0, min(first_pos + r0 / share + 1, (int64_t)reach));
-    if (lane == 0 && su.len > reach) record_status(ICX_DEVICE_BAD_PAGE);
+    if (lane == 0 && su.len > reach) record_bad_page();
 
     // ------------------------------------------------------- codes on their way
     uint8_t* ring = smem + warp * C::kStages * C::kStage;
@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(32 * kAttWarps, (AttConfig<T, D, BITS, GROUP, 
     auto fetch_pages = [&](int from) {   // from: a tile, a multiple of 32
       const int i = from + lane, p = p0 + i / SUB * kStep + i % SUB * 16;
       my_page = p < end ? (int)kv_page(c, w, seq, p) : -1;
-      if (p < end && my_page < 0) record_status(ICX_DEVICE_BAD_PAGE);
+      if (p < end && my_page < 0) record_bad_page();
     };
     // bits SUB st ..: which tiles of stage st have a page and positions
     uint32_t there = 0;

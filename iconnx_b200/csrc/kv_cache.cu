@@ -321,7 +321,7 @@ __device__ __forceinline__ WarpPart warp_part(const KvView& c, const KvTokens& w
       const int64_t page = kv_page(c, w, b, p.pos);
       if (page < 0) {
         p.pos = -1;
-        record_status(ICX_DEVICE_BAD_PAGE);
+        record_bad_page();
       } else {
         p.row0 = kv_row(c, page, 0, p.pos);
       }

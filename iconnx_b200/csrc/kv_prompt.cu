@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(kPrThreads, 2)
     const int see_all = (int)max((int64_t)0, min(first_pos + r0 / share + 1, (int64_t)reach));
     const PromptShare part(see_any, kPrKeys, splits);
     const int tiles = part.tiles, p0 = part.first, p_end = part.end;
-    if (threadIdx.x == 0 && su.len > reach) record_status(ICX_DEVICE_BAD_PAGE);
+    if (threadIdx.x == 0 && su.len > reach) record_bad_page();
 
     if (warp >= 4) {
       // ------------------------------------------------------------ codes
@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kPrThreads, 2)
         const int pos = p0 + i * kPrKeys + key;
         const int64_t page = pos < p_end ? kv_page(c, w, seq, pos) : -1;
         hole = pos < p_end && page < 0;
-        if (hole && half == 0) record_status(ICX_DEVICE_BAD_PAGE);
+        if (hole && half == 0) record_bad_page();
         if (page >= 0) raw.load(c, kv_row(c, page, head, pos), pos, half);
         if (warp == 4) {
 #pragma unroll

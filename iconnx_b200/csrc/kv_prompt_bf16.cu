@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kB16Threads, 1)
     const int see_any = (int)max((int64_t)0, min(first_pos + (r0 + nrows - 1) / share + 1, (int64_t)reach));
     const PromptShare part(see_any, kB16Keys, splits);
     const int tiles = part.tiles, p0 = part.first, p_end = part.end;
-    if (threadIdx.x == 0 && su.len > reach) record_status(ICX_DEVICE_BAD_PAGE);
+    if (threadIdx.x == 0 && su.len > reach) record_bad_page();
 
     // the first look
     {
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(kB16Threads, 1)
         const int64_t page = kv_page(c, w, seq, pos);
         if (page < 0) {
           special = 1;
-          record_status(ICX_DEVICE_BAD_PAGE);
+          record_bad_page();
           continue;
         }
         uint32_t prm[2][G];
